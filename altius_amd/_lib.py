@@ -48,6 +48,59 @@ class FusedStep(ctypes.Structure):
                 ("pow_scalar_exponent", c_int)]
 
 
+class Rotary(ctypes.Structure):
+    """ahip_rotary"""
+    _fields_ = [("frequencies", c_void_p), ("dim", ctypes.c_int32), ("layout", ctypes.c_int32), ("magnitude", c_float)]
+
+    def __init__(self, frequencies=None, dim=0, layout=0, magnitude=1.0):
+        super().__init__(frequencies, dim, layout, magnitude)
+
+
+class _Described(ctypes.Structure):
+    """Fields by name; those left out take the class's defaults."""
+    _defaults = {}
+
+    def __init__(self, **fields):
+        super().__init__(**{**self._defaults, **fields})
+
+
+class HeadRows(_Described):
+    """ahip_head_rows; pointers as integers, strides as tuples (batch, token, head)."""
+    _fields_ = [("out", c_void_p), ("x", c_void_p), ("batch", c_size_t), ("tokens", c_size_t), ("heads", c_size_t), ("head_size", c_size_t),
+                ("out_strides", c_size_t * 3), ("x_strides", c_size_t * 3), ("positions", c_void_p), ("position_size", ctypes.c_int32),
+                ("position_stride", c_size_t), ("first_position", c_int64), ("gamma", c_void_p), ("epsilon", c_float)]
+    _defaults = {"position_size": 4}
+
+
+class KvCache(_Described):
+    """ahip_kv_cache"""
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("elem", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_size", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("pages", c_int64), ("page_stride", c_int64), ("head_stride", c_int64), ("slot_stride", c_int64)]
+
+
+class KvBatch(_Described):
+    """ahip_kv_batch"""
+    _fields_ = [("sequences", ctypes.c_int32), ("table_pages", ctypes.c_int32), ("table_stride", c_int64), ("query_starts", c_void_p),
+                ("lengths", c_void_p), ("page_table", c_void_p)]
+
+
+class KvTokens(_Described):
+    """ahip_kv_tokens; strides as tuples (token, head)."""
+    _fields_ = [("tokens", c_size_t), ("q_heads", ctypes.c_int32), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p),
+                ("q_strides", c_size_t * 2), ("k_strides", c_size_t * 2), ("v_strides", c_size_t * 2), ("q_out_strides", c_size_t * 2),
+                ("q_gamma", c_void_p), ("k_gamma", c_void_p), ("epsilon", c_float), ("positions", c_void_p), ("position_size", ctypes.c_int32)]
+    _defaults = {"position_size": 4}
+
+
+class KvAttend(_Described):
+    """ahip_kv_attend; strides as tuples (token, head)."""
+    _fields_ = [("tokens", c_size_t), ("q_heads", ctypes.c_int32), ("q", c_void_p), ("out", c_void_p), ("q_strides", c_size_t * 2),
+                ("out_strides", c_size_t * 2), ("scale", c_float), ("softcap", c_float), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("slopes", c_void_p), ("prefix", c_void_p), ("first_keys", c_void_p), ("max_tokens", c_size_t), ("max_keys", c_size_t),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+    _defaults = {"scale": 1.0, "causal": 1}
+
+
 FUSED_ACC = -1
 FUSED_MAX_INPUTS = 6
 FUSED_MAX_STEPS = 16
@@ -97,6 +150,11 @@ def _declare(L):
       + [c_size_t] * 5 + [c_float, c_float])
     f("ahip_gemm_post", [c_void_p] * 5 + [c_size_t] * 3 + [c_int, c_int] + [c_size_t] * 5 + [c_float, c_float, c_int, c_void_p])
     f("ahip_attention", [c_void_p] * 5 + [c_size_t] * 9 + [P(c_size_t)] * 4 + [c_int, c_float, c_void_p, c_size_t])
+    f("ahip_rotary_frequencies", [P(ctypes.c_double), c_int, ctypes.c_double, c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double])
+    f("ahip_rotary_heads", [c_void_p, P(HeadRows), P(Rotary)])
+    f("ahip_kv_append", [c_void_p, P(KvCache), P(KvBatch), P(KvTokens), P(Rotary)])
+    f("ahip_kv_attention_workspace", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), P(c_size_t)])
+    f("ahip_kv_attention", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend)])
     f("ahip_gemm_set_algorithm", [c_void_p, c_int])
     f("ahip_set_streaming_threshold", [c_void_p, c_size_t])
     f("ahip_set_load_streaming_threshold", [c_void_p, c_size_t])

@@ -46,6 +46,12 @@ int create_ctx(int device, hipStream_t stream, bool own_stream, ahip_ctx **out) 
     return AHIP_OK;
 }
 
+// The next ahip_sync looks at the error flags; every later one too if this call is being recorded, since its replays are not seen here.
+void arm_flags(DeviceCtx &d) {
+    d.flags_armed = true;
+    if (!d.flags_recorded && altius::stream_is_recording(d)) d.flags_recorded = true;
+}
+
 }  // namespace
 
 #define REQUIRE_CTX(ctx, name)                                                       \
@@ -573,6 +579,48 @@ int ahip_attention(ahip_ctx *ctx, float *o, const float *q, const float *k, cons
                                     k_batch_strides, v_batch_strides, o_batch_strides, scale_op, scale, mask, mask_outer_stride);
 } catch (...) {
     return altius::caught_at_boundary("ahip_attention");
+}
+
+int ahip_rotary_frequencies(double *frequencies, int dim, double base, int scaling, double factor, double length, double slow_turns,
+                            double fast_turns) try {
+    return altius::rotary_frequencies(frequencies, dim, base, scaling, factor, length, slow_turns, fast_turns);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_rotary_frequencies");
+}
+
+int ahip_rotary_heads(ahip_ctx *ctx, const ahip_head_rows *rows, const ahip_rotary *rotary) try {
+    REQUIRE_CTX(ctx, "ahip_rotary_heads");
+    if (!rows) return ctx->d.fail(AHIP_ERR_ARG, "ahip_rotary_heads: null rows");
+    if (!rows->gamma && !rotary) return ctx->d.fail(AHIP_ERR_ARG, "ahip_rotary_heads: neither a norm nor a rotation");
+    return altius::launch_rotary_heads(ctx->d, *rows, rotary);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_rotary_heads");
+}
+
+int ahip_kv_append(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_tokens *tokens,
+                   const ahip_rotary *rotary) try {
+    REQUIRE_CTX(ctx, "ahip_kv_append");
+    if (!cache || !batch || !tokens) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_append: null cache, batch or tokens");
+    arm_flags(ctx->d);
+    return altius::launch_kv_append(ctx->d, *cache, *batch, *tokens, rotary);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_append");
+}
+
+int ahip_kv_attention_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
+                                size_t *bytes) try {
+    return altius::kv_attention_workspace(ctx ? &ctx->d : nullptr, cache, batch, attend, bytes);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention_workspace");
+}
+
+int ahip_kv_attention(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend) try {
+    REQUIRE_CTX(ctx, "ahip_kv_attention");
+    if (!cache || !batch || !attend) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_attention: null cache, batch or attend");
+    arm_flags(ctx->d);
+    return altius::launch_kv_attention(ctx->d, *cache, *batch, *attend);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention");
 }
 
 int ahip_gemm_set_algorithm(ahip_ctx *ctx, int algorithm) try {

@@ -102,12 +102,12 @@ int create_device_ctx(int device, hipStream_t stream, bool own_stream, DeviceCtx
 }
 
 int check_device_flags(DeviceCtx &ctx) {
-    if (!ctx.flags_armed) return AHIP_OK;
+    if (!ctx.flags_armed && !ctx.flags_recorded) return AHIP_OK;
     ctx.flags_armed = false;
-    int raised[2] = {0, 0};
+    int raised[3] = {0, 0, 0};
     int rc = ctx.check(hipMemcpy(raised, ctx.flags, sizeof(raised), hipMemcpyDeviceToHost), "hipMemcpy(flags)");
     if (rc) return rc;
-    if (!raised[0] && !raised[1]) return AHIP_OK;
+    if (!raised[0] && !raised[1] && !raised[2]) return AHIP_OK;
     rc = ctx.check(hipMemset(ctx.flags, 0, sizeof(raised)), "hipMemset(flags)");
     if (rc) return rc;
     if (raised[1]) {
@@ -117,6 +117,8 @@ int check_device_flags(DeviceCtx &ctx) {
         return ctx.fail(AHIP_ERR_HIP, "MatMul: the slices of a tile cut along k ran on different XCDs, so their partial sums could not be "
                                       "combined; the in-kernel cut is now switched off for this context, run the product again");
     }
+    if (raised[2])
+        return ctx.fail(AHIP_ERR_ARG, "paged cache: a sequence's rows, length or pages do not fit the call's tensors, page table or cache");
     return ctx.fail(AHIP_ERR_ARG, "Gather: an index is outside the gathered axis");
 }
 

@@ -41,10 +41,11 @@ struct DeviceCtx {
     float *scratch = nullptr;
     size_t scratch_floats = 0;
     // Error flags kernels raise (device memory; int 0: Gather's index check, int 1: the slices of a GEMM tile
-    // cut along k did not share an XCD); read back by check_device_flags after a synchronisation, only when a
-    // kernel that can raise one has run.
+    // cut along k did not share an XCD, int 2: a batch's lengths or pages do not fit its cache); read back by
+    // check_device_flags after a synchronisation, only when a kernel that can raise one has run, or has been recorded by
+    // the caller, who may replay it unseen.
     int *flags = nullptr;
-    bool flags_armed = false;
+    bool flags_armed = false, flags_recorded = false;
     // Tensors of at least this many bytes are streamed with non-temporal accesses (a session raises it to
     // SESSION_NT_THRESHOLD_BYTES: its results are read by the node behind, out of the Infinity Cache if they fit).
     size_t nt_threshold_bytes = (size_t)64 << 20;
@@ -251,6 +252,14 @@ int launch_attention(DeviceCtx &ctx, float *o, const float *q, const float *k, c
 // of the product on the bf16 route that reads it (gemm_planes_bytes(batch_outer * tq, batch_inner * 64) bytes).  Only
 // where attention_writes_planes says so.
 bool attention_writes_planes(const DeviceCtx &ctx, size_t batch_outer, size_t batch_inner, size_t tq);
+
+// Rotary positions, a paged cache and attention over it (rotary.hip, kv_attention.hip); the structs are the C interface's.
+int launch_rotary_heads(DeviceCtx &ctx, const ahip_head_rows &rows, const ahip_rotary *rotary);
+int launch_kv_append(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_tokens &tokens, const ahip_rotary *rotary);
+int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend);
+// Host only; ctx may be null.
+int kv_attention_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, size_t *bytes);
+int rotary_frequencies(double *frequencies, int dim, double base, int scaling, double factor, double length, double slow_turns, double fast_turns);
 
 // The same product for one batch through three bf16 planes per operand and six bf16 MFMAs per fp32
 // product (gemm_split.hip): as accurate as an fp32 multiply-add chain, about 1.6 times the fp32 matrix

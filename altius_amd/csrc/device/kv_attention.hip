@@ -1,0 +1,631 @@
+// Attention of a batch's newest tokens over a paged cache of keys and values:
+//   x(row, j) = cap tanh(q k_j scale / cap) - slope |p - j|,   out = sum_j softmax(x)_j v_j   over low <= j < high,
+// a row being one query head of one token.  The rows of one kv head -- its group of query heads, times the sequence's new
+// tokens -- read the same keys, so they are computed together: row r is token r / group, head r % group of the group.
+//
+// One pass over the keys with a running maximum m and sum l of 2^(x log2(e)): where m rises, what has been summed is rescaled
+// by 2^(old - new).  Parts of a row's keys (wavefronts of a block, blocks of a sequence) keep their own m, l and sum and are
+// joined by the same rescaling.  All of it is held in fp32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "kv.h"
+#include "math.h"
+#include "split3.h"
+
+namespace altius {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.44269504088896341f;
+// Sequences with at most so many rows for a kv head share their keys' blocks out (attend_rows16, SPLIT); longer ones have
+// blocks enough.
+constexpr uint32_t FEW_ROWS = 64;
+
+struct AttendArgs {
+    dev::KvView kv;
+    const float *q;
+    float *out;
+    int64_t q_token, q_head, out_token, out_head;
+    uint32_t q_heads, group, d;
+    dev::FastDiv by_group;
+    float scale, cap;  // scale: with log2(e) where there is no cap; cap: 0, or the cap
+    int causal, window;
+    const float *slopes;
+    const int32_t *prefix, *first_keys;
+    uint32_t max_tokens, max_keys;
+    uint32_t row_tiles, splits, split_keys;
+    // Partial results of (sequence, kv head, row < rows_kept, split): maximum and sum, and the weighted sum of values.
+    float *part_stats, *part_out;
+    uint32_t rows_kept;
+};
+
+// The sequence, with n == 0 where the call's bounds leave it out (too long for them: the flag is raised).
+__device__ __forceinline__ dev::KvSequence sequence_of(const AttendArgs &g, uint32_t s) {
+    dev::KvSequence q = dev::kv_sequence(g.kv, s);
+    if ((uint32_t)q.n > g.max_tokens || (uint32_t)q.length > g.max_keys) {
+        *g.kv.flag = 1;
+        q.n = 0;
+    }
+    return q;
+}
+
+struct RowRange {
+    int32_t low, high, place;
+};
+__device__ __forceinline__ RowRange row_range(const AttendArgs &g, const dev::KvSequence &q, uint32_t s, uint32_t token) {
+    RowRange r;
+    r.place = q.length - q.n + (int32_t)token;
+    r.high = g.causal ? r.place + 1 : q.length;
+    if (g.prefix) r.high = max(r.high, g.prefix[s]);
+    r.high = min(r.high, q.length);
+    r.low = g.window ? max(0, r.place - g.window + 1) : 0;
+    if (g.first_keys) r.low = max(r.low, g.first_keys[q.start + (int32_t)token]);
+    return r;
+}
+
+// 2^(the score that the product `dot` of a query and a key stands for): scaled, capped and biased, in units of log2(e).
+__device__ __forceinline__ float score(const AttendArgs &g, float dot, float slope, int32_t distance) {
+    float x = dot * g.scale;
+    if (g.cap != 0.0f) x = g.cap * LOG2E * dev::tanh_elem(x / g.cap);
+    if (g.slopes) x -= slope * (float)abs(distance);
+    return x;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
+template <bool BF16> __device__ __forceinline__ float cache_value(const void *base, int64_t at) {
+    return BF16 ? __uint_as_float((uint32_t)static_cast<const uint16_t *>(base)[at] << 16) : static_cast<const float *>(base)[at];
+}
+
+// ---------------------------------------------------------------- 16 rows a wavefront, keys straight from memory
+// Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T, with 16 rows as columns.  The accumulator of S^T has in
+// lane l, register r the score of row l % 16 and key 4 (l / 16) + r of the tile, which is where the second product wants P^T:
+// the k slots of its instructions are declared to be keys in that order.  Keys and values go from memory into registers in the
+// layout of the instructions' first operand, without LDS: a row of keys is read along its channels, 16 bytes a lane, a row of
+// values by 16 lanes side by side, each lane's channels being rows of O^T.
+//   fp32 cache: v_mfma_f32_16x16x4_f32, tiles of 16 keys.
+//   bf16 cache: v_mfma_f32_16x16x32_bf16, tiles of 32 keys; q and the weights as three bf16 numbers each, whose sum they are
+//   exactly (split3.h), so that each of the three products is exact in the fp32 sum; a lane holds 8 keys x DP / 16 channels of
+//   V and turns them with v_perm.
+template <bool BF16> constexpr int KEYS = BF16 ? 32 : 16;
+constexpr int ROW_WAVES = 4;
+
+template <int DP, bool BF16> struct RowTile;
+template <int DP> struct RowTile<DP, false> {
+    f32x4 k[DP / 16], v[4][DP / 64];
+};
+template <int DP> struct RowTile<DP, true> {
+    u32x4 k[2][DP / 32];
+    uint32_t v[8][DP / 32];
+};
+template <int DP, bool BF16> struct RowQuery;
+template <int DP> struct RowQuery<DP, false> {
+    f32x4 q[DP / 16];
+};
+template <int DP> struct RowQuery<DP, true> {
+    u32x4 q[3][DP / 32];
+};
+
+#define ALTIUS_MFMA16_F32(A, B, C) C = __builtin_amdgcn_mfma_f32_16x16x4f32(A, B, C, 0, 0, 0)
+#define ALTIUS_MFMA16_BF16(A, B, C) \
+    C = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, A), __builtin_bit_cast(bf16x8, B), C, 0, 0, 0)
+
+// Row of O^T (channel) of accumulator i, register r, in lane group `part` = lane / 16.
+template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int i, int r, uint32_t part) {
+    return BF16 ? (DP / 16) * (4 * part + r) + i : 64 * (i / 4) + 4 * (4 * part + r) + i % 4;
+}
+
+// UNIFORM: pages hold whole tiles, so a tile's keys are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
+template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
+__global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows16(AttendArgs g) {
+    constexpr int KT = KEYS<BF16>, NACC = DP / 16, PITCH = DP + 4;
+    __shared__ __align__(16) float sums[ROW_WAVES][16 * PITCH];
+    __shared__ float stats[ROW_WAVES][2][16];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 15u, part = lane >> 4;
+
+    uint32_t id = blockIdx.x;
+    const uint32_t kvh = id % g.kv.kv_heads;
+    id /= g.kv.kv_heads;
+    const uint32_t tile = id % g.row_tiles;
+    id /= g.row_tiles;
+    const uint32_t split = id % g.splits, s = id / g.splits;
+
+    const dev::KvSequence seq = sequence_of(g, s);
+    const uint32_t rows = (uint32_t)seq.n * g.group;
+    if ((rows <= FEW_ROWS) != SPLIT || tile * 16 >= rows) return;
+    const uint32_t row = tile * 16 + col;
+    const bool valid = row < rows;
+    const uint32_t token = g.by_group.div(valid ? row : 0), head = kvh * g.group + (valid ? row : 0) - token * g.group;
+    const RowRange range = row_range(g, seq, s, token);
+    const int32_t low = range.low, high = range.high, place = range.place;
+    const bool sees = valid && low < high;
+    const float slope = g.slopes ? g.slopes[head] * LOG2E : 0.0f;
+
+    // What any row sees, and what all see.
+    int32_t any_low = sees ? low : INT32_MAX, any_high = sees ? high : 0, all_low = valid ? low : 0, all_high = valid ? high : INT32_MAX;
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+        any_low = min(any_low, __shfl_xor(any_low, m)), any_high = max(any_high, __shfl_xor(any_high, m));
+        all_low = max(all_low, __shfl_xor(all_low, m)), all_high = min(all_high, __shfl_xor(all_high, m));
+    }
+    int32_t begin = any_low, end = any_high;
+    if (SPLIT) begin = max(begin, (int32_t)(split * g.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * g.split_keys));
+    begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
+    const int32_t first = begin / KT, tiles = begin < end ? (end + KT - 1) / KT - first : 0;
+
+    const char *keys = static_cast<const char *>(g.kv.keys), *values = static_cast<const char *>(g.kv.values);
+    constexpr int SIZE = BF16 ? 2 : 4;
+    const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
+
+    RowQuery<DP, BF16> q;
+    const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
+    if constexpr (BF16) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+            const uint32_t c = 32 * i + 8 * part;
+            f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+            if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c), hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4);
+            uint32_t h[3][4];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                dev::split3_pair(lo[2 * e], lo[2 * e + 1], h[0][e], h[1][e], h[2][e]);
+                dev::split3_pair(hi[2 * e], hi[2 * e + 1], h[0][2 + e], h[1][2 + e], h[2][2 + e]);
+            }
+#pragma unroll
+            for (int p = 0; p < 3; p++) q.q[p][i] = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) {
+            const uint32_t c = 16 * i + 4 * part;
+            q.q[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (valid && c < g.d) q.q[i] = *reinterpret_cast<const f32x4 *>(q_row + c);
+        }
+    }
+
+    // Wavefront w takes tiles w, w + 4, ... of the block's; the pages of its next 64 tiles wait in one register.
+    const int32_t mine = tiles > (int32_t)wave ? (tiles - (int32_t)wave + ROW_WAVES - 1) / ROW_WAVES : 0;
+    int32_t pages = 0;
+    auto fetch_pages = [&](int32_t from) {
+        const int32_t i = from + (int32_t)lane;
+        pages = 0;
+        if (UNIFORM && i < mine) pages = g.kv.page_of(s, g.kv.by_page_size.div((uint32_t)((first + (int32_t)wave + i * ROW_WAVES) * KT)), 0);
+    };
+    auto tile_key = [&](int32_t i) { return (first + (int32_t)wave + i * ROW_WAVES) * KT; };
+    auto row_at = [&](uint32_t key) {  // elements from the start of the cache
+        const uint32_t index = g.kv.by_page_size.div(key);
+        return (int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
+    };
+    // Which key of its tile a lane's i-th row of values is, and (bf16) that of its rows of keys in half t.
+    auto value_key = [&](int i) { return BF16 ? 16 * (i / 4) + 4 * part + i % 4 : 4 * part + i; };
+    constexpr int VROWS = BF16 ? 8 : 4;
+
+    auto load = [&](int32_t i, RowTile<DP, BF16> &t) {
+        const int32_t key0 = tile_key(i);
+        int64_t k_at[2], v_at[VROWS];
+        if (UNIFORM) {
+            const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
+            const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
+            const int64_t base = (int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at;
+            for (int h = 0; h < (BF16 ? 2 : 1); h++) k_at[h] = base + (int64_t)(col + 16 * h) * g.kv.slot_stride;
+            for (int r = 0; r < VROWS; r++) v_at[r] = base + (int64_t)value_key(r) * g.kv.slot_stride;
+        } else {
+            // Keys behind the last that is seen have no page to be read from: the last one stands in for them.
+            for (int h = 0; h < (BF16 ? 2 : 1); h++) k_at[h] = row_at((uint32_t)min(key0 + (int32_t)col + 16 * h, end - 1));
+            for (int r = 0; r < VROWS; r++) v_at[r] = row_at((uint32_t)min(key0 + (int32_t)value_key(r), end - 1));
+        }
+        if constexpr (BF16) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    t.k[h][c] = u32x4{0, 0, 0, 0};
+                    if (32 * c + 8 * part < g.d) t.k[h][c] = *reinterpret_cast<const u32x4 *>(keys + (k_at[h] + 32 * c + 8 * part) * SIZE);
+                }
+#pragma unroll
+            for (int r = 0; r < VROWS; r++) {
+                const char *p = values + (v_at[r] + (DP / 16) * col) * SIZE;
+#pragma unroll
+                for (int w = 0; w < DP / 32; w++) t.v[r][w] = 0;
+                if (DP == 64) {
+                    if (4 * col < g.d) {
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+                        t.v[r][0] = x.x, t.v[r][1] = x.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < DP / 128; w++) {
+                        if ((DP / 16) * col + 8 * w < g.d) {
+                            const u32x4 x = *reinterpret_cast<const u32x4 *>(p + 16 * w);
+                            t.v[r][4 * w] = x.x, t.v[r][4 * w + 1] = x.y, t.v[r][4 * w + 2] = x.z, t.v[r][4 * w + 3] = x.w;
+                        }
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) {
+                t.k[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (16 * c + 4 * part < g.d) t.k[c] = *reinterpret_cast<const f32x4 *>(keys + (k_at[0] + 16 * c + 4 * part) * SIZE);
+            }
+#pragma unroll
+            for (int r = 0; r < VROWS; r++)
+#pragma unroll
+                for (int j = 0; j < DP / 64; j++) {
+                    t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (64 * j + 4 * col < g.d) t.v[r][j] = *reinterpret_cast<const f32x4 *>(values + (v_at[r] + 64 * j + 4 * col) * SIZE);
+                }
+        }
+        if (key0 < begin || key0 + KT > end) {  // slots that no row sees may hold anything: their weight is 0, so is their value then
+#pragma unroll
+            for (int r = 0; r < VROWS; r++) {
+                const int32_t key = key0 + (int32_t)value_key(r);
+                if (key < begin || key >= end) {
+                    if constexpr (BF16) {
+#pragma unroll
+                        for (int w = 0; w < DP / 32; w++) t.v[r][w] = 0;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < DP / 64; j++) t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
+                }
+            }
+        }
+    };
+
+    float top = -INFINITY, total = 0.0f;
+    f32x4 acc[NACC];
+#pragma unroll
+    for (int i = 0; i < NACC; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // Scores of the tile (NS registers a lane, key0 + value_key(r)), running maximum and sum, weights in their place.
+    constexpr int NS = VROWS;
+    auto weigh = [&](int32_t key0, float (&x)[NS]) {
+        const bool full = key0 >= all_low && key0 + KT <= all_high && key0 >= begin && key0 + KT <= end;
+        float most = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < NS; r++) {
+            const int32_t key = key0 + (int32_t)value_key(r);
+            x[r] = score(g, x[r], slope, place - key);
+            if (full || (key >= low && key < high && key >= begin && key < end)) most = fmaxf(most, x[r]);
+        }
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const float now = fmaxf(top, most);
+        if (__any(now != top)) {
+            const float corr = weight_of(top, now);
+            total *= corr;
+#pragma unroll
+            for (int i = 0; i < NACC; i++) acc[i] *= corr;
+            top = now;
+        }
+        const float base = now == -INFINITY ? 0.0f : now;
+#pragma unroll
+        for (int r = 0; r < NS; r++) {
+            const int32_t key = key0 + (int32_t)value_key(r);
+            const bool seen = full || (key >= low && key < high && key >= begin && key < end);
+            x[r] = seen ? exp2_fast(x[r] - base) : 0.0f;
+            total += x[r];
+        }
+    };
+
+    auto products = [&](int32_t i, const RowTile<DP, BF16> &t) {
+        const int32_t key0 = tile_key(i);
+        float x[NS];
+        if constexpr (BF16) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                f32x4 large = {0.0f, 0.0f, 0.0f, 0.0f}, small = large;
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    ALTIUS_MFMA16_BF16(t.k[h][c], q.q[2][c], small);
+                    ALTIUS_MFMA16_BF16(t.k[h][c], q.q[0][c], large);
+                    ALTIUS_MFMA16_BF16(t.k[h][c], q.q[1][c], small);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[4 * h + r] = large[r] + small[r];
+            }
+            weigh(key0, x);
+            u32x4 p[3];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t w[3];
+                dev::split3_pair(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
+                p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
+            }
+#pragma unroll
+            for (int c = 0; c < NACC; c++) {
+                u32x4 v;
+#pragma unroll
+                for (int m = 0; m < 4; m++) v[m] = __builtin_amdgcn_perm(t.v[2 * m + 1][c / 2], t.v[2 * m][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int e = 2; e >= 0; e--) ALTIUS_MFMA16_BF16(v, p[e], acc[c]);
+            }
+        } else {
+            f32x4 even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;
+#pragma unroll
+            for (int c = 0; c < DP / 16; c += 2) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    ALTIUS_MFMA16_F32(t.k[c][e], q.q[c][e], even);
+                    ALTIUS_MFMA16_F32(t.k[c + 1][e], q.q[c + 1][e], odd);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[r] = even[r] + odd[r];
+            weigh(key0, x);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int j = 0; j < DP / 64; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ALTIUS_MFMA16_F32(t.v[r][j][e], x[r], acc[4 * j + e]);
+        }
+    };
+
+    fetch_pages(0);
+    RowTile<DP, BF16> now, next;
+    if (mine > 0) load(0, now);
+    for (int32_t i = 0; i < mine; i++) {
+        if (i + 1 < mine) {
+            if (((i + 1) & 63) == 0) fetch_pages(i + 1);
+            load(i + 1, next);  // on its way during the products
+        }
+        products(i, now);
+        now = next;
+    }
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+
+    // An infinity or NaN among the keys or values, or a score beyond fp32, has left one here, and not always where the
+    // definition has it (0 x infinity of a key that the row does not see; parts of infinity of opposite signs).  Once more then,
+    // value by value.
+    float check = total * 0.0f;
+#pragma unroll
+    for (int i = 0; i < NACC; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) check = __builtin_fmaf(acc[i][r], 0.0f, check);
+    if (__any(valid && check != 0.0f)) {
+        top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NACC; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int32_t i = 0; i < mine; i++) {
+            const int32_t from = max(tile_key(i), begin), to = min(tile_key(i) + KT, end);
+            for (int32_t key = from; key < to; key++) {
+                const int64_t at = row_at((uint32_t)key);
+                float dot = 0.0f;
+                if (valid)
+                    for (uint32_t c = part; c < g.d; c += 4) dot = __builtin_fmaf(q_row[c], cache_value<BF16>(keys, at + c), dot);
+                dot += __shfl_xor(dot, 16);
+                dot += __shfl_xor(dot, 32);
+                if (!sees || key < low || key >= high) continue;
+                const float x = score(g, dot, slope, place - key), now_top = fmaxf(top, x);
+                const float corr = weight_of(top, now_top), p = exp2_fast(x - (now_top == -INFINITY ? 0.0f : now_top));
+                top = now_top;
+                total = total * corr + p;
+#pragma unroll
+                for (int j = 0; j < NACC; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t c = channel_of<DP, BF16>(j, r, part);
+                        if (c < g.d) acc[j][r] = acc[j][r] * corr + p * cache_value<BF16>(values, at + c);
+                    }
+            }
+        }
+    }
+
+    // The block's wavefronts join their parts.
+    if (part == 0) stats[wave][0][col] = top, stats[wave][1][col] = total;
+#pragma unroll
+    for (int i = 0; i < NACC; i += 4)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *reinterpret_cast<f32x4 *>(&sums[wave][col * PITCH + channel_of<DP, BF16>(i, r, part)]) = f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+    __syncthreads();
+
+    for (uint32_t unit = threadIdx.x; unit < 16 * (DP / 4); unit += 64 * ROW_WAVES) {
+        const uint32_t r = unit / (DP / 4), c = 4 * (unit % (DP / 4)), mine_row = tile * 16 + r;
+        if (mine_row >= rows || c >= g.d) continue;
+        float m = stats[0][0][r];
+#pragma unroll
+        for (int w = 1; w < ROW_WAVES; w++) m = fmaxf(m, stats[w][0][r]);
+        float l = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < ROW_WAVES; w++) {
+            const float f = weight_of(stats[w][0][r], m);
+            l = __builtin_fmaf(stats[w][1][r], f, l);
+            o += *reinterpret_cast<const f32x4 *>(&sums[w][r * PITCH + c]) * f;
+        }
+        if (SPLIT && g.splits > 1) {
+            const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * g.rows_kept + mine_row) * g.splits + split;
+            *reinterpret_cast<f32x4 *>(g.part_out + at * g.d + c) = o;
+            if (c == 0) g.part_stats[2 * at] = m, g.part_stats[2 * at + 1] = l;
+        } else {
+            const uint32_t t = g.by_group.div(mine_row), h = kvh * g.group + mine_row - t * g.group;
+            const RowRange of = row_range(g, seq, s, t);
+            const float recip = of.low < of.high ? 1.0f / l : 0.0f;
+            *reinterpret_cast<f32x4 *>(g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + c) =
+                of.low < of.high ? o * recip : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+}
+
+// Joins the splits of a row: a block per row, the splits dealt to its threads' groups of d / 4 lanes.
+constexpr int JOIN = 256;
+__global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g) {
+    __shared__ float tops[JOIN / 64], totals[JOIN / 64];
+    __shared__ __align__(16) f32x4 sums[JOIN];
+    uint32_t id = blockIdx.x;
+    const uint32_t row = id % g.rows_kept;
+    id /= g.rows_kept;
+    const uint32_t kvh = id % g.kv.kv_heads, s = id / g.kv.kv_heads;
+    const dev::KvSequence seq = sequence_of(g, s);
+    const uint32_t rows = (uint32_t)seq.n * g.group;
+    if (rows > FEW_ROWS || row >= rows) return;
+    const uint32_t t = g.by_group.div(row), h = kvh * g.group + row - t * g.group;
+    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * g.rows_kept + row) * g.splits;
+
+    float top = -INFINITY;
+    for (uint32_t i = threadIdx.x; i < g.splits; i += JOIN) top = fmaxf(top, g.part_stats[2 * (at + i)]);
+    top = dev::wave_reduce<dev::MaxOp>(top);
+    if ((threadIdx.x & 63u) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < JOIN / 64; w++) top = fmaxf(top, tops[w]);
+    float total = 0.0f;
+    for (uint32_t i = threadIdx.x; i < g.splits; i += JOIN) total = __builtin_fmaf(g.part_stats[2 * (at + i) + 1], weight_of(g.part_stats[2 * (at + i)], top), total);
+    total = dev::wave_reduce<dev::SumOp>(total);
+    if ((threadIdx.x & 63u) == 0) totals[threadIdx.x >> 6] = total;
+
+    const uint32_t lanes = g.d / 4, groups = JOIN / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (group < groups) {
+        for (uint32_t i = group; i < g.splits; i += groups) {
+            const float f = weight_of(g.part_stats[2 * (at + i)], top);
+            if (f != 0.0f) o += *reinterpret_cast<const f32x4 *>(g.part_out + (at + i) * g.d + 4 * lane) * f;
+        }
+    }
+    sums[threadIdx.x] = o;
+    __syncthreads();
+    if (group != 0) return;
+    total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < JOIN / 64; w++) total += totals[w];
+    for (uint32_t i = 1; i < groups; i++) o += sums[i * lanes + lane];
+    const RowRange of = row_range(g, seq, s, t);
+    *reinterpret_cast<f32x4 *>(g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + 4 * lane) =
+        of.low < of.high ? o * (1.0f / total) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+struct Plan {
+    uint32_t rows, rows_kept, splits, split_keys;
+    size_t bytes;
+};
+
+Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
+    Plan p = {};
+    const uint32_t group = (uint32_t)(attend.q_heads / cache.kv_heads);
+    const size_t held = std::min((size_t)batch.table_pages * (size_t)cache.page_size, (size_t)INT32_MAX);
+    const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
+    const size_t max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
+    p.rows = (uint32_t)std::min(max_tokens * group, (size_t)1 << 30);
+    p.rows_kept = std::min(p.rows, FEW_ROWS);
+    const uint32_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
+    // Blocks enough for every CU to have several in turn, since sequences are of different lengths; no split shorter than 256 KiB.
+    const uint64_t blocks = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads * ((p.rows_kept + 15) / 16);
+    const uint64_t key_bytes = 2 * (uint64_t)cache.head_size * (cache.elem == AHIP_KV_BF16 ? 2 : 4);
+    const uint64_t least = std::max<uint64_t>(64, (256 * 1024 / key_bytes + 63) / 64 * 64);
+    const uint64_t wanted = std::max<uint64_t>(1, 8 * cus / std::max<uint64_t>(1, blocks));
+    const uint64_t each = std::max<uint64_t>(least, ((max_keys + wanted - 1) / wanted + 63) / 64 * 64);
+    p.split_keys = (uint32_t)std::min<uint64_t>(each, (uint64_t)1 << 31);
+    p.splits = (uint32_t)std::max<uint64_t>(1, (max_keys + p.split_keys - 1) / p.split_keys);
+    if (p.splits > 1) p.bytes = (size_t)batch.sequences * (size_t)cache.kv_heads * p.rows_kept * p.splits * ((size_t)cache.head_size + 2) * sizeof(float);
+    return p;
+}
+
+int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, dev::KvView *view) {
+    const std::string name = "kv attention: ";
+    if (!attend) return kv_fail(ctx, AHIP_ERR_ARG, name + "null attend");
+    if (int rc = make_kv_view(ctx, "kv attention", cache, batch, attend->tokens, view)) return rc;
+    if (attend->q_heads <= 0 || attend->q_heads > 65535 || attend->q_heads % cache->kv_heads)
+        return kv_fail(ctx, AHIP_ERR_SHAPE, name + std::to_string(attend->q_heads) + " query heads do not share " + std::to_string(cache->kv_heads) + " heads of keys");
+    if (!std::isfinite(attend->scale) || !std::isfinite(attend->softcap) || attend->softcap < 0 || attend->window < 0)
+        return kv_fail(ctx, AHIP_ERR_ARG, name + "the scale, the cap or the window is out of range");
+    const bool bf16 = cache->elem == AHIP_KV_BF16;
+    const int64_t unit = bf16 ? 8 : 4;
+    if (cache->head_size > 256 || cache->head_size % unit) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "no kernel for heads of " + std::to_string(cache->head_size));
+    bool on = aligned16(attend->q) && aligned16(attend->out) && aligned16(cache->keys) && aligned16(cache->values) && cache->page_stride % unit == 0 &&
+              cache->head_stride % unit == 0 && cache->slot_stride % unit == 0 && (!attend->workspace || aligned16(attend->workspace));
+    for (int i = 0; i < 2; i++) {
+        if (attend->q_strides[i] > ((size_t)1 << 48) || attend->out_strides[i] > ((size_t)1 << 48)) return kv_fail(ctx, AHIP_ERR_ARG, name + "a stride is out of range");
+        on = on && attend->q_strides[i] % 4 == 0 && attend->out_strides[i] % 4 == 0;
+    }
+    if (!on) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "a tensor or stride is not on 16-byte boundaries");
+    return AHIP_OK;
+}
+
+template <int DP, bool BF16, bool UNIFORM> int launch_rows(DeviceCtx &ctx, AttendArgs g, const Plan &plan) {
+    const uint64_t most = ((uint64_t)1 << 24) - 1;  // a grid ends at 2^32 threads
+    g.splits = plan.splits, g.split_keys = plan.split_keys, g.rows_kept = plan.rows_kept;
+    g.row_tiles = (plan.rows_kept + 15) / 16;
+    const uint64_t few = (uint64_t)g.kv.sequences * g.kv.kv_heads * g.row_tiles * g.splits, rows = (uint64_t)g.kv.sequences * g.kv.kv_heads * g.rows_kept;
+    const uint64_t many_tiles = (plan.rows + 15) / 16, many = (uint64_t)g.kv.sequences * g.kv.kv_heads * many_tiles;
+    if (few > most || rows > most || (plan.rows > FEW_ROWS && many > most)) return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
+    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, true>), dim3((uint32_t)few), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+    if (int rc = ctx.check(hipGetLastError(), "kv attention launch")) return rc;
+    if (g.splits > 1) {
+        hipLaunchKernelGGL(join_splits, dim3((uint32_t)rows), dim3(JOIN), 0, ctx.stream, g);
+        if (int rc = ctx.check(hipGetLastError(), "kv attention launch")) return rc;
+    }
+    if (plan.rows > FEW_ROWS) {
+        g.row_tiles = (uint32_t)many_tiles;
+        g.splits = 1;
+        hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, false>), dim3((uint32_t)many), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+        return ctx.check(hipGetLastError(), "kv attention launch");
+    }
+    return AHIP_OK;
+}
+
+template <bool BF16, bool UNIFORM> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g, const Plan &plan) {
+    if (g.d <= 64) return launch_rows<64, BF16, UNIFORM>(ctx, g, plan);
+    if (g.d <= 128) return launch_rows<128, BF16, UNIFORM>(ctx, g, plan);
+    return launch_rows<256, BF16, UNIFORM>(ctx, g, plan);
+}
+
+}  // namespace
+
+int kv_attention_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, size_t *bytes) {
+    if (!bytes) return kv_fail(ctx, AHIP_ERR_ARG, "kv attention: null output");
+    *bytes = 0;
+    dev::KvView view = {};
+    // The sizes alone: neither the tensors nor the arrays on the device need exist yet.
+    if (int rc = check_attend(ctx, cache, batch, attend, &view)) return rc;
+    *bytes = plan_of(ctx, *cache, *batch, *attend).bytes;
+    return AHIP_OK;
+}
+
+int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
+    AttendArgs g = {};
+    if (int rc = check_attend(&ctx, &cache, &batch, &attend, &g.kv)) return rc;
+    if (attend.tokens == 0 || batch.sequences == 0) return AHIP_OK;
+    if (int rc = require_kv_arrays(ctx, "kv attention", cache, batch)) return rc;
+    if (!attend.q || !attend.out) return ctx.fail(AHIP_ERR_ARG, "kv attention: null pointer");
+    const Plan plan = plan_of(&ctx, cache, batch, attend);
+    if (plan.bytes && (!attend.workspace || attend.workspace_bytes < plan.bytes))
+        return ctx.fail(AHIP_ERR_ARG, "kv attention: the workspace holds " + std::to_string(attend.workspace ? attend.workspace_bytes : 0) + " bytes of " +
+                                          std::to_string(plan.bytes));
+    g.q = attend.q, g.out = attend.out;
+    g.q_token = (int64_t)attend.q_strides[0], g.q_head = (int64_t)attend.q_strides[1];
+    g.out_token = (int64_t)attend.out_strides[0], g.out_head = (int64_t)attend.out_strides[1];
+    g.q_heads = (uint32_t)attend.q_heads, g.group = (uint32_t)(attend.q_heads / cache.kv_heads), g.d = (uint32_t)cache.head_size;
+    g.by_group = dev::make_fastdiv(g.group);
+    g.cap = attend.softcap;
+    g.scale = g.cap != 0.0f ? attend.scale : attend.scale * LOG2E;
+    g.causal = attend.causal, g.window = attend.window, g.slopes = attend.slopes, g.prefix = attend.prefix, g.first_keys = attend.first_keys;
+    g.max_tokens = (uint32_t)(attend.max_tokens ? std::min(attend.max_tokens, attend.tokens) : attend.tokens);
+    g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
+    g.part_stats = static_cast<float *>(attend.workspace);
+    const size_t parts = (size_t)g.kv.sequences * g.kv.kv_heads * plan.rows_kept * plan.splits;
+    g.part_out = g.part_stats ? g.part_stats + 2 * parts : nullptr;
+    // Pages that hold whole tiles: a tile's page is looked up once, not key by key.
+    const bool bf16 = cache.elem == AHIP_KV_BF16;
+    if (cache.page_size % (bf16 ? KEYS<true> : KEYS<false>) == 0) return bf16 ? launch_by_size<true, true>(ctx, g, plan) : launch_by_size<false, true>(ctx, g, plan);
+    return bf16 ? launch_by_size<true, false>(ctx, g, plan) : launch_by_size<false, false>(ctx, g, plan);
+}
+
+}  // namespace altius

@@ -9,7 +9,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from ._lib import check, i64_array
+from ._lib import HeadRows, KvAttend, KvBatch, KvCache, KvTokens, Rotary, check, i64_array  # noqa: F401 (described here for callers)
 
 ADD, SUB, MUL, DIV, POW = 0, 1, 2, 3, 4
 SQRT, ERF, GELU, SIGMOID, HARDSIGMOID, RELU, TANH, LEAKYRELU, EXP, ROUND, CLIP = range(11)
@@ -17,6 +17,9 @@ REDUCE_MEAN, REDUCE_MAX, REDUCE_SUM = 0, 1, 2
 BOOL, F32, I32, I64 = 0, 1, 2, 3
 GEMM_AUTO, GEMM_FP32, GEMM_BF16X3 = 0, 1, 2
 GEMM_DEFAULT = GEMM_FP32  # what a new context or session uses: the reference's results for every operand value
+ROTARY_HALVES, ROTARY_INTERLEAVED = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_TURNS = range(4)
+KV_F32, KV_BF16 = 0, 1
 _ELEM_OF = {np.dtype(np.bool_): BOOL, np.dtype(np.float32): F32, np.dtype(np.int32): I32, np.dtype(np.int64): I64}
 
 
@@ -36,6 +39,21 @@ def gemm_f32_grid(batch, m, n, k):
 def attention_rows_fits(batch, tq, tk):
     """Whether a session runs attention over that many heads, queries and keys (64 columns) as one kernel (host only)."""
     return bool(_lib.lib().ahip_attention_rows_fits(batch, tq, tk))
+
+
+def rotary_frequencies(dim, base=10000.0, scaling=ROTARY_PLAIN, factor=1.0, length=0.0, slow_turns=1.0, fast_turns=4.0):
+    """Radians per position of each pair of `dim` channels (float64, host only); scaling: ROTARY_PLAIN / LINEAR / BASE / TURNS."""
+    out = np.empty(max(dim // 2, 0), np.float64)
+    check(_lib.lib().ahip_rotary_frequencies(out.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), dim, base, scaling, factor, length, slow_turns, fast_turns))
+    return out
+
+
+def kv_attention_workspace(ctx, cache, batch, attend):
+    """Bytes of workspace that kv_attention_raw wants for these arguments; ctx may be None (host only)."""
+    n = ctypes.c_size_t()
+    handle = ctx.handle if ctx else None
+    check(_lib.lib().ahip_kv_attention_workspace(handle, ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(attend), ctypes.byref(n)), handle)
+    return n.value
 
 
 def broadcast_shape(a_dims, b_dims):
@@ -77,12 +95,15 @@ class DeviceBuffer:
 
 
 class Context:
-    """One device + one stream.  Not thread-safe; create one per thread."""
+    """One device + one stream (its own, or the hipStream_t given as an integer).  Not thread-safe; create one per thread."""
 
-    def __init__(self, device=0):
+    def __init__(self, device=0, stream=None):
         self.L = _lib.lib()
         h = ctypes.c_void_p()
-        check(self.L.ahip_init(int(device), ctypes.byref(h)))
+        if stream is None:
+            check(self.L.ahip_init(int(device), ctypes.byref(h)))
+        else:
+            check(self.L.ahip_init_on_stream(int(device), stream, ctypes.byref(h)))
         self.handle = h
         self._buffers = []
 
@@ -191,6 +212,25 @@ class Context:
     def reduce_static_raw(self, kind, out_ptr, in_ptr, outer, red, inner):
         """ahip_reduce_static: the reduction that allocates nothing (partial results in a fixed array)."""
         check(self.L.ahip_reduce_static(self.handle, kind, out_ptr, in_ptr, outer, red, inner), self.handle)
+
+    # --- positions by rotation, a paged cache, attention over it ------------
+    def rotary_raw(self, rows, rotary=None):
+        """ahip_rotary_heads: the norm (rows.gamma) and rotation of HeadRows `rows`."""
+        rc = self.L.ahip_rotary_heads(self.handle, rows, rotary)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_append_raw(self, cache, batch, tokens, rotary=None):
+        """ahip_kv_append: the KvTokens into the KvCache, queries turned on the way."""
+        rc = self.L.ahip_kv_append(self.handle, cache, batch, tokens, rotary)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_attention_raw(self, cache, batch, attend):
+        """ahip_kv_attention."""
+        rc = self.L.ahip_kv_attention(self.handle, cache, batch, attend)
+        if rc:
+            check(rc, self.handle)
 
     # --- convenience: numpy in, numpy out (upload, one kernel, download) ----
     def binary(self, op, a, b):

@@ -333,6 +333,127 @@ int ahip_attention(ahip_ctx *ctx, float *o, const float *q, const float *k, cons
                    const size_t q_batch_strides[2], const size_t k_batch_strides[2], const size_t v_batch_strides[2],
                    const size_t o_batch_strides[2], int scale_op, float scale, const float *mask, size_t mask_outer_stride);
 
+/* ------------------------------------------------------------------------
+ * What serves a decoder token by token: positions by rotation, a paged cache of keys and values, and attention
+ * that reads it.  No counterpart in the reference, which recomputes a whole prompt for each token.  Everything a
+ * batch's shape depends on (lengths, page tables, positions) is read from device memory by the kernels, so a
+ * recorded call can be replayed with other lengths.  Such a value out of range -- a page outside the cache, a length
+ * beyond the page table, a batch that does not fit the call -- never makes a kernel read or write elsewhere: the
+ * token is left out or page 0 is read, and the next ahip_sync on the context fails with AHIP_ERR_ARG.
+ * ---------------------------------------------------------------------- */
+
+/* Which channels of a head turn together: i and i + dim / 2, or 2 i and 2 i + 1. */
+#define AHIP_ROTARY_HALVES 0
+#define AHIP_ROTARY_INTERLEAVED 1
+/* Pair i of the first `dim` channels of a head, (a, b), becomes magnitude * (a cos t - b sin t, a sin t + b cos t) with
+ * t = position * frequencies[i]; the other channels stay.  The angle is reduced in 64 bits, so that far positions turn
+ * as exactly as near ones. */
+typedef struct ahip_rotary {
+    const double *frequencies; /* device, dim / 2 values: radians per position */
+    int32_t dim;               /* even */
+    int32_t layout;            /* AHIP_ROTARY_* */
+    float magnitude;           /* 1 where a scheme for long contexts asks for nothing else */
+} ahip_rotary;
+
+/* Frequencies base^(-2 i / dim) on the host, i < dim / 2, stretched for contexts longer than the one trained on (no GPU
+ * needed).  PLAIN: as they are.  LINEAR: all divided by factor (positions interpolated).  BASE: base multiplied by
+ * factor^(dim / (dim - 2)), which leaves the fastest pair and divides the slowest by factor.  TURNS: a pair that makes at
+ * most slow_turns turns over `length` positions is divided by factor, one that makes at least fast_turns is left, between
+ * the two the frequency is the mean of both weighted by where its turns lie. */
+enum ahip_rotary_scaling { AHIP_ROTARY_PLAIN = 0, AHIP_ROTARY_LINEAR = 1, AHIP_ROTARY_BASE = 2, AHIP_ROTARY_TURNS = 3 };
+int ahip_rotary_frequencies(double *frequencies, int dim, double base, int scaling, double factor, double length,
+                            double slow_turns, double fast_turns);
+
+/* Rows of head_size adjacent channels, one for each batch, token and head, read at x and written at out with strides in
+ * elements.  out may be x with the same strides; otherwise the two must not overlap, and rows of out never may. */
+typedef struct ahip_head_rows {
+    float *out;
+    const float *x;
+    size_t batch, tokens, heads, head_size;
+    size_t out_strides[3], x_strides[3]; /* batch, token, head */
+    const void *positions;               /* device, i32 or i64; NULL: first_position + token */
+    int32_t position_size;               /* 4 or 8 */
+    size_t position_stride;              /* from one batch's positions to the next one's; 0: all batches share them */
+    int64_t first_position;
+    const float *gamma; /* head_size weights: row * gamma / sqrt(mean(row^2) + epsilon) before it turns; NULL: no norm */
+    float epsilon;
+} ahip_head_rows;
+/* The norm (where rows->gamma is not NULL), then the rotation (where rotary is not NULL) of every row, in one pass. */
+int ahip_rotary_heads(ahip_ctx *ctx, const ahip_head_rows *rows, const ahip_rotary *rotary);
+
+/* Keys and values in pages: channel c of head h in slot s of page p is at p * page_stride + h * head_stride +
+ * s * slot_stride + c of `keys` and of `values` (elements).  A dense cache of one sequence is one long page. */
+#define AHIP_KV_F32 0
+#define AHIP_KV_BF16 1 /* rounded to nearest even when appended, taken as they are when read: half the bytes and memory */
+typedef struct ahip_kv_cache {
+    void *keys, *values;
+    int32_t elem; /* AHIP_KV_* */
+    int32_t kv_heads, head_size, page_size;
+    int64_t pages, page_stride, head_stride, slot_stride;
+} ahip_kv_cache;
+
+/* The sequences of a call.  Rows query_starts[s] .. query_starts[s + 1] - 1 of its tensors are the newest tokens of
+ * sequence s, which holds lengths[s] tokens with them; none is a sequence that sits the call out.  Rows behind the last
+ * sequence's are padding: not read, and left as they are where written.  The token at place j of sequence s is in slot
+ * j % page_size of page page_table[s * table_stride + j / page_size].  All three arrays are device memory. */
+typedef struct ahip_kv_batch {
+    int32_t sequences, table_pages; /* table_pages: entries of one sequence's row of the table */
+    int64_t table_stride;
+    const int32_t *query_starts; /* sequences + 1 */
+    const int32_t *lengths;      /* sequences */
+    const int32_t *page_table;
+} ahip_kv_batch;
+
+/* New tokens: k and v (kv_heads rows a token) and, where q_heads is not 0, q, whose rows are written to q_out (which may be
+ * q with the same strides).  Strides in elements: token, head. */
+typedef struct ahip_kv_tokens {
+    size_t tokens; /* rows of the tensors, padding included */
+    int32_t q_heads;
+    const float *q, *k, *v;
+    float *q_out;
+    size_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2];
+    const float *q_gamma, *k_gamma; /* norms of heads as in ahip_head_rows; NULL: none */
+    float epsilon;
+    const void *positions; /* device, one per row, to turn by; NULL: the token's place in its sequence */
+    int32_t position_size; /* 4 or 8 */
+} ahip_kv_tokens;
+/* Writes each token's keys, normed and turned as ahip_rotary_heads does it, and its values into its slot, and turns the
+ * queries on the way: one launch.  rotary may be NULL.  Two tokens of a call must not have the same slot. */
+int ahip_kv_append(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_tokens *tokens,
+                   const ahip_rotary *rotary);
+
+/* Attention of the newest tokens of each sequence over all of its keys, query head h with kv head h / (q_heads / kv_heads).
+ * The token at place p = lengths[s] - n + t (t of the sequence's n rows) sees the keys low <= j < high:
+ *     high = min(lengths[s], max(causal ? p + 1 : lengths[s], prefix ? prefix[s] : 0))
+ *     low  = max(0, window ? p - window + 1 : 0, first_keys ? first_keys[row] : 0)
+ * with the score  x = q k * scale,  softcap ? softcap * tanh(x / softcap) : x,  less slopes[h] * |p - j|.
+ * out = sum softmax(score) v; a row that sees no key is 0.  Documents packed into one sequence have their first keys as
+ * first_keys.  What lies in slots that a row does not see never reaches it, not even as infinity or NaN; sums and the
+ * softmax are held in 32 bits, and a bf16 cache's products with q and with the weights are exact to fp32. */
+typedef struct ahip_kv_attend {
+    size_t tokens; /* rows of q and out, padding included */
+    int32_t q_heads;
+    const float *q;
+    float *out;
+    size_t q_strides[2], out_strides[2]; /* token, head */
+    float scale, softcap;                /* softcap 0: none */
+    int32_t causal, window;              /* window 0: none */
+    const float *slopes;                 /* device, q_heads; NULL: none */
+    const int32_t *prefix;               /* device, sequences; NULL: none */
+    const int32_t *first_keys;           /* device, tokens; NULL: none */
+    size_t max_tokens, max_keys; /* no sequence of the batch has more rows or is longer; 0: as the tensors and the table allow */
+    void *workspace;
+    size_t workspace_bytes;
+} ahip_kv_attend;
+/* Bytes of device memory that a call of ahip_kv_attention with these arguments wants as its workspace (often 0), from the
+ * sizes alone: the lengths on the device do not matter.  ctx may be NULL (no GPU needed). */
+int ahip_kv_attention_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch,
+                                const ahip_kv_attend *attend, size_t *bytes);
+/* head_size up to 256 and a multiple of 4 (of 8 with a bf16 cache); q, out and the cache, with their strides, on 16-byte
+ * boundaries (AHIP_ERR_UNSUPPORTED otherwise, nothing launched).  The workspace holds partial results during the call:
+ * calls that run at the same time need one each.  out must not overlap q. */
+int ahip_kv_attention(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend);
+
 /* Which kernel ahip_gemm (and the MatMul / Gemm / Conv2d operators of a session on this context) uses
  * for a single-batch product.  AHIP_GEMM_FP32: v_mfma_f32_32x32x2_f32 on the operands as they are.
  * AHIP_GEMM_BF16X3: every operand value is split exactly into three bf16 numbers and six bf16 MFMAs per

@@ -1,0 +1,82 @@
+"""The host side of the decoder's operators, no GPU needed: frequencies of rotary positions, the workspace that attention
+over a paged cache wants, and what it refuses."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from altius_amd import _lib
+from altius_amd import device as D
+from altius_amd._lib import ERR_ARG, ERR_SHAPE, ERR_UNSUPPORTED, AltiusHipError
+
+
+def test_frequencies_by_their_formulas():
+    plain = 10000.0 ** (-np.arange(0, 64, 2) / 64)
+    np.testing.assert_allclose(D.rotary_frequencies(64), plain, rtol=1e-14)
+    np.testing.assert_allclose(D.rotary_frequencies(64, base=5e5), 5e5 ** (-np.arange(0, 64, 2) / 64), rtol=1e-14)
+    np.testing.assert_allclose(D.rotary_frequencies(64, scaling=D.ROTARY_LINEAR, factor=4), plain / 4, rtol=1e-14)
+    stretched = D.rotary_frequencies(64, scaling=D.ROTARY_BASE, factor=8)
+    assert stretched[0] == 1.0 and math.isclose(stretched[-1], plain[-1] / 8, rel_tol=1e-12) and (np.diff(stretched / plain) < 0).all()
+    by_turns = D.rotary_frequencies(64, scaling=D.ROTARY_TURNS, factor=8, length=1024, slow_turns=1, fast_turns=4)
+    turns = 1024 * plain / (2 * math.pi)
+    keep = np.clip((turns - 1) / 3, 0, 1)
+    np.testing.assert_allclose(by_turns, plain * (keep + (1 - keep) / 8), rtol=1e-13)
+    assert (by_turns[turns >= 4] == D.rotary_frequencies(64)[turns >= 4]).all() and D.rotary_frequencies(0).size == 0
+
+
+@pytest.mark.parametrize("arguments", [dict(dim=7), dict(dim=-2), dict(dim=8, base=0.0), dict(dim=8, base=math.inf), dict(dim=8, scaling=4), dict(dim=8, scaling=-1),
+                                       dict(dim=8, scaling=D.ROTARY_LINEAR, factor=0.0), dict(dim=8, scaling=D.ROTARY_LINEAR, factor=math.nan),
+                                       dict(dim=2, scaling=D.ROTARY_BASE, factor=2.0), dict(dim=8, scaling=D.ROTARY_TURNS, factor=2.0),
+                                       dict(dim=8, scaling=D.ROTARY_TURNS, factor=2.0, length=64.0, slow_turns=4.0, fast_turns=4.0)])
+def test_frequencies_refused(arguments):
+    with pytest.raises(AltiusHipError) as e:
+        D.rotary_frequencies(**arguments)
+    assert e.value.code == ERR_ARG
+
+
+CACHE = dict(elem=D.KV_F32, kv_heads=8, head_size=128, page_size=16, pages=100, page_stride=8 * 16 * 128, head_stride=16 * 128, slot_stride=128)
+BATCH = dict(sequences=4, table_pages=50, table_stride=50)
+ATTEND = dict(tokens=4, q_heads=32, q_strides=(32 * 128, 128), out_strides=(32 * 128, 128), scale=0.1, max_tokens=1)
+
+
+def workspace(**changed):
+    one = lambda base, kind: kind(**{**base, **{k: v for k, v in changed.items() if k in base or (k in dict(kind._fields_) and k not in {**CACHE, **BATCH, **ATTEND})}})  # noqa: E731
+    return D.kv_attention_workspace(None, one(CACHE, D.KvCache), one(BATCH, D.KvBatch), one(ATTEND, D.KvAttend))
+
+
+def test_the_workspace_goes_by_the_sizes():
+    few = workspace()
+    assert few >= 0 and few % 4 == 0
+    long = workspace(sequences=1, tokens=1, table_pages=4096, table_stride=4096)
+    row = (128 + 2) * 4
+    assert long > 0 and long % row == 0 and long // row % 32 == 0  # whole splits of 32 rows
+    assert workspace(sequences=1, tokens=1, table_pages=4096, table_stride=4096, max_keys=64) == 0  # short sequences are not split
+    # Many rows of a sequence have blocks enough: what is kept does not grow with the prompt.
+    assert workspace(sequences=1, tokens=100000, max_tokens=100000, table_pages=8000) <= 64 * 8 * 8000 * 16 // 64 * row
+
+
+@pytest.mark.parametrize("code,changed", [
+    (ERR_ARG, dict(elem=2)), (ERR_ARG, dict(kv_heads=0)), (ERR_ARG, dict(kv_heads=-1)), (ERR_ARG, dict(kv_heads=40000, q_heads=40000)), (ERR_ARG, dict(page_size=0)),
+    (ERR_ARG, dict(head_size=0)), (ERR_ARG, dict(pages=-1)), (ERR_ARG, dict(pages=1 << 31)), (ERR_ARG, dict(page_stride=-4)), (ERR_ARG, dict(slot_stride=1 << 31)),
+    (ERR_ARG, dict(sequences=-1)), (ERR_ARG, dict(table_pages=-1)), (ERR_ARG, dict(table_stride=-1)), (ERR_UNSUPPORTED, dict(table_pages=1 << 30)),
+    (ERR_SHAPE, dict(q_heads=31)), (ERR_SHAPE, dict(q_heads=0)), (ERR_SHAPE, dict(q_heads=-8)), (ERR_ARG, dict(scale=math.inf)), (ERR_ARG, dict(scale=math.nan)),
+    (ERR_ARG, dict(softcap=-1.0)), (ERR_ARG, dict(softcap=math.nan)), (ERR_ARG, dict(window=-1)), (ERR_UNSUPPORTED, dict(head_size=260)),
+    (ERR_UNSUPPORTED, dict(head_size=130)), (ERR_UNSUPPORTED, dict(elem=D.KV_BF16, head_size=100)), (ERR_UNSUPPORTED, dict(slot_stride=130)),
+    (ERR_UNSUPPORTED, dict(elem=D.KV_BF16, page_stride=4)), (ERR_UNSUPPORTED, dict(q=8)), (ERR_UNSUPPORTED, dict(out=4)), (ERR_UNSUPPORTED, dict(keys=2)),
+    (ERR_UNSUPPORTED, dict(workspace=8)), (ERR_UNSUPPORTED, dict(q_strides=(4096, 126))), (ERR_UNSUPPORTED, dict(out_strides=(4098, 128))),
+    (ERR_UNSUPPORTED, dict(tokens=1 << 23))])
+def test_attention_refuses(code, changed):
+    with pytest.raises(AltiusHipError) as e:
+        workspace(**changed)
+    assert e.value.code == code and str(e.value)
+
+
+def test_null_arguments_are_refused():
+    L = _lib.lib()
+    n = ctypes.c_size_t()
+    assert L.ahip_kv_attention_workspace(None, None, None, None, ctypes.byref(n)) == ERR_ARG
+    assert L.ahip_kv_attention_workspace(None, D.KvCache(**CACHE), D.KvBatch(**BATCH), D.KvAttend(**ATTEND), None) == ERR_ARG
+    assert L.ahip_rotary_heads(None, None, None) == ERR_ARG and L.ahip_kv_append(None, None, None, None, None) == ERR_ARG
+    assert L.ahip_kv_attention(None, None, None, None) == ERR_ARG
+    assert L.ahip_rotary_frequencies(None, 8, 10000.0, 0, 1.0, 0.0, 0.0, 0.0) == ERR_ARG
