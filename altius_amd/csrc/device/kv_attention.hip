@@ -20,6 +20,7 @@ namespace altius {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -31,6 +32,15 @@ constexpr float LOG2E = 1.44269504088896341f;
 // blocks enough.
 constexpr uint32_t FEW_ROWS = 64;
 
+// How the blocks share the work on the sequences of one kind: row tiles, and splits of split_keys keys each.  Where there are
+// several, the partial results of (sequence, kv head, row < rows, split) wait in the workspace: maximum and sum, and the weighted
+// sum of values.
+struct Share {
+    uint32_t row_tiles, splits, split_keys, rows;
+    uint32_t blocks;
+    float *part_stats, *part_out;
+};
+
 struct AttendArgs {
     dev::KvView kv;
     const float *q;
@@ -38,15 +48,12 @@ struct AttendArgs {
     int64_t q_token, q_head, out_token, out_head;
     uint32_t q_heads, group, d;
     dev::FastDiv by_group;
-    float scale, cap;  // scale: with log2(e) where there is no cap; cap: 0, or the cap
+    float scale, cap;  // scale: with log2(e), or by the cap where there is one; cap: 0, or the cap with log2(e)
     int causal, window;
     const float *slopes;
     const int32_t *prefix, *first_keys;
     uint32_t max_tokens, max_keys;
-    uint32_t row_tiles, splits, split_keys;
-    // Partial results of (sequence, kv head, row < rows_kept, split): maximum and sum, and the weighted sum of values.
-    float *part_stats, *part_out;
-    uint32_t rows_kept;
+    Share few, many;  // of sequences with up to FEW_ROWS rows, and with more
 };
 
 // The sequence, with n == 0 where the call's bounds leave it out (too long for them: the flag is raised).
@@ -73,16 +80,49 @@ __device__ __forceinline__ RowRange row_range(const AttendArgs &g, const dev::Kv
     return r;
 }
 
-// 2^(the score that the product `dot` of a query and a key stands for): scaled, capped and biased, in units of log2(e).
-__device__ __forceinline__ float score(const AttendArgs &g, float dot, float slope, int32_t distance) {
-    float x = dot * g.scale;
-    if (g.cap != 0.0f) x = g.cap * LOG2E * dev::tanh_elem(x / g.cap);
-    if (g.slopes) x -= slope * (float)abs(distance);
-    return x;
-}
-
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
+// tanh, as dev::rational_tanh has it, but for the division: a reciprocal and one step of Newton's, off by an fp32 step more at most.
+__device__ __forceinline__ float fast_tanh(float v) {
+    v = dev::rclamp(v, -9.0f, 9.0f);
+    const float v2 = v * v;
+    float p = __builtin_fmaf(v2, -2.76076847742355e-16f, 2.00018790482477e-13f);
+    p = __builtin_fmaf(p, v2, -8.60467152213735e-11f);
+    p = __builtin_fmaf(p, v2, 5.12229709037114e-08f);
+    p = __builtin_fmaf(p, v2, 1.48572235717979e-05f);
+    p = __builtin_fmaf(p, v2, 6.37261928875436e-04f);
+    p = __builtin_fmaf(p, v2, 4.89352455891786e-03f);
+    float q = __builtin_fmaf(v2, 1.19825839466702e-06f, 1.18534705686654e-04f);
+    q = __builtin_fmaf(q, v2, 2.26843463243900e-03f);
+    q = __builtin_fmaf(q, v2, 4.89352518554385e-03f);
+    float r = __builtin_amdgcn_rcpf(q);
+    r = __builtin_fmaf(__builtin_fmaf(-q, r, 1.0f), r, r);
+    return p * v * r;
+}
+
+// Products of a query and keys become scores in units of log2(e): scaled, capped, biased.  first_key + place(r) is the key of x[r].
+template <int N, class Place> __device__ __forceinline__ void scores(const AttendArgs &g, float (&x)[N], float slope, int32_t distance, Place place) {
+#pragma unroll
+    for (int r = 0; r < N; r++) x[r] *= g.scale;
+    if (g.cap != 0.0f) {
+#pragma unroll
+        for (int r = 0; r < N; r++) x[r] = g.cap * fast_tanh(x[r]);
+    }
+    if (g.slopes) {
+#pragma unroll
+        for (int r = 0; r < N; r++) x[r] -= slope * (float)abs(distance - (int32_t)place(r));
+    }
+}
+
+// A weight and its neighbour as three pairs of bf16 whose sums they are (weights are in [0, 1], or NaN).
+__device__ __forceinline__ void split_weights(float e0, float e1, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+    p0 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){e0, e1}, bf16x2));
+    const float r0 = e0 - __uint_as_float(p0 << 16), r1 = e1 - __uint_as_float(p0 & 0xffff0000u);
+    p1 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){r0, r1}, bf16x2));
+    const float s0 = r0 - __uint_as_float(p1 << 16), s1 = r1 - __uint_as_float(p1 & 0xffff0000u);
+    p2 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){s0, s1}, bf16x2));
+}
 
 template <bool BF16> __device__ __forceinline__ float cache_value(const void *base, int64_t at) {
     return BF16 ? __uint_as_float((uint32_t)static_cast<const uint16_t *>(base)[at] << 16) : static_cast<const float *>(base)[at];
@@ -127,20 +167,26 @@ template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int 
 }
 
 // UNIFORM: pages hold whole tiles, so a tile's keys are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
+template <int DP> struct RowLds {
+    static constexpr int PITCH = DP + 4;
+    float sums[ROW_WAVES][16 * PITCH];
+    float stats[ROW_WAVES][2][16];
+};
+
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
-__global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows16(AttendArgs g) {
-    constexpr int KT = KEYS<BF16>, NACC = DP / 16, PITCH = DP + 4;
-    __shared__ __align__(16) float sums[ROW_WAVES][16 * PITCH];
-    __shared__ float stats[ROW_WAVES][2][16];
+__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP> &lds) {
+    constexpr int KT = KEYS<BF16>, NACC = DP / 16, PITCH = RowLds<DP>::PITCH;
+    auto &sums = lds.sums;
+    auto &stats = lds.stats;
+    const Share &share = SPLIT ? g.few : g.many;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, part = lane >> 4;
 
-    uint32_t id = blockIdx.x;
     const uint32_t kvh = id % g.kv.kv_heads;
     id /= g.kv.kv_heads;
-    const uint32_t tile = id % g.row_tiles;
-    id /= g.row_tiles;
-    const uint32_t split = id % g.splits, s = id / g.splits;
+    const uint32_t tile = id % share.row_tiles;
+    id /= share.row_tiles;
+    const uint32_t split = SPLIT ? id % share.splits : 0, s = SPLIT ? id / share.splits : id;
 
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
@@ -161,7 +207,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
         all_low = max(all_low, __shfl_xor(all_low, m)), all_high = min(all_high, __shfl_xor(all_high, m));
     }
     int32_t begin = any_low, end = any_high;
-    if (SPLIT) begin = max(begin, (int32_t)(split * g.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * g.split_keys));
+    if (SPLIT) begin = max(begin, (int32_t)(split * share.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * share.split_keys));
     begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
     const int32_t first = begin / KT, tiles = begin < end ? (end + KT - 1) / KT - first : 0;
 
@@ -294,11 +340,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
     constexpr int NS = VROWS;
     auto weigh = [&](int32_t key0, float (&x)[NS]) {
         const bool full = key0 >= all_low && key0 + KT <= all_high && key0 >= begin && key0 + KT <= end;
+        scores(g, x, slope, place - key0, value_key);
         float most = -INFINITY;
 #pragma unroll
         for (int r = 0; r < NS; r++) {
             const int32_t key = key0 + (int32_t)value_key(r);
-            x[r] = score(g, x[r], slope, place - key);
             if (full || (key >= low && key < high && key >= begin && key < end)) most = fmaxf(most, x[r]);
         }
         most = fmaxf(most, __shfl_xor(most, 16));
@@ -342,7 +388,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 uint32_t w[3];
-                dev::split3_pair(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
+                split_weights(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
                 p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
             }
 #pragma unroll
@@ -411,8 +457,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
                 dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
                 if (!sees || key < low || key >= high) continue;
-                const float x = score(g, dot, slope, place - key), now_top = fmaxf(top, x);
-                const float corr = weight_of(top, now_top), p = exp2_fast(x - (now_top == -INFINITY ? 0.0f : now_top));
+                float x[1] = {dot};
+                scores(g, x, slope, place - key, [](int) { return 0; });
+                const float now_top = fmaxf(top, x[0]);
+                const float corr = weight_of(top, now_top), p = exp2_fast(x[0] - (now_top == -INFINITY ? 0.0f : now_top));
                 top = now_top;
                 total = total * corr + p;
 #pragma unroll
@@ -449,10 +497,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
             l = __builtin_fmaf(stats[w][1][r], f, l);
             o += *reinterpret_cast<const f32x4 *>(&sums[w][r * PITCH + c]) * f;
         }
-        if (SPLIT && g.splits > 1) {
-            const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * g.rows_kept + mine_row) * g.splits + split;
-            *reinterpret_cast<f32x4 *>(g.part_out + at * g.d + c) = o;
-            if (c == 0) g.part_stats[2 * at] = m, g.part_stats[2 * at + 1] = l;
+        if (SPLIT && share.splits > 1) {
+            const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + mine_row) * share.splits + split;
+            *reinterpret_cast<f32x4 *>(share.part_out + at * g.d + c) = o;
+            if (c == 0) share.part_stats[2 * at] = m, share.part_stats[2 * at + 1] = l;
         } else {
             const uint32_t t = g.by_group.div(mine_row), h = kvh * g.group + mine_row - t * g.group;
             const RowRange of = row_range(g, seq, s, t);
@@ -463,39 +511,406 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
     }
 }
 
+// Heads of more than 128 channels have no tiles of their own yet: all their rows go 16 a wavefront.
+template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
+__global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows16(AttendArgs g) {
+    __shared__ __align__(16) RowLds<DP> lds;
+    rows16<DP, BF16, UNIFORM, SPLIT>(g, blockIdx.x, lds);
+}
+
+// ---------------------------------------------------------------- 128 rows a block, keys through LDS
+// A wavefront owns 32 rows; the block's four share tiles of 32 keys in LDS.  S^T = K Q^T and O^T = V^T P^T again, by
+// v_mfma_f32_32x32x16_bf16: accumulator register r of lane l holds row l % 32 and key 8 (r / 4) + 4 (l / 32) + r % 4, and the
+// second product takes its k slots in that order, in which V^T lies in LDS.  Queries and weights are three bf16 numbers each, as
+// above; so are the values of an fp32 cache, split on their way into LDS, and six products of the parts are what fp32 holds of the
+// whole (the three left out are below 2^-24 of it).  A bf16 cache's values are one number: three products.
+//   The next tile's loads are in flight during the products; where LDS has room for two blocks' worth of two tiles the next one is
+// written while the other is read, with one barrier a tile.
+constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
+
+#define ALTIUS_MFMA32_BF16(A, B, C) \
+    C = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, A), __builtin_bit_cast(bf16x8, B), C, 0, 0, 0)
+
+template <int DP, bool BF16> struct TileLds {
+    static constexpr int PLANES = BF16 ? 1 : 3;
+    static constexpr int K_PITCH = DP + 8;          // 16-bit words; 16 rows of 16-byte reads cover all banks
+    static constexpr int V_PITCH = TILE_KEYS + 8;   // a row is a channel
+    static constexpr int BUFFERS = 2 * 2 * PLANES * (TILE_KEYS * K_PITCH + DP * V_PITCH) <= 80 * 1024 ? 2 : 1;
+    uint16_t k[BUFFERS][PLANES][TILE_KEYS * K_PITCH], v[BUFFERS][PLANES][DP * V_PITCH];
+    int32_t bounds[4][2];
+};
+
+template <int DP, bool BF16, bool UNIFORM>
+__device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLds<DP, BF16> &lds) {
+    using Lds = TileLds<DP, BF16>;
+    constexpr int PLANES = Lds::PLANES, K_PITCH = Lds::K_PITCH, V_PITCH = Lds::V_PITCH, BUFFERS = Lds::BUFFERS;
+    constexpr int STEPS = DP / 16, PARTS = DP / 32;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31u, h = lane >> 5;
+
+    // The last rows of a causal sequence see most keys: they start first.  Blocks that follow each other work on different heads.
+    const Share &share = g.many;
+    const uint32_t kvh = id % g.kv.kv_heads;
+    id /= g.kv.kv_heads;
+    const uint32_t s = id % g.kv.sequences;
+    id /= g.kv.sequences;
+    const uint32_t split = id % share.splits, tile = share.row_tiles - 1 - id / share.splits;
+
+    const dev::KvSequence seq = sequence_of(g, s);
+    const uint32_t rows = (uint32_t)seq.n * g.group;
+    if (rows <= FEW_ROWS || tile * TILE_ROWS >= rows) return;
+    const uint32_t row = tile * TILE_ROWS + wave * 32 + col;
+    const bool valid = row < rows;
+    const uint32_t token = g.by_group.div(valid ? row : 0), head = kvh * g.group + (valid ? row : 0) - token * g.group;
+    const RowRange range = row_range(g, seq, s, token);
+    const int32_t low = range.low, high = range.high, place = range.place;
+    const bool sees = valid && low < high;
+    const float slope = g.slopes ? g.slopes[head] * LOG2E : 0.0f;
+
+    int32_t any_low = sees ? low : INT32_MAX, any_high = sees ? high : 0, all_low = valid ? low : 0, all_high = valid ? high : INT32_MAX;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        any_low = min(any_low, __shfl_xor(any_low, m)), any_high = max(any_high, __shfl_xor(any_high, m));
+        all_low = max(all_low, __shfl_xor(all_low, m)), all_high = min(all_high, __shfl_xor(all_high, m));
+    }
+    if (lane == 0) lds.bounds[wave][0] = any_low, lds.bounds[wave][1] = any_high;
+    __syncthreads();
+    int32_t begin = INT32_MAX, end = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) begin = min(begin, lds.bounds[w][0]), end = max(end, lds.bounds[w][1]);
+    if (share.splits > 1)
+        begin = max(begin, (int32_t)(split * share.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * share.split_keys));
+    begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
+    any_low = __builtin_amdgcn_readfirstlane(any_low), any_high = __builtin_amdgcn_readfirstlane(any_high);
+    all_low = __builtin_amdgcn_readfirstlane(all_low), all_high = __builtin_amdgcn_readfirstlane(all_high);
+    const int32_t first = begin / TILE_KEYS, tiles = begin < end ? (end + TILE_KEYS - 1) / TILE_KEYS - first : 0;
+
+    const char *keys = static_cast<const char *>(g.kv.keys), *values = static_cast<const char *>(g.kv.values);
+    constexpr int SIZE = BF16 ? 2 : 4;
+    const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
+
+    // Staging.  Keys: 16-byte units, a row after the other.  Values: blocks of 4 keys (which lie side by side in V^T) and VC
+    // channels.  Where there are at most 128 blocks of values two wavefronts fetch them and the other two the keys.
+    constexpr int VC = BF16 && DP >= 96 ? 8 : 4, V_BLOCKS = 8 * (DP / VC), K_UNITS_ROW = DP * SIZE / 16, K_UNITS = TILE_KEYS * K_UNITS_ROW;
+    constexpr bool APART = V_BLOCKS <= 128;
+    constexpr int K_THREADS = APART ? 128 : 256, K_EACH = (K_UNITS + K_THREADS - 1) / K_THREADS;
+    static_assert(K_UNITS % K_THREADS == 0 && V_BLOCKS <= 256, "staging");
+    const bool stages_k = !APART || tid >= 128, stages_v = tid < V_BLOCKS;
+    const uint32_t k_tid = APART ? tid & 127u : tid;
+    const uint32_t v_block = tid & 7u, v_channel = VC * (tid >> 3);
+    // Keys 4 b .. 4 b + 3 of a tile are slots 16 (b / 4) + 8 (b % 2) + 4 (b / 2 % 2) on.
+    const uint32_t v_slot = 16 * (v_block >> 2) + 8 * (v_block & 1u) + 4 * ((v_block >> 1) & 1u);
+
+    u32x4 k_stage[K_EACH];
+    uint32_t v_stage[4][BF16 ? VC / 2 : VC];
+
+    int32_t pages = 0;
+    auto fetch_pages = [&](int32_t from) {
+        const int32_t i = from + (int32_t)lane;
+        pages = 0;
+        if (UNIFORM && i < tiles) pages = g.kv.page_of(s, g.kv.by_page_size.div((uint32_t)((first + i) * TILE_KEYS)), 0);
+    };
+    auto row_at = [&](uint32_t key) {  // elements from the start of the cache
+        const uint32_t index = g.kv.by_page_size.div(key);
+        return (int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
+    };
+    auto fetch = [&](int32_t i) {
+        const int32_t key0 = (first + i) * TILE_KEYS;
+        int64_t base = 0;
+        if (UNIFORM) {
+            const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
+            const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
+            base = (int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at;
+        }
+        auto at = [&](uint32_t key) { return UNIFORM ? base + (int64_t)key * g.kv.slot_stride : row_at((uint32_t)min(key0 + (int32_t)key, end - 1)); };
+        if (stages_k) {
+#pragma unroll
+            for (int e = 0; e < K_EACH; e++) {
+                const uint32_t unit = e * K_THREADS + k_tid, key = unit / K_UNITS_ROW, c = (16 / SIZE) * (unit % K_UNITS_ROW);
+                k_stage[e] = u32x4{0, 0, 0, 0};
+                if (c < g.d) k_stage[e] = *reinterpret_cast<const u32x4 *>(keys + (at(key) + c) * SIZE);
+            }
+        }
+        if (stages_v) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int32_t key = key0 + 4 * (int32_t)v_block + e;
+                constexpr int WORDS = BF16 ? VC / 2 : VC;
+#pragma unroll
+                for (int w = 0; w < WORDS; w++) v_stage[e][w] = 0;
+                // Slots that no row sees may hold anything: their weight is 0, so is their value then.
+                if (v_channel < g.d && key >= begin && key < end) {
+                    const char *p = values + (at(4 * v_block + e) + v_channel) * SIZE;
+                    if constexpr (WORDS == 4) {
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(p);
+                        v_stage[e][0] = x.x, v_stage[e][1] = x.y, v_stage[e][2] = x.z, v_stage[e][3] = x.w;
+                    } else {
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+                        v_stage[e][0] = x.x, v_stage[e][1] = x.y;
+                    }
+                }
+            }
+        }
+    };
+    auto park = [&](int buffer) {
+        if (stages_k) {
+#pragma unroll
+            for (int e = 0; e < K_EACH; e++) {
+                const uint32_t unit = e * K_THREADS + k_tid, key = unit / K_UNITS_ROW, c = (16 / SIZE) * (unit % K_UNITS_ROW);
+                uint16_t *to = &lds.k[buffer][0][key * K_PITCH + c];
+                if constexpr (BF16) {
+                    *reinterpret_cast<u32x4 *>(to) = k_stage[e];
+                } else {
+                    uint32_t p[3][2];
+#pragma unroll
+                    for (int w = 0; w < 2; w++) dev::split3_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
+#pragma unroll
+                    for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
+                }
+            }
+        }
+        if (stages_v) {
+#pragma unroll
+            for (int c = 0; c < VC; c++) {
+                uint16_t *to = &lds.v[buffer][0][(v_channel + c) * V_PITCH + v_slot];
+                if constexpr (BF16) {
+                    const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
+                    *reinterpret_cast<u32x2 *>(to) = u32x2{__builtin_amdgcn_perm(v_stage[1][c / 2], v_stage[0][c / 2], pick), __builtin_amdgcn_perm(v_stage[3][c / 2], v_stage[2][c / 2], pick)};
+                } else {
+                    uint32_t p[3][2];
+#pragma unroll
+                    for (int w = 0; w < 2; w++) dev::split3_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
+#pragma unroll
+                    for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
+                }
+            }
+        }
+    };
+
+    const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
+    u32x4 q[3][STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const uint32_t c = 16 * i + 8 * h;
+        f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+        if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c);
+        if (valid && c + 4 < g.d) hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4);
+        uint32_t w[3][4];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            dev::split3_pair(lo[2 * e], lo[2 * e + 1], w[0][e], w[1][e], w[2][e]);
+            dev::split3_pair(hi[2 * e], hi[2 * e + 1], w[0][2 + e], w[1][2 + e], w[2][2 + e]);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) q[p][i] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+    }
+
+    float top = -INFINITY, total = 0.0f;
+    f32x16 acc[PARTS];
+#pragma unroll
+    for (int i = 0; i < PARTS; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][r] = 0.0f;
+
+    auto key_of = [&](int r) { return 8 * (r >> 2) + 4 * (int32_t)h + (r & 3); };
+    // Smallest terms first.
+    auto multiply = [&](const u32x4 (&a)[PLANES], const u32x4 &b0, const u32x4 &b1, const u32x4 &b2, f32x16 &c) {
+        if constexpr (BF16) {
+            ALTIUS_MFMA32_BF16(a[0], b2, c);
+            ALTIUS_MFMA32_BF16(a[0], b1, c);
+            ALTIUS_MFMA32_BF16(a[0], b0, c);
+        } else {
+            ALTIUS_MFMA32_BF16(a[0], b2, c);
+            ALTIUS_MFMA32_BF16(a[2], b0, c);
+            ALTIUS_MFMA32_BF16(a[1], b1, c);
+            ALTIUS_MFMA32_BF16(a[0], b1, c);
+            ALTIUS_MFMA32_BF16(a[1], b0, c);
+            ALTIUS_MFMA32_BF16(a[0], b0, c);
+        }
+    };
+    auto attend = [&](int32_t i, int buffer) {
+        const int32_t key0 = (first + i) * TILE_KEYS;
+        if (key0 >= any_high || key0 + TILE_KEYS <= any_low) return;  // for this wavefront's rows
+        f32x16 st;
+#pragma unroll
+        for (int r = 0; r < 16; r++) st[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < STEPS; c++) {
+            u32x4 k[PLANES];
+#pragma unroll
+            for (int p = 0; p < PLANES; p++) k[p] = *reinterpret_cast<const u32x4 *>(&lds.k[buffer][p][col * K_PITCH + 16 * c + 8 * h]);
+            multiply(k, q[0][c], q[1][c], q[2][c], st);
+        }
+        float x[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[r] = st[r];
+        scores(g, x, slope, place - key0, key_of);
+        if (key0 < max(all_low, begin) || key0 + TILE_KEYS > min(all_high, end)) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int32_t key = key0 + key_of(r);
+                // A score that is not there is minus infinity: its weight is 0 once a finite maximum is known, and the row that has
+                // none yet takes 0 for it.
+                x[r] = key >= max(low, begin) && key < min(high, end) ? x[r] : -INFINITY;
+            }
+        }
+        float most = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) most = fmaxf(most, x[r]);
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const float now = fmaxf(top, most);
+        if (__any(now != top)) {
+            const float corr = weight_of(top, now);
+            total *= corr;
+#pragma unroll
+            for (int t = 0; t < PARTS; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[t][r] *= corr;
+            top = now;
+        }
+        const float base = now == -INFINITY ? 0.0f : now;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            x[r] = exp2_fast(x[r] - base);
+            total += x[r];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            u32x4 p[3];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t w[3];
+                split_weights(x[8 * u + 2 * e], x[8 * u + 2 * e + 1], w[0], w[1], w[2]);
+                p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
+            }
+#pragma unroll
+            for (int t = 0; t < PARTS; t++) {
+                u32x4 v[PLANES];
+#pragma unroll
+                for (int q = 0; q < PLANES; q++) v[q] = *reinterpret_cast<const u32x4 *>(&lds.v[buffer][q][(32 * t + col) * V_PITCH + 16 * u + 8 * h]);
+                multiply(v, p[0], p[1], p[2], acc[t]);
+            }
+        }
+    };
+
+    fetch_pages(0);
+    if (tiles > 0) fetch(0);
+    if (BUFFERS == 2 && tiles > 0) park(0);
+    for (int32_t i = 0; i < tiles; i++) {
+        const bool more = i + 1 < tiles;
+        if (BUFFERS == 1) {
+            __syncthreads();  // nobody reads the tile before any more
+            park(0);
+        }
+        __syncthreads();
+        if (more) {
+            if (((i + 1) & 63) == 0) fetch_pages(i + 1);
+            fetch(i + 1);
+        }
+        attend(i, BUFFERS == 2 ? i & 1 : 0);
+        if (BUFFERS == 2 && more) park((i + 1) & 1);
+    }
+    total += __shfl_xor(total, 32);
+
+    // As in rows16: what is not finite is computed once more, value by value.
+    float check = total * 0.0f;
+#pragma unroll
+    for (int t = 0; t < PARTS; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) check = __builtin_fmaf(acc[t][r], 0.0f, check);
+    if (__any(valid && check != 0.0f)) {
+        top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int t = 0; t < PARTS; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
+        for (int32_t key = max(begin, any_low); key < min(end, any_high); key++) {
+            const int64_t at = row_at((uint32_t)key);
+            float dot = 0.0f;
+            if (valid)
+                for (uint32_t c = h; c < g.d; c += 2) dot = __builtin_fmaf(q_row[c], cache_value<BF16>(keys, at + c), dot);
+            dot += __shfl_xor(dot, 32);
+            if (!sees || key < low || key >= high) continue;
+            float x[1] = {dot};
+            scores(g, x, slope, place - key, [](int) { return 0; });
+            const float now = fmaxf(top, x[0]);
+            const float corr = weight_of(top, now), p = exp2_fast(x[0] - (now == -INFINITY ? 0.0f : now));
+            top = now;
+            total = total * corr + p;
+#pragma unroll
+            for (int t = 0; t < PARTS; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const uint32_t c = 32 * t + (uint32_t)key_of(r);
+                    if (c < g.d) acc[t][r] = acc[t][r] * corr + p * cache_value<BF16>(values, at + c);
+                }
+        }
+    }
+
+    if (!valid) return;
+    const bool whole = share.splits == 1;
+    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits + split;
+    float *to = whole ? g.out + (int64_t)(seq.start + (int32_t)token) * g.out_token + (int64_t)head * g.out_head : share.part_out + at * g.d;
+    const float factor = !whole ? 1.0f : 1.0f / total;
+    if (!whole && h == 0) share.part_stats[2 * at] = top, share.part_stats[2 * at + 1] = total;
+#pragma unroll
+    for (int t = 0; t < PARTS; t++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const uint32_t c = 32 * t + 8 * b + 4 * h;
+            if (c >= g.d) continue;
+            f32x4 o = {acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]};
+            *reinterpret_cast<f32x4 *>(to + c) = !whole ? o : sees ? o * factor : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+}
+
+// Prompts, and the sequences of few rows that share a batch with them: the first blocks are the latter's.
+template <int DP, bool BF16, bool UNIFORM>
+__global__ __launch_bounds__(256, 2) void attend_rows128(AttendArgs g) {
+    __shared__ __align__(16) union {
+        RowLds<DP <= 64 ? 64 : 128> few;
+        TileLds<DP, BF16> many;
+    } lds;
+    if (blockIdx.x < g.few.blocks) rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true>(g, blockIdx.x, lds.few);
+    else rows128<DP, BF16, UNIFORM>(g, blockIdx.x - g.few.blocks, lds.many);
+}
+
 // Joins the splits of a row: a block per row, the splits dealt to its threads' groups of d / 4 lanes.
 constexpr int JOIN = 256;
-__global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g) {
+__global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_rows) {
     __shared__ float tops[JOIN / 64], totals[JOIN / 64];
     __shared__ __align__(16) f32x4 sums[JOIN];
-    uint32_t id = blockIdx.x;
-    const uint32_t row = id % g.rows_kept;
-    id /= g.rows_kept;
+    const bool few = blockIdx.x < few_rows;
+    const Share &share = few ? g.few : g.many;
+    uint32_t id = few ? blockIdx.x : blockIdx.x - few_rows;
+    const uint32_t row = id % share.rows;
+    id /= share.rows;
     const uint32_t kvh = id % g.kv.kv_heads, s = id / g.kv.kv_heads;
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
-    if (rows > FEW_ROWS || row >= rows) return;
+    if ((rows <= FEW_ROWS) != few || row >= rows) return;
     const uint32_t t = g.by_group.div(row), h = kvh * g.group + row - t * g.group;
-    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * g.rows_kept + row) * g.splits;
+    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits;
 
     float top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < g.splits; i += JOIN) top = fmaxf(top, g.part_stats[2 * (at + i)]);
+    for (uint32_t i = threadIdx.x; i < share.splits; i += JOIN) top = fmaxf(top, share.part_stats[2 * (at + i)]);
     top = dev::wave_reduce<dev::MaxOp>(top);
     if ((threadIdx.x & 63u) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < JOIN / 64; w++) top = fmaxf(top, tops[w]);
     float total = 0.0f;
-    for (uint32_t i = threadIdx.x; i < g.splits; i += JOIN) total = __builtin_fmaf(g.part_stats[2 * (at + i) + 1], weight_of(g.part_stats[2 * (at + i)], top), total);
+    for (uint32_t i = threadIdx.x; i < share.splits; i += JOIN)
+        total = __builtin_fmaf(share.part_stats[2 * (at + i) + 1], weight_of(share.part_stats[2 * (at + i)], top), total);
     total = dev::wave_reduce<dev::SumOp>(total);
     if ((threadIdx.x & 63u) == 0) totals[threadIdx.x >> 6] = total;
 
     const uint32_t lanes = g.d / 4, groups = JOIN / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     if (group < groups) {
-        for (uint32_t i = group; i < g.splits; i += groups) {
-            const float f = weight_of(g.part_stats[2 * (at + i)], top);
-            if (f != 0.0f) o += *reinterpret_cast<const f32x4 *>(g.part_out + (at + i) * g.d + 4 * lane) * f;
+        for (uint32_t i = group; i < share.splits; i += groups) {
+            const float f = weight_of(share.part_stats[2 * (at + i)], top);
+            if (f != 0.0f) o += *reinterpret_cast<const f32x4 *>(share.part_out + (at + i) * g.d + 4 * lane) * f;
         }
     }
     sums[threadIdx.x] = o;
@@ -512,8 +927,11 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g) {
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// The largest head that blocks of 128 rows are built for.
+constexpr int TILE_CHANNELS = 128;
+
 struct Plan {
-    uint32_t rows, rows_kept, splits, split_keys;
+    Share few, many;  // their pointers from the start of the workspace, as yet
     size_t bytes;
 };
 
@@ -523,18 +941,36 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const size_t held = std::min((size_t)batch.table_pages * (size_t)cache.page_size, (size_t)INT32_MAX);
     const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
     const size_t max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
-    p.rows = (uint32_t)std::min(max_tokens * group, (size_t)1 << 30);
-    p.rows_kept = std::min(p.rows, FEW_ROWS);
-    const uint32_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
-    // Blocks enough for every CU to have several in turn, since sequences are of different lengths; no split shorter than 256 KiB.
-    const uint64_t blocks = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads * ((p.rows_kept + 15) / 16);
+    const uint32_t rows = (uint32_t)std::min(max_tokens * group, (size_t)1 << 30);
+    const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256, pairs = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads;
     const uint64_t key_bytes = 2 * (uint64_t)cache.head_size * (cache.elem == AHIP_KV_BF16 ? 2 : 4);
-    const uint64_t least = std::max<uint64_t>(64, (256 * 1024 / key_bytes + 63) / 64 * 64);
-    const uint64_t wanted = std::max<uint64_t>(1, 8 * cus / std::max<uint64_t>(1, blocks));
-    const uint64_t each = std::max<uint64_t>(least, ((max_keys + wanted - 1) / wanted + 63) / 64 * 64);
-    p.split_keys = (uint32_t)std::min<uint64_t>(each, (uint64_t)1 << 31);
-    p.splits = (uint32_t)std::max<uint64_t>(1, (max_keys + p.split_keys - 1) / p.split_keys);
-    if (p.splits > 1) p.bytes = (size_t)batch.sequences * (size_t)cache.kv_heads * p.rows_kept * p.splits * ((size_t)cache.head_size + 2) * sizeof(float);
+    auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, uint64_t wanted_blocks, uint64_t least) {
+        s.rows = most_rows;
+        s.row_tiles = (most_rows + tile - 1) / tile;
+        const uint64_t blocks = std::max<uint64_t>(1, pairs * s.row_tiles), splits = std::max<uint64_t>(1, wanted_blocks / blocks);
+        const uint64_t each = std::max<uint64_t>(least, ((max_keys + splits - 1) / splits + 63) / 64 * 64);
+        s.split_keys = (uint32_t)std::min<uint64_t>(each, (uint64_t)1 << 31);
+        s.splits = (uint32_t)std::max<uint64_t>(1, (max_keys + s.split_keys - 1) / s.split_keys);
+        s.blocks = (uint32_t)std::min<uint64_t>(blocks * s.splits, UINT32_MAX);
+        if (s.splits > 1) {
+            const size_t parts = pairs * s.rows * s.splits;
+            s.part_stats = reinterpret_cast<float *>(p.bytes);
+            p.bytes += (2 * parts * sizeof(float) + 15) / 16 * 16;
+            s.part_out = reinterpret_cast<float *>(p.bytes);
+            p.bytes += parts * (size_t)cache.head_size * sizeof(float);
+        }
+    };
+    // Few rows: blocks enough for every CU to have several in turn, since sequences are of different lengths; no split shorter than
+    // 256 KiB of keys and values.
+    share(p.few, std::min(rows, FEW_ROWS), 16, 8 * cus, std::max<uint64_t>(64, (256 * 1024 / key_bytes + 63) / 64 * 64));
+    if (rows > FEW_ROWS) {
+        if (cache.head_size <= TILE_CHANNELS) {
+            // Two blocks of 128 rows are at work on a CU.
+            share(p.many, rows, TILE_ROWS, 4 * cus, 512);
+        } else {
+            share(p.many, rows, 16, 1, 1);
+        }
+    }
     return p;
 }
 
@@ -559,32 +995,26 @@ int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
     return AHIP_OK;
 }
 
-template <int DP, bool BF16, bool UNIFORM> int launch_rows(DeviceCtx &ctx, AttendArgs g, const Plan &plan) {
-    const uint64_t most = ((uint64_t)1 << 24) - 1;  // a grid ends at 2^32 threads
-    g.splits = plan.splits, g.split_keys = plan.split_keys, g.rows_kept = plan.rows_kept;
-    g.row_tiles = (plan.rows_kept + 15) / 16;
-    const uint64_t few = (uint64_t)g.kv.sequences * g.kv.kv_heads * g.row_tiles * g.splits, rows = (uint64_t)g.kv.sequences * g.kv.kv_heads * g.rows_kept;
-    const uint64_t many_tiles = (plan.rows + 15) / 16, many = (uint64_t)g.kv.sequences * g.kv.kv_heads * many_tiles;
-    if (few > most || rows > most || (plan.rows > FEW_ROWS && many > most)) return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
-    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, true>), dim3((uint32_t)few), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+template <int DP, bool BF16, bool UNIFORM> int launch_wide(DeviceCtx &ctx, const AttendArgs &g) {
+    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, true>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
     if (int rc = ctx.check(hipGetLastError(), "kv attention launch")) return rc;
-    if (g.splits > 1) {
-        hipLaunchKernelGGL(join_splits, dim3((uint32_t)rows), dim3(JOIN), 0, ctx.stream, g);
-        if (int rc = ctx.check(hipGetLastError(), "kv attention launch")) return rc;
-    }
-    if (plan.rows > FEW_ROWS) {
-        g.row_tiles = (uint32_t)many_tiles;
-        g.splits = 1;
-        hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, false>), dim3((uint32_t)many), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
-        return ctx.check(hipGetLastError(), "kv attention launch");
-    }
-    return AHIP_OK;
+    if (!g.many.blocks) return AHIP_OK;
+    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, false>), dim3(g.many.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+    return ctx.check(hipGetLastError(), "kv attention launch");
+}
+template <int DP, bool BF16, bool UNIFORM> int launch_tiled(DeviceCtx &ctx, const AttendArgs &g) {
+    if (!g.many.blocks)
+        hipLaunchKernelGGL((attend_rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+    else
+        hipLaunchKernelGGL((attend_rows128<DP, BF16, UNIFORM>), dim3(g.few.blocks + g.many.blocks), dim3(256), 0, ctx.stream, g);
+    return ctx.check(hipGetLastError(), "kv attention launch");
 }
 
-template <bool BF16, bool UNIFORM> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g, const Plan &plan) {
-    if (g.d <= 64) return launch_rows<64, BF16, UNIFORM>(ctx, g, plan);
-    if (g.d <= 128) return launch_rows<128, BF16, UNIFORM>(ctx, g, plan);
-    return launch_rows<256, BF16, UNIFORM>(ctx, g, plan);
+template <bool BF16, bool UNIFORM> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g) {
+    if (g.d <= 64) return launch_tiled<64, BF16, UNIFORM>(ctx, g);
+    if (g.d <= 96) return launch_tiled<96, BF16, UNIFORM>(ctx, g);
+    if (g.d <= TILE_CHANNELS) return launch_tiled<128, BF16, UNIFORM>(ctx, g);
+    return launch_wide<256, BF16, UNIFORM>(ctx, g);
 }
 
 }  // namespace
@@ -614,18 +1044,27 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
     g.out_token = (int64_t)attend.out_strides[0], g.out_head = (int64_t)attend.out_strides[1];
     g.q_heads = (uint32_t)attend.q_heads, g.group = (uint32_t)(attend.q_heads / cache.kv_heads), g.d = (uint32_t)cache.head_size;
     g.by_group = dev::make_fastdiv(g.group);
-    g.cap = attend.softcap;
-    g.scale = g.cap != 0.0f ? attend.scale : attend.scale * LOG2E;
+    g.cap = attend.softcap * LOG2E;
+    g.scale = attend.softcap != 0.0f ? attend.scale / attend.softcap : attend.scale * LOG2E;
     g.causal = attend.causal, g.window = attend.window, g.slopes = attend.slopes, g.prefix = attend.prefix, g.first_keys = attend.first_keys;
     g.max_tokens = (uint32_t)(attend.max_tokens ? std::min(attend.max_tokens, attend.tokens) : attend.tokens);
     g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
-    g.part_stats = static_cast<float *>(attend.workspace);
-    const size_t parts = (size_t)g.kv.sequences * g.kv.kv_heads * plan.rows_kept * plan.splits;
-    g.part_out = g.part_stats ? g.part_stats + 2 * parts : nullptr;
+    g.few = plan.few, g.many = plan.many;
+    for (Share *s : {&g.few, &g.many})
+        if (s->splits > 1) {
+            s->part_stats = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_stats));
+            s->part_out = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_out));
+        }
+    const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, few_rows = g.few.splits > 1 ? pairs * g.few.rows : 0, many_rows = g.many.splits > 1 ? pairs * g.many.rows : 0;
+    if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_rows + many_rows >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
+        return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
     // Pages that hold whole tiles: a tile's page is looked up once, not key by key.
-    const bool bf16 = cache.elem == AHIP_KV_BF16;
-    if (cache.page_size % (bf16 ? KEYS<true> : KEYS<false>) == 0) return bf16 ? launch_by_size<true, true>(ctx, g, plan) : launch_by_size<false, true>(ctx, g, plan);
-    return bf16 ? launch_by_size<true, false>(ctx, g, plan) : launch_by_size<false, false>(ctx, g, plan);
+    const bool bf16 = cache.elem == AHIP_KV_BF16, uniform = cache.page_size % TILE_KEYS == 0 || (!bf16 && !g.many.blocks && cache.page_size % KEYS<false> == 0);
+    int rc = bf16 ? (uniform ? launch_by_size<true, true>(ctx, g) : launch_by_size<true, false>(ctx, g))
+                  : (uniform ? launch_by_size<false, true>(ctx, g) : launch_by_size<false, false>(ctx, g));
+    if (rc || few_rows + many_rows == 0) return rc;
+    hipLaunchKernelGGL(join_splits, dim3((uint32_t)(few_rows + many_rows)), dim3(JOIN), 0, ctx.stream, g, (uint32_t)few_rows);
+    return ctx.check(hipGetLastError(), "kv attention launch");
 }
 
 }  // namespace altius
