@@ -10,10 +10,10 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv.h"
 #include "math.h"
-#include "split3.h"
 
 namespace altius {
 
@@ -101,13 +101,29 @@ __device__ __forceinline__ float fast_tanh(float v) {
     return p * v * r;
 }
 
-// Products of a query and keys become scores in units of log2(e): scaled, capped, biased.  first_key + place(r) is the key of x[r].
+// Products of a (scaled) query and keys become scores in units of log2(e): capped, biased.  Key place(r) of the tile, which starts
+// `distance` in front of the row's place, is that of x[r].
 template <int N, class Place> __device__ __forceinline__ void scores(const AttendArgs &g, float (&x)[N], float slope, int32_t distance, Place place) {
-#pragma unroll
-    for (int r = 0; r < N; r++) x[r] *= g.scale;
     if (g.cap != 0.0f) {
+        // Up to 3/4 of the cap, where nearly all scores are, tanh(x) / x is a polynomial of degree 5 in x^2, off by 2.9e-8 of
+        // itself at most (a fit of the least largest error): 8 operations a score instead of 20.
+        float most = fabsf(x[0]);
 #pragma unroll
-        for (int r = 0; r < N; r++) x[r] = g.cap * fast_tanh(x[r]);
+        for (int r = 1; r < N; r++) most = fmaxf(most, fabsf(x[r]));
+        if (__any(most > 0.75f)) {
+#pragma unroll
+            for (int r = 0; r < N; r++) x[r] = g.cap * fast_tanh(x[r]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < N; r++) {
+                const float z = x[r] * x[r], c = g.cap * x[r];
+                float p = __builtin_fmaf(z, -0.004716264083981514f, 0.01958294026553631f);
+                p = __builtin_fmaf(p, z, -0.05334445834159851f);
+                p = __builtin_fmaf(p, z, 0.1332540661096573f);
+                p = __builtin_fmaf(p, z, -0.33332958817481995f);
+                x[r] = __builtin_fmaf(c * z, p, c);
+            }
+        }
     }
     if (g.slopes) {
 #pragma unroll
@@ -115,8 +131,9 @@ template <int N, class Place> __device__ __forceinline__ void scores(const Atten
     }
 }
 
-// A weight and its neighbour as three pairs of bf16 whose sums they are (weights are in [0, 1], or NaN).
-__device__ __forceinline__ void split_weights(float e0, float e1, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+// Two values as three pairs of bf16 whose sums they are (split3.h, without its care for infinities and what rounds up to one: those
+// become NaN, and rows that see them are computed once more).
+__device__ __forceinline__ void split_pair(float e0, float e1, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
     p0 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){e0, e1}, bf16x2));
     const float r0 = e0 - __uint_as_float(p0 << 16), r1 = e1 - __uint_as_float(p0 & 0xffff0000u);
     p1 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){r0, r1}, bf16x2));
@@ -136,7 +153,7 @@ template <bool BF16> __device__ __forceinline__ float cache_value(const void *ba
 // values by 16 lanes side by side, each lane's channels being rows of O^T.
 //   fp32 cache: v_mfma_f32_16x16x4_f32, tiles of 16 keys.
 //   bf16 cache: v_mfma_f32_16x16x32_bf16, tiles of 32 keys; q and the weights as three bf16 numbers each, whose sum they are
-//   exactly (split3.h), so that each of the three products is exact in the fp32 sum; a lane holds 8 keys x DP / 16 channels of
+//   exactly, so that each of the three products is exact in the fp32 sum; a lane holds 8 keys x DP / 16 channels of
 //   V and turns them with v_perm.
 template <bool BF16> constexpr int KEYS = BF16 ? 32 : 16;
 constexpr int ROW_WAVES = 4;
@@ -222,12 +239,12 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         for (int i = 0; i < DP / 32; i++) {
             const uint32_t c = 32 * i + 8 * part;
             f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
-            if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c), hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4);
+            if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale, hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4) * g.scale;
             uint32_t h[3][4];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                dev::split3_pair(lo[2 * e], lo[2 * e + 1], h[0][e], h[1][e], h[2][e]);
-                dev::split3_pair(hi[2 * e], hi[2 * e + 1], h[0][2 + e], h[1][2 + e], h[2][2 + e]);
+                split_pair(lo[2 * e], lo[2 * e + 1], h[0][e], h[1][e], h[2][e]);
+                split_pair(hi[2 * e], hi[2 * e + 1], h[0][2 + e], h[1][2 + e], h[2][2 + e]);
             }
 #pragma unroll
             for (int p = 0; p < 3; p++) q.q[p][i] = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
@@ -237,7 +254,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         for (int i = 0; i < DP / 16; i++) {
             const uint32_t c = 16 * i + 4 * part;
             q.q[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (valid && c < g.d) q.q[i] = *reinterpret_cast<const f32x4 *>(q_row + c);
+            if (valid && c < g.d) q.q[i] = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
         }
     }
 
@@ -258,45 +275,35 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     auto value_key = [&](int i) { return BF16 ? 16 * (i / 4) + 4 * part + i % 4 : 4 * part + i; };
     constexpr int VROWS = BF16 ? 8 : 4;
 
-    auto load = [&](int32_t i, RowTile<DP, BF16> &t) {
-        const int32_t key0 = tile_key(i);
-        int64_t k_at[2], v_at[VROWS];
-        if (UNIFORM) {
-            const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
-            const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
-            const int64_t base = (int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at;
-            for (int h = 0; h < (BF16 ? 2 : 1); h++) k_at[h] = base + (int64_t)(col + 16 * h) * g.kv.slot_stride;
-            for (int r = 0; r < VROWS; r++) v_at[r] = base + (int64_t)value_key(r) * g.kv.slot_stride;
-        } else {
-            // Keys behind the last that is seen have no page to be read from: the last one stands in for them.
-            for (int h = 0; h < (BF16 ? 2 : 1); h++) k_at[h] = row_at((uint32_t)min(key0 + (int32_t)col + 16 * h, end - 1));
-            for (int r = 0; r < VROWS; r++) v_at[r] = row_at((uint32_t)min(key0 + (int32_t)value_key(r), end - 1));
-        }
+    // Where pages hold whole tiles a tile starts at one address for the whole wavefront, and a lane's parts lie at fixed distances from
+    // it (below 2^31 bytes, or the call takes the other kernel).
+    const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
+    const uint32_t k_off = col * slot_bytes + 16 * part, v_off = 4 * part * slot_bytes + (BF16 ? (DP / 16) * SIZE : 16) * col;
+    auto load_parts = [&](RowTile<DP, BF16> &t, auto whole, auto k_part, auto v_part) {
+        // k_part(h, c): channels from 64 bytes x c on, of the lane's key in half h; v_part(r, j): 256 bytes x j (fp32), 16 x j (bf16) on.
+        constexpr bool WHOLE = decltype(whole)::value;
         if constexpr (BF16) {
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int c = 0; c < DP / 32; c++) {
                     t.k[h][c] = u32x4{0, 0, 0, 0};
-                    if (32 * c + 8 * part < g.d) t.k[h][c] = *reinterpret_cast<const u32x4 *>(keys + (k_at[h] + 32 * c + 8 * part) * SIZE);
+                    if (WHOLE || 32 * c + 8 * part < g.d) t.k[h][c] = *reinterpret_cast<const u32x4 *>(k_part(h) + 64 * c);
                 }
 #pragma unroll
             for (int r = 0; r < VROWS; r++) {
-                const char *p = values + (v_at[r] + (DP / 16) * col) * SIZE;
-#pragma unroll
-                for (int w = 0; w < DP / 32; w++) t.v[r][w] = 0;
                 if (DP == 64) {
-                    if (4 * col < g.d) {
-                        const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+                    t.v[r][0] = t.v[r][1] = 0;
+                    if (WHOLE || 4 * col < g.d) {
+                        const u32x2 x = *reinterpret_cast<const u32x2 *>(v_part(r));
                         t.v[r][0] = x.x, t.v[r][1] = x.y;
                     }
                 } else {
 #pragma unroll
                     for (int w = 0; w < DP / 128; w++) {
-                        if ((DP / 16) * col + 8 * w < g.d) {
-                            const u32x4 x = *reinterpret_cast<const u32x4 *>(p + 16 * w);
-                            t.v[r][4 * w] = x.x, t.v[r][4 * w + 1] = x.y, t.v[r][4 * w + 2] = x.z, t.v[r][4 * w + 3] = x.w;
-                        }
+                        u32x4 x = {0, 0, 0, 0};
+                        if (WHOLE || (DP / 16) * col + 8 * w < g.d) x = *reinterpret_cast<const u32x4 *>(v_part(r) + 16 * w);
+                        t.v[r][4 * w] = x.x, t.v[r][4 * w + 1] = x.y, t.v[r][4 * w + 2] = x.z, t.v[r][4 * w + 3] = x.w;
                     }
                 }
             }
@@ -304,28 +311,51 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
 #pragma unroll
             for (int c = 0; c < DP / 16; c++) {
                 t.k[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (16 * c + 4 * part < g.d) t.k[c] = *reinterpret_cast<const f32x4 *>(keys + (k_at[0] + 16 * c + 4 * part) * SIZE);
+                if (WHOLE || 16 * c + 4 * part < g.d) t.k[c] = *reinterpret_cast<const f32x4 *>(k_part(0) + 64 * c);
             }
 #pragma unroll
             for (int r = 0; r < VROWS; r++)
 #pragma unroll
                 for (int j = 0; j < DP / 64; j++) {
                     t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (64 * j + 4 * col < g.d) t.v[r][j] = *reinterpret_cast<const f32x4 *>(values + (v_at[r] + 64 * j + 4 * col) * SIZE);
+                    if (WHOLE || 64 * j + 4 * col < g.d) t.v[r][j] = *reinterpret_cast<const f32x4 *>(v_part(r) + 256 * j);
                 }
         }
-        if (key0 < begin || key0 + KT > end) {  // slots that no row sees may hold anything: their weight is 0, so is their value then
+    };
+    auto load = [&](int32_t i, RowTile<DP, BF16> &t) {
+        const int32_t key0 = tile_key(i);
+        if constexpr (UNIFORM) {
+            const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
+            const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
+            const int64_t base = ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
+            const char *kb = keys + base, *vb = values + base;
+            auto k_part = [&](int h) { return kb + (uint64_t)(16 * h) * slot_bytes + k_off; };
+            auto v_part = [&](int r) { return vb + (uint64_t)(BF16 ? 16 * (r / 4) + r % 4 : r) * slot_bytes + v_off; };
+            if (g.d == DP) load_parts(t, std::true_type(), k_part, v_part);
+            else load_parts(t, std::false_type(), k_part, v_part);
+        } else {
+            // Keys behind the last that is seen have no page to be read from: the last one stands in for them.
+            const char *k_at[2], *v_at[VROWS];
 #pragma unroll
-            for (int r = 0; r < VROWS; r++) {
-                const int32_t key = key0 + (int32_t)value_key(r);
-                if (key < begin || key >= end) {
-                    if constexpr (BF16) {
+            for (int h = 0; h < (BF16 ? 2 : 1); h++) k_at[h] = keys + row_at((uint32_t)min(key0 + (int32_t)col + 16 * h, end - 1)) * SIZE + 16 * part;
 #pragma unroll
-                        for (int w = 0; w < DP / 32; w++) t.v[r][w] = 0;
-                    } else {
+            for (int r = 0; r < VROWS; r++) v_at[r] = values + row_at((uint32_t)min(key0 + (int32_t)value_key(r), end - 1)) * SIZE + (BF16 ? (DP / 16) * SIZE : 16) * col;
+            load_parts(t, std::false_type(), [&](int h) { return k_at[h]; }, [&](int r) { return v_at[r]; });
+        }
+    };
+    // Slots that no row sees may hold anything: their weight is 0, so is their value then.
+    auto clear_unseen = [&](int32_t key0, RowTile<DP, BF16> &t) {
+        if (key0 >= begin && key0 + KT <= end) return;
 #pragma unroll
-                        for (int j = 0; j < DP / 64; j++) t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    }
+        for (int r = 0; r < VROWS; r++) {
+            const int32_t key = key0 + (int32_t)value_key(r);
+            if (key < begin || key >= end) {
+                if constexpr (BF16) {
+#pragma unroll
+                    for (int w = 0; w < DP / 32; w++) t.v[r][w] = 0;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < DP / 64; j++) t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
             }
         }
@@ -367,7 +397,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         }
     };
 
-    auto products = [&](int32_t i, const RowTile<DP, BF16> &t) {
+    auto products = [&](int32_t i, RowTile<DP, BF16> &t) {
         const int32_t key0 = tile_key(i);
         float x[NS];
         if constexpr (BF16) {
@@ -384,11 +414,12 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
                 for (int r = 0; r < 4; r++) x[4 * h + r] = large[r] + small[r];
             }
             weigh(key0, x);
+            clear_unseen(key0, t);
             u32x4 p[3];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 uint32_t w[3];
-                split_weights(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
+                split_pair(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
                 p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
             }
 #pragma unroll
@@ -412,6 +443,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
 #pragma unroll
             for (int r = 0; r < 4; r++) x[r] = even[r] + odd[r];
             weigh(key0, x);
+            clear_unseen(key0, t);
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -421,16 +453,21 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         }
     };
 
+    // Two tiles take turns: one is on its way during the other's products.
     fetch_pages(0);
-    RowTile<DP, BF16> now, next;
-    if (mine > 0) load(0, now);
-    for (int32_t i = 0; i < mine; i++) {
-        if (i + 1 < mine) {
-            if (((i + 1) & 63) == 0) fetch_pages(i + 1);
-            load(i + 1, next);  // on its way during the products
-        }
-        products(i, now);
-        now = next;
+    RowTile<DP, BF16> a, b;
+    auto load_next = [&](int32_t i, RowTile<DP, BF16> &t) {
+        if (i >= mine) return;
+        if ((i & 63) == 0) fetch_pages(i);
+        load(i, t);
+    };
+    if (mine > 0) load(0, a);
+    for (int32_t i = 0; i < mine; i += 2) {
+        load_next(i + 1, b);
+        products(i, a);
+        if (i + 1 >= mine) break;
+        load_next(i + 2, a);
+        products(i + 1, b);
     }
     total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
@@ -453,7 +490,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
                 const int64_t at = row_at((uint32_t)key);
                 float dot = 0.0f;
                 if (valid)
-                    for (uint32_t c = part; c < g.d; c += 4) dot = __builtin_fmaf(q_row[c], cache_value<BF16>(keys, at + c), dot);
+                    for (uint32_t c = part; c < g.d; c += 4) dot = __builtin_fmaf(q_row[c] * g.scale, cache_value<BF16>(keys, at + c), dot);
                 dot += __shfl_xor(dot, 16);
                 dot += __shfl_xor(dot, 32);
                 if (!sees || key < low || key >= high) continue;
@@ -614,21 +651,31 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         const uint32_t index = g.kv.by_page_size.div(key);
         return (int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
     };
+    const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
+    uint32_t k_off[K_EACH], k_channel[K_EACH], k_key[K_EACH];
+#pragma unroll
+    for (int e = 0; e < K_EACH; e++) {
+        const uint32_t unit = e * K_THREADS + k_tid;
+        k_key[e] = unit / K_UNITS_ROW, k_channel[e] = (16 / SIZE) * (unit % K_UNITS_ROW);
+        k_off[e] = k_key[e] * slot_bytes + 16 * (unit % K_UNITS_ROW);
+    }
+    const uint32_t v_off = 4 * v_block * slot_bytes + SIZE * v_channel;
     auto fetch = [&](int32_t i) {
         const int32_t key0 = (first + i) * TILE_KEYS;
-        int64_t base = 0;
+        const char *kb = keys, *vb = values;
         if (UNIFORM) {
             const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
             const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
-            base = (int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at;
+            const int64_t base = ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
+            kb += base, vb += base;
         }
-        auto at = [&](uint32_t key) { return UNIFORM ? base + (int64_t)key * g.kv.slot_stride : row_at((uint32_t)min(key0 + (int32_t)key, end - 1)); };
+        auto stand_in = [&](int32_t key) { return row_at((uint32_t)min(key, end - 1)) * SIZE; };  // for keys behind the last that is seen
         if (stages_k) {
 #pragma unroll
             for (int e = 0; e < K_EACH; e++) {
-                const uint32_t unit = e * K_THREADS + k_tid, key = unit / K_UNITS_ROW, c = (16 / SIZE) * (unit % K_UNITS_ROW);
                 k_stage[e] = u32x4{0, 0, 0, 0};
-                if (c < g.d) k_stage[e] = *reinterpret_cast<const u32x4 *>(keys + (at(key) + c) * SIZE);
+                if (k_channel[e] < g.d)
+                    k_stage[e] = *reinterpret_cast<const u32x4 *>(UNIFORM ? kb + k_off[e] : keys + stand_in(key0 + (int32_t)k_key[e]) + SIZE * k_channel[e]);
             }
         }
         if (stages_v) {
@@ -640,7 +687,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
                 for (int w = 0; w < WORDS; w++) v_stage[e][w] = 0;
                 // Slots that no row sees may hold anything: their weight is 0, so is their value then.
                 if (v_channel < g.d && key >= begin && key < end) {
-                    const char *p = values + (at(4 * v_block + e) + v_channel) * SIZE;
+                    const char *p = UNIFORM ? vb + (uint64_t)e * slot_bytes + v_off : values + stand_in(key) + SIZE * v_channel;
                     if constexpr (WORDS == 4) {
                         const u32x4 x = *reinterpret_cast<const u32x4 *>(p);
                         v_stage[e][0] = x.x, v_stage[e][1] = x.y, v_stage[e][2] = x.z, v_stage[e][3] = x.w;
@@ -656,14 +703,13 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         if (stages_k) {
 #pragma unroll
             for (int e = 0; e < K_EACH; e++) {
-                const uint32_t unit = e * K_THREADS + k_tid, key = unit / K_UNITS_ROW, c = (16 / SIZE) * (unit % K_UNITS_ROW);
-                uint16_t *to = &lds.k[buffer][0][key * K_PITCH + c];
+                uint16_t *to = &lds.k[buffer][0][k_key[e] * K_PITCH + k_channel[e]];
                 if constexpr (BF16) {
                     *reinterpret_cast<u32x4 *>(to) = k_stage[e];
                 } else {
                     uint32_t p[3][2];
 #pragma unroll
-                    for (int w = 0; w < 2; w++) dev::split3_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
+                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
                     for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
                 }
@@ -679,7 +725,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
                 } else {
                     uint32_t p[3][2];
 #pragma unroll
-                    for (int w = 0; w < 2; w++) dev::split3_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
+                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
                     for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
                 }
@@ -693,13 +739,13 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     for (int i = 0; i < STEPS; i++) {
         const uint32_t c = 16 * i + 8 * h;
         f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
-        if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c);
-        if (valid && c + 4 < g.d) hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4);
+        if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
+        if (valid && c + 4 < g.d) hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4) * g.scale;
         uint32_t w[3][4];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            dev::split3_pair(lo[2 * e], lo[2 * e + 1], w[0][e], w[1][e], w[2][e]);
-            dev::split3_pair(hi[2 * e], hi[2 * e + 1], w[0][2 + e], w[1][2 + e], w[2][2 + e]);
+            split_pair(lo[2 * e], lo[2 * e + 1], w[0][e], w[1][e], w[2][e]);
+            split_pair(hi[2 * e], hi[2 * e + 1], w[0][2 + e], w[1][2 + e], w[2][2 + e]);
         }
 #pragma unroll
         for (int p = 0; p < 3; p++) q[p][i] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
@@ -780,7 +826,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 uint32_t w[3];
-                split_weights(x[8 * u + 2 * e], x[8 * u + 2 * e + 1], w[0], w[1], w[2]);
+                split_pair(x[8 * u + 2 * e], x[8 * u + 2 * e + 1], w[0], w[1], w[2]);
                 p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
             }
 #pragma unroll
@@ -828,7 +874,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             const int64_t at = row_at((uint32_t)key);
             float dot = 0.0f;
             if (valid)
-                for (uint32_t c = h; c < g.d; c += 2) dot = __builtin_fmaf(q_row[c], cache_value<BF16>(keys, at + c), dot);
+                for (uint32_t c = h; c < g.d; c += 2) dot = __builtin_fmaf(q_row[c] * g.scale, cache_value<BF16>(keys, at + c), dot);
             dot += __shfl_xor(dot, 32);
             if (!sees || key < low || key >= high) continue;
             float x[1] = {dot};
@@ -875,43 +921,62 @@ __global__ __launch_bounds__(256, 2) void attend_rows128(AttendArgs g) {
     else rows128<DP, BF16, UNIFORM>(g, blockIdx.x - g.few.blocks, lds.many);
 }
 
-// Joins the splits of a row: a block per row, the splits dealt to its threads' groups of d / 4 lanes.
-constexpr int JOIN = 256;
-__global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_rows) {
-    __shared__ float tops[JOIN / 64], totals[JOIN / 64];
+// Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
+// channels, four a lane.  few: a block per row, whose groups of lanes deal the splits out among themselves; else a group per row.
+constexpr int JOIN = 256, MOST_SPLITS = 512;
+__global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_blocks) {
+    __shared__ float factors[MOST_SPLITS];
     __shared__ __align__(16) f32x4 sums[JOIN];
-    const bool few = blockIdx.x < few_rows;
+    __shared__ float totals[JOIN / 64];
+    const bool few = blockIdx.x < few_blocks;
     const Share &share = few ? g.few : g.many;
-    uint32_t id = few ? blockIdx.x : blockIdx.x - few_rows;
+    const uint32_t lanes = g.d / 4, groups = JOIN / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    uint32_t id = few ? blockIdx.x : (blockIdx.x - few_blocks) * groups + group;
     const uint32_t row = id % share.rows;
     id /= share.rows;
     const uint32_t kvh = id % g.kv.kv_heads, s = id / g.kv.kv_heads;
+    if (s >= g.kv.sequences || (!few && group >= groups)) return;
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
     if ((rows <= FEW_ROWS) != few || row >= rows) return;
     const uint32_t t = g.by_group.div(row), h = kvh * g.group + row - t * g.group;
-    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits;
+    const RowRange of = row_range(g, seq, s, t);
+    float *to = g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + 4 * lane;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (of.low >= of.high) {
+        if (!few || group == 0) *reinterpret_cast<f32x4 *>(to) = zero;
+        return;
+    }
+    const uint32_t from = (uint32_t)of.low / share.split_keys, count = (uint32_t)(of.high - 1) / share.split_keys + 1 - from;
+    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits + from;
+    const float *stats = share.part_stats + 2 * at;
+    const f32x4 *parts = reinterpret_cast<const f32x4 *>(share.part_out + at * g.d) + lane;
 
-    float top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < share.splits; i += JOIN) top = fmaxf(top, share.part_stats[2 * (at + i)]);
+    float top = -INFINITY, total = 0.0f;
+    f32x4 o = zero;
+    if (!few) {
+        for (uint32_t i = 0; i < count; i++) top = fmaxf(top, stats[2 * i]);
+        for (uint32_t i = 0; i < count; i++) {
+            const float f = weight_of(stats[2 * i], top);
+            total = __builtin_fmaf(stats[2 * i + 1], f, total);
+            o += parts[i * lanes] * f;
+        }
+        *reinterpret_cast<f32x4 *>(to) = o * (1.0f / total);
+        return;
+    }
+    // Every wavefront finds the maximum by itself; the weights of the splits wait in LDS.
+    for (uint32_t i = threadIdx.x & 63u; i < count; i += 64) top = fmaxf(top, stats[2 * i]);
     top = dev::wave_reduce<dev::MaxOp>(top);
-    if ((threadIdx.x & 63u) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < JOIN / 64; w++) top = fmaxf(top, tops[w]);
-    float total = 0.0f;
-    for (uint32_t i = threadIdx.x; i < share.splits; i += JOIN)
-        total = __builtin_fmaf(share.part_stats[2 * (at + i) + 1], weight_of(share.part_stats[2 * (at + i)], top), total);
+    for (uint32_t i = threadIdx.x; i < count; i += JOIN) {
+        factors[i] = weight_of(stats[2 * i], top);
+        total = __builtin_fmaf(stats[2 * i + 1], factors[i], total);
+    }
     total = dev::wave_reduce<dev::SumOp>(total);
     if ((threadIdx.x & 63u) == 0) totals[threadIdx.x >> 6] = total;
-
-    const uint32_t lanes = g.d / 4, groups = JOIN / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    __syncthreads();
     if (group < groups) {
-        for (uint32_t i = group; i < share.splits; i += groups) {
-            const float f = weight_of(share.part_stats[2 * (at + i)], top);
-            if (f != 0.0f) o += *reinterpret_cast<const f32x4 *>(share.part_out + (at + i) * g.d + 4 * lane) * f;
-        }
+#pragma unroll 4
+        for (uint32_t i = group; i < count; i += groups) o += parts[(size_t)i * lanes] * factors[i];
     }
     sums[threadIdx.x] = o;
     __syncthreads();
@@ -920,9 +985,7 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_r
 #pragma unroll
     for (int w = 0; w < JOIN / 64; w++) total += totals[w];
     for (uint32_t i = 1; i < groups; i++) o += sums[i * lanes + lane];
-    const RowRange of = row_range(g, seq, s, t);
-    *reinterpret_cast<f32x4 *>(g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + 4 * lane) =
-        of.low < of.high ? o * (1.0f / total) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    *reinterpret_cast<f32x4 *>(to) = o * (1.0f / total);
 }
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -945,10 +1008,11 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256, pairs = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads;
     const uint64_t key_bytes = 2 * (uint64_t)cache.head_size * (cache.elem == AHIP_KV_BF16 ? 2 : 4);
     auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, uint64_t wanted_blocks, uint64_t least) {
+        least = std::max<uint64_t>(least, (max_keys + MOST_SPLITS - 1) / MOST_SPLITS);
         s.rows = most_rows;
         s.row_tiles = (most_rows + tile - 1) / tile;
         const uint64_t blocks = std::max<uint64_t>(1, pairs * s.row_tiles), splits = std::max<uint64_t>(1, wanted_blocks / blocks);
-        const uint64_t each = std::max<uint64_t>(least, ((max_keys + splits - 1) / splits + 63) / 64 * 64);
+        const uint64_t each = (std::max<uint64_t>(least, (max_keys + splits - 1) / splits) + 63) / 64 * 64;
         s.split_keys = (uint32_t)std::min<uint64_t>(each, (uint64_t)1 << 31);
         s.splits = (uint32_t)std::max<uint64_t>(1, (max_keys + s.split_keys - 1) / s.split_keys);
         s.blocks = (uint32_t)std::min<uint64_t>(blocks * s.splits, UINT32_MAX);
@@ -962,11 +1026,11 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     };
     // Few rows: blocks enough for every CU to have several in turn, since sequences are of different lengths; no split shorter than
     // 256 KiB of keys and values.
-    share(p.few, std::min(rows, FEW_ROWS), 16, 8 * cus, std::max<uint64_t>(64, (256 * 1024 / key_bytes + 63) / 64 * 64));
+    share(p.few, std::min(rows, FEW_ROWS), 16, 4 * cus, std::max<uint64_t>(64, 256 * 1024 / key_bytes));
     if (rows > FEW_ROWS) {
         if (cache.head_size <= TILE_CHANNELS) {
             // Two blocks of 128 rows are at work on a CU.
-            share(p.many, rows, TILE_ROWS, 4 * cus, 512);
+            share(p.many, rows, TILE_ROWS, 2 * cus, 512);
         } else {
             share(p.many, rows, 16, 1, 1);
         }
@@ -1055,15 +1119,17 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
             s->part_stats = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_stats));
             s->part_out = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_out));
         }
-    const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, few_rows = g.few.splits > 1 ? pairs * g.few.rows : 0, many_rows = g.many.splits > 1 ? pairs * g.many.rows : 0;
-    if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_rows + many_rows >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
+    const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, groups = JOIN / (g.d / 4);
+    const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? (pairs * g.many.rows + groups - 1) / groups : 0;
+    if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_joins + many_joins >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
-    // Pages that hold whole tiles: a tile's page is looked up once, not key by key.
-    const bool bf16 = cache.elem == AHIP_KV_BF16, uniform = cache.page_size % TILE_KEYS == 0 || (!bf16 && !g.many.blocks && cache.page_size % KEYS<false> == 0);
+    // Pages that hold whole tiles: a tile's page is looked up once, not key by key, and its slots lie within 2^31 bytes.
+    const bool bf16 = cache.elem == AHIP_KV_BF16, near = cache.slot_stride < (int64_t)1 << 23;
+    const bool uniform = near && (cache.page_size % TILE_KEYS == 0 || (!bf16 && !g.many.blocks && cache.page_size % KEYS<false> == 0));
     int rc = bf16 ? (uniform ? launch_by_size<true, true>(ctx, g) : launch_by_size<true, false>(ctx, g))
                   : (uniform ? launch_by_size<false, true>(ctx, g) : launch_by_size<false, false>(ctx, g));
-    if (rc || few_rows + many_rows == 0) return rc;
-    hipLaunchKernelGGL(join_splits, dim3((uint32_t)(few_rows + many_rows)), dim3(JOIN), 0, ctx.stream, g, (uint32_t)few_rows);
+    if (rc || few_joins + many_joins == 0) return rc;
+    hipLaunchKernelGGL(join_splits, dim3((uint32_t)(few_joins + many_joins)), dim3(JOIN), 0, ctx.stream, g, (uint32_t)few_joins);
     return ctx.check(hipGetLastError(), "kv attention launch");
 }
 
