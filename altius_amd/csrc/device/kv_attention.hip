@@ -158,12 +158,18 @@ template <bool BF16> __device__ __forceinline__ float cache_value(const void *ba
 template <bool BF16> constexpr int KEYS = BF16 ? 32 : 16;
 constexpr int ROW_WAVES = 4;
 
-template <int DP, bool BF16> struct RowTile;
-template <int DP> struct RowTile<DP, false> {
-    f32x4 k[DP / 16], v[4][DP / 64];
+template <int DP, bool BF16> struct RowKeys;
+template <int DP> struct RowKeys<DP, false> {
+    f32x4 k[DP / 16];
 };
-template <int DP> struct RowTile<DP, true> {
+template <int DP> struct RowKeys<DP, true> {
     u32x4 k[2][DP / 32];
+};
+template <int DP, bool BF16> struct RowValues;
+template <int DP> struct RowValues<DP, false> {
+    f32x4 v[4][DP / 64];
+};
+template <int DP> struct RowValues<DP, true> {
     uint32_t v[8][DP / 32];
 };
 template <int DP, bool BF16> struct RowQuery;
@@ -279,8 +285,8 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     // it (below 2^31 bytes, or the call takes the other kernel).
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
     const uint32_t k_off = col * slot_bytes + 16 * part, v_off = 4 * part * slot_bytes + (BF16 ? (DP / 16) * SIZE : 16) * col;
-    auto load_parts = [&](RowTile<DP, BF16> &t, auto whole, auto k_part, auto v_part) {
-        // k_part(h, c): channels from 64 bytes x c on, of the lane's key in half h; v_part(r, j): 256 bytes x j (fp32), 16 x j (bf16) on.
+    // at(h): where the lane's row of keys (in half h of the tile) or its h-th row of values starts.
+    auto load_keys_at = [&](RowKeys<DP, BF16> &t, auto whole, auto at) {
         constexpr bool WHOLE = decltype(whole)::value;
         if constexpr (BF16) {
 #pragma unroll
@@ -288,63 +294,76 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
 #pragma unroll
                 for (int c = 0; c < DP / 32; c++) {
                     t.k[h][c] = u32x4{0, 0, 0, 0};
-                    if (WHOLE || 32 * c + 8 * part < g.d) t.k[h][c] = *reinterpret_cast<const u32x4 *>(k_part(h) + 64 * c);
+                    if (WHOLE || 32 * c + 8 * part < g.d) t.k[h][c] = *reinterpret_cast<const u32x4 *>(at(h) + 64 * c);
                 }
-#pragma unroll
-            for (int r = 0; r < VROWS; r++) {
-                if (DP == 64) {
-                    t.v[r][0] = t.v[r][1] = 0;
-                    if (WHOLE || 4 * col < g.d) {
-                        const u32x2 x = *reinterpret_cast<const u32x2 *>(v_part(r));
-                        t.v[r][0] = x.x, t.v[r][1] = x.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < DP / 128; w++) {
-                        u32x4 x = {0, 0, 0, 0};
-                        if (WHOLE || (DP / 16) * col + 8 * w < g.d) x = *reinterpret_cast<const u32x4 *>(v_part(r) + 16 * w);
-                        t.v[r][4 * w] = x.x, t.v[r][4 * w + 1] = x.y, t.v[r][4 * w + 2] = x.z, t.v[r][4 * w + 3] = x.w;
-                    }
-                }
-            }
         } else {
 #pragma unroll
             for (int c = 0; c < DP / 16; c++) {
                 t.k[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (WHOLE || 16 * c + 4 * part < g.d) t.k[c] = *reinterpret_cast<const f32x4 *>(k_part(0) + 64 * c);
+                if (WHOLE || 16 * c + 4 * part < g.d) t.k[c] = *reinterpret_cast<const f32x4 *>(at(0) + 64 * c);
             }
+        }
+    };
+    auto load_values_at = [&](RowValues<DP, BF16> &t, auto whole, auto at) {
+        constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-            for (int r = 0; r < VROWS; r++)
+        for (int r = 0; r < VROWS; r++) {
+            if constexpr (!BF16) {
 #pragma unroll
                 for (int j = 0; j < DP / 64; j++) {
                     t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (WHOLE || 64 * j + 4 * col < g.d) t.v[r][j] = *reinterpret_cast<const f32x4 *>(v_part(r) + 256 * j);
+                    if (WHOLE || 64 * j + 4 * col < g.d) t.v[r][j] = *reinterpret_cast<const f32x4 *>(at(r) + 256 * j);
                 }
+            } else if constexpr (DP == 64) {
+                u32x2 x = {0, 0};
+                if (WHOLE || 4 * col < g.d) x = *reinterpret_cast<const u32x2 *>(at(r));
+                t.v[r][0] = x.x, t.v[r][1] = x.y;
+            } else {
+#pragma unroll
+                for (int w = 0; w < DP / 128; w++) {
+                    u32x4 x = {0, 0, 0, 0};
+                    if (WHOLE || (DP / 16) * col + 8 * w < g.d) x = *reinterpret_cast<const u32x4 *>(at(r) + 16 * w);
+                    t.v[r][4 * w] = x.x, t.v[r][4 * w + 1] = x.y, t.v[r][4 * w + 2] = x.z, t.v[r][4 * w + 3] = x.w;
+                }
+            }
         }
     };
-    auto load = [&](int32_t i, RowTile<DP, BF16> &t) {
-        const int32_t key0 = tile_key(i);
+    // The page of key lane % KT of a tile, where pages do not hold whole tiles.  Keys behind the last that is seen have none: the last
+    // one stands in for them.
+    auto standing_in = [&](int32_t key) { return (uint32_t)min(key, end - 1); };
+    auto tile_base = [&](int32_t i) {
+        const int32_t key0 = tile_key(i), page = __builtin_amdgcn_readlane(pages, i & 63);
+        const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
+        return ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
+    };
+    auto load_keys = [&](int32_t i, RowKeys<DP, BF16> &t) {
         if constexpr (UNIFORM) {
-            const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
-            const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
-            const int64_t base = ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
-            const char *kb = keys + base, *vb = values + base;
-            auto k_part = [&](int h) { return kb + (uint64_t)(16 * h) * slot_bytes + k_off; };
-            auto v_part = [&](int r) { return vb + (uint64_t)(BF16 ? 16 * (r / 4) + r % 4 : r) * slot_bytes + v_off; };
-            if (g.d == DP) load_parts(t, std::true_type(), k_part, v_part);
-            else load_parts(t, std::false_type(), k_part, v_part);
+            const char *base = keys + tile_base(i);
+            auto at = [&](int h) { return base + (uint64_t)(16 * h) * slot_bytes + k_off; };
+            if (g.d == DP) load_keys_at(t, std::true_type(), at);
+            else load_keys_at(t, std::false_type(), at);
         } else {
-            // Keys behind the last that is seen have no page to be read from: the last one stands in for them.
-            const char *k_at[2], *v_at[VROWS];
+            const char *at[2];
 #pragma unroll
-            for (int h = 0; h < (BF16 ? 2 : 1); h++) k_at[h] = keys + row_at((uint32_t)min(key0 + (int32_t)col + 16 * h, end - 1)) * SIZE + 16 * part;
+            for (int h = 0; h < (BF16 ? 2 : 1); h++) at[h] = keys + row_at(standing_in(tile_key(i) + (int32_t)col + 16 * h)) * SIZE + 16 * part;
+            load_keys_at(t, std::false_type(), [&](int h) { return at[h]; });
+        }
+    };
+    auto load_values = [&](int32_t i, RowValues<DP, BF16> &t) {
+        if constexpr (UNIFORM) {
+            const char *base = values + tile_base(i);
+            auto at = [&](int r) { return base + (uint64_t)(BF16 ? 16 * (r / 4) + r % 4 : r) * slot_bytes + v_off; };
+            if (g.d == DP) load_values_at(t, std::true_type(), at);
+            else load_values_at(t, std::false_type(), at);
+        } else {
+            const char *at[VROWS];
 #pragma unroll
-            for (int r = 0; r < VROWS; r++) v_at[r] = values + row_at((uint32_t)min(key0 + (int32_t)value_key(r), end - 1)) * SIZE + (BF16 ? (DP / 16) * SIZE : 16) * col;
-            load_parts(t, std::false_type(), [&](int h) { return k_at[h]; }, [&](int r) { return v_at[r]; });
+            for (int r = 0; r < VROWS; r++) at[r] = values + row_at(standing_in(tile_key(i) + (int32_t)value_key(r))) * SIZE + (BF16 ? (DP / 16) * SIZE : 16) * col;
+            load_values_at(t, std::false_type(), [&](int r) { return at[r]; });
         }
     };
     // Slots that no row sees may hold anything: their weight is 0, so is their value then.
-    auto clear_unseen = [&](int32_t key0, RowTile<DP, BF16> &t) {
+    auto clear_unseen = [&](int32_t key0, RowValues<DP, BF16> &t) {
         if (key0 >= begin && key0 + KT <= end) return;
 #pragma unroll
         for (int r = 0; r < VROWS; r++) {
@@ -397,7 +416,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         }
     };
 
-    auto products = [&](int32_t i, RowTile<DP, BF16> &t) {
+    auto products = [&](int32_t i, const RowKeys<DP, BF16> &t, RowValues<DP, BF16> &u) {
         const int32_t key0 = tile_key(i);
         float x[NS];
         if constexpr (BF16) {
@@ -414,7 +433,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
                 for (int r = 0; r < 4; r++) x[4 * h + r] = large[r] + small[r];
             }
             weigh(key0, x);
-            clear_unseen(key0, t);
+            clear_unseen(key0, u);
             u32x4 p[3];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -426,7 +445,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             for (int c = 0; c < NACC; c++) {
                 u32x4 v;
 #pragma unroll
-                for (int m = 0; m < 4; m++) v[m] = __builtin_amdgcn_perm(t.v[2 * m + 1][c / 2], t.v[2 * m][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+                for (int m = 0; m < 4; m++) v[m] = __builtin_amdgcn_perm(u.v[2 * m + 1][c / 2], u.v[2 * m][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                 for (int e = 2; e >= 0; e--) ALTIUS_MFMA16_BF16(v, p[e], acc[c]);
             }
@@ -443,31 +462,32 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
 #pragma unroll
             for (int r = 0; r < 4; r++) x[r] = even[r] + odd[r];
             weigh(key0, x);
-            clear_unseen(key0, t);
+            clear_unseen(key0, u);
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int j = 0; j < DP / 64; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) ALTIUS_MFMA16_F32(t.v[r][j][e], x[r], acc[4 * j + e]);
+                    for (int e = 0; e < 4; e++) ALTIUS_MFMA16_F32(u.v[r][j][e], x[r], acc[4 * j + e]);
         }
     };
 
-    // Two tiles take turns: one is on its way during the other's products.
+    // The next tile's keys are on their way during a tile's products, its values during the first of them.
     fetch_pages(0);
-    RowTile<DP, BF16> a, b;
-    auto load_next = [&](int32_t i, RowTile<DP, BF16> &t) {
-        if (i >= mine) return;
-        if ((i & 63) == 0) fetch_pages(i);
-        load(i, t);
+    RowKeys<DP, BF16> a, b;
+    RowValues<DP, BF16> v;
+    auto step = [&](int32_t i, const RowKeys<DP, BF16> &now, RowKeys<DP, BF16> &next) {
+        load_values(i, v);
+        if (i + 1 < mine) {
+            if (((i + 1) & 63) == 0) fetch_pages(i + 1);
+            load_keys(i + 1, next);
+        }
+        products(i, now, v);
     };
-    if (mine > 0) load(0, a);
+    if (mine > 0) load_keys(0, a);
     for (int32_t i = 0; i < mine; i += 2) {
-        load_next(i + 1, b);
-        products(i, a);
-        if (i + 1 >= mine) break;
-        load_next(i + 2, a);
-        products(i + 1, b);
+        step(i, a, b);
+        if (i + 1 < mine) step(i + 1, b, a);
     }
     total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
@@ -638,8 +658,10 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     // Keys 4 b .. 4 b + 3 of a tile are slots 16 (b / 4) + 8 (b % 2) + 4 (b / 2 % 2) on.
     const uint32_t v_slot = 16 * (v_block >> 2) + 8 * (v_block & 1u) + 4 * ((v_block >> 1) & 1u);
 
-    u32x4 k_stage[K_EACH];
-    uint32_t v_stage[4][BF16 ? VC / 2 : VC];
+    // In registers on their way: a thread's units of keys and its block of values, or (APART) either of them in the same ones.
+    constexpr int V_WORDS = BF16 ? VC / 2 : VC, V_REGS = V_WORDS;  // 4 keys of V_WORDS words are V_WORDS registers of four
+    u32x4 stage[APART ? (K_EACH > V_REGS ? K_EACH : V_REGS) : K_EACH + V_REGS];
+    auto v_word = [&](int key, int w) -> uint32_t { return stage[(APART ? 0 : K_EACH) + (key * V_WORDS + w) / 4][(key * V_WORDS + w) % 4]; };
 
     int32_t pages = 0;
     auto fetch_pages = [&](int32_t from) {
@@ -652,14 +674,12 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         return (int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
     };
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
-    uint32_t k_off[K_EACH], k_channel[K_EACH], k_key[K_EACH];
-#pragma unroll
-    for (int e = 0; e < K_EACH; e++) {
-        const uint32_t unit = e * K_THREADS + k_tid;
-        k_key[e] = unit / K_UNITS_ROW, k_channel[e] = (16 / SIZE) * (unit % K_UNITS_ROW);
-        k_off[e] = k_key[e] * slot_bytes + 16 * (unit % K_UNITS_ROW);
-    }
-    const uint32_t v_off = 4 * v_block * slot_bytes + SIZE * v_channel;
+    // Unit e of a thread is K_ROWS keys behind the one before, in the same channels, where that divides the rows up evenly.
+    constexpr bool EVEN = K_THREADS % K_UNITS_ROW == 0;
+    constexpr int K_ROWS = K_THREADS / K_UNITS_ROW;
+    auto k_key = [&](int e) { return EVEN ? k_tid / K_UNITS_ROW + e * K_ROWS : (e * K_THREADS + k_tid) / K_UNITS_ROW; };
+    auto k_unit = [&](int e) { return EVEN ? k_tid % K_UNITS_ROW : (e * K_THREADS + k_tid) % K_UNITS_ROW; };
+    const uint32_t k_off = (k_tid / K_UNITS_ROW) * slot_bytes + 16 * (k_tid % K_UNITS_ROW), v_off = 4 * v_block * slot_bytes + SIZE * v_channel;
     auto fetch = [&](int32_t i) {
         const int32_t key0 = (first + i) * TILE_KEYS;
         const char *kb = keys, *vb = values;
@@ -673,29 +693,33 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         if (stages_k) {
 #pragma unroll
             for (int e = 0; e < K_EACH; e++) {
-                k_stage[e] = u32x4{0, 0, 0, 0};
-                if (k_channel[e] < g.d)
-                    k_stage[e] = *reinterpret_cast<const u32x4 *>(UNIFORM ? kb + k_off[e] : keys + stand_in(key0 + (int32_t)k_key[e]) + SIZE * k_channel[e]);
+                stage[e] = u32x4{0, 0, 0, 0};
+                if ((16 / SIZE) * k_unit(e) < g.d) {
+                    const char *p = !UNIFORM ? keys + stand_in(key0 + (int32_t)k_key(e)) + 16 * k_unit(e)
+                                    : EVEN   ? kb + (uint64_t)(e * K_ROWS) * slot_bytes + k_off
+                                             : kb + (uint32_t)(k_key(e) * slot_bytes + 16 * k_unit(e));
+                    stage[e] = *reinterpret_cast<const u32x4 *>(p);
+                }
             }
         }
         if (stages_v) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int32_t key = key0 + 4 * (int32_t)v_block + e;
-                constexpr int WORDS = BF16 ? VC / 2 : VC;
-#pragma unroll
-                for (int w = 0; w < WORDS; w++) v_stage[e][w] = 0;
+                constexpr int AT = APART ? 0 : K_EACH;
+                u32x4 x = {0, 0, 0, 0};
                 // Slots that no row sees may hold anything: their weight is 0, so is their value then.
                 if (v_channel < g.d && key >= begin && key < end) {
                     const char *p = UNIFORM ? vb + (uint64_t)e * slot_bytes + v_off : values + stand_in(key) + SIZE * v_channel;
-                    if constexpr (WORDS == 4) {
-                        const u32x4 x = *reinterpret_cast<const u32x4 *>(p);
-                        v_stage[e][0] = x.x, v_stage[e][1] = x.y, v_stage[e][2] = x.z, v_stage[e][3] = x.w;
+                    if constexpr (V_WORDS == 4) {
+                        x = *reinterpret_cast<const u32x4 *>(p);
                     } else {
-                        const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
-                        v_stage[e][0] = x.x, v_stage[e][1] = x.y;
+                        const u32x2 y = *reinterpret_cast<const u32x2 *>(p);
+                        x.x = y.x, x.y = y.y;
                     }
                 }
+                if constexpr (V_WORDS == 4) stage[AT + e] = x;
+                else stage[AT + e / 2][2 * (e % 2)] = x.x, stage[AT + e / 2][2 * (e % 2) + 1] = x.y;
             }
         }
     };
@@ -703,13 +727,13 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         if (stages_k) {
 #pragma unroll
             for (int e = 0; e < K_EACH; e++) {
-                uint16_t *to = &lds.k[buffer][0][k_key[e] * K_PITCH + k_channel[e]];
+                uint16_t *to = &lds.k[buffer][0][k_key(e) * K_PITCH + (16 / SIZE) * k_unit(e)];
                 if constexpr (BF16) {
-                    *reinterpret_cast<u32x4 *>(to) = k_stage[e];
+                    *reinterpret_cast<u32x4 *>(to) = stage[e];
                 } else {
                     uint32_t p[3][2];
 #pragma unroll
-                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
+                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(stage[e][2 * w]), __uint_as_float(stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
                     for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
                 }
@@ -721,11 +745,12 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
                 uint16_t *to = &lds.v[buffer][0][(v_channel + c) * V_PITCH + v_slot];
                 if constexpr (BF16) {
                     const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
-                    *reinterpret_cast<u32x2 *>(to) = u32x2{__builtin_amdgcn_perm(v_stage[1][c / 2], v_stage[0][c / 2], pick), __builtin_amdgcn_perm(v_stage[3][c / 2], v_stage[2][c / 2], pick)};
+                    *reinterpret_cast<u32x2 *>(to) =
+                        u32x2{__builtin_amdgcn_perm(v_word(1, c / 2), v_word(0, c / 2), pick), __builtin_amdgcn_perm(v_word(3, c / 2), v_word(2, c / 2), pick)};
                 } else {
                     uint32_t p[3][2];
 #pragma unroll
-                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
+                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_word(2 * w, c)), __uint_as_float(v_word(2 * w + 1, c)), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
                     for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
                 }
