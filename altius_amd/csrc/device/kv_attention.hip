@@ -28,6 +28,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504088896341f;
+// The maximum that weights are relative to stays until one is this much (in powers of two) above it: fp32 holds weights up to 2^8 as
+// exactly as those up to 1, and most of the rescaling of what has been summed falls away.
+constexpr float SLACK = 8.0f;
 // Sequences with at most so many rows for a kv head share their keys' blocks out (attend_rows16, SPLIT); longer ones have
 // blocks enough.
 constexpr uint32_t FEW_ROWS = 64;
@@ -141,6 +144,19 @@ __device__ __forceinline__ void split_pair(float e0, float e1, uint32_t &p0, uin
     p2 = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){s0, s1}, bf16x2));
 }
 
+// The largest of three, without the instructions that make a signalling NaN quiet in front of fmaxf.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// v of lane ^ 32 next to the lane's own, without LDS: the first is the lower half's value in both halves, the second the upper half's.
+__device__ __forceinline__ void halves(float v, float &lower, float &upper) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    lower = __uint_as_float(r[0]), upper = __uint_as_float(r[1]);
+}
+
 template <bool BF16> __device__ __forceinline__ float cache_value(const void *base, int64_t at) {
     return BF16 ? __uint_as_float((uint32_t)static_cast<const uint16_t *>(base)[at] << 16) : static_cast<const float *>(base)[at];
 }
@@ -189,7 +205,7 @@ template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int 
     return BF16 ? (DP / 16) * (4 * part + r) + i : 64 * (i / 4) + 4 * (4 * part + r) + i % 4;
 }
 
-// UNIFORM: pages hold whole tiles, so a tile's keys are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
+// UNIFORM: 16 keys that start at a multiple of 16 are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
 template <int DP> struct RowLds {
     static constexpr int PITCH = DP + 4;
     float sums[ROW_WAVES][16 * PITCH];
@@ -264,13 +280,14 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         }
     }
 
-    // Wavefront w takes tiles w, w + 4, ... of the block's; the pages of its next 64 tiles wait in one register.
+    // Wavefront w takes tiles w, w + 4, ... of the block's; the pages of its next 64 groups of 16 keys wait in one register.
+    constexpr int HALVES = KT / 16;
     const int32_t mine = tiles > (int32_t)wave ? (tiles - (int32_t)wave + ROW_WAVES - 1) / ROW_WAVES : 0;
     int32_t pages = 0;
     auto fetch_pages = [&](int32_t from) {
-        const int32_t i = from + (int32_t)lane;
+        const int32_t i = from + (int32_t)lane / HALVES, key = (first + (int32_t)wave + i * ROW_WAVES) * KT + 16 * (int32_t)(lane % HALVES);
         pages = 0;
-        if (UNIFORM && i < mine) pages = g.kv.page_of(s, g.kv.by_page_size.div((uint32_t)((first + (int32_t)wave + i * ROW_WAVES) * KT)), 0);
+        if (UNIFORM && i < mine && key < end) pages = g.kv.page_of(s, g.kv.by_page_size.div((uint32_t)key), 0);
     };
     auto tile_key = [&](int32_t i) { return (first + (int32_t)wave + i * ROW_WAVES) * KT; };
     auto row_at = [&](uint32_t key) {  // elements from the start of the cache
@@ -281,7 +298,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     auto value_key = [&](int i) { return BF16 ? 16 * (i / 4) + 4 * part + i % 4 : 4 * part + i; };
     constexpr int VROWS = BF16 ? 8 : 4;
 
-    // Where pages hold whole tiles a tile starts at one address for the whole wavefront, and a lane's parts lie at fixed distances from
+    // 16 keys of one page start at one address for the whole wavefront, and a lane's parts lie at fixed distances from
     // it (below 2^31 bytes, or the call takes the other kernel).
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
     const uint32_t k_off = col * slot_bytes + 16 * part, v_off = 4 * part * slot_bytes + (BF16 ? (DP / 16) * SIZE : 16) * col;
@@ -328,18 +345,17 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             }
         }
     };
-    // The page of key lane % KT of a tile, where pages do not hold whole tiles.  Keys behind the last that is seen have none: the last
-    // one stands in for them.
+    // Keys behind the last that is seen have no page: the last one stands in for them.
     auto standing_in = [&](int32_t key) { return (uint32_t)min(key, end - 1); };
-    auto tile_base = [&](int32_t i) {
-        const int32_t key0 = tile_key(i), page = __builtin_amdgcn_readlane(pages, i & 63);
-        const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
+    auto half_at = [&](int32_t i, int half) {
+        const int32_t page = __builtin_amdgcn_readlane(pages, (HALVES * i + half) & 63);
+        const uint32_t key = (uint32_t)tile_key(i) + 16 * half, slot = key - g.kv.by_page_size.div(key) * g.kv.page_size;
         return ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
     };
     auto load_keys = [&](int32_t i, RowKeys<DP, BF16> &t) {
         if constexpr (UNIFORM) {
-            const char *base = keys + tile_base(i);
-            auto at = [&](int h) { return base + (uint64_t)(16 * h) * slot_bytes + k_off; };
+            const char *base[2] = {keys + half_at(i, 0), keys + half_at(i, HALVES - 1)};
+            auto at = [&](int h) { return base[h] + k_off; };
             if (g.d == DP) load_keys_at(t, std::true_type(), at);
             else load_keys_at(t, std::false_type(), at);
         } else {
@@ -351,8 +367,8 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     };
     auto load_values = [&](int32_t i, RowValues<DP, BF16> &t) {
         if constexpr (UNIFORM) {
-            const char *base = values + tile_base(i);
-            auto at = [&](int r) { return base + (uint64_t)(BF16 ? 16 * (r / 4) + r % 4 : r) * slot_bytes + v_off; };
+            const char *base[2] = {values + half_at(i, 0), values + half_at(i, HALVES - 1)};
+            auto at = [&](int r) { return base[r / 4] + (uint64_t)(r % 4) * slot_bytes + v_off; };
             if (g.d == DP) load_values_at(t, std::true_type(), at);
             else load_values_at(t, std::false_type(), at);
         } else {
@@ -399,14 +415,14 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
         const float now = fmaxf(top, most);
-        if (__any(now != top)) {
+        if (__any(now > top + SLACK)) {
             const float corr = weight_of(top, now);
             total *= corr;
 #pragma unroll
             for (int i = 0; i < NACC; i++) acc[i] *= corr;
             top = now;
         }
-        const float base = now == -INFINITY ? 0.0f : now;
+        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int r = 0; r < NS; r++) {
             const int32_t key = key0 + (int32_t)value_key(r);
@@ -479,7 +495,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     auto step = [&](int32_t i, const RowKeys<DP, BF16> &now, RowKeys<DP, BF16> &next) {
         load_values(i, v);
         if (i + 1 < mine) {
-            if (((i + 1) & 63) == 0) fetch_pages(i + 1);
+            if (((i + 1) & (64 / HALVES - 1)) == 0) fetch_pages(i + 1);
             load_keys(i + 1, next);
         }
         products(i, now, v);
@@ -581,8 +597,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows
 // second product takes its k slots in that order, in which V^T lies in LDS.  Queries and weights are three bf16 numbers each, as
 // above; so are the values of an fp32 cache, split on their way into LDS, and six products of the parts are what fp32 holds of the
 // whole (the three left out are below 2^-24 of it).  A bf16 cache's values are one number: three products.
-//   The next tile's loads are in flight during the products; where LDS has room for two blocks' worth of two tiles the next one is
-// written while the other is read, with one barrier a tile.
+//   Two tiles of each operand in LDS, one barrier a tile.
 constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
 
 #define ALTIUS_MFMA32_BF16(A, B, C) \
@@ -592,15 +607,14 @@ template <int DP, bool BF16> struct TileLds {
     static constexpr int PLANES = BF16 ? 1 : 3;
     static constexpr int K_PITCH = DP + 8;          // 16-bit words; 16 rows of 16-byte reads cover all banks
     static constexpr int V_PITCH = TILE_KEYS + 8;   // a row is a channel
-    static constexpr int BUFFERS = 2 * 2 * PLANES * (TILE_KEYS * K_PITCH + DP * V_PITCH) <= 80 * 1024 ? 2 : 1;
-    uint16_t k[BUFFERS][PLANES][TILE_KEYS * K_PITCH], v[BUFFERS][PLANES][DP * V_PITCH];
+    uint16_t k[2][PLANES][TILE_KEYS * K_PITCH], v[2][PLANES][DP * V_PITCH];
     int32_t bounds[4][2];
 };
 
 template <int DP, bool BF16, bool UNIFORM>
 __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLds<DP, BF16> &lds) {
     using Lds = TileLds<DP, BF16>;
-    constexpr int PLANES = Lds::PLANES, K_PITCH = Lds::K_PITCH, V_PITCH = Lds::V_PITCH, BUFFERS = Lds::BUFFERS;
+    constexpr int PLANES = Lds::PLANES, K_PITCH = Lds::K_PITCH, V_PITCH = Lds::V_PITCH;
     constexpr int STEPS = DP / 16, PARTS = DP / 32;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, h = lane >> 5;
@@ -638,126 +652,140 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     if (share.splits > 1)
         begin = max(begin, (int32_t)(split * share.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * share.split_keys));
     begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
-    any_low = __builtin_amdgcn_readfirstlane(any_low), any_high = __builtin_amdgcn_readfirstlane(any_high);
-    all_low = __builtin_amdgcn_readfirstlane(all_low), all_high = __builtin_amdgcn_readfirstlane(all_high);
+    any_low = max(begin, __builtin_amdgcn_readfirstlane(any_low)), any_high = min(end, __builtin_amdgcn_readfirstlane(any_high));
+    all_low = max(begin, __builtin_amdgcn_readfirstlane(all_low)), all_high = min(end, __builtin_amdgcn_readfirstlane(all_high));
     const int32_t first = begin / TILE_KEYS, tiles = begin < end ? (end + TILE_KEYS - 1) / TILE_KEYS - first : 0;
+    // The tiles that this wavefront's rows see.
+    const int32_t mine_from = any_low < any_high ? any_low / TILE_KEYS - first : INT32_MAX - 1, mine_to = any_low < any_high ? (any_high + TILE_KEYS - 1) / TILE_KEYS - first : 0;
 
     const char *keys = static_cast<const char *>(g.kv.keys), *values = static_cast<const char *>(g.kv.values);
     constexpr int SIZE = BF16 ? 2 : 4;
     const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
 
     // Staging.  Keys: 16-byte units, a row after the other.  Values: blocks of 4 keys (which lie side by side in V^T) and VC
-    // channels.  Where there are at most 128 blocks of values two wavefronts fetch them and the other two the keys.
-    constexpr int VC = BF16 && DP >= 96 ? 8 : 4, V_BLOCKS = 8 * (DP / VC), K_UNITS_ROW = DP * SIZE / 16, K_UNITS = TILE_KEYS * K_UNITS_ROW;
-    constexpr bool APART = V_BLOCKS <= 128;
-    constexpr int K_THREADS = APART ? 128 : 256, K_EACH = (K_UNITS + K_THREADS - 1) / K_THREADS;
-    static_assert(K_UNITS % K_THREADS == 0 && V_BLOCKS <= 256, "staging");
-    const bool stages_k = !APART || tid >= 128, stages_v = tid < V_BLOCKS;
-    const uint32_t k_tid = APART ? tid & 127u : tid;
-    const uint32_t v_block = tid & 7u, v_channel = VC * (tid >> 3);
+    // channels.  All threads do the same, without a branch: where the units or blocks are fewer, some are fetched and written twice.
+    constexpr int VC = DP == 64 ? 2 : 4, V_BLOCKS = 8 * (DP / VC), K_UNITS_ROW = DP * SIZE / 16, K_UNITS = TILE_KEYS * K_UNITS_ROW, K_EACH = (K_UNITS + 255) / 256;
+    static_assert(V_BLOCKS <= 256 && DP % VC == 0, "staging");
+    const uint32_t v_tid = V_BLOCKS == 256 ? tid : tid % V_BLOCKS, v_block = v_tid & 7u, v_channel = VC * (v_tid >> 3);
     // Keys 4 b .. 4 b + 3 of a tile are slots 16 (b / 4) + 8 (b % 2) + 4 (b / 2 % 2) on.
     const uint32_t v_slot = 16 * (v_block >> 2) + 8 * (v_block & 1u) + 4 * ((v_block >> 1) & 1u);
+    // Unit e of a thread is K_ROWS keys behind the one before, in the same channels, where that divides the rows up evenly.
+    constexpr bool EVEN = 256 % K_UNITS_ROW == 0 && K_UNITS % 256 == 0;
+    constexpr int K_ROWS = 256 / K_UNITS_ROW;
+    auto k_key = [&](int e) { return EVEN ? tid / K_UNITS_ROW + e * K_ROWS : (e * 256 + tid) % K_UNITS / K_UNITS_ROW; };
+    auto k_unit = [&](int e) { return EVEN ? tid % K_UNITS_ROW : (e * 256 + tid) % K_UNITS % K_UNITS_ROW; };
+    constexpr int V_WORDS = VC * SIZE / 4;  // of a key
+    typedef uint32_t VWords __attribute__((ext_vector_type(V_WORDS == 1 ? 2 : V_WORDS)));
+    u32x4 k_stage[K_EACH];
+    VWords v_stage[4];
 
-    // In registers on their way: a thread's units of keys and its block of values, or (APART) either of them in the same ones.
-    constexpr int V_WORDS = BF16 ? VC / 2 : VC, V_REGS = V_WORDS;  // 4 keys of V_WORDS words are V_WORDS registers of four
-    u32x4 stage[APART ? (K_EACH > V_REGS ? K_EACH : V_REGS) : K_EACH + V_REGS];
-    auto v_word = [&](int key, int w) -> uint32_t { return stage[(APART ? 0 : K_EACH) + (key * V_WORDS + w) / 4][(key * V_WORDS + w) % 4]; };
-
-    int32_t pages = 0;
-    auto fetch_pages = [&](int32_t from) {
-        const int32_t i = from + (int32_t)lane;
-        pages = 0;
-        if (UNIFORM && i < tiles) pages = g.kv.page_of(s, g.kv.by_page_size.div((uint32_t)((first + i) * TILE_KEYS)), 0);
+    // Where pages hold at least half a tile: where the next 32 tiles' halves start, in bytes from the start of the cache, a half a lane.
+    int64_t starts = 0;
+    auto fetch_starts = [&](int32_t from) {
+        const int32_t key = (first + from) * TILE_KEYS + 16 * (int32_t)lane;
+        if (!UNIFORM) return;
+        const uint32_t index = g.kv.by_page_size.div((uint32_t)min(key, end - 1));
+        starts = ((int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)((uint32_t)key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
+        if (key >= end) starts = 0;
     };
     auto row_at = [&](uint32_t key) {  // elements from the start of the cache
         const uint32_t index = g.kv.by_page_size.div(key);
         return (int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
     };
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
-    // Unit e of a thread is K_ROWS keys behind the one before, in the same channels, where that divides the rows up evenly.
-    constexpr bool EVEN = K_THREADS % K_UNITS_ROW == 0;
-    constexpr int K_ROWS = K_THREADS / K_UNITS_ROW;
-    auto k_key = [&](int e) { return EVEN ? k_tid / K_UNITS_ROW + e * K_ROWS : (e * K_THREADS + k_tid) / K_UNITS_ROW; };
-    auto k_unit = [&](int e) { return EVEN ? k_tid % K_UNITS_ROW : (e * K_THREADS + k_tid) % K_UNITS_ROW; };
-    const uint32_t k_off = (k_tid / K_UNITS_ROW) * slot_bytes + 16 * (k_tid % K_UNITS_ROW), v_off = 4 * v_block * slot_bytes + SIZE * v_channel;
-    auto fetch = [&](int32_t i) {
+    // No load below depends on a condition, which would have the compiler wait for those before it.  Channels that a head does not
+    // have are read as its first ones: their queries are 0, their sums go nowhere.
+    auto k_byte = [&](int e) { return (16 / SIZE) * k_unit(e) < g.d ? 16 * k_unit(e) : 0u; };
+    const uint32_t v_byte = v_channel < g.d ? SIZE * v_channel : 0;
+    const uint32_t k_off = tid / K_UNITS_ROW % 16 * slot_bytes + k_byte(0), v_off = 4 * (v_block & 3u) * slot_bytes + v_byte;
+    struct Halves {
+        int64_t at[2];
+    };
+    auto halves_of = [&](int32_t i) {
+        Halves t;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const uint32_t low_word = __builtin_amdgcn_readlane((int32_t)starts, (2 * i + half) & 63), high_word = __builtin_amdgcn_readlane((int32_t)(starts >> 32), (2 * i + half) & 63);
+            t.at[half] = (int64_t)((uint64_t)high_word << 32 | low_word);
+        }
+        return t;
+    };
+    auto stand_in = [&](int32_t key) { return row_at((uint32_t)min(key, end - 1)) * SIZE; };  // for keys behind the last that is seen
+    auto fetch_keys = [&](int32_t i, const Halves &half) {
         const int32_t key0 = (first + i) * TILE_KEYS;
-        const char *kb = keys, *vb = values;
-        if (UNIFORM) {
-            const int32_t page = __builtin_amdgcn_readlane(pages, i & 63);
-            const uint32_t slot = (uint32_t)key0 - g.kv.by_page_size.div((uint32_t)key0) * g.kv.page_size;
-            const int64_t base = ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
-            kb += base, vb += base;
-        }
-        auto stand_in = [&](int32_t key) { return row_at((uint32_t)min(key, end - 1)) * SIZE; };  // for keys behind the last that is seen
-        if (stages_k) {
 #pragma unroll
-            for (int e = 0; e < K_EACH; e++) {
-                stage[e] = u32x4{0, 0, 0, 0};
-                if ((16 / SIZE) * k_unit(e) < g.d) {
-                    const char *p = !UNIFORM ? keys + stand_in(key0 + (int32_t)k_key(e)) + 16 * k_unit(e)
-                                    : EVEN   ? kb + (uint64_t)(e * K_ROWS) * slot_bytes + k_off
-                                             : kb + (uint32_t)(k_key(e) * slot_bytes + 16 * k_unit(e));
-                    stage[e] = *reinterpret_cast<const u32x4 *>(p);
-                }
-            }
+        for (int e = 0; e < K_EACH; e++) {
+            const char *p;
+            if constexpr (!UNIFORM) p = keys + stand_in(key0 + (int32_t)k_key(e)) + k_byte(e);
+            else if constexpr (EVEN && K_ROWS <= 16) p = keys + half.at[e * K_ROWS / 16] + (uint64_t)(e * K_ROWS % 16) * slot_bytes + k_off;
+            else if constexpr (EVEN) p = keys + (k_key(e) < 16 ? half.at[0] : half.at[1]) + k_off;
+            else p = keys + (k_key(e) < 16 ? half.at[0] : half.at[1]) + (k_key(e) % 16 * slot_bytes + k_byte(e));
+            k_stage[e] = *reinterpret_cast<const u32x4 *>(p);
         }
-        if (stages_v) {
+    };
+    auto fetch_values = [&](int32_t i, const Halves &half) {
+        const int32_t key0 = (first + i) * TILE_KEYS;
+        const char *base = values + (v_block < 4 ? half.at[0] : half.at[1]) + v_off;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int32_t key = key0 + 4 * (int32_t)v_block + e;
-                constexpr int AT = APART ? 0 : K_EACH;
-                u32x4 x = {0, 0, 0, 0};
-                // Slots that no row sees may hold anything: their weight is 0, so is their value then.
-                if (v_channel < g.d && key >= begin && key < end) {
-                    const char *p = UNIFORM ? vb + (uint64_t)e * slot_bytes + v_off : values + stand_in(key) + SIZE * v_channel;
-                    if constexpr (V_WORDS == 4) {
-                        x = *reinterpret_cast<const u32x4 *>(p);
-                    } else {
-                        const u32x2 y = *reinterpret_cast<const u32x2 *>(p);
-                        x.x = y.x, x.y = y.y;
-                    }
-                }
-                if constexpr (V_WORDS == 4) stage[AT + e] = x;
-                else stage[AT + e / 2][2 * (e % 2)] = x.x, stage[AT + e / 2][2 * (e % 2) + 1] = x.y;
+        for (int e = 0; e < 4; e++) {
+            const char *p = UNIFORM ? base + (uint64_t)e * slot_bytes : values + stand_in(key0 + 4 * (int32_t)v_block + e) + v_byte;
+            if constexpr (V_WORDS == 1) v_stage[e][0] = *reinterpret_cast<const uint32_t *>(p);
+            else v_stage[e] = *reinterpret_cast<const VWords *>(p);
+        }
+    };
+    // Slots that no row sees may hold anything: their weight is 0, so is their value then.
+    auto clear_unseen = [&](int32_t i) {
+        const int32_t key0 = (first + i) * TILE_KEYS;
+        if (key0 >= begin && key0 + TILE_KEYS <= end) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int32_t key = key0 + 4 * (int32_t)v_block + e;
+            const bool seen = key >= begin && key < end;
+#pragma unroll
+            for (int w = 0; w < V_WORDS; w++) v_stage[e][w] = seen ? v_stage[e][w] : 0;
+        }
+    };
+    auto park_keys = [&](int buffer) {
+#pragma unroll
+        for (int e = 0; e < K_EACH; e++) {
+            uint16_t *to = &lds.k[buffer][0][k_key(e) * K_PITCH + (16 / SIZE) * k_unit(e)];
+            if constexpr (BF16) {
+                *reinterpret_cast<u32x4 *>(to) = k_stage[e];
+            } else {
+                uint32_t p[3][2];
+#pragma unroll
+                for (int w = 0; w < 2; w++) split_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
+#pragma unroll
+                for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
             }
         }
     };
-    auto park = [&](int buffer) {
-        if (stages_k) {
+    auto park_values = [&](int buffer) {
 #pragma unroll
-            for (int e = 0; e < K_EACH; e++) {
-                uint16_t *to = &lds.k[buffer][0][k_key(e) * K_PITCH + (16 / SIZE) * k_unit(e)];
-                if constexpr (BF16) {
-                    *reinterpret_cast<u32x4 *>(to) = stage[e];
-                } else {
-                    uint32_t p[3][2];
+        for (int c = 0; c < VC; c++) {
+            uint16_t *to = &lds.v[buffer][0][(v_channel + c) * V_PITCH + v_slot];
+            if constexpr (BF16) {
+                const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
+                *reinterpret_cast<u32x2 *>(to) =
+                    u32x2{__builtin_amdgcn_perm(v_stage[1][c / 2], v_stage[0][c / 2], pick), __builtin_amdgcn_perm(v_stage[3][c / 2], v_stage[2][c / 2], pick)};
+            } else {
+                uint32_t p[3][2];
 #pragma unroll
-                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(stage[e][2 * w]), __uint_as_float(stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
+                for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
-                    for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
-                }
-            }
-        }
-        if (stages_v) {
-#pragma unroll
-            for (int c = 0; c < VC; c++) {
-                uint16_t *to = &lds.v[buffer][0][(v_channel + c) * V_PITCH + v_slot];
-                if constexpr (BF16) {
-                    const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
-                    *reinterpret_cast<u32x2 *>(to) =
-                        u32x2{__builtin_amdgcn_perm(v_word(1, c / 2), v_word(0, c / 2), pick), __builtin_amdgcn_perm(v_word(3, c / 2), v_word(2, c / 2), pick)};
-                } else {
-                    uint32_t p[3][2];
-#pragma unroll
-                    for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_word(2 * w, c)), __uint_as_float(v_word(2 * w + 1, c)), p[0][w], p[1][w], p[2][w]);
-#pragma unroll
-                    for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
-                }
+                for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
             }
         }
     };
 
+    // The first tile's keys and values and the second's keys, while the queries are split.
+    Halves next = {};  // of the tile whose values are fetched next: its keys were a tile ago
+    if (tiles > 0) {
+        fetch_starts(0);
+        next = halves_of(0);
+        fetch_keys(0, next), fetch_values(0, next);
+        next = halves_of(1);
+    }
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
     u32x4 q[3][STEPS];
 #pragma unroll
@@ -777,7 +805,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     }
 
     float top = -INFINITY, total = 0.0f;
-    f32x16 acc[PARTS];
+    f32x16 acc[PARTS], st;
 #pragma unroll
     for (int i = 0; i < PARTS; i++)
 #pragma unroll
@@ -799,10 +827,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             ALTIUS_MFMA32_BF16(a[0], b0, c);
         }
     };
-    auto attend = [&](int32_t i, int buffer) {
-        const int32_t key0 = (first + i) * TILE_KEYS;
-        if (key0 >= any_high || key0 + TILE_KEYS <= any_low) return;  // for this wavefront's rows
-        f32x16 st;
+    auto first_product = [&](int buffer) {
 #pragma unroll
         for (int r = 0; r < 16; r++) st[r] = 0.0f;
 #pragma unroll
@@ -812,76 +837,93 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             for (int p = 0; p < PLANES; p++) k[p] = *reinterpret_cast<const u32x4 *>(&lds.k[buffer][p][col * K_PITCH + 16 * c + 8 * h]);
             multiply(k, q[0][c], q[1][c], q[2][c], st);
         }
-        float x[16];
-#pragma unroll
-        for (int r = 0; r < 16; r++) x[r] = st[r];
-        scores(g, x, slope, place - key0, key_of);
-        if (key0 < max(all_low, begin) || key0 + TILE_KEYS > min(all_high, end)) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int32_t key = key0 + key_of(r);
-                // A score that is not there is minus infinity: its weight is 0 once a finite maximum is known, and the row that has
-                // none yet takes 0 for it.
-                x[r] = key >= max(low, begin) && key < min(high, end) ? x[r] : -INFINITY;
-            }
-        }
-        float most = x[0];
-#pragma unroll
-        for (int r = 1; r < 16; r++) most = fmaxf(most, x[r]);
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const float now = fmaxf(top, most);
-        if (__any(now != top)) {
-            const float corr = weight_of(top, now);
-            total *= corr;
-#pragma unroll
-            for (int t = 0; t < PARTS; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) acc[t][r] *= corr;
-            top = now;
-        }
-        const float base = now == -INFINITY ? 0.0f : now;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            x[r] = exp2_fast(x[r] - base);
-            total += x[r];
-        }
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            u32x4 p[3];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                uint32_t w[3];
-                split_pair(x[8 * u + 2 * e], x[8 * u + 2 * e + 1], w[0], w[1], w[2]);
-                p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
-            }
-#pragma unroll
-            for (int t = 0; t < PARTS; t++) {
-                u32x4 v[PLANES];
-#pragma unroll
-                for (int q = 0; q < PLANES; q++) v[q] = *reinterpret_cast<const u32x4 *>(&lds.v[buffer][q][(32 * t + col) * V_PITCH + 16 * u + 8 * h]);
-                multiply(v, p[0], p[1], p[2], acc[t]);
-            }
-        }
     };
 
-    fetch_pages(0);
-    if (tiles > 0) fetch(0);
-    if (BUFFERS == 2 && tiles > 0) park(0);
-    for (int32_t i = 0; i < tiles; i++) {
-        const bool more = i + 1 < tiles;
-        if (BUFFERS == 1) {
-            __syncthreads();  // nobody reads the tile before any more
-            park(0);
+    if (tiles > 0) {
+        clear_unseen(0);
+        park_keys(0), park_values(0);
+        if (tiles > 1) {
+            fetch_keys(1, next);
+            park_keys(1);
         }
         __syncthreads();
-        if (more) {
-            if (((i + 1) & 63) == 0) fetch_pages(i + 1);
-            fetch(i + 1);
-        }
-        attend(i, BUFFERS == 2 ? i & 1 : 0);
-        if (BUFFERS == 2 && more) park((i + 1) & 1);
+        if (mine_from == 0) first_product(0);
     }
-    total += __shfl_xor(total, 32);
+    // Tile i: its scores are in registers, its values and the next tile's keys in LDS.  The next tile's first product runs beside the
+    // exponentials and splits of this one's weights, this one's second product beside the staging of the tiles behind: the matrix
+    // cores and the vector unit have work at the same time, in one wavefront as in two.
+    for (int32_t i = 0; i < tiles; i++) {
+        __syncthreads();
+        const int32_t key0 = (first + i) * TILE_KEYS;
+        // Tiles i + 2 and i + 1; behind the last one it is fetched again, and not read.
+        const int32_t ahead = min(i + 2, tiles - 1);
+        fetch_values(min(i + 1, tiles - 1), next);
+        if ((ahead & 31) == 0) fetch_starts(ahead);
+        next = halves_of(ahead);
+        fetch_keys(ahead, next);
+        if (i >= mine_from && i < mine_to) {
+            float x[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[r] = st[r];
+            scores(g, x, slope, place - key0, key_of);
+            if (key0 < all_low || key0 + TILE_KEYS > all_high) {
+                // A score that is not there is minus infinity: its weight is 0 once a finite maximum is known, and the row that has none
+                // yet takes 0 for it.
+                const int32_t from = max(low, begin) - key0, to = min(high, end) - key0;
+#pragma unroll
+                for (int r = 0; r < 16; r++) x[r] = key_of(r) >= from && key_of(r) < to ? x[r] : -INFINITY;
+            }
+            float most = x[0], lower, upper;
+#pragma unroll
+            for (int r = 1; r < 15; r += 2) most = max3(most, x[r], x[r + 1]);
+            most = max3(most, x[15], x[15]);
+            halves(most, lower, upper);
+            const float now = max3(top, lower, upper);
+            if (__any(now > top + SLACK)) {
+                const float corr = weight_of(top, now);
+                total *= corr;
+#pragma unroll
+                for (int t = 0; t < PARTS; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[t][r] *= corr;
+                top = now;
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            if (i + 1 == tiles - 1) clear_unseen(i + 1);
+            first_product((i + 1) & 1);
+            u32x4 p[2][3];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float a = exp2_fast(x[8 * u + 2 * e] - base), b = exp2_fast(x[8 * u + 2 * e + 1] - base);
+                    total += a;
+                    total += b;
+                    uint32_t w[3];
+                    split_pair(a, b, w[0], w[1], w[2]);
+                    p[u][0][e] = w[0], p[u][1][e] = w[1], p[u][2][e] = w[2];
+                }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int t = 0; t < PARTS; t++) {
+                    u32x4 v[PLANES];
+#pragma unroll
+                    for (int w = 0; w < PLANES; w++) v[w] = *reinterpret_cast<const u32x4 *>(&lds.v[i & 1][w][(32 * t + col) * V_PITCH + 16 * u + 8 * h]);
+                    multiply(v, p[u][0], p[u][1], p[u][2], acc[t]);
+                }
+            park_keys(i & 1), park_values((i + 1) & 1);
+        } else {
+            if (i + 1 == mine_from) first_product((i + 1) & 1);
+            if (i + 1 == tiles - 1) clear_unseen(i + 1);
+            park_keys(i & 1), park_values((i + 1) & 1);
+        }
+    }
+    {
+        float lower, upper;
+        halves(total, lower, upper);
+        total = lower + upper;
+    }
 
     // As in rows16: what is not finite is computed once more, value by value.
     float check = total * 0.0f;
@@ -935,15 +977,16 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         }
 }
 
-// Prompts, and the sequences of few rows that share a batch with them: the first blocks are the latter's.
+// Prompts, and the sequences of few rows that share a batch with them: the last blocks are the latter's, and end at once where there
+// are none.
 template <int DP, bool BF16, bool UNIFORM>
-__global__ __launch_bounds__(256, 2) void attend_rows128(AttendArgs g) {
+__global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(AttendArgs g) {
     __shared__ __align__(16) union {
         RowLds<DP <= 64 ? 64 : 128> few;
         TileLds<DP, BF16> many;
     } lds;
-    if (blockIdx.x < g.few.blocks) rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true>(g, blockIdx.x, lds.few);
-    else rows128<DP, BF16, UNIFORM>(g, blockIdx.x - g.few.blocks, lds.many);
+    if (blockIdx.x < g.many.blocks) rows128<DP, BF16, UNIFORM>(g, blockIdx.x, lds.many);
+    else rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true>(g, blockIdx.x - g.many.blocks, lds.few);
 }
 
 // Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
@@ -1148,9 +1191,8 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
     const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? (pairs * g.many.rows + groups - 1) / groups : 0;
     if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_joins + many_joins >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
-    // Pages that hold whole tiles: a tile's page is looked up once, not key by key, and its slots lie within 2^31 bytes.
-    const bool bf16 = cache.elem == AHIP_KV_BF16, near = cache.slot_stride < (int64_t)1 << 23;
-    const bool uniform = near && (cache.page_size % TILE_KEYS == 0 || (!bf16 && !g.many.blocks && cache.page_size % KEYS<false> == 0));
+    // Pages of whole groups of 16 keys: a group's page is looked up once, not key by key, and its slots lie within 2^31 bytes.
+    const bool bf16 = cache.elem == AHIP_KV_BF16, uniform = cache.page_size % 16 == 0 && cache.slot_stride < (int64_t)1 << 23;
     int rc = bf16 ? (uniform ? launch_by_size<true, true>(ctx, g) : launch_by_size<true, false>(ctx, g))
                   : (uniform ? launch_by_size<false, true>(ctx, g) : launch_by_size<false, false>(ctx, g));
     if (rc || few_joins + many_joins == 0) return rc;
