@@ -607,7 +607,10 @@ template <int DP, bool BF16> struct TileLds {
     static constexpr int PLANES = BF16 ? 1 : 3;
     static constexpr int K_PITCH = DP + 8;          // 16-bit words; 16 rows of 16-byte reads cover all banks
     static constexpr int V_PITCH = TILE_KEYS + 8;   // a row is a channel
+    // The queries' third parts, read once a tile, where registers do not hold all three.
+    static constexpr bool Q_HERE = DP > 64;
     uint16_t k[2][PLANES][TILE_KEYS * K_PITCH], v[2][PLANES][DP * V_PITCH];
+    uint16_t q[Q_HERE ? 4 : 1][Q_HERE ? 32 * K_PITCH : 8];
     int32_t bounds[4][2];
 };
 
@@ -787,7 +790,8 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         next = halves_of(1);
     }
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
-    u32x4 q[3][STEPS];
+    u32x4 q[Lds::Q_HERE ? 2 : 3][STEPS];
+    uint16_t *q_here = &lds.q[Lds::Q_HERE ? wave : 0][Lds::Q_HERE ? col * K_PITCH + 8 * h : 0];
 #pragma unroll
     for (int i = 0; i < STEPS; i++) {
         const uint32_t c = 16 * i + 8 * h;
@@ -801,7 +805,8 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             split_pair(hi[2 * e], hi[2 * e + 1], w[0][2 + e], w[1][2 + e], w[2][2 + e]);
         }
 #pragma unroll
-        for (int p = 0; p < 3; p++) q[p][i] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+        for (int p = 0; p < (Lds::Q_HERE ? 2 : 3); p++) q[p][i] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+        if (Lds::Q_HERE) *reinterpret_cast<u32x4 *>(q_here + 16 * i) = u32x4{w[2][0], w[2][1], w[2][2], w[2][3]};
     }
 
     float top = -INFINITY, total = 0.0f;
@@ -835,7 +840,10 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             u32x4 k[PLANES];
 #pragma unroll
             for (int p = 0; p < PLANES; p++) k[p] = *reinterpret_cast<const u32x4 *>(&lds.k[buffer][p][col * K_PITCH + 16 * c + 8 * h]);
-            multiply(k, q[0][c], q[1][c], q[2][c], st);
+            u32x4 third;
+            if constexpr (Lds::Q_HERE) third = *reinterpret_cast<const u32x4 *>(q_here + 16 * c);
+            else third = q[2][c];
+            multiply(k, q[0][c], q[1][c], third, st);
         }
     };
 
