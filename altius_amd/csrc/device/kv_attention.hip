@@ -345,8 +345,22 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             }
         }
     };
-    // Keys behind the last that is seen have no page: the last one stands in for them.
-    auto standing_in = [&](int32_t key) { return (uint32_t)min(key, end - 1); };
+    // Where pages do not hold whole groups: lane l has the row of key l % KT of a tile, looked up a tile ahead of its first use.  Keys
+    // behind the last that is seen have no page: the last one stands in for them.
+    int32_t page_ahead = 0;
+    int64_t rows_next = 0;  // bytes from the start of the cache
+    auto key_ahead = [&](int32_t i) { return (uint32_t)min(tile_key(i) + (int32_t)(lane % KT), end - 1); };
+    auto look_up = [&](int32_t i) { page_ahead = g.kv.table[(int64_t)s * g.kv.table_stride + g.kv.by_page_size.div(key_ahead(i))]; };
+    auto advance = [&](int32_t i) {  // to tile i, whose pages are known
+        const uint32_t key = key_ahead(i);
+        if ((uint32_t)page_ahead >= g.kv.pages) *g.kv.flag = 1;
+        const int32_t page = (uint32_t)page_ahead < g.kv.pages ? page_ahead : 0;
+        rows_next = ((int64_t)page * g.kv.page_stride + (int64_t)(key - g.kv.by_page_size.div(key) * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
+    };
+    auto row_of = [&](int64_t rows_of_tile, uint32_t key) {
+        const uint32_t low_word = __shfl((int32_t)rows_of_tile, key), high_word = __shfl((int32_t)(rows_of_tile >> 32), key);
+        return (int64_t)((uint64_t)high_word << 32 | low_word);
+    };
     auto half_at = [&](int32_t i, int half) {
         const int32_t page = __builtin_amdgcn_readlane(pages, (HALVES * i + half) & 63);
         const uint32_t key = (uint32_t)tile_key(i) + 16 * half, slot = key - g.kv.by_page_size.div(key) * g.kv.page_size;
@@ -361,11 +375,11 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         } else {
             const char *at[2];
 #pragma unroll
-            for (int h = 0; h < (BF16 ? 2 : 1); h++) at[h] = keys + row_at(standing_in(tile_key(i) + (int32_t)col + 16 * h)) * SIZE + 16 * part;
+            for (int h = 0; h < HALVES; h++) at[h] = keys + row_of(rows_next, col + 16 * h) + 16 * part;
             load_keys_at(t, std::false_type(), [&](int h) { return at[h]; });
         }
     };
-    auto load_values = [&](int32_t i, RowValues<DP, BF16> &t) {
+    auto load_values = [&](int32_t i, RowValues<DP, BF16> &t, int64_t rows_of_tile) {
         if constexpr (UNIFORM) {
             const char *base[2] = {values + half_at(i, 0), values + half_at(i, HALVES - 1)};
             auto at = [&](int r) { return base[r / 4] + (uint64_t)(r % 4) * slot_bytes + v_off; };
@@ -374,7 +388,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         } else {
             const char *at[VROWS];
 #pragma unroll
-            for (int r = 0; r < VROWS; r++) at[r] = values + row_at(standing_in(tile_key(i) + (int32_t)value_key(r))) * SIZE + (BF16 ? (DP / 16) * SIZE : 16) * col;
+            for (int r = 0; r < VROWS; r++) at[r] = values + row_of(rows_of_tile, value_key(r)) + (BF16 ? (DP / 16) * SIZE : 16) * col;
             load_values_at(t, std::false_type(), [&](int r) { return at[r]; });
         }
     };
@@ -493,14 +507,19 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     RowKeys<DP, BF16> a, b;
     RowValues<DP, BF16> v;
     auto step = [&](int32_t i, const RowKeys<DP, BF16> &now, RowKeys<DP, BF16> &next) {
-        load_values(i, v);
+        load_values(i, v, rows_next);
         if (i + 1 < mine) {
-            if (((i + 1) & (64 / HALVES - 1)) == 0) fetch_pages(i + 1);
+            if (!UNIFORM) advance(i + 1);
+            else if (((i + 1) & (64 / HALVES - 1)) == 0) fetch_pages(i + 1);
             load_keys(i + 1, next);
+            if (!UNIFORM) look_up(min(i + 2, mine - 1));
         }
         products(i, now, v);
     };
-    if (mine > 0) load_keys(0, a);
+    if (mine > 0) {
+        if (!UNIFORM) look_up(0), advance(0), look_up(min(1, mine - 1));
+        load_keys(0, a);
+    }
     for (int32_t i = 0; i < mine; i += 2) {
         step(i, a, b);
         if (i + 1 < mine) step(i + 1, b, a);
@@ -713,25 +732,39 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         }
         return t;
     };
-    auto stand_in = [&](int32_t key) { return row_at((uint32_t)min(key, end - 1)) * SIZE; };  // for keys behind the last that is seen
-    auto fetch_keys = [&](int32_t i, const Halves &half) {
-        const int32_t key0 = (first + i) * TILE_KEYS;
+    // Where they do not: lane l has the row of key l % 32 of a tile, looked up a tile ahead of its first use.  Keys behind the last that
+    // is seen have no page: the last one stands in for them.
+    int32_t page_ahead = 0;
+    int64_t rows_next = 0, rows_ahead = 0;  // bytes from the start of the cache, of tiles i + 1 and i + 2 while tile i is computed
+    auto key_ahead = [&](int32_t i) { return (uint32_t)min((first + i) * TILE_KEYS + (int32_t)col, end - 1); };
+    auto look_up = [&](int32_t i) { page_ahead = g.kv.table[(int64_t)s * g.kv.table_stride + g.kv.by_page_size.div(key_ahead(i))]; };
+    auto advance = [&](int32_t i) {  // to tile i, whose pages are known
+        const uint32_t key = key_ahead(i);
+        if ((uint32_t)page_ahead >= g.kv.pages) *g.kv.flag = 1;
+        const int32_t page = (uint32_t)page_ahead < g.kv.pages ? page_ahead : 0;
+        rows_next = rows_ahead;
+        rows_ahead = ((int64_t)page * g.kv.page_stride + (int64_t)(key - g.kv.by_page_size.div(key) * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
+    };
+    auto row_of = [&](int64_t rows_of_tile, uint32_t key) {
+        const uint32_t low_word = __shfl((int32_t)rows_of_tile, key), high_word = __shfl((int32_t)(rows_of_tile >> 32), key);
+        return (int64_t)((uint64_t)high_word << 32 | low_word);
+    };
+    auto fetch_keys = [&](const Halves &half) {
 #pragma unroll
         for (int e = 0; e < K_EACH; e++) {
             const char *p;
-            if constexpr (!UNIFORM) p = keys + stand_in(key0 + (int32_t)k_key(e)) + k_byte(e);
+            if constexpr (!UNIFORM) p = keys + row_of(rows_ahead, k_key(e)) + k_byte(e);
             else if constexpr (EVEN && K_ROWS <= 16) p = keys + half.at[e * K_ROWS / 16] + (uint64_t)(e * K_ROWS % 16) * slot_bytes + k_off;
             else if constexpr (EVEN) p = keys + (k_key(e) < 16 ? half.at[0] : half.at[1]) + k_off;
             else p = keys + (k_key(e) < 16 ? half.at[0] : half.at[1]) + (k_key(e) % 16 * slot_bytes + k_byte(e));
             k_stage[e] = *reinterpret_cast<const u32x4 *>(p);
         }
     };
-    auto fetch_values = [&](int32_t i, const Halves &half) {
-        const int32_t key0 = (first + i) * TILE_KEYS;
+    auto fetch_values = [&](const Halves &half, int64_t rows_of_tile) {
         const char *base = values + (v_block < 4 ? half.at[0] : half.at[1]) + v_off;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const char *p = UNIFORM ? base + (uint64_t)e * slot_bytes : values + stand_in(key0 + 4 * (int32_t)v_block + e) + v_byte;
+            const char *p = UNIFORM ? base + (uint64_t)e * slot_bytes : values + row_of(rows_of_tile, 4 * v_block + e) + v_byte;
             if constexpr (V_WORDS == 1) v_stage[e][0] = *reinterpret_cast<const uint32_t *>(p);
             else v_stage[e] = *reinterpret_cast<const VWords *>(p);
         }
@@ -784,10 +817,11 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     // The first tile's keys and values and the second's keys, while the queries are split.
     Halves next = {};  // of the tile whose values are fetched next: its keys were a tile ago
     if (tiles > 0) {
-        fetch_starts(0);
-        next = halves_of(0);
-        fetch_keys(0, next), fetch_values(0, next);
-        next = halves_of(1);
+        if (UNIFORM) fetch_starts(0), next = halves_of(0);
+        else look_up(0), advance(0), look_up(min(1, tiles - 1));
+        fetch_keys(next), fetch_values(next, rows_ahead);
+        if (UNIFORM) next = halves_of(1);
+        else advance(min(1, tiles - 1)), look_up(min(2, tiles - 1));
     }
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
     u32x4 q[Lds::Q_HERE ? 2 : 3][STEPS];
@@ -851,7 +885,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         clear_unseen(0);
         park_keys(0), park_values(0);
         if (tiles > 1) {
-            fetch_keys(1, next);
+            fetch_keys(next);
             park_keys(1);
         }
         __syncthreads();
@@ -865,10 +899,16 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         const int32_t key0 = (first + i) * TILE_KEYS;
         // Tiles i + 2 and i + 1; behind the last one it is fetched again, and not read.
         const int32_t ahead = min(i + 2, tiles - 1);
-        fetch_values(min(i + 1, tiles - 1), next);
-        if ((ahead & 31) == 0) fetch_starts(ahead);
-        next = halves_of(ahead);
-        fetch_keys(ahead, next);
+        if (UNIFORM) {
+            fetch_values(next, 0);
+            if ((ahead & 31) == 0) fetch_starts(ahead);
+            next = halves_of(ahead);
+        } else {
+            advance(ahead);
+            fetch_values(next, rows_next);
+            look_up(min(i + 3, tiles - 1));
+        }
+        fetch_keys(next);
         if (i >= mine_from && i < mine_to) {
             float x[16];
 #pragma unroll
@@ -1105,8 +1145,9 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     share(p.few, std::min(rows, FEW_ROWS), 16, 4 * cus, std::max<uint64_t>(64, 256 * 1024 / key_bytes));
     if (rows > FEW_ROWS) {
         if (cache.head_size <= TILE_CHANNELS) {
-            // Two blocks of 128 rows are at work on a CU.
-            share(p.many, rows, TILE_ROWS, 2 * cus, 512);
+            // So many blocks are at work at once.  Fewer of them are cut until there are two rounds.
+            const uint64_t at_once = cus * (cache.elem == AHIP_KV_BF16 || cache.head_size <= 64 ? 2 : 1), blocks = std::max<uint64_t>(1, pairs * ((rows + TILE_ROWS - 1) / TILE_ROWS));
+            share(p.many, rows, TILE_ROWS, blocks < at_once / 2 ? 2 * at_once + blocks - 1 : 1, 256);
         } else {
             share(p.many, rows, 16, 1, 1);
         }
