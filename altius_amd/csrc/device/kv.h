@@ -39,29 +39,52 @@ struct KvView {
 struct KvSequence {
     int32_t start, n, length;
 };
-__device__ __forceinline__ KvSequence kv_sequence(const KvView &kv, uint32_t s) {
+__device__ __forceinline__ KvSequence kv_checked(const KvView &kv, int32_t start, int32_t next, int32_t length) {
     KvSequence q;
-    q.start = kv.starts[s];
-    const int64_t n = (int64_t)kv.starts[s + 1] - q.start;
-    q.length = kv.lengths[s];
-    const bool fits = q.start >= 0 && n >= 0 && q.start + n <= (int64_t)kv.tokens && q.length >= 0 &&
-                      (uint64_t)q.length <= (uint64_t)kv.table_pages * kv.page_size;
+    q.start = start;
+    q.length = length;
+    const int64_t n = (int64_t)next - start;
+    const bool fits = start >= 0 && n >= 0 && start + n <= (int64_t)kv.tokens && length >= 0 && (uint64_t)length <= (uint64_t)kv.table_pages * kv.page_size;
     if (!fits) *kv.flag = 1;
     q.n = fits ? (int32_t)n : 0;
     return q;
 }
+__device__ __forceinline__ KvSequence kv_sequence(const KvView &kv, uint32_t s) { return kv_checked(kv, kv.starts[s], kv.starts[s + 1], kv.lengths[s]); }
 
-// The sequence that row `token` belongs to, kv.sequences if it is behind the last one's.  Most calls that matter for their
-// latency have one row per sequence, so that guess is tried before a search.
-__device__ __forceinline__ uint32_t kv_sequence_of(const KvView &kv, uint32_t token) {
+// The sequence that row `token` belongs to, kv.sequences if it is behind the last one's, and what there is to know of it.  For whole
+// wavefronts: up to 64 sequences are read at once, a lane each.  More are searched, one row per sequence first, then by cutting the range
+// in eight with loads that do not wait for each other.
+__device__ __forceinline__ uint32_t kv_sequence_of(const KvView &kv, uint32_t token, KvSequence &q) {
     const int32_t t = (int32_t)token;
-    if (token < kv.sequences && kv.starts[token] <= t && t < kv.starts[token + 1]) return token;
-    uint32_t low = 0, high = kv.sequences;  // how many of starts[1 ..] are <= t
-    while (low < high) {
-        const uint32_t mid = (low + high) >> 1;
-        if (kv.starts[mid + 1] <= t) low = mid + 1;
-        else high = mid;
+    if (kv.sequences <= 64) {
+        const uint32_t lane = threadIdx.x & 63u;
+        const int32_t first = kv.starts[0], next = lane < kv.sequences ? kv.starts[lane + 1] : INT32_MAX, length = lane < kv.sequences ? kv.lengths[lane] : 0;
+        uint32_t s = 0;
+        for (uint64_t left = ~(uint64_t)0; left;) {  // each row of the wavefront in turn
+            const int32_t one = __builtin_amdgcn_readlane(t, __builtin_ctzll(left));
+            const uint32_t before = (uint32_t)__popcll(__ballot(next <= one));
+            const bool mine = t == one;
+            if (mine) s = before;
+            left &= ~__ballot(mine);
+        }
+        const int32_t before = __shfl(next, (int)s - 1), behind = __shfl(next, (int)s), its_length = __shfl(length, (int)s);
+        if (s < kv.sequences) q = kv_checked(kv, s ? before : first, behind, its_length);
+        return s;
     }
+    uint32_t low = 0, high = kv.sequences;  // how many of starts[1 ..] are <= t: low to high
+    if (token < kv.sequences && kv.starts[token] <= t && t < kv.starts[token + 1]) low = high = token;
+    while (low < high) {
+        const uint32_t step = (high - low + 7) / 8;
+        uint32_t below = 0;
+#pragma unroll
+        for (uint32_t i = 1; i <= 7; i++) {
+            const uint32_t at = low + i * step, in = at <= high ? at : high;
+            below += at <= high && kv.starts[in] <= t ? 1u : 0u;
+        }
+        low += below * step;
+        if (below < 7 && low + step - 1 < high) high = low + step - 1;
+    }
+    if (low < kv.sequences) q = kv_sequence(kv, low);
     return low;
 }
 

@@ -18,6 +18,9 @@ namespace altius {
 
 namespace {
 
+using dev::FastDiv;
+using dev::make_fastdiv;
+
 constexpr int BLOCK = 256;
 
 struct RowsOf {  // rows at base + token * token_stride + head * head_stride (+ batch * batch_stride)
@@ -33,9 +36,11 @@ struct RotateArgs {
     uint32_t heads;       // ends[2]
     uint32_t tokens, batch;
     uint32_t d, dim;      // channels of a row, of which the first dim turn
-    uint32_t lanes_log2;  // of lanes per row
-    uint32_t heads_log2;  // of head groups per block
     uint32_t interleaved;
+    // Threads are lanes of rows, `threads` of them; rows of one lane group lie `groups` heads apart.  Which comes next after the lane:
+    // the group of heads (then the token), or the token (then the group).
+    uint32_t threads, token_next;
+    FastDiv lanes, groups, by_tokens;
     const double *frequencies;
     float magnitude, epsilon;
     const void *positions;
@@ -48,9 +53,10 @@ struct RotateArgs {
 // |r| <= pi / 4: r^11 / 11! = 1.8e-9, r^12 / 12! = 1.1e-10.
 __device__ __forceinline__ void turn(double position, double frequency, float magnitude, float &cos_out, float &sin_out) {
     const double quarters = position * frequency * 0.63661977236758134308;  // 2 / pi
-    const double whole = rint(quarters);
-    const float r = (float)((quarters - whole) * 1.57079632679489661923);
-    const uint32_t quadrant = (uint32_t)(int64_t)whole & 3u;
+    // A sum beyond 2^52 is whole, its lowest bits are the quarter turns.
+    const double shifted = quarters + 6755399441055744.0;  // 1.5 x 2^52
+    const float r = (float)((quarters - (shifted - 6755399441055744.0)) * 1.57079632679489661923);
+    const uint32_t quadrant = (uint32_t)__double2loint(shifted);
     const float r2 = r * r;
     float s = __builtin_fmaf(r2, 2.75573192e-6f, -1.98412698e-4f);
     s = __builtin_fmaf(s, r2, 8.33333333e-3f);
@@ -85,7 +91,7 @@ template <bool BF16> __device__ __forceinline__ void cache_store1(void *base, in
     else static_cast<float *>(base)[at] = v;
 }
 
-// Where a token's row goes in the cache (elements), and whether it goes anywhere.
+// Where a token's row goes in the cache (elements), and whether it goes anywhere.  For whole wavefronts.
 struct Slot {
     int64_t at;
     bool live;
@@ -93,9 +99,9 @@ struct Slot {
 __device__ __forceinline__ Slot slot_of(const dev::KvView &kv, uint32_t token, int64_t &place) {
     Slot slot = {0, false};
     place = 0;
-    const uint32_t s = dev::kv_sequence_of(kv, token);
+    dev::KvSequence q = {};
+    const uint32_t s = dev::kv_sequence_of(kv, token, q);
     if (s >= kv.sequences) return slot;  // padding behind the last sequence
-    const dev::KvSequence q = dev::kv_sequence(kv, s);
     const int64_t p = (int64_t)q.length - q.n + ((int64_t)token - q.start);
     if (q.n == 0 || (int64_t)token < q.start || (int64_t)token >= (int64_t)q.start + q.n || p < 0) {  // starts out of order, or shorter than its rows
         *kv.flag = 1;
@@ -110,17 +116,26 @@ __device__ __forceinline__ Slot slot_of(const dev::KvView &kv, uint32_t token, i
     return slot;
 }
 
+// One of three arguments by selection: indexing them would read them from memory in front of every address.
+#define ALTIUS_ROWS_FIELD(which, field) ((which) == 0 ? g.rows[0].field : (which) == 1 ? g.rows[1].field : g.rows[2].field)
+
 // Eight channels a lane, in two float4 A and B: the two halves' channels (4 u, dim / 2 + 4 u) of the part that turns where
-// halves turn together, neighbours (8 u, 8 u + 4) otherwise; a row is 2^lanes_log2 lanes, a block 2^heads_log2 groups of heads
-// of one token or several tokens.  N heads of its token per lane, all loads in front of the first use.
+// halves turn together, neighbours (8 u, 8 u + 4) otherwise.  N heads of its token per lane, all loads in front of the first use.
+// Rows that are normed have a power of two of lanes, which add up their squares; others exactly as many as they need.
 template <int N, bool CACHE, bool BF16>
 __global__ __launch_bounds__(BLOCK) void rotate_rows_vec4(RotateArgs g) {
-    const uint32_t lane = threadIdx.x & ((1u << g.lanes_log2) - 1), group = threadIdx.x >> g.lanes_log2;
-    const uint32_t first = group & ((1u << g.heads_log2) - 1);
-    const uint32_t per_block = BLOCK >> (g.lanes_log2 + g.heads_log2);
-    const uint32_t item = blockIdx.x * per_block + (group >> g.heads_log2);
-    if (item >= g.tokens * g.batch) return;
-    const uint32_t b = CACHE ? 0 : item / g.tokens, token = CACHE ? item : item - b * g.tokens;
+    const uint32_t mine = blockIdx.x * BLOCK + threadIdx.x, thread = min(mine, g.threads - 1);
+    const uint32_t of = g.lanes.div(thread), lane = thread - of * g.lanes.d;
+    uint32_t group, item;
+    if (g.token_next) {  // of = (batch * groups + group) * tokens + token
+        const uint32_t outer = g.by_tokens.div(of), b = g.groups.div(outer);
+        group = outer - b * g.groups.d;
+        item = b * g.tokens + (of - outer * g.tokens);
+    } else {
+        item = g.groups.div(of);
+        group = of - item * g.groups.d;
+    }
+    const uint32_t b = CACHE ? 0 : g.by_tokens.div(item), token = CACHE ? item : item - b * g.tokens;
 
     const uint32_t half = g.dim / 2;
     const bool split = !g.interleaved && 4 * lane < half;  // this lane's A and B are the halves of a pair
@@ -128,29 +143,28 @@ __global__ __launch_bounds__(BLOCK) void rotate_rows_vec4(RotateArgs g) {
     const uint32_t a_at = offset, b_at = split ? half + offset : offset + 4;
     const bool has_a = a_at < g.d, has_b = b_at < g.d;
 
+    f32x4 a[N], c[N];
+    uint32_t which[N], head[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint32_t h = group + (uint32_t)i * g.groups.d;
+        const bool live = h < g.heads && mine < g.threads;
+        if (!live) h = 0;
+        which[i] = CACHE ? (h >= g.ends[0]) + (h >= g.ends[1]) : 0;
+        head[i] = h - (which[i] ? g.ends[which[i] - 1] : 0);
+        const float *src = ALTIUS_ROWS_FIELD(which[i], src) + (int64_t)b * g.rows[0].src_batch + (int64_t)token * ALTIUS_ROWS_FIELD(which[i], src_token) +
+                           (int64_t)head[i] * ALTIUS_ROWS_FIELD(which[i], src_head);
+        a[i] = c[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (live && has_a) a[i] = *reinterpret_cast<const f32x4 *>(src + a_at);
+        if (live && has_b) c[i] = *reinterpret_cast<const f32x4 *>(src + b_at);
+        if (!live) which[i] = 3;
+    }
+
     int64_t place = (int64_t)g.first_position + token;
     Slot slot = {0, true};
     if (CACHE) {
         slot = slot_of(g.kv, token, place);
         if (!slot.live) return;
-    }
-
-    const float *src[N];
-    f32x4 a[N], c[N];
-    uint32_t which[N], head[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        uint32_t h = blockIdx.y * (N << g.heads_log2) + first + ((uint32_t)i << g.heads_log2);
-        const bool live = h < g.heads;
-        if (!live) h = 0;
-        which[i] = CACHE ? (h >= g.ends[0]) + (h >= g.ends[1]) : 0;
-        head[i] = h - (which[i] ? g.ends[which[i] - 1] : 0);
-        if (!live) which[i] = 3;
-        const RowsOf &r = g.rows[live ? which[i] : 0];
-        src[i] = r.src + (int64_t)b * r.src_batch + (int64_t)token * r.src_token + (int64_t)head[i] * r.src_head;
-        a[i] = c[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (live && has_a) a[i] = *reinterpret_cast<const f32x4 *>(src[i] + a_at);
-        if (live && has_b) c[i] = *reinterpret_cast<const f32x4 *>(src[i] + b_at);
     }
 
     // The angles: of pairs (4 u + j) where halves turn together, of pairs (4 u + j) of neighbours in A and B alike.
@@ -169,17 +183,17 @@ __global__ __launch_bounds__(BLOCK) void rotate_rows_vec4(RotateArgs g) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
         if (which[i] == 3) continue;  // alike in all lanes of a row
-        const RowsOf &r = g.rows[which[i]];
-        if (r.gamma) {
+        const float *gamma = ALTIUS_ROWS_FIELD(which[i], gamma);
+        if (gamma) {
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; j++) sum = __builtin_fmaf(a[i][j], a[i][j], sum);
 #pragma unroll
             for (int j = 0; j < 4; j++) sum = __builtin_fmaf(c[i][j], c[i][j], sum);
-            for (uint32_t m = 1; m < (1u << g.lanes_log2); m <<= 1) sum += __shfl_xor(sum, m);
+            for (uint32_t m = 1; m < g.lanes.d; m <<= 1) sum += __shfl_xor(sum, m);
             const float scale = 1.0f / sqrtf(sum / (float)g.d + g.epsilon);
             const f32x4 ones = {1.0f, 1.0f, 1.0f, 1.0f};
-            const f32x4 ga = has_a ? *reinterpret_cast<const f32x4 *>(r.gamma + a_at) : ones, gb = has_b ? *reinterpret_cast<const f32x4 *>(r.gamma + b_at) : ones;
+            const f32x4 ga = has_a ? *reinterpret_cast<const f32x4 *>(gamma + a_at) : ones, gb = has_b ? *reinterpret_cast<const f32x4 *>(gamma + b_at) : ones;
             a[i] = a[i] * scale * ga;
             c[i] = c[i] * scale * gb;
         }
@@ -210,6 +224,7 @@ __global__ __launch_bounds__(BLOCK) void rotate_rows_vec4(RotateArgs g) {
             if (has_a) cache_store4<BF16>(base, at + a_at, a[i]);
             if (has_b) cache_store4<BF16>(base, at + b_at, c[i]);
         } else {
+            const RowsOf &r = g.rows[0];
             float *dst = r.dst + (int64_t)b * r.dst_batch + (int64_t)token * r.dst_token + (int64_t)head[i] * r.dst_head;
             if (has_a) *reinterpret_cast<f32x4 *>(dst + a_at) = a[i];
             if (has_b) *reinterpret_cast<f32x4 *>(dst + b_at) = c[i];
@@ -267,6 +282,8 @@ uint32_t log2_up(size_t n) {
 bool quads(int64_t stride) { return stride % 4 == 0; }
 bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
+constexpr uint64_t MANY = (uint64_t)1 << 18;
+
 template <bool CACHE, bool BF16> int launch_rotate(DeviceCtx &ctx, const RotateArgs &g, const char *what) {
     // Float4s wherever rows and their parts allow it; a row of up to 512 channels is one lane group of a wavefront.
     bool vec = g.d % 4 == 0 && g.d <= 512 && g.dim % (g.interleaved ? 4 : 8) == 0;
@@ -280,18 +297,25 @@ template <bool CACHE, bool BF16> int launch_rotate(DeviceCtx &ctx, const RotateA
         vec = vec && aligned(g.kv.keys, BF16 ? 8 : 16) && aligned(g.kv.values, BF16 ? 8 : 16) && quads(g.kv.page_stride) && quads(g.kv.head_stride) &&
               quads(g.kv.slot_stride);
     const uint64_t items = (uint64_t)g.tokens * g.batch;
+    const uint32_t units = g.interleaved ? (g.d + 7) / 8 : g.dim / 8 + (g.d - g.dim + 7) / 8;
+    const uint32_t lanes = g.rows[0].gamma || g.rows[1].gamma ? 1u << log2_up(units) : units;
+    const uint64_t work = items * g.heads * lanes;
+    // Two heads a lane where there are threads enough for the whole part all the same.
+    const uint32_t n = work >= MANY ? 2 : 1, groups = (g.heads + n - 1) / n;
+    const uint64_t threads = items * groups * lanes;
+    vec = vec && threads < ((uint64_t)1 << 31);
     if (!vec) {
         hipLaunchKernelGGL((rotate_rows_any<CACHE, BF16>), dim3((uint32_t)items, (g.heads + BLOCK / 64 - 1) / (BLOCK / 64)), dim3(BLOCK), 0, ctx.stream, g);
         return ctx.check(hipGetLastError(), what);
     }
     RotateArgs a = g;
-    const uint32_t units = a.interleaved ? (a.d + 7) / 8 : a.dim / 8 + (a.d - a.dim + 7) / 8;
-    a.lanes_log2 = log2_up(units);
-    const uint32_t n = 1;
-    a.heads_log2 = std::min(log2_up((a.heads + n - 1) / n), log2_up(BLOCK) - a.lanes_log2);
-    const uint32_t per_block = BLOCK >> (a.lanes_log2 + a.heads_log2);
-    const dim3 grid((uint32_t)((items + per_block - 1) / per_block), (a.heads + (n << a.heads_log2) - 1) / (n << a.heads_log2));
-    hipLaunchKernelGGL((rotate_rows_vec4<1, CACHE, BF16>), grid, dim3(BLOCK), 0, ctx.stream, a);
+    a.threads = (uint32_t)threads;
+    // Rows next to each other in memory are next to each other in a block.
+    a.token_next = !CACHE && g.rows[0].src_token < g.rows[0].src_head;
+    a.lanes = make_fastdiv(lanes), a.groups = make_fastdiv(groups), a.by_tokens = make_fastdiv(g.tokens);
+    const dim3 grid((a.threads + BLOCK - 1) / BLOCK);
+    if (n == 2) hipLaunchKernelGGL((rotate_rows_vec4<2, CACHE, BF16>), grid, dim3(BLOCK), 0, ctx.stream, a);
+    else hipLaunchKernelGGL((rotate_rows_vec4<1, CACHE, BF16>), grid, dim3(BLOCK), 0, ctx.stream, a);
     return ctx.check(hipGetLastError(), what);
 }
 
