@@ -25,6 +25,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504088896341f;
@@ -167,38 +168,23 @@ template <bool BF16> __device__ __forceinline__ float cache_value(const void *ba
 // the k slots of its instructions are declared to be keys in that order.  Keys and values go from memory into registers in the
 // layout of the instructions' first operand, without LDS: a row of keys is read along its channels, 16 bytes a lane, a row of
 // values by 16 lanes side by side, each lane's channels being rows of O^T.
-//   fp32 cache: v_mfma_f32_16x16x4_f32, tiles of 16 keys.
-//   bf16 cache: v_mfma_f32_16x16x32_bf16, tiles of 32 keys; q and the weights as three bf16 numbers each, whose sum they are
-//   exactly, so that each of the three products is exact in the fp32 sum; a lane holds 8 keys x DP / 16 channels of
-//   V and turns them with v_perm.
-template <bool BF16> constexpr int KEYS = BF16 ? 32 : 16;
-constexpr int ROW_WAVES = 4;
+//   fp32 cache: v_mfma_f32_16x16x4_f32.
+//   bf16 cache: v_mfma_f32_16x16x32_bf16 over the channels and _16x16x16_bf16 over the keys; q and the weights as three bf16 numbers
+//   each, whose sum they are exactly, so that each of the three products is exact in the fp32 sum; a lane holds 4 keys x DP / 16
+//   channels of V and turns them with v_perm.
+constexpr int ROW_WAVES = 4, ROW_KEYS = 16;
 
-template <int DP, bool BF16> struct RowKeys;
-template <int DP> struct RowKeys<DP, false> {
-    f32x4 k[DP / 16];
-};
-template <int DP> struct RowKeys<DP, true> {
-    u32x4 k[2][DP / 32];
-};
-template <int DP, bool BF16> struct RowValues;
-template <int DP> struct RowValues<DP, false> {
-    f32x4 v[4][DP / 64];
-};
-template <int DP> struct RowValues<DP, true> {
-    uint32_t v[8][DP / 32];
-};
-template <int DP, bool BF16> struct RowQuery;
-template <int DP> struct RowQuery<DP, false> {
-    f32x4 q[DP / 16];
-};
-template <int DP> struct RowQuery<DP, true> {
-    u32x4 q[3][DP / 32];
+template <int DP, bool BF16> struct RowTile {
+    static constexpr int K_UNITS = DP * (BF16 ? 2 : 4) / 64, V_WORDS = DP * (BF16 ? 2 : 4) / 64;  // 16 bytes of keys; words of a row of values
+    u32x4 k[K_UNITS];
+    uint32_t v[4][V_WORDS];
 };
 
 #define ALTIUS_MFMA16_F32(A, B, C) C = __builtin_amdgcn_mfma_f32_16x16x4f32(A, B, C, 0, 0, 0)
 #define ALTIUS_MFMA16_BF16(A, B, C) \
     C = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, A), __builtin_bit_cast(bf16x8, B), C, 0, 0, 0)
+#define ALTIUS_MFMA16_BF16_K16(A, B, C) \
+    C = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, A), __builtin_bit_cast(s16x4, B), C, 0, 0, 0)
 
 // Row of O^T (channel) of accumulator i, register r, in lane group `part` = lane / 16.
 template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int i, int r, uint32_t part) {
@@ -214,7 +200,7 @@ template <int DP> struct RowLds {
 
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
 __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP> &lds) {
-    constexpr int KT = KEYS<BF16>, NACC = DP / 16, PITCH = RowLds<DP>::PITCH;
+    constexpr int KT = ROW_KEYS, NACC = DP / 16, PITCH = RowLds<DP>::PITCH;
     auto &sums = lds.sums;
     auto &stats = lds.stats;
     const Share &share = SPLIT ? g.few : g.many;
@@ -254,7 +240,8 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     constexpr int SIZE = BF16 ? 2 : 4;
     const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
 
-    RowQuery<DP, BF16> q;
+    // fp32: channels 16 i + 4 part on; bf16: parts of channels 32 i + 8 part on.
+    u32x4 q[BF16 ? 3 : 1][BF16 ? DP / 32 : DP / 16];
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
     if constexpr (BF16) {
 #pragma unroll
@@ -262,151 +249,115 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             const uint32_t c = 32 * i + 8 * part;
             f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
             if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale, hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4) * g.scale;
-            uint32_t h[3][4];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                split_pair(lo[2 * e], lo[2 * e + 1], h[0][e], h[1][e], h[2][e]);
-                split_pair(hi[2 * e], hi[2 * e + 1], h[0][2 + e], h[1][2 + e], h[2][2 + e]);
+                uint32_t w[3];
+                split_pair(lo[2 * e], lo[2 * e + 1], w[0], w[1], w[2]);
+                q[0][i][e] = w[0], q[1][i][e] = w[1], q[2][i][e] = w[2];
+                split_pair(hi[2 * e], hi[2 * e + 1], w[0], w[1], w[2]);
+                q[0][i][2 + e] = w[0], q[1][i][2 + e] = w[1], q[2][i][2 + e] = w[2];
             }
-#pragma unroll
-            for (int p = 0; p < 3; p++) q.q[p][i] = u32x4{h[p][0], h[p][1], h[p][2], h[p][3]};
         }
     } else {
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) {
             const uint32_t c = 16 * i + 4 * part;
-            q.q[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (valid && c < g.d) q.q[i] = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (valid && c < g.d) x = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
+            q[0][i] = __builtin_bit_cast(u32x4, x);
         }
     }
 
-    // Wavefront w takes tiles w, w + 4, ... of the block's; the pages of its next 64 groups of 16 keys wait in one register.
-    constexpr int HALVES = KT / 16;
+    // Wavefront w takes tiles w, w + 4, ... of the block's.
     const int32_t mine = tiles > (int32_t)wave ? (tiles - (int32_t)wave + ROW_WAVES - 1) / ROW_WAVES : 0;
-    int32_t pages = 0;
-    auto fetch_pages = [&](int32_t from) {
-        const int32_t i = from + (int32_t)lane / HALVES, key = (first + (int32_t)wave + i * ROW_WAVES) * KT + 16 * (int32_t)(lane % HALVES);
-        pages = 0;
-        if (UNIFORM && i < mine && key < end) pages = g.kv.page_of(s, g.kv.by_page_size.div((uint32_t)key), 0);
-    };
     auto tile_key = [&](int32_t i) { return (first + (int32_t)wave + i * ROW_WAVES) * KT; };
     auto row_at = [&](uint32_t key) {  // elements from the start of the cache
         const uint32_t index = g.kv.by_page_size.div(key);
         return (int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
     };
-    // Which key of its tile a lane's i-th row of values is, and (bf16) that of its rows of keys in half t.
-    auto value_key = [&](int i) { return BF16 ? 16 * (i / 4) + 4 * part + i % 4 : 4 * part + i; };
-    constexpr int VROWS = BF16 ? 8 : 4;
-
-    // 16 keys of one page start at one address for the whole wavefront, and a lane's parts lie at fixed distances from
-    // it (below 2^31 bytes, or the call takes the other kernel).
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
-    const uint32_t k_off = col * slot_bytes + 16 * part, v_off = 4 * part * slot_bytes + (BF16 ? (DP / 16) * SIZE : 16) * col;
-    // at(h): where the lane's row of keys (in half h of the tile) or its h-th row of values starts.
-    auto load_keys_at = [&](RowKeys<DP, BF16> &t, auto whole, auto at) {
-        constexpr bool WHOLE = decltype(whole)::value;
-        if constexpr (BF16) {
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int c = 0; c < DP / 32; c++) {
-                    t.k[h][c] = u32x4{0, 0, 0, 0};
-                    if (WHOLE || 32 * c + 8 * part < g.d) t.k[h][c] = *reinterpret_cast<const u32x4 *>(at(h) + 64 * c);
-                }
-        } else {
-#pragma unroll
-            for (int c = 0; c < DP / 16; c++) {
-                t.k[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (WHOLE || 16 * c + 4 * part < g.d) t.k[c] = *reinterpret_cast<const f32x4 *>(at(0) + 64 * c);
-            }
-        }
+    // Where pages hold whole tiles: where the wavefront's next 64 tiles start, in bytes from the start of the cache, a tile a lane.  A
+    // tile then starts at one address for all lanes, whose parts lie at fixed distances from it (below 2^31 bytes, or the call takes the
+    // other kernel).
+    int64_t starts = 0;
+    auto fetch_starts = [&](int32_t from) {
+        const int32_t i = from + (int32_t)lane;
+        const uint32_t key = (uint32_t)tile_key(i < mine ? i : mine - 1), index = g.kv.by_page_size.div(key);
+        starts = ((int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
     };
-    auto load_values_at = [&](RowValues<DP, BF16> &t, auto whole, auto at) {
-        constexpr bool WHOLE = decltype(whole)::value;
-#pragma unroll
-        for (int r = 0; r < VROWS; r++) {
-            if constexpr (!BF16) {
-#pragma unroll
-                for (int j = 0; j < DP / 64; j++) {
-                    t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (WHOLE || 64 * j + 4 * col < g.d) t.v[r][j] = *reinterpret_cast<const f32x4 *>(at(r) + 256 * j);
-                }
-            } else if constexpr (DP == 64) {
-                u32x2 x = {0, 0};
-                if (WHOLE || 4 * col < g.d) x = *reinterpret_cast<const u32x2 *>(at(r));
-                t.v[r][0] = x.x, t.v[r][1] = x.y;
-            } else {
-#pragma unroll
-                for (int w = 0; w < DP / 128; w++) {
-                    u32x4 x = {0, 0, 0, 0};
-                    if (WHOLE || (DP / 16) * col + 8 * w < g.d) x = *reinterpret_cast<const u32x4 *>(at(r) + 16 * w);
-                    t.v[r][4 * w] = x.x, t.v[r][4 * w + 1] = x.y, t.v[r][4 * w + 2] = x.z, t.v[r][4 * w + 3] = x.w;
-                }
-            }
-        }
-    };
-    // Where pages do not hold whole groups: lane l has the row of key l % KT of a tile, looked up a tile ahead of its first use.  Keys
-    // behind the last that is seen have no page: the last one stands in for them.
+    // Where they do not: lane l has the row of key l % 16 of a tile, looked up a tile ahead of its use.  Keys behind the last that is
+    // seen have no page: the last one stands in for them.
     int32_t page_ahead = 0;
-    int64_t rows_next = 0;  // bytes from the start of the cache
-    auto key_ahead = [&](int32_t i) { return (uint32_t)min(tile_key(i) + (int32_t)(lane % KT), end - 1); };
+    auto key_ahead = [&](int32_t i) { return (uint32_t)min(tile_key(i) + (int32_t)col, end - 1); };
     auto look_up = [&](int32_t i) { page_ahead = g.kv.table[(int64_t)s * g.kv.table_stride + g.kv.by_page_size.div(key_ahead(i))]; };
-    auto advance = [&](int32_t i) {  // to tile i, whose pages are known
+    auto row_ahead = [&](int32_t i) {  // of tile i, whose pages are known
         const uint32_t key = key_ahead(i);
         if ((uint32_t)page_ahead >= g.kv.pages) *g.kv.flag = 1;
         const int32_t page = (uint32_t)page_ahead < g.kv.pages ? page_ahead : 0;
-        rows_next = ((int64_t)page * g.kv.page_stride + (int64_t)(key - g.kv.by_page_size.div(key) * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
+        return ((int64_t)page * g.kv.page_stride + (int64_t)(key - g.kv.by_page_size.div(key) * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
     };
-    auto row_of = [&](int64_t rows_of_tile, uint32_t key) {
-        const uint32_t low_word = __shfl((int32_t)rows_of_tile, key), high_word = __shfl((int32_t)(rows_of_tile >> 32), key);
-        return (int64_t)((uint64_t)high_word << 32 | low_word);
-    };
-    auto half_at = [&](int32_t i, int half) {
-        const int32_t page = __builtin_amdgcn_readlane(pages, (HALVES * i + half) & 63);
-        const uint32_t key = (uint32_t)tile_key(i) + 16 * half, slot = key - g.kv.by_page_size.div(key) * g.kv.page_size;
-        return ((int64_t)page * g.kv.page_stride + (int64_t)slot * g.kv.slot_stride + head_at) * SIZE;
-    };
-    auto load_keys = [&](int32_t i, RowKeys<DP, BF16> &t) {
-        if constexpr (UNIFORM) {
-            const char *base[2] = {keys + half_at(i, 0), keys + half_at(i, HALVES - 1)};
-            auto at = [&](int h) { return base[h] + k_off; };
-            if (g.d == DP) load_keys_at(t, std::true_type(), at);
-            else load_keys_at(t, std::false_type(), at);
-        } else {
-            const char *at[2];
+
+    // A lane's parts of a tile: of row `col` of the keys 16 bytes at 64 c + 16 part; of row 4 part + r of the values, fp32: 16 bytes at
+    // 256 j + 16 col, bf16: DP / 8 bytes.  No load depends on a condition, which would have the compiler wait for those before it:
+    // channels that a head does not have are read as others (their queries are 0, their sums go nowhere).
+    typedef RowTile<DP, BF16> Tile;
+    const uint32_t row_bytes = g.d * SIZE;
+    constexpr uint32_t V_STEP = BF16 ? DP / 8 : 16;
+    auto load_parts = [&](Tile &t, auto whole, const char *k_row, auto v_row) {
+        constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-            for (int h = 0; h < HALVES; h++) at[h] = keys + row_of(rows_next, col + 16 * h) + 16 * part;
-            load_keys_at(t, std::false_type(), [&](int h) { return at[h]; });
+        for (int c = 0; c < Tile::K_UNITS; c++) {
+            if (WHOLE) t.k[c] = *reinterpret_cast<const u32x4 *>(k_row + 64 * c);
+            else t.k[c] = *reinterpret_cast<const u32x4 *>(k_row + (64 * c + 16 * part < row_bytes ? 64 * c : 0));
         }
-    };
-    auto load_values = [&](int32_t i, RowValues<DP, BF16> &t, int64_t rows_of_tile) {
-        if constexpr (UNIFORM) {
-            const char *base[2] = {values + half_at(i, 0), values + half_at(i, HALVES - 1)};
-            auto at = [&](int r) { return base[r / 4] + (uint64_t)(r % 4) * slot_bytes + v_off; };
-            if (g.d == DP) load_values_at(t, std::true_type(), at);
-            else load_values_at(t, std::false_type(), at);
-        } else {
-            const char *at[VROWS];
 #pragma unroll
-            for (int r = 0; r < VROWS; r++) at[r] = values + row_of(rows_of_tile, value_key(r)) + (BF16 ? (DP / 16) * SIZE : 16) * col;
-            load_values_at(t, std::false_type(), [&](int r) { return at[r]; });
-        }
-    };
-    // Slots that no row sees may hold anything: their weight is 0, so is their value then.
-    auto clear_unseen = [&](int32_t key0, RowValues<DP, BF16> &t) {
-        if (key0 >= begin && key0 + KT <= end) return;
+        for (int r = 0; r < 4; r++) {
+            const char *p = v_row(r);
+            if constexpr (BF16 && DP == 64) {
+                const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+                t.v[r][0] = x.x, t.v[r][1] = x.y;
+            } else {
+                constexpr uint32_t APART = BF16 ? 16 : 256;
 #pragma unroll
-        for (int r = 0; r < VROWS; r++) {
-            const int32_t key = key0 + (int32_t)value_key(r);
-            if (key < begin || key >= end) {
-                if constexpr (BF16) {
+                for (int w = 0; w < Tile::V_WORDS / 4; w++) {
+                    const char *at = p + (WHOLE || APART * w + V_STEP * col < row_bytes ? APART * w : 0);
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
 #pragma unroll
-                    for (int w = 0; w < DP / 32; w++) t.v[r][w] = 0;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < DP / 64; j++) t.v[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int e = 0; e < 4; e++) t.v[r][4 * w + e] = x[e];
                 }
             }
+        }
+    };
+    // Lanes without channels of their own read the first ones.
+    const uint32_t k_byte = 16 * part < row_bytes ? 16 * part : 0, v_byte = V_STEP * col < row_bytes ? V_STEP * col : 0;
+    const uint32_t k_off = col * slot_bytes + k_byte, v_off = 4 * part * slot_bytes + v_byte;
+    auto load = [&](int32_t i, Tile &t) {
+        if constexpr (UNIFORM) {
+            const uint32_t low_word = __builtin_amdgcn_readlane((int32_t)starts, i & 63), high_word = __builtin_amdgcn_readlane((int32_t)(starts >> 32), i & 63);
+            const int64_t start = (int64_t)((uint64_t)high_word << 32 | low_word);
+            const char *k_tile = keys + start, *v_tile = values + start;
+            auto v_row = [&](int r) { return v_tile + (uint64_t)r * slot_bytes + v_off; };
+            if (g.d == DP) load_parts(t, std::true_type(), k_tile + k_off, v_row);
+            else load_parts(t, std::false_type(), k_tile + k_off, v_row);
+        } else {
+            const int64_t row = row_ahead(i);
+            auto v_row = [&](int r) {
+                const uint32_t low_word = __shfl((int32_t)row, 4 * part + r), high_word = __shfl((int32_t)(row >> 32), 4 * part + r);
+                return values + (int64_t)((uint64_t)high_word << 32 | low_word) + v_byte;
+            };
+            load_parts(t, std::false_type(), keys + row + k_byte, v_row);
+        }
+    };
+    auto value_key = [&](int r) { return 4 * (int32_t)part + r; };
+    // Slots that no row sees may hold anything: their weight is 0, so is their value then.
+    auto clear_unseen = [&](int32_t key0, Tile &t) {
+        if (key0 >= begin && key0 + KT <= end) return;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int32_t key = key0 + value_key(r);
+            const bool seen = key >= begin && key < end;
+#pragma unroll
+            for (int w = 0; w < Tile::V_WORDS; w++) t.v[r][w] = seen ? t.v[r][w] : 0;
         }
     };
 
@@ -416,14 +367,14 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     for (int i = 0; i < NACC; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     // Scores of the tile (NS registers a lane, key0 + value_key(r)), running maximum and sum, weights in their place.
-    constexpr int NS = VROWS;
+    constexpr int NS = 4;
     auto weigh = [&](int32_t key0, float (&x)[NS]) {
         const bool full = key0 >= all_low && key0 + KT <= all_high && key0 >= begin && key0 + KT <= end;
         scores(g, x, slope, place - key0, value_key);
         float most = -INFINITY;
 #pragma unroll
         for (int r = 0; r < NS; r++) {
-            const int32_t key = key0 + (int32_t)value_key(r);
+            const int32_t key = key0 + value_key(r);
             if (full || (key >= low && key < high && key >= begin && key < end)) most = fmaxf(most, x[r]);
         }
         most = fmaxf(most, __shfl_xor(most, 16));
@@ -439,90 +390,78 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int r = 0; r < NS; r++) {
-            const int32_t key = key0 + (int32_t)value_key(r);
+            const int32_t key = key0 + value_key(r);
             const bool seen = full || (key >= low && key < high && key >= begin && key < end);
             x[r] = seen ? exp2_fast(x[r] - base) : 0.0f;
             total += x[r];
         }
     };
 
-    auto products = [&](int32_t i, const RowKeys<DP, BF16> &t, RowValues<DP, BF16> &u) {
+    auto products = [&](int32_t i, Tile &t) {
         const int32_t key0 = tile_key(i);
         float x[NS];
-        if constexpr (BF16) {
+        f32x4 large = {0.0f, 0.0f, 0.0f, 0.0f}, small = large;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                f32x4 large = {0.0f, 0.0f, 0.0f, 0.0f}, small = large;
+        for (int c = 0; c < Tile::K_UNITS; c++) {
+            if constexpr (BF16) {
+                ALTIUS_MFMA16_BF16(t.k[c], q[2][c], small);
+                ALTIUS_MFMA16_BF16(t.k[c], q[0][c], large);
+                ALTIUS_MFMA16_BF16(t.k[c], q[1][c], small);
+            } else {
 #pragma unroll
-                for (int c = 0; c < DP / 32; c++) {
-                    ALTIUS_MFMA16_BF16(t.k[h][c], q.q[2][c], small);
-                    ALTIUS_MFMA16_BF16(t.k[h][c], q.q[0][c], large);
-                    ALTIUS_MFMA16_BF16(t.k[h][c], q.q[1][c], small);
+                for (int e = 0; e < 4; e++) {
+                    if (c % 2 == 0) ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[0][c][e]), large);
+                    else ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[0][c][e]), small);
                 }
-#pragma unroll
-                for (int r = 0; r < 4; r++) x[4 * h + r] = large[r] + small[r];
             }
-            weigh(key0, x);
-            clear_unseen(key0, u);
-            u32x4 p[3];
+        }
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
+        for (int r = 0; r < 4; r++) x[r] = large[r] + small[r];
+        weigh(key0, x);
+        clear_unseen(key0, t);
+        if constexpr (BF16) {
+            u32x2 p[3];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
                 uint32_t w[3];
                 split_pair(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
                 p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
             }
 #pragma unroll
             for (int c = 0; c < NACC; c++) {
-                u32x4 v;
+                const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
+                const u32x2 v = {__builtin_amdgcn_perm(t.v[1][c / 2], t.v[0][c / 2], pick), __builtin_amdgcn_perm(t.v[3][c / 2], t.v[2][c / 2], pick)};
 #pragma unroll
-                for (int m = 0; m < 4; m++) v[m] = __builtin_amdgcn_perm(u.v[2 * m + 1][c / 2], u.v[2 * m][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                for (int e = 2; e >= 0; e--) ALTIUS_MFMA16_BF16(v, p[e], acc[c]);
+                for (int e = 2; e >= 0; e--) ALTIUS_MFMA16_BF16_K16(v, p[e], acc[c]);
             }
         } else {
-            f32x4 even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;
-#pragma unroll
-            for (int c = 0; c < DP / 16; c += 2) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    ALTIUS_MFMA16_F32(t.k[c][e], q.q[c][e], even);
-                    ALTIUS_MFMA16_F32(t.k[c + 1][e], q.q[c + 1][e], odd);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) x[r] = even[r] + odd[r];
-            weigh(key0, x);
-            clear_unseen(key0, u);
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int j = 0; j < DP / 64; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) ALTIUS_MFMA16_F32(u.v[r][j][e], x[r], acc[4 * j + e]);
+                for (int w = 0; w < Tile::V_WORDS; w++) ALTIUS_MFMA16_F32(__uint_as_float(t.v[r][w]), x[r], acc[w]);
         }
     };
 
-    // The next tile's keys are on their way during a tile's products, its values during the first of them.
-    fetch_pages(0);
-    RowKeys<DP, BF16> a, b;
-    RowValues<DP, BF16> v;
-    auto step = [&](int32_t i, const RowKeys<DP, BF16> &now, RowKeys<DP, BF16> &next) {
-        load_values(i, v, rows_next);
-        if (i + 1 < mine) {
-            if (!UNIFORM) advance(i + 1);
-            else if (((i + 1) & (64 / HALVES - 1)) == 0) fetch_pages(i + 1);
-            load_keys(i + 1, next);
-            if (!UNIFORM) look_up(min(i + 2, mine - 1));
-        }
-        products(i, now, v);
+    // Two tiles take turns: one is on its way during the other's products.
+    Tile a, b;
+    auto step = [&](int32_t i, Tile &now, Tile &after) {
+        const int32_t ahead = min(i + 1, mine - 1);
+        if (UNIFORM && (ahead & 63) == 0) fetch_starts(ahead);
+        load(ahead, after);
+        if (!UNIFORM) look_up(min(i + 2, mine - 1));
+        products(i, now);
     };
     if (mine > 0) {
-        if (!UNIFORM) look_up(0), advance(0), look_up(min(1, mine - 1));
-        load_keys(0, a);
-    }
-    for (int32_t i = 0; i < mine; i += 2) {
-        step(i, a, b);
-        if (i + 1 < mine) step(i + 1, b, a);
+        if (UNIFORM) fetch_starts(0);
+        else look_up(0);
+        load(0, a);
+        if (!UNIFORM) look_up(min(1, mine - 1));
+        for (int32_t i = 0;;) {
+            step(i, a, b);
+            if (++i >= mine) break;
+            step(i, b, a);
+            if (++i >= mine) break;
+        }
     }
     total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
