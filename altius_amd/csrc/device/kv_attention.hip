@@ -194,7 +194,10 @@ template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int 
 // UNIFORM: 16 keys that start at a multiple of 16 are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
 template <int DP> struct RowLds {
     static constexpr int PITCH = DP + 4;
-    float sums[ROW_WAVES][16 * PITCH];
+    union {
+        float sums[ROW_WAVES][16 * PITCH];
+        uint16_t q[3][16 * (DP + 8)];  // a bf16 cache's: the parts of the queries, which all wavefronts share
+    };
     float stats[ROW_WAVES][2][16];
 };
 
@@ -241,7 +244,9 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
 
     // fp32: channels 16 i + 4 part on; bf16: parts of channels 32 i + 8 part on.
-    u32x4 q[BF16 ? 3 : 1][BF16 ? DP / 32 : DP / 16];
+    u32x4 q[BF16 ? 1 : DP / 16];
+    uint32_t q_at = col * (DP + 8) + 8 * part;
+    constexpr int Q_PART = 16 * (DP + 8);
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
     if constexpr (BF16) {
 #pragma unroll
@@ -249,14 +254,18 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             const uint32_t c = 32 * i + 8 * part;
             f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
             if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale, hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4) * g.scale;
+            u32x4 parts[3];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 uint32_t w[3];
                 split_pair(lo[2 * e], lo[2 * e + 1], w[0], w[1], w[2]);
-                q[0][i][e] = w[0], q[1][i][e] = w[1], q[2][i][e] = w[2];
+                parts[0][e] = w[0], parts[1][e] = w[1], parts[2][e] = w[2];
                 split_pair(hi[2 * e], hi[2 * e + 1], w[0], w[1], w[2]);
-                q[0][i][2 + e] = w[0], q[1][i][2 + e] = w[1], q[2][i][2 + e] = w[2];
+                parts[0][2 + e] = w[0], parts[1][2 + e] = w[1], parts[2][2 + e] = w[2];
             }
+            // Every wavefront writes the same.
+#pragma unroll
+            for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4 *>(&lds.q[0][q_at + p * Q_PART + 32 * i]) = parts[p];
         }
     } else {
 #pragma unroll
@@ -264,7 +273,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             const uint32_t c = 16 * i + 4 * part;
             f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
             if (valid && c < g.d) x = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
-            q[0][i] = __builtin_bit_cast(u32x4, x);
+            q[i] = __builtin_bit_cast(u32x4, x);
         }
     }
 
@@ -401,17 +410,19 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         const int32_t key0 = tile_key(i);
         float x[NS];
         f32x4 large = {0.0f, 0.0f, 0.0f, 0.0f}, small = large;
+        if (BF16) asm volatile("" : "+v"(q_at));  // or the parts in LDS would move to registers in front of the loop
 #pragma unroll
         for (int c = 0; c < Tile::K_UNITS; c++) {
             if constexpr (BF16) {
-                ALTIUS_MFMA16_BF16(t.k[c], q[2][c], small);
-                ALTIUS_MFMA16_BF16(t.k[c], q[0][c], large);
-                ALTIUS_MFMA16_BF16(t.k[c], q[1][c], small);
+                auto part_of = [&](int p) { return *reinterpret_cast<const u32x4 *>(&lds.q[0][q_at + p * Q_PART + 32 * c]); };
+                ALTIUS_MFMA16_BF16(t.k[c], part_of(2), small);
+                ALTIUS_MFMA16_BF16(t.k[c], part_of(0), large);
+                ALTIUS_MFMA16_BF16(t.k[c], part_of(1), small);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    if (c % 2 == 0) ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[0][c][e]), large);
-                    else ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[0][c][e]), small);
+                    if (c % 2 == 0) ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[c][e]), large);
+                    else ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[c][e]), small);
                 }
             }
         }
@@ -505,7 +516,8 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         }
     }
 
-    // The block's wavefronts join their parts.
+    // The block's wavefronts join their parts, where the queries' parts were.
+    if (BF16) __syncthreads();
     if (part == 0) stats[wave][0][col] = top, stats[wave][1][col] = total;
 #pragma unroll
     for (int i = 0; i < NACC; i += 4)
@@ -544,7 +556,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
 
 // Heads of more than 128 channels have no tiles of their own yet: all their rows go 16 a wavefront.
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
-__global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : 2) void attend_rows16(AttendArgs g) {
+__global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ? 3 : 2) void attend_rows16(AttendArgs g) {
     __shared__ __align__(16) RowLds<DP> lds;
     rows16<DP, BF16, UNIFORM, SPLIT>(g, blockIdx.x, lds);
 }
