@@ -38,7 +38,8 @@ constexpr uint32_t FEW_ROWS = 64;
 
 // How the blocks share the work on the sequences of one kind: row tiles, and splits of split_keys keys each.  Where there are
 // several, the partial results of (sequence, kv head, row < rows, split) wait in the workspace: maximum and sum, and the weighted
-// sum of values.
+// sum of values.  The sequences of few rows are cut otherwise (Cut): there splits is 1 or 2, not cut or cut, and a block's part has
+// split_keys keys at least.
 struct Share {
     uint32_t row_tiles, splits, split_keys, rows;
     uint32_t blocks;
@@ -79,7 +80,7 @@ __device__ __forceinline__ RowRange row_range(const AttendArgs &g, const dev::Kv
     r.high = g.causal ? r.place + 1 : q.length;
     if (g.prefix) r.high = max(r.high, g.prefix[s]);
     r.high = min(r.high, q.length);
-    r.low = g.window ? max(0, r.place - g.window + 1) : 0;
+    r.low = g.window ? max(0, max(0, r.place) - g.window + 1) : 0;
     if (g.first_keys) r.low = max(r.low, g.first_keys[q.start + (int32_t)token]);
     return r;
 }
@@ -201,20 +202,95 @@ template <int DP> struct RowLds {
     float stats[ROW_WAVES][2][16];
 };
 
+// The keys of sequences of few rows, cut into equal parts, one a block, whatever the sequences' lengths: a line of units of 64 keys, the
+// sequences one after the other, in each of them the row tiles and kv heads (its pairs).  A block's part may end inside one pair and
+// go on in others; each piece of a pair leaves its partial result in a place of its own, the (block + pair)-th.  Found by every block for
+// itself, from the lengths, by a scan over the sequences, 64 at a time.
+constexpr uint32_t UNIT = 64;
+struct SequenceWork {
+    uint32_t units, pairs;  // units of one pair; pairs
+    int32_t begin;          // the first unit's first key
+};
+__device__ __forceinline__ SequenceWork sequence_work(const AttendArgs &g, uint32_t s) {
+    const dev::KvSequence q = sequence_of(g, s);
+    const uint32_t rows = (uint32_t)q.n * g.group;
+    SequenceWork w = {0, 0, 0};
+    if (rows == 0 || rows > FEW_ROWS) return w;
+    if (g.window) w.begin = max(0, max(0, q.length - q.n) - g.window + 1) & ~(int32_t)(UNIT - 1);
+    w.units = max(1u, (uint32_t)(q.length - w.begin + (int32_t)UNIT - 1) / UNIT);
+    w.pairs = (rows + 15) / 16 * g.kv.kv_heads;
+    return w;
+}
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // over the lanes up to this one
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t t = __shfl_up(v, m);
+        if (lane >= (uint32_t)m) v += t;
+    }
+    return v;
+}
+struct Cut {
+    uint32_t units, blocks;  // in all
+    __device__ __forceinline__ uint32_t first_unit(uint32_t block) const { return (uint32_t)((uint64_t)block * units / blocks); }
+    __device__ __forceinline__ uint32_t block_of(uint32_t unit) const { return (uint32_t)(((uint64_t)(unit + 1) * blocks - 1) / units); }
+};
+__device__ __forceinline__ Cut cut_of(const AttendArgs &g) {
+    Cut cut = {0, 0};
+    for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
+        const uint32_t s = base + (threadIdx.x & 63u);
+        SequenceWork w = {0, 0, 0};
+        if (s < g.kv.sequences) w = sequence_work(g, s);
+        cut.units += __builtin_amdgcn_readlane(wave_prefix(w.units * w.pairs), 63);
+    }
+    cut.blocks = min(g.few.blocks, max(1u, cut.units / (g.few.split_keys / UNIT)));
+    return cut;
+}
+struct Found {
+    uint32_t s, units_before, pairs_before;
+    SequenceWork work;
+};
+// The sequence that a unit (below cut.units) belongs to, or, by_sequence, the one asked for.
+__device__ __forceinline__ Found find(const AttendArgs &g, bool by_sequence, uint32_t what) {
+    Found f = {0, 0, 0, {1, 1, 0}};
+    uint32_t units = 0, pairs = 0;
+    for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
+        const uint32_t s = base + (threadIdx.x & 63u);
+        SequenceWork w = {0, 0, 0};
+        if (s < g.kv.sequences) w = sequence_work(g, s);
+        const uint32_t u = wave_prefix(w.units * w.pairs), p = wave_prefix(w.pairs);
+        const uint64_t here = __ballot(by_sequence ? s == what : units + u > what);
+        if (here) {
+            const int lane = __builtin_ctzll(here);
+            f.s = base + lane;
+            f.work.units = __builtin_amdgcn_readlane(w.units, lane), f.work.pairs = __builtin_amdgcn_readlane(w.pairs, lane);
+            f.work.begin = __builtin_amdgcn_readlane(w.begin, lane);
+            f.units_before = units + __builtin_amdgcn_readlane(u, lane) - f.work.units * f.work.pairs;
+            f.pairs_before = pairs + __builtin_amdgcn_readlane(p, lane) - f.work.pairs;
+            break;
+        }
+        units += __builtin_amdgcn_readlane(u, 63), pairs += __builtin_amdgcn_readlane(p, 63);
+    }
+    return f;
+}
+
+// What a block does for 16 rows of a kv head: the keys from .. to - 1.  whole: that is all there is to them; else the partial result
+// goes to place `slot`.
+struct Piece {
+    uint32_t s, kvh, tile;
+    int32_t from, to;
+    bool whole;
+    uint32_t slot;
+};
+
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
-__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP> &lds) {
+__device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece, RowLds<DP> &lds) {
     constexpr int KT = ROW_KEYS, NACC = DP / 16, PITCH = RowLds<DP>::PITCH;
     auto &sums = lds.sums;
     auto &stats = lds.stats;
-    const Share &share = SPLIT ? g.few : g.many;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, part = lane >> 4;
-
-    const uint32_t kvh = id % g.kv.kv_heads;
-    id /= g.kv.kv_heads;
-    const uint32_t tile = id % share.row_tiles;
-    id /= share.row_tiles;
-    const uint32_t split = SPLIT ? id % share.splits : 0, s = SPLIT ? id / share.splits : id;
+    const uint32_t s = piece.s, kvh = piece.kvh, tile = piece.tile;
 
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
@@ -234,8 +310,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         any_low = min(any_low, __shfl_xor(any_low, m)), any_high = max(any_high, __shfl_xor(any_high, m));
         all_low = max(all_low, __shfl_xor(all_low, m)), all_high = min(all_high, __shfl_xor(all_high, m));
     }
-    int32_t begin = any_low, end = any_high;
-    if (SPLIT) begin = max(begin, (int32_t)(split * share.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * share.split_keys));
+    int32_t begin = max(any_low, piece.from), end = min(any_high, piece.to);
     begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
     const int32_t first = begin / KT, tiles = begin < end ? (end + KT - 1) / KT - first : 0;
 
@@ -540,10 +615,10 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             l = __builtin_fmaf(stats[w][1][r], f, l);
             o += *reinterpret_cast<const f32x4 *>(&sums[w][r * PITCH + c]) * f;
         }
-        if (SPLIT && share.splits > 1) {
-            const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + mine_row) * share.splits + split;
-            *reinterpret_cast<f32x4 *>(share.part_out + at * g.d + c) = o;
-            if (c == 0) share.part_stats[2 * at] = m, share.part_stats[2 * at + 1] = l;
+        if (SPLIT && !piece.whole) {
+            const size_t at = (size_t)piece.slot * 16 + r;
+            *reinterpret_cast<f32x4 *>(g.few.part_out + at * g.d + c) = o;
+            if (c == 0) g.few.part_stats[2 * at] = m, g.few.part_stats[2 * at + 1] = l;
         } else {
             const uint32_t t = g.by_group.div(mine_row), h = kvh * g.group + mine_row - t * g.group;
             const RowRange of = row_range(g, seq, s, t);
@@ -551,6 +626,38 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
             *reinterpret_cast<f32x4 *>(g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + c) =
                 of.low < of.high ? o * recip : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+    }
+}
+
+template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
+__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP> &lds) {
+    const Share &share = SPLIT ? g.few : g.many;
+    Piece piece = {0, 0, 0, 0, INT32_MAX, true, 0};
+    uint32_t unit = 0, last = 1;
+    Cut cut = {0, 0};
+    const bool is_cut = SPLIT && share.splits > 1;
+    if (is_cut) {
+        cut = cut_of(g);
+        if (id >= cut.blocks) return;
+        unit = cut.first_unit(id), last = cut.first_unit(id + 1);
+    }
+    for (; unit < last;) {
+        if (is_cut) {
+            const Found f = find(g, false, unit);
+            const uint32_t inside = unit - f.units_before, pair = inside / f.work.units, off = inside - pair * f.work.units, count = min(last - unit, f.work.units - off);
+            piece.s = f.s, piece.tile = pair / g.kv.kv_heads, piece.kvh = pair - piece.tile * g.kv.kv_heads;
+            piece.from = f.work.begin + (int32_t)(off * UNIT), piece.to = off + count == f.work.units ? INT32_MAX : piece.from + (int32_t)(count * UNIT);
+            piece.whole = count == f.work.units;
+            piece.slot = id + f.pairs_before + pair;
+            unit += count;
+        } else {
+            piece.kvh = id % g.kv.kv_heads;
+            id /= g.kv.kv_heads;
+            piece.tile = id % share.row_tiles, piece.s = id / share.row_tiles;
+            unit = last;
+        }
+        piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds);
+        if (unit < last) __syncthreads();  // LDS is used again
     }
 }
 
@@ -990,7 +1097,7 @@ __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(
 
 // Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
 // channels, four a lane.  few: a block per row, whose groups of lanes deal the splits out among themselves; else a group per row.
-constexpr int JOIN = 256, MOST_SPLITS = 512;
+constexpr int JOIN = 256, MOST_SPLITS = 1024;
 __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_blocks) {
     __shared__ float factors[MOST_SPLITS];
     __shared__ __align__(16) f32x4 sums[JOIN];
@@ -1014,36 +1121,49 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_b
         if (!few || group == 0) *reinterpret_cast<f32x4 *>(to) = zero;
         return;
     }
-    const uint32_t from = (uint32_t)of.low / share.split_keys, count = (uint32_t)(of.high - 1) / share.split_keys + 1 - from;
-    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits + from;
+    uint32_t count, apart;  // partial results, and how many rows they are apart
+    size_t at;
+    if (few) {
+        const Cut cut = cut_of(g);
+        const Found f = find(g, true, s);
+        const uint32_t pair = row / 16 * g.kv.kv_heads + kvh, unit = f.units_before + pair * f.work.units, block = cut.block_of(unit);
+        count = cut.block_of(unit + f.work.units - 1) + 1 - block;
+        if (count == 1) return;  // one block did it all
+        at = (size_t)(block + f.pairs_before + pair) * 16 + row % 16, apart = 16;
+    } else {
+        const uint32_t from = (uint32_t)of.low / share.split_keys;
+        count = (uint32_t)(of.high - 1) / share.split_keys + 1 - from;
+        at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits + from, apart = 1;
+    }
     const float *stats = share.part_stats + 2 * at;
     const f32x4 *parts = reinterpret_cast<const f32x4 *>(share.part_out + at * g.d) + lane;
+    const size_t stats_apart = 2 * apart, parts_apart = (size_t)apart * lanes;
 
     float top = -INFINITY, total = 0.0f;
     f32x4 o = zero;
     if (!few) {
-        for (uint32_t i = 0; i < count; i++) top = fmaxf(top, stats[2 * i]);
+        for (uint32_t i = 0; i < count; i++) top = fmaxf(top, stats[stats_apart * i]);
         for (uint32_t i = 0; i < count; i++) {
-            const float f = weight_of(stats[2 * i], top);
-            total = __builtin_fmaf(stats[2 * i + 1], f, total);
-            o += parts[i * lanes] * f;
+            const float f = weight_of(stats[stats_apart * i], top);
+            total = __builtin_fmaf(stats[stats_apart * i + 1], f, total);
+            o += parts[i * parts_apart] * f;
         }
         *reinterpret_cast<f32x4 *>(to) = o * (1.0f / total);
         return;
     }
     // Every wavefront finds the maximum by itself; the weights of the splits wait in LDS.
-    for (uint32_t i = threadIdx.x & 63u; i < count; i += 64) top = fmaxf(top, stats[2 * i]);
+    for (uint32_t i = threadIdx.x & 63u; i < count; i += 64) top = fmaxf(top, stats[stats_apart * i]);
     top = dev::wave_reduce<dev::MaxOp>(top);
     for (uint32_t i = threadIdx.x; i < count; i += JOIN) {
-        factors[i] = weight_of(stats[2 * i], top);
-        total = __builtin_fmaf(stats[2 * i + 1], factors[i], total);
+        factors[i] = weight_of(stats[stats_apart * i], top);
+        total = __builtin_fmaf(stats[stats_apart * i + 1], factors[i], total);
     }
     total = dev::wave_reduce<dev::SumOp>(total);
     if ((threadIdx.x & 63u) == 0) totals[threadIdx.x >> 6] = total;
     __syncthreads();
     if (group < groups) {
 #pragma unroll 4
-        for (uint32_t i = group; i < count; i += groups) o += parts[(size_t)i * lanes] * factors[i];
+        for (uint32_t i = group; i < count; i += groups) o += parts[i * parts_apart] * factors[i];
     }
     sums[threadIdx.x] = o;
     __syncthreads();
@@ -1091,9 +1211,22 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
             p.bytes += parts * (size_t)cache.head_size * sizeof(float);
         }
     };
-    // Few rows: blocks enough for every CU to have several in turn, since sequences are of different lengths; no split shorter than
-    // 256 KiB of keys and values.
-    share(p.few, std::min(rows, FEW_ROWS), 16, 4 * cus, std::max<uint64_t>(64, 256 * 1024 / key_bytes));
+    // Few rows: a part for each block that is at work at once, none shorter than 256 KiB of keys and values or 64 keys.
+    p.few.rows = std::min(rows, FEW_ROWS);
+    p.few.row_tiles = (p.few.rows + 15) / 16;
+    p.few.split_keys = (uint32_t)((std::max<uint64_t>(UNIT, 256 * 1024 / key_bytes) + UNIT - 1) / UNIT * UNIT);
+    const uint64_t few_pairs = pairs * p.few.row_tiles, units = few_pairs * ((max_keys + UNIT - 1) / UNIT);
+    p.few.splits = max_keys > p.few.split_keys && units < UINT32_MAX ? 2 : 1;
+    p.few.blocks = (uint32_t)std::min<uint64_t>(few_pairs, UINT32_MAX);
+    if (p.few.splits > 1) {
+        const uint64_t at_once = cus * (cache.head_size <= 64 || (cache.elem == AHIP_KV_BF16 && cache.head_size <= 128) ? 3 : cache.head_size <= 128 ? 2 : 1);
+        p.few.blocks = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(at_once, MOST_SPLITS), std::max<uint64_t>(1, units * UNIT / p.few.split_keys));
+        const size_t parts = (size_t)(p.few.blocks + few_pairs) * 16;
+        p.few.part_stats = reinterpret_cast<float *>(p.bytes);
+        p.bytes += 2 * parts * sizeof(float);
+        p.few.part_out = reinterpret_cast<float *>(p.bytes);
+        p.bytes += parts * (size_t)cache.head_size * sizeof(float);
+    }
     if (rows > FEW_ROWS) {
         if (cache.head_size <= TILE_CHANNELS) {
             // So many blocks are at work at once.  Fewer of them are cut until there are two rounds.
