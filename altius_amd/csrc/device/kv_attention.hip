@@ -38,11 +38,11 @@ constexpr uint32_t FEW_ROWS = 64;
 
 // How the blocks share the work on the sequences of one kind: row tiles, and splits of split_keys keys each.  Where there are
 // several, the partial results of (sequence, kv head, row < rows, split) wait in the workspace: maximum and sum, and the weighted
-// sum of values.  The sequences of few rows are cut otherwise (Cut): there splits is 1 or 2, not cut or cut, and a block's part has
-// split_keys keys at least.
+// sum of values.  The sequences of few rows are cut otherwise (part_of): there splits is 1 or 2, not cut or cut, a block's part has
+// split_keys keys at least, and at_once blocks are at work at once.
 struct Share {
     uint32_t row_tiles, splits, split_keys, rows;
-    uint32_t blocks;
+    uint32_t blocks, at_once;
     float *part_stats, *part_out;
 };
 
@@ -193,28 +193,31 @@ template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int 
 }
 
 // UNIFORM: 16 keys that start at a multiple of 16 are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
-template <int DP> struct RowLds {
+template <int DP, bool BF16> struct RowLds {
     static constexpr int PITCH = DP + 4;
     union {
         float sums[ROW_WAVES][16 * PITCH];
-        uint16_t q[3][16 * (DP + 8)];  // a bf16 cache's: the parts of the queries, which all wavefronts share
+        // The parts of the queries, a bf16 cache's, or the queries, where registers do not hold them: all wavefronts share them.
+        uint16_t q[3][16 * (DP + 8)];
+        float whole_q[16 * PITCH];
     };
     float stats[ROW_WAVES][2][16];
 };
 
-// The keys of sequences of few rows, cut into equal parts, one a block, whatever the sequences' lengths: a line of units of 64 keys, the
-// sequences one after the other, in each of them the row tiles and kv heads (its pairs).  A block's part may end inside one pair and
-// go on in others; each piece of a pair leaves its partial result in a place of its own, the (block + pair)-th.  Found by every block for
-// itself, from the lengths, by a scan over the sequences, 64 at a time.
+// The keys of sequences of few rows, cut into parts of about the same size, one a block, whatever the sequences' lengths.  In units of 64
+// keys: a part is as large as leaves no more parts than blocks that are at work at once, as far as the pairs (row tiles x kv
+// heads of all sequences), which are cut one by one, allow.  Every block finds its part for itself, from the lengths, by a scan over the
+// sequences, 64 at a time; its partial results wait in the place of its number.
 constexpr uint32_t UNIT = 64;
 struct SequenceWork {
     uint32_t units, pairs;  // units of one pair; pairs
     int32_t begin;          // the first unit's first key
 };
 __device__ __forceinline__ SequenceWork sequence_work(const AttendArgs &g, uint32_t s) {
+    SequenceWork w = {0, 0, 0};
+    if (s >= g.kv.sequences) return w;
     const dev::KvSequence q = sequence_of(g, s);
     const uint32_t rows = (uint32_t)q.n * g.group;
-    SequenceWork w = {0, 0, 0};
     if (rows == 0 || rows > FEW_ROWS) return w;
     if (g.window) w.begin = max(0, max(0, q.length - q.n) - g.window + 1) & ~(int32_t)(UNIT - 1);
     w.units = max(1u, (uint32_t)(q.length - w.begin + (int32_t)UNIT - 1) / UNIT);
@@ -230,52 +233,46 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // over the lanes
     }
     return v;
 }
-struct Cut {
-    uint32_t units, blocks;  // in all
-    __device__ __forceinline__ uint32_t first_unit(uint32_t block) const { return (uint32_t)((uint64_t)block * units / blocks); }
-    __device__ __forceinline__ uint32_t block_of(uint32_t unit) const { return (uint32_t)(((uint64_t)(unit + 1) * blocks - 1) / units); }
-};
-__device__ __forceinline__ Cut cut_of(const AttendArgs &g) {
-    Cut cut = {0, 0};
-    for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
-        const uint32_t s = base + (threadIdx.x & 63u);
-        SequenceWork w = {0, 0, 0};
-        if (s < g.kv.sequences) w = sequence_work(g, s);
-        cut.units += __builtin_amdgcn_readlane(wave_prefix(w.units * w.pairs), 63);
-    }
-    cut.blocks = min(g.few.blocks, max(1u, cut.units / (g.few.split_keys / UNIT)));
-    return cut;
-}
-struct Found {
-    uint32_t s, units_before, pairs_before;
-    SequenceWork work;
-};
-// The sequence that a unit (below cut.units) belongs to, or, by_sequence, the one asked for.
-__device__ __forceinline__ Found find(const AttendArgs &g, bool by_sequence, uint32_t what) {
-    Found f = {0, 0, 0, {1, 1, 0}};
+// The units of a part.
+__device__ __forceinline__ uint32_t part_of(const AttendArgs &g, const SequenceWork &first) {
     uint32_t units = 0, pairs = 0;
     for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
+        const SequenceWork w = base ? sequence_work(g, base + (threadIdx.x & 63u)) : first;
+        units += __builtin_amdgcn_readlane(wave_prefix(w.units * w.pairs), 63), pairs += __builtin_amdgcn_readlane(wave_prefix(w.pairs), 63);
+    }
+    const uint32_t blocks = 2 * pairs < g.few.at_once ? g.few.at_once - pairs : g.few.at_once;
+    return max((units + blocks - 1) / blocks, g.few.split_keys / UNIT);
+}
+struct Found {
+    uint32_t s, before, parts;  // of a pair; before: the sequence's first block
+    SequenceWork work;
+};
+// The sequence that a block is at work on, or, by_sequence, the one asked for.  False where there is none.
+__device__ __forceinline__ bool find(const AttendArgs &g, bool by_sequence, uint32_t what, Found &f) {
+    const SequenceWork first = sequence_work(g, threadIdx.x & 63u);
+    const uint32_t part = part_of(g, first);
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
         const uint32_t s = base + (threadIdx.x & 63u);
-        SequenceWork w = {0, 0, 0};
-        if (s < g.kv.sequences) w = sequence_work(g, s);
-        const uint32_t u = wave_prefix(w.units * w.pairs), p = wave_prefix(w.pairs);
-        const uint64_t here = __ballot(by_sequence ? s == what : units + u > what);
+        const SequenceWork w = base ? sequence_work(g, s) : first;
+        const uint32_t parts = (w.units + part - 1) / part, up_to = wave_prefix(parts * w.pairs);
+        const uint64_t here = __ballot(by_sequence ? s == what : before + up_to > what);
         if (here) {
             const int lane = __builtin_ctzll(here);
             f.s = base + lane;
             f.work.units = __builtin_amdgcn_readlane(w.units, lane), f.work.pairs = __builtin_amdgcn_readlane(w.pairs, lane);
             f.work.begin = __builtin_amdgcn_readlane(w.begin, lane);
-            f.units_before = units + __builtin_amdgcn_readlane(u, lane) - f.work.units * f.work.pairs;
-            f.pairs_before = pairs + __builtin_amdgcn_readlane(p, lane) - f.work.pairs;
-            break;
+            f.parts = __builtin_amdgcn_readlane(parts, lane);
+            f.before = before + __builtin_amdgcn_readlane(up_to, lane) - f.parts * f.work.pairs;
+            return true;
         }
-        units += __builtin_amdgcn_readlane(u, 63), pairs += __builtin_amdgcn_readlane(p, 63);
+        before += __builtin_amdgcn_readlane(up_to, 63);
     }
-    return f;
+    return false;
 }
 
-// What a block does for 16 rows of a kv head: the keys from .. to - 1.  whole: that is all there is to them; else the partial result
-// goes to place `slot`.
+// What a block does for 16 rows of a kv head: the keys from .. to - 1, which its wavefronts share tile by tile.  whole: that is all there
+// is to them; else the partial results go to place `slot`.
 struct Piece {
     uint32_t s, kvh, tile;
     int32_t from, to;
@@ -284,13 +281,13 @@ struct Piece {
 };
 
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
-__device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece, RowLds<DP> &lds) {
-    constexpr int KT = ROW_KEYS, NACC = DP / 16, PITCH = RowLds<DP>::PITCH;
+__device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece, RowLds<DP, BF16> &lds) {
+    constexpr int KT = ROW_KEYS, NACC = DP / 16, PITCH = RowLds<DP, BF16>::PITCH;
     auto &sums = lds.sums;
     auto &stats = lds.stats;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, part = lane >> 4;
-    const uint32_t s = piece.s, kvh = piece.kvh, tile = piece.tile;
+    const uint32_t s = piece.s, tile = piece.tile, kvh = piece.kvh;
 
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
@@ -319,8 +316,9 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
 
     // fp32: channels 16 i + 4 part on; bf16: parts of channels 32 i + 8 part on.
-    u32x4 q[BF16 ? 1 : DP / 16];
-    uint32_t q_at = col * (DP + 8) + 8 * part;
+    constexpr bool Q_HERE = DP > 128 && !BF16;
+    u32x4 q[BF16 || Q_HERE ? 1 : DP / 16];
+    uint32_t q_at = BF16 ? col * (DP + 8) + 8 * part : col * PITCH + 4 * part;
     constexpr int Q_PART = 16 * (DP + 8);
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
     if constexpr (BF16) {
@@ -338,7 +336,6 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
                 split_pair(hi[2 * e], hi[2 * e + 1], w[0], w[1], w[2]);
                 parts[0][2 + e] = w[0], parts[1][2 + e] = w[1], parts[2][2 + e] = w[2];
             }
-            // Every wavefront writes the same.
 #pragma unroll
             for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4 *>(&lds.q[0][q_at + p * Q_PART + 32 * i]) = parts[p];
         }
@@ -348,7 +345,8 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
             const uint32_t c = 16 * i + 4 * part;
             f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
             if (valid && c < g.d) x = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
-            q[i] = __builtin_bit_cast(u32x4, x);
+            if constexpr (Q_HERE) *reinterpret_cast<f32x4 *>(&lds.whole_q[q_at + 16 * i]) = x;
+            else q[i] = __builtin_bit_cast(u32x4, x);
         }
     }
 
@@ -485,7 +483,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
         const int32_t key0 = tile_key(i);
         float x[NS];
         f32x4 large = {0.0f, 0.0f, 0.0f, 0.0f}, small = large;
-        if (BF16) asm volatile("" : "+v"(q_at));  // or the parts in LDS would move to registers in front of the loop
+        if (BF16 || Q_HERE) asm volatile("" : "+v"(q_at));  // or what is in LDS would move to registers in front of the loop
 #pragma unroll
         for (int c = 0; c < Tile::K_UNITS; c++) {
             if constexpr (BF16) {
@@ -494,10 +492,13 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
                 ALTIUS_MFMA16_BF16(t.k[c], part_of(0), large);
                 ALTIUS_MFMA16_BF16(t.k[c], part_of(1), small);
             } else {
+                u32x4 its_q;
+                if constexpr (Q_HERE) its_q = *reinterpret_cast<const u32x4 *>(&lds.whole_q[q_at + 16 * c]);
+                else its_q = q[c];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    if (c % 2 == 0) ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[c][e]), large);
-                    else ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(q[c][e]), small);
+                    if (c % 2 == 0) ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(its_q[e]), large);
+                    else ALTIUS_MFMA16_F32(__uint_as_float(t.k[c][e]), __uint_as_float(its_q[e]), small);
                 }
             }
         }
@@ -513,13 +514,16 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
                 split_pair(x[2 * e], x[2 * e + 1], w[0], w[1], w[2]);
                 p[0][e] = w[0], p[1][e] = w[1], p[2][e] = w[2];
             }
+            u32x2 v[NACC];
 #pragma unroll
             for (int c = 0; c < NACC; c++) {
                 const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
-                const u32x2 v = {__builtin_amdgcn_perm(t.v[1][c / 2], t.v[0][c / 2], pick), __builtin_amdgcn_perm(t.v[3][c / 2], t.v[2][c / 2], pick)};
-#pragma unroll
-                for (int e = 2; e >= 0; e--) ALTIUS_MFMA16_BF16_K16(v, p[e], acc[c]);
+                v[c] = u32x2{__builtin_amdgcn_perm(t.v[1][c / 2], t.v[0][c / 2], pick), __builtin_amdgcn_perm(t.v[3][c / 2], t.v[2][c / 2], pick)};
             }
+#pragma unroll
+            for (int e = 2; e >= 0; e--)  // a sum's next term comes after all others': none waits for the one before
+#pragma unroll
+                for (int c = 0; c < NACC; c++) ALTIUS_MFMA16_BF16_K16(v[c], p[e], acc[c]);
         } else {
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -528,24 +532,28 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
         }
     };
 
-    // Two tiles take turns: one is on its way during the other's products.
-    Tile a, b;
-    auto step = [&](int32_t i, Tile &now, Tile &after) {
-        const int32_t ahead = min(i + 1, mine - 1);
-        if (UNIFORM && (ahead & 63) == 0) fetch_starts(ahead);
-        load(ahead, after);
-        if (!UNIFORM) look_up(min(i + 2, mine - 1));
-        products(i, now);
+    // Two tiles take turns, one on its way during the other's products; heads of more than 128 channels have registers for one.
+    auto load_one = [&](int32_t i, Tile &t) {
+        if (UNIFORM && (i & 63) == 0) fetch_starts(i);
+        load(i, t);
+        if (!UNIFORM) look_up(min(i + 1, mine - 1));
     };
-    if (mine > 0) {
-        if (UNIFORM) fetch_starts(0);
-        else look_up(0);
-        load(0, a);
-        if (!UNIFORM) look_up(min(1, mine - 1));
+    Tile a;
+    if (mine > 0 && !UNIFORM) look_up(0);
+    if constexpr (DP > 128) {
+        for (int32_t i = 0; i < mine; i++) {
+            load_one(i, a);
+            products(i, a);
+        }
+    } else if (mine > 0) {
+        Tile b;
+        load_one(0, a);
         for (int32_t i = 0;;) {
-            step(i, a, b);
+            load_one(min(i + 1, mine - 1), b);
+            products(i, a);
             if (++i >= mine) break;
-            step(i, b, a);
+            load_one(min(i + 1, mine - 1), a);
+            products(i, b);
             if (++i >= mine) break;
         }
     }
@@ -591,8 +599,8 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
         }
     }
 
-    // The block's wavefronts join their parts, where the queries' parts were.
-    if (BF16) __syncthreads();
+    // The block's wavefronts join their parts, where queries were.
+    if (BF16 || Q_HERE) __syncthreads();
     if (part == 0) stats[wave][0][col] = top, stats[wave][1][col] = total;
 #pragma unroll
     for (int i = 0; i < NACC; i += 4)
@@ -630,41 +638,31 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
 }
 
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
-__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP> &lds) {
+__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP, BF16> &lds) {
     const Share &share = SPLIT ? g.few : g.many;
     Piece piece = {0, 0, 0, 0, INT32_MAX, true, 0};
-    uint32_t unit = 0, last = 1;
-    Cut cut = {0, 0};
-    const bool is_cut = SPLIT && share.splits > 1;
-    if (is_cut) {
-        cut = cut_of(g);
-        if (id >= cut.blocks) return;
-        unit = cut.first_unit(id), last = cut.first_unit(id + 1);
-    }
-    for (; unit < last;) {
-        if (is_cut) {
-            const Found f = find(g, false, unit);
-            const uint32_t inside = unit - f.units_before, pair = inside / f.work.units, off = inside - pair * f.work.units, count = min(last - unit, f.work.units - off);
-            piece.s = f.s, piece.tile = pair / g.kv.kv_heads, piece.kvh = pair - piece.tile * g.kv.kv_heads;
-            piece.from = f.work.begin + (int32_t)(off * UNIT), piece.to = off + count == f.work.units ? INT32_MAX : piece.from + (int32_t)(count * UNIT);
-            piece.whole = count == f.work.units;
-            piece.slot = id + f.pairs_before + pair;
-            unit += count;
-        } else {
-            piece.kvh = id % g.kv.kv_heads;
-            id /= g.kv.kv_heads;
-            piece.tile = id % share.row_tiles, piece.s = id / share.row_tiles;
-            unit = last;
-        }
+    if (!SPLIT || share.splits == 1) {
+        const uint32_t outer = id / g.kv.kv_heads;
+        piece.kvh = id - outer * g.kv.kv_heads;
+        piece.tile = outer % share.row_tiles, piece.s = outer / share.row_tiles;
         piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds);
-        if (unit < last) __syncthreads();  // LDS is used again
+        return;
     }
+    Found f;
+    if (!find(g, false, id, f)) return;
+    const uint32_t inside = id - f.before, pair = inside / f.parts, part = inside - pair * f.parts;
+    piece.s = f.s, piece.tile = pair / g.kv.kv_heads, piece.kvh = pair - piece.tile * g.kv.kv_heads;
+    auto key = [&](uint32_t p) { return f.work.begin + (int32_t)((uint32_t)((uint64_t)p * f.work.units / f.parts) * UNIT); };
+    piece.from = key(part), piece.to = part + 1 == f.parts ? INT32_MAX : key(part + 1);
+    piece.whole = f.parts == 1;
+    piece.slot = id;
+    piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds);
 }
 
 // Heads of more than 128 channels have no tiles of their own yet: all their rows go 16 a wavefront.
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
 __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ? 3 : 2) void attend_rows16(AttendArgs g) {
-    __shared__ __align__(16) RowLds<DP> lds;
+    __shared__ __align__(16) RowLds<DP, BF16> lds;
     rows16<DP, BF16, UNIFORM, SPLIT>(g, blockIdx.x, lds);
 }
 
@@ -1088,7 +1086,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
 template <int DP, bool BF16, bool UNIFORM>
 __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(AttendArgs g) {
     __shared__ __align__(16) union {
-        RowLds<DP <= 64 ? 64 : 128> few;
+        RowLds<DP <= 64 ? 64 : 128, BF16> few;
         TileLds<DP, BF16> many;
     } lds;
     if (blockIdx.x < g.many.blocks) rows128<DP, BF16, UNIFORM>(g, blockIdx.x, lds.many);
@@ -1124,12 +1122,10 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_b
     uint32_t count, apart;  // partial results, and how many rows they are apart
     size_t at;
     if (few) {
-        const Cut cut = cut_of(g);
-        const Found f = find(g, true, s);
-        const uint32_t pair = row / 16 * g.kv.kv_heads + kvh, unit = f.units_before + pair * f.work.units, block = cut.block_of(unit);
-        count = cut.block_of(unit + f.work.units - 1) + 1 - block;
-        if (count == 1) return;  // one block did it all
-        at = (size_t)(block + f.pairs_before + pair) * 16 + row % 16, apart = 16;
+        Found f;
+        if (!find(g, true, s, f) || f.parts <= 1) return;  // one block did it all
+        count = f.parts;
+        at = (size_t)(f.before + (row / 16 * g.kv.kv_heads + kvh) * f.parts) * 16 + row % 16, apart = 16;
     } else {
         const uint32_t from = (uint32_t)of.low / share.split_keys;
         count = (uint32_t)(of.high - 1) / share.split_keys + 1 - from;
@@ -1220,8 +1216,10 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     p.few.blocks = (uint32_t)std::min<uint64_t>(few_pairs, UINT32_MAX);
     if (p.few.splits > 1) {
         const uint64_t at_once = cus * (cache.head_size <= 64 || (cache.elem == AHIP_KV_BF16 && cache.head_size <= 128) ? 3 : cache.head_size <= 128 ? 2 : 1);
-        p.few.blocks = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(at_once, MOST_SPLITS), std::max<uint64_t>(1, units * UNIT / p.few.split_keys));
-        const size_t parts = (size_t)(p.few.blocks + few_pairs) * 16;
+        p.few.at_once = (uint32_t)std::min<uint64_t>(at_once, MOST_SPLITS);
+        // No more parts than both the parts' least size and at_once allow, and one more a pair.
+        p.few.blocks = (uint32_t)(std::min<uint64_t>(p.few.at_once, units * UNIT / p.few.split_keys) + few_pairs);
+        const size_t parts = (size_t)p.few.blocks * 16;
         p.few.part_stats = reinterpret_cast<float *>(p.bytes);
         p.bytes += 2 * parts * sizeof(float);
         p.few.part_out = reinterpret_cast<float *>(p.bytes);

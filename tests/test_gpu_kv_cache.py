@@ -245,6 +245,14 @@ SHAPES = [  # n, lengths, heads, kv heads, d, page, type, order
     ([2, 5], [19, 300], 6, 3, 80, 8, "bf16", "head"),
     ([1, 1], [100, 64], 4, 4, 256, 16, "f32", "head"),
     ([4, 1], [200, 129], 16, 2, 256, 64, "bf16", "slot"),
+    ([1, 3], [1000, 700], 4, 4, 256, 16, "f32", "head"),
+    ([1, 3], [1000, 700], 8, 1, 256, 48, "f32", "slot"),
+    ([2], [3000], 4, 2, 256, 16, "bf16", "slot"),
+    ([1, 1], [2500, 90], 2, 1, 256, 20, "bf16", "head"),
+    ([1], [1111], 6, 6, 132, 16, "f32", "head"),
+    ([1] * 70, [5 * i + 1 for i in range(69)] + [1500], 8, 4, 64, 16, "f32", "slot"),
+    ([1] * 66 + [0, 3], [1700] + [330 - 5 * i for i in range(65)] + [5, 900], 6, 6, 64, 16, "bf16", "head"),
+    ([70, 1], [400, 3000], 2, 2, 256, 16, "f32", "slot"),
     ([1, 2], [33, 50], 3, 1, 200, 7, "bf16", "head"),
     ([1, 2], [33, 50], 3, 1, 20, 5, "f32", "slot"),
     ([17], [17], 2, 2, 64, 16, "f32", "head"),
