@@ -233,15 +233,21 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // over the lanes
     }
     return v;
 }
-// The units of a part.
+// The units of a part: the least of a few that leave no more parts than blocks at work at once, so that few of those go without one.
 __device__ __forceinline__ uint32_t part_of(const AttendArgs &g, const SequenceWork &first) {
-    uint32_t units = 0, pairs = 0;
-    for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
-        const SequenceWork w = base ? sequence_work(g, base + (threadIdx.x & 63u)) : first;
-        units += __builtin_amdgcn_readlane(wave_prefix(w.units * w.pairs), 63), pairs += __builtin_amdgcn_readlane(wave_prefix(w.pairs), 63);
+    auto sum = [&](auto of) {
+        uint32_t total = 0;
+        for (uint32_t base = 0; base < g.kv.sequences; base += 64)
+            total += __builtin_amdgcn_readlane(wave_prefix(of(base ? sequence_work(g, base + (threadIdx.x & 63u)) : first)), 63);
+        return total;
+    };
+    const uint32_t units = sum([](const SequenceWork &w) { return w.units * w.pairs; });
+    uint32_t part = max((units + g.few.at_once - 1) / g.few.at_once, g.few.split_keys / UNIT);
+    for (int i = 0; i < 4; i++) {
+        if (sum([&](const SequenceWork &w) { return (w.units + part - 1) / part * w.pairs; }) <= g.few.at_once) break;
+        part += (part + 15) / 16;
     }
-    const uint32_t blocks = 2 * pairs < g.few.at_once ? g.few.at_once - pairs : g.few.at_once;
-    return max((units + blocks - 1) / blocks, g.few.split_keys / UNIT);
+    return part;
 }
 struct Found {
     uint32_t s, before, parts;  // of a pair; before: the sequence's first block
