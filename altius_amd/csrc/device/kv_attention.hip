@@ -843,36 +843,39 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             for (int w = 0; w < V_WORDS; w++) v_stage[e][w] = seen ? v_stage[e][w] : 0;
         }
     };
-    auto park_keys = [&](int buffer) {
+    auto park_key = [&](int buffer, int e) {
+        uint16_t *to = &lds.k[buffer][0][k_key(e) * K_PITCH + (16 / SIZE) * k_unit(e)];
+        if constexpr (BF16) {
+            *reinterpret_cast<u32x4 *>(to) = k_stage[e];
+        } else {
+            uint32_t p[3][2];
 #pragma unroll
-        for (int e = 0; e < K_EACH; e++) {
-            uint16_t *to = &lds.k[buffer][0][k_key(e) * K_PITCH + (16 / SIZE) * k_unit(e)];
-            if constexpr (BF16) {
-                *reinterpret_cast<u32x4 *>(to) = k_stage[e];
-            } else {
-                uint32_t p[3][2];
+            for (int w = 0; w < 2; w++) split_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
-                for (int w = 0; w < 2; w++) split_pair(__uint_as_float(k_stage[e][2 * w]), __uint_as_float(k_stage[e][2 * w + 1]), p[0][w], p[1][w], p[2][w]);
-#pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
-            }
+            for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (TILE_KEYS * K_PITCH)) = u32x2{p[q][0], p[q][1]};
         }
     };
-    auto park_values = [&](int buffer) {
+    auto park_value = [&](int buffer, int c) {
+        uint16_t *to = &lds.v[buffer][0][(v_channel + c) * V_PITCH + v_slot];
+        if constexpr (BF16) {
+            const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
+            *reinterpret_cast<u32x2 *>(to) =
+                u32x2{__builtin_amdgcn_perm(v_stage[1][c / 2], v_stage[0][c / 2], pick), __builtin_amdgcn_perm(v_stage[3][c / 2], v_stage[2][c / 2], pick)};
+        } else {
+            uint32_t p[3][2];
 #pragma unroll
-        for (int c = 0; c < VC; c++) {
-            uint16_t *to = &lds.v[buffer][0][(v_channel + c) * V_PITCH + v_slot];
-            if constexpr (BF16) {
-                const uint32_t pick = c % 2 ? 0x07060302u : 0x05040100u;
-                *reinterpret_cast<u32x2 *>(to) =
-                    u32x2{__builtin_amdgcn_perm(v_stage[1][c / 2], v_stage[0][c / 2], pick), __builtin_amdgcn_perm(v_stage[3][c / 2], v_stage[2][c / 2], pick)};
-            } else {
-                uint32_t p[3][2];
+            for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
 #pragma unroll
-                for (int w = 0; w < 2; w++) split_pair(__uint_as_float(v_stage[2 * w][c]), __uint_as_float(v_stage[2 * w + 1][c]), p[0][w], p[1][w], p[2][w]);
+            for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
+        }
+    };
+    // Of the units of keys and channels of values that a thread puts into LDS, keys first, those from .. to - 1.
+    constexpr int PARKED = K_EACH + VC;
+    auto park = [&](int from, int to, int key_buffer, int value_buffer) {
 #pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<u32x2 *>(to + q * (DP * V_PITCH)) = u32x2{p[q][0], p[q][1]};
-            }
+        for (int n = from; n < to; n++) {
+            if (n < K_EACH) park_key(key_buffer, n);
+            else park_value(value_buffer, n - K_EACH);
         }
     };
 
@@ -928,30 +931,50 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             ALTIUS_MFMA32_BF16(a[0], b0, c);
         }
     };
-    auto first_product = [&](int buffer) {
+    // FENCED: operands are read from LDS a step before they are used, and what is done beside a step stays between its fences, where
+    // the compiler deals it out among the matrix instructions.  One wavefront a SIMD has nothing else to fill the waits with: 3 prompts
+    // of documents, fp32, d = 128: 108 -> 99 us; d = 64, two a SIMD: 63 -> 60 us.  A bf16 cache's kernel has no registers left for
+    // it: a prompt of 4096 with a window takes 152 us without and 194 us with it.
+    constexpr bool FENCED = !BF16;
+    auto fence = [] { if constexpr (FENCED) __builtin_amdgcn_sched_barrier(0); };
+    struct Operand {
+        u32x4 of[PLANES], third;
+    };
+    auto key_operand = [&](int buffer, int c, Operand &a) {
+#pragma unroll
+        for (int p = 0; p < PLANES; p++) a.of[p] = *reinterpret_cast<const u32x4 *>(&lds.k[buffer][p][col * K_PITCH + 16 * c + 8 * h]);
+        if constexpr (Lds::Q_HERE) a.third = *reinterpret_cast<const u32x4 *>(q_here + 16 * c);
+    };
+    auto value_operand = [&](int buffer, int step, Operand &a) {
+#pragma unroll
+        for (int w = 0; w < PLANES; w++)
+            a.of[w] = *reinterpret_cast<const u32x4 *>(&lds.v[buffer][w][(32 * (step % PARTS) + col) * V_PITCH + 16 * (step / PARTS) + 8 * h]);
+    };
+    auto first_product = [&](int buffer, auto beside) {
 #pragma unroll
         for (int r = 0; r < 16; r++) st[r] = 0.0f;
+        Operand a[2];
+        if (FENCED) key_operand(buffer, 0, a[0]);
 #pragma unroll
         for (int c = 0; c < STEPS; c++) {
-            u32x4 k[PLANES];
-#pragma unroll
-            for (int p = 0; p < PLANES; p++) k[p] = *reinterpret_cast<const u32x4 *>(&lds.k[buffer][p][col * K_PITCH + 16 * c + 8 * h]);
-            u32x4 third;
-            if constexpr (Lds::Q_HERE) third = *reinterpret_cast<const u32x4 *>(q_here + 16 * c);
-            else third = q[2][c];
-            multiply(k, q[0][c], q[1][c], third, st);
+            if (!FENCED) key_operand(buffer, c, a[c & 1]);
+            else if (c + 1 < STEPS) key_operand(buffer, c + 1, a[(c + 1) & 1]);
+            if constexpr (Lds::Q_HERE) multiply(a[c & 1].of, q[0][c], q[1][c], a[c & 1].third, st);
+            else multiply(a[c & 1].of, q[0][c], q[1][c], q[2][c], st);
+            beside(c);
+            fence();
         }
     };
 
     if (tiles > 0) {
         clear_unseen(0);
-        park_keys(0), park_values(0);
+        park(0, PARKED, 0, 0);
         if (tiles > 1) {
             fetch_keys(next);
-            park_keys(1);
+            park(0, K_EACH, 1, 0);
         }
         __syncthreads();
-        if (mine_from == 0) first_product(0);
+        if (mine_from == 0) first_product(0, [](int) {});
     }
     // Tile i: its scores are in registers, its values and the next tile's keys in LDS.  The next tile's first product runs beside the
     // exponentials and splits of this one's weights, this one's second product beside the staging of the tiles behind: the matrix
@@ -1000,33 +1023,41 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             }
             const float base = top == -INFINITY ? 0.0f : top;
             if (i + 1 == tiles - 1) clear_unseen(i + 1);
-            first_product((i + 1) & 1);
+            Operand v[2];
             u32x4 p[2][3];
+            auto weights = [&](int from, int to) {  // pairs of them
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float a = exp2_fast(x[8 * u + 2 * e] - base), b = exp2_fast(x[8 * u + 2 * e + 1] - base);
+                for (int n = from; n < to; n++) {
+                    const float a = exp2_fast(x[2 * n] - base), b = exp2_fast(x[2 * n + 1] - base);
                     total += a;
                     total += b;
                     uint32_t w[3];
                     split_pair(a, b, w[0], w[1], w[2]);
-                    p[u][0][e] = w[0], p[u][1][e] = w[1], p[u][2][e] = w[2];
+#pragma unroll
+                    for (int e = 0; e < 3; e++) p[n / 4][e][n % 4] = w[e];
                 }
+            };
+            if (!FENCED) weights(0, 8);
+            fence();
+            first_product((i + 1) & 1, [&](int c) {
+                if (!FENCED) return;
+                if (c + 1 == STEPS) value_operand(i & 1, 0, v[0]);
+                weights(8 * c / STEPS, 8 * (c + 1) / STEPS);
+            });
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int t = 0; t < PARTS; t++) {
-                    u32x4 v[PLANES];
-#pragma unroll
-                    for (int w = 0; w < PLANES; w++) v[w] = *reinterpret_cast<const u32x4 *>(&lds.v[i & 1][w][(32 * t + col) * V_PITCH + 16 * u + 8 * h]);
-                    multiply(v, p[u][0], p[u][1], p[u][2], acc[t]);
-                }
-            park_keys(i & 1), park_values((i + 1) & 1);
+            for (int step = 0; step < 2 * PARTS; step++) {
+                if (!FENCED) value_operand(i & 1, step, v[step & 1]);
+                else if (step + 1 < 2 * PARTS) value_operand(i & 1, step + 1, v[(step + 1) & 1]);
+                const auto &w = p[step / PARTS];
+                multiply(v[step & 1].of, w[0], w[1], w[2], acc[step % PARTS]);
+                if (FENCED) park(step * PARKED / (2 * PARTS), (step + 1) * PARKED / (2 * PARTS), i & 1, (i + 1) & 1);
+                fence();
+            }
+            if (!FENCED) park(0, PARKED, i & 1, (i + 1) & 1);
         } else {
-            if (i + 1 == mine_from) first_product((i + 1) & 1);
+            if (i + 1 == mine_from) first_product((i + 1) & 1, [](int) {});
             if (i + 1 == tiles - 1) clear_unseen(i + 1);
-            park_keys(i & 1), park_values((i + 1) & 1);
+            park(0, PARKED, i & 1, (i + 1) & 1);
         }
     }
     {
