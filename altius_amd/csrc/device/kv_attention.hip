@@ -703,13 +703,14 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, h = lane >> 5;
 
-    // The last rows of a causal sequence see most keys: they start first.  Blocks that follow each other work on different heads.
+    // The last rows of a causal sequence see most keys: they start first.  Of documents whose first keys are open to all rows (or later
+    // ones to earlier rows) the first rows see most.  Blocks that follow each other work on different heads.
     const Share &share = g.many;
     const uint32_t kvh = id % g.kv.kv_heads;
     id /= g.kv.kv_heads;
     const uint32_t s = id % g.kv.sequences;
     id /= g.kv.sequences;
-    const uint32_t split = id % share.splits, tile = share.row_tiles - 1 - id / share.splits;
+    const uint32_t split = id % share.splits, order = id / share.splits, tile = g.first_keys && (g.prefix || !g.causal) ? order : share.row_tiles - 1 - order;
 
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
@@ -891,21 +892,62 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
     u32x4 q[Lds::Q_HERE ? 2 : 3][STEPS];
     uint16_t *q_here = &lds.q[Lds::Q_HERE ? wave : 0][Lds::Q_HERE ? col * K_PITCH + 8 * h : 0];
+    if constexpr (Lds::Q_HERE) {
+        // A row of queries by DP / 4 lanes side by side, all loads on their way at once, then part by part through LDS, where the third
+        // ones stay.  (A lane that reads its own row asks for 64 lines with each load.)
+        constexpr int UNITS = 32 * (DP / 4) / 64;
+        const int64_t mine = (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
+        f32x4 whole[UNITS];
+        auto row_unit = [&](int e) { return (64 * e + lane) / (DP / 4); };
+        auto channel_unit = [&](int e) { return 4 * ((64 * e + lane) % (DP / 4)); };
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-        const uint32_t c = 16 * i + 8 * h;
-        f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
-        if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
-        if (valid && c + 4 < g.d) hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4) * g.scale;
-        uint32_t w[3][4];
+        for (int e = 0; e < UNITS; e++) {
+            const uint32_t low_word = __shfl((int32_t)mine, row_unit(e)), high_word = __shfl((int32_t)(mine >> 32), row_unit(e));
+            whole[e] = *reinterpret_cast<const f32x4 *>(g.q + (int64_t)((uint64_t)high_word << 32 | low_word) + (channel_unit(e) < g.d ? channel_unit(e) : 0));
+        }
+        const float scale = g.scale;
+        u32x2 third[UNITS], second[UNITS];
+        uint16_t *shared = lds.q[wave];
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            split_pair(lo[2 * e], lo[2 * e + 1], w[0][e], w[1][e], w[2][e]);
-            split_pair(hi[2 * e], hi[2 * e + 1], w[0][2 + e], w[1][2 + e], w[2][2 + e]);
+        for (int e = 0; e < UNITS; e++) {
+            const float by = channel_unit(e) < g.d ? scale : 0.0f;
+            uint32_t w[3][2];
+            split_pair(whole[e][0] * by, whole[e][1] * by, w[0][0], w[1][0], w[2][0]);
+            split_pair(whole[e][2] * by, whole[e][3] * by, w[0][1], w[1][1], w[2][1]);
+            *reinterpret_cast<u32x2 *>(shared + row_unit(e) * K_PITCH + channel_unit(e)) = u32x2{w[0][0], w[0][1]};
+            second[e] = u32x2{w[1][0], w[1][1]}, third[e] = u32x2{w[2][0], w[2][1]};
+        }
+        auto wait = [] { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"), __builtin_amdgcn_wave_barrier(); };
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            wait();
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) q[p][i] = *reinterpret_cast<const u32x4 *>(q_here + 16 * i);
+            wait();
+#pragma unroll
+            for (int e = 0; e < UNITS; e++) *reinterpret_cast<u32x2 *>(shared + row_unit(e) * K_PITCH + channel_unit(e)) = p == 0 ? second[e] : third[e];
+        }
+        wait();
+    } else {
+        f32x4 lo[STEPS], hi[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            const uint32_t c = 16 * i + 8 * h;
+            lo[i] = *reinterpret_cast<const f32x4 *>(q_row + (c < g.d ? c : 0)), hi[i] = *reinterpret_cast<const f32x4 *>(q_row + (c + 4 < g.d ? c + 4 : 0));
         }
 #pragma unroll
-        for (int p = 0; p < (Lds::Q_HERE ? 2 : 3); p++) q[p][i] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
-        if (Lds::Q_HERE) *reinterpret_cast<u32x4 *>(q_here + 16 * i) = u32x4{w[2][0], w[2][1], w[2][2], w[2][3]};
+        for (int i = 0; i < STEPS; i++) {
+            const uint32_t c = 16 * i + 8 * h;
+            const float by[2] = {c < g.d ? g.scale : 0.0f, c + 4 < g.d ? g.scale : 0.0f};
+            uint32_t w[3][4];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                split_pair(lo[i][2 * e] * by[0], lo[i][2 * e + 1] * by[0], w[0][e], w[1][e], w[2][e]);
+                split_pair(hi[i][2 * e] * by[1], hi[i][2 * e + 1] * by[1], w[0][2 + e], w[1][2 + e], w[2][2 + e]);
+            }
+#pragma unroll
+            for (int p = 0; p < 3; p++) q[p][i] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
+        }
     }
 
     float top = -INFINITY, total = 0.0f;
