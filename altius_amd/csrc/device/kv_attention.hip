@@ -32,14 +32,15 @@ constexpr float LOG2E = 1.44269504088896341f;
 // The maximum that weights are relative to stays until one is this much (in powers of two) above it: fp32 holds weights up to 2^8 as
 // exactly as those up to 1, and most of the rescaling of what has been summed falls away.
 constexpr float SLACK = 8.0f;
-// Sequences with at most so many rows for a kv head share their keys' blocks out (attend_rows16, SPLIT); longer ones have
-// blocks enough.
-constexpr uint32_t FEW_ROWS = 64;
+// Sequences with at most so many rows for a kv head go 16 rows a block (attend_rows16, SPLIT), longer ones 128 (rows128): FEW_ROWS, or
+// FEW_BESIDE_CUT in a batch whose longer ones' keys are cut as well.
+constexpr uint32_t FEW_ROWS = 64, FEW_BESIDE_CUT = 16;
+constexpr int TILE_ROWS = 128;  // a block's, of the longer ones
 
-// How the blocks share the work on the sequences of one kind: row tiles, and splits of split_keys keys each.  Where there are
-// several, the partial results of (sequence, kv head, row < rows, split) wait in the workspace: maximum and sum, and the weighted
-// sum of values.  The sequences of few rows are cut otherwise (part_of): there splits is 1 or 2, not cut or cut, a block's part has
-// split_keys keys at least, and at_once blocks are at work at once.
+// How the blocks share the work on the sequences of one kind.  splits 1: a block per (sequence, kv head, row tile).  Else their keys are
+// cut (part_of) so that at_once blocks, which are at work at once, have parts of about the same size, of split_keys keys at least, and
+// the partial results of a part's rows wait in the workspace in the place of its number: maximum and sum, and the weighted sum of
+// values.
 struct Share {
     uint32_t row_tiles, splits, split_keys, rows;
     uint32_t blocks, at_once;
@@ -51,14 +52,14 @@ struct AttendArgs {
     const float *q;
     float *out;
     int64_t q_token, q_head, out_token, out_head;
-    uint32_t q_heads, group, d;
+    uint32_t q_heads, group, d, few_rows;
     dev::FastDiv by_group;
     float scale, cap;  // scale: with log2(e), or by the cap where there is one; cap: 0, or the cap with log2(e)
     int causal, window;
     const float *slopes;
     const int32_t *prefix, *first_keys;
     uint32_t max_tokens, max_keys;
-    Share few, many;  // of sequences with up to FEW_ROWS rows, and with more
+    Share few, many;  // of sequences with up to few_rows rows, and with more
 };
 
 // The sequence, with n == 0 where the call's bounds leave it out (too long for them: the flag is raised).
@@ -204,24 +205,24 @@ template <int DP, bool BF16> struct RowLds {
     float stats[ROW_WAVES][2][16];
 };
 
-// The keys of sequences of few rows, cut into parts of about the same size, one a block, whatever the sequences' lengths.  In units of 64
-// keys: a part is as large as leaves no more parts than blocks that are at work at once, as far as the pairs (row tiles x kv
+// The keys of the sequences of one kind, cut into parts of about the same size, one a block, whatever the sequences' lengths.  In
+// units of 64 keys: a part is as large as leaves no more parts than blocks that are at work at once, as far as the pairs (row tiles x kv
 // heads of all sequences), which are cut one by one, allow.  Every block finds its part for itself, from the lengths, by a scan over the
-// sequences, 64 at a time; its partial results wait in the place of its number.
+// sequences, 64 at a time.
 constexpr uint32_t UNIT = 64;
 struct SequenceWork {
     uint32_t units, pairs;  // units of one pair; pairs
     int32_t begin;          // the first unit's first key
 };
-__device__ __forceinline__ SequenceWork sequence_work(const AttendArgs &g, uint32_t s) {
+template <bool FEW> __device__ __forceinline__ SequenceWork sequence_work(const AttendArgs &g, uint32_t s) {
     SequenceWork w = {0, 0, 0};
     if (s >= g.kv.sequences) return w;
     const dev::KvSequence q = sequence_of(g, s);
     const uint32_t rows = (uint32_t)q.n * g.group;
-    if (rows == 0 || rows > FEW_ROWS) return w;
+    if (rows == 0 || (rows <= g.few_rows) != FEW) return w;
     if (g.window) w.begin = max(0, max(0, q.length - q.n) - g.window + 1) & ~(int32_t)(UNIT - 1);
     w.units = max(1u, (uint32_t)(q.length - w.begin + (int32_t)UNIT - 1) / UNIT);
-    w.pairs = (rows + 15) / 16 * g.kv.kv_heads;
+    w.pairs = (rows + (FEW ? 15 : TILE_ROWS - 1)) / (FEW ? 16 : TILE_ROWS) * g.kv.kv_heads;
     return w;
 }
 __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // over the lanes up to this one
@@ -234,17 +235,18 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // over the lanes
     return v;
 }
 // The units of a part: the least of a few that leave no more parts than blocks at work at once, so that few of those go without one.
-__device__ __forceinline__ uint32_t part_of(const AttendArgs &g, const SequenceWork &first) {
+template <bool FEW> __device__ __forceinline__ uint32_t part_of(const AttendArgs &g, const SequenceWork &first) {
+    const Share &share = FEW ? g.few : g.many;
     auto sum = [&](auto of) {
         uint32_t total = 0;
         for (uint32_t base = 0; base < g.kv.sequences; base += 64)
-            total += __builtin_amdgcn_readlane(wave_prefix(of(base ? sequence_work(g, base + (threadIdx.x & 63u)) : first)), 63);
+            total += __builtin_amdgcn_readlane(wave_prefix(of(base ? sequence_work<FEW>(g, base + (threadIdx.x & 63u)) : first)), 63);
         return total;
     };
     const uint32_t units = sum([](const SequenceWork &w) { return w.units * w.pairs; });
-    uint32_t part = max((units + g.few.at_once - 1) / g.few.at_once, g.few.split_keys / UNIT);
+    uint32_t part = max((units + share.at_once - 1) / share.at_once, share.split_keys / UNIT);
     for (int i = 0; i < 4; i++) {
-        if (sum([&](const SequenceWork &w) { return (w.units + part - 1) / part * w.pairs; }) <= g.few.at_once) break;
+        if (sum([&](const SequenceWork &w) { return (w.units + part - 1) / part * w.pairs; }) <= share.at_once) break;
         part += (part + 15) / 16;
     }
     return part;
@@ -252,15 +254,21 @@ __device__ __forceinline__ uint32_t part_of(const AttendArgs &g, const SequenceW
 struct Found {
     uint32_t s, before, parts;  // of a pair; before: the sequence's first block
     SequenceWork work;
+    __device__ __forceinline__ int32_t first_key(uint32_t part) const {
+        return work.begin + (int32_t)((uint32_t)((uint64_t)part * work.units / parts) * UNIT);
+    }
+    __device__ __forceinline__ uint32_t part_with(int32_t key) const {  // the last part that starts at that key's unit or in front of it
+        return (uint32_t)(((uint64_t)((uint32_t)(key - work.begin) / UNIT + 1) * parts - 1) / work.units);
+    }
 };
 // The sequence that a block is at work on, or, by_sequence, the one asked for.  False where there is none.
-__device__ __forceinline__ bool find(const AttendArgs &g, bool by_sequence, uint32_t what, Found &f) {
-    const SequenceWork first = sequence_work(g, threadIdx.x & 63u);
-    const uint32_t part = part_of(g, first);
+template <bool FEW> __device__ __forceinline__ bool find(const AttendArgs &g, bool by_sequence, uint32_t what, Found &f) {
+    const SequenceWork first = sequence_work<FEW>(g, threadIdx.x & 63u);
+    const uint32_t part = part_of<FEW>(g, first);
     uint32_t before = 0;
     for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
         const uint32_t s = base + (threadIdx.x & 63u);
-        const SequenceWork w = base ? sequence_work(g, s) : first;
+        const SequenceWork w = base ? sequence_work<FEW>(g, s) : first;
         const uint32_t parts = (w.units + part - 1) / part, up_to = wave_prefix(parts * w.pairs);
         const uint64_t here = __ballot(by_sequence ? s == what : before + up_to > what);
         if (here) {
@@ -297,7 +305,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
 
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
-    if ((rows <= FEW_ROWS) != SPLIT || tile * 16 >= rows) return;
+    if ((rows <= g.few_rows) != SPLIT || tile * 16 >= rows) return;
     const uint32_t row = tile * 16 + col;
     const bool valid = row < rows;
     const uint32_t token = g.by_group.div(valid ? row : 0), head = kvh * g.group + (valid ? row : 0) - token * g.group;
@@ -655,11 +663,10 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
         return;
     }
     Found f;
-    if (!find(g, false, id, f)) return;
+    if (!find<true>(g, false, id, f)) return;
     const uint32_t inside = id - f.before, pair = inside / f.parts, part = inside - pair * f.parts;
     piece.s = f.s, piece.tile = pair / g.kv.kv_heads, piece.kvh = pair - piece.tile * g.kv.kv_heads;
-    auto key = [&](uint32_t p) { return f.work.begin + (int32_t)((uint32_t)((uint64_t)p * f.work.units / f.parts) * UNIT); };
-    piece.from = key(part), piece.to = part + 1 == f.parts ? INT32_MAX : key(part + 1);
+    piece.from = f.first_key(part), piece.to = part + 1 == f.parts ? INT32_MAX : f.first_key(part + 1);
     piece.whole = f.parts == 1;
     piece.slot = id;
     piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds);
@@ -679,7 +686,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ?
 // above; so are the values of an fp32 cache, split on their way into LDS, and six products of the parts are what fp32 holds of the
 // whole (the three left out are below 2^-24 of it).  A bf16 cache's values are one number: three products.
 //   Two tiles of each operand in LDS, one barrier a tile.
-constexpr int TILE_ROWS = 128, TILE_KEYS = 32;
+constexpr int TILE_KEYS = 32;
 
 #define ALTIUS_MFMA32_BF16(A, B, C) \
     C = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, A), __builtin_bit_cast(bf16x8, B), C, 0, 0, 0)
@@ -703,18 +710,29 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, h = lane >> 5;
 
-    // The last rows of a causal sequence see most keys: they start first.  Of documents whose first keys are open to all rows (or later
-    // ones to earlier rows) the first rows see most.  Blocks that follow each other work on different heads.
     const Share &share = g.many;
-    const uint32_t kvh = id % g.kv.kv_heads;
-    id /= g.kv.kv_heads;
-    const uint32_t s = id % g.kv.sequences;
-    id /= g.kv.sequences;
-    const uint32_t split = id % share.splits, order = id / share.splits, tile = g.first_keys && (g.prefix || !g.causal) ? order : share.row_tiles - 1 - order;
+    uint32_t kvh, s, tile;
+    int32_t from = 0, to = INT32_MAX;
+    bool whole = true;
+    if (share.splits == 1) {
+        // The last rows of a causal sequence see most keys: they start first.  Of documents whose first keys are open to all rows (or
+        // later ones to earlier rows) the first rows see most.  Blocks that follow each other work on different heads.
+        kvh = id % g.kv.kv_heads;
+        const uint32_t outer = id / g.kv.kv_heads, order = outer / g.kv.sequences;
+        s = outer % g.kv.sequences;
+        tile = g.first_keys && (g.prefix || !g.causal) ? order : share.row_tiles - 1 - order;
+    } else {
+        Found f;
+        if (!find<false>(g, false, id, f)) return;
+        const uint32_t inside = id - f.before, pair = inside / f.parts, part = inside - pair * f.parts;
+        s = f.s, tile = pair / g.kv.kv_heads, kvh = pair - tile * g.kv.kv_heads;
+        from = f.first_key(part), to = part + 1 == f.parts ? INT32_MAX : f.first_key(part + 1);
+        whole = f.parts == 1;
+    }
 
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
-    if (rows <= FEW_ROWS || tile * TILE_ROWS >= rows) return;
+    if (rows <= g.few_rows || tile * TILE_ROWS >= rows) return;
     const uint32_t row = tile * TILE_ROWS + wave * 32 + col;
     const bool valid = row < rows;
     const uint32_t token = g.by_group.div(valid ? row : 0), head = kvh * g.group + (valid ? row : 0) - token * g.group;
@@ -734,8 +752,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     int32_t begin = INT32_MAX, end = 0;
 #pragma unroll
     for (int w = 0; w < 4; w++) begin = min(begin, lds.bounds[w][0]), end = max(end, lds.bounds[w][1]);
-    if (share.splits > 1)
-        begin = max(begin, (int32_t)(split * share.split_keys)), end = min(end, (int32_t)min((uint64_t)INT32_MAX, (uint64_t)(split + 1) * share.split_keys));
+    begin = max(begin, from), end = min(end, to);
     begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
     any_low = max(begin, __builtin_amdgcn_readfirstlane(any_low)), any_high = min(end, __builtin_amdgcn_readfirstlane(any_high));
     all_low = max(begin, __builtin_amdgcn_readfirstlane(all_low)), all_high = min(end, __builtin_amdgcn_readfirstlane(all_high));
@@ -1144,9 +1161,8 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     }
 
     if (!valid) return;
-    const bool whole = share.splits == 1;
-    const size_t at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits + split;
-    float *to = whole ? g.out + (int64_t)(seq.start + (int32_t)token) * g.out_token + (int64_t)head * g.out_head : share.part_out + at * g.d;
+    const size_t at = (size_t)id * TILE_ROWS + wave * 32 + col;
+    float *const row_out = whole ? g.out + (int64_t)(seq.start + (int32_t)token) * g.out_token + (int64_t)head * g.out_head : share.part_out + at * g.d;
     const float factor = !whole ? 1.0f : 1.0f / total;
     if (!whole && h == 0) share.part_stats[2 * at] = top, share.part_stats[2 * at + 1] = total;
 #pragma unroll
@@ -1156,7 +1172,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
             const uint32_t c = 32 * t + 8 * b + 4 * h;
             if (c >= g.d) continue;
             f32x4 o = {acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3]};
-            *reinterpret_cast<f32x4 *>(to + c) = !whole ? o : sees ? o * factor : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            *reinterpret_cast<f32x4 *>(row_out + c) = !whole ? o : sees ? o * factor : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 }
 
@@ -1182,14 +1198,15 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_b
     const bool few = blockIdx.x < few_blocks;
     const Share &share = few ? g.few : g.many;
     const uint32_t lanes = g.d / 4, groups = JOIN / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
-    uint32_t id = few ? blockIdx.x : (blockIdx.x - few_blocks) * groups + group;
-    const uint32_t row = id % share.rows;
-    id /= share.rows;
-    const uint32_t kvh = id % g.kv.kv_heads, s = id / g.kv.kv_heads;
-    if (s >= g.kv.sequences || (!few && group >= groups)) return;
+    const uint32_t id = few ? blockIdx.x : blockIdx.x - few_blocks, chunks = few ? share.rows : (share.rows + groups - 1) / groups;
+    const uint32_t outer = id / chunks, row = few ? id - outer * chunks : (id - outer * chunks) * groups + group;
+    const uint32_t kvh = outer % g.kv.kv_heads, s = outer / g.kv.kv_heads;
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
-    if ((rows <= FEW_ROWS) != few || row >= rows) return;
+    if ((rows <= g.few_rows) != few || row - (few ? 0 : group) >= rows) return;
+    Found f;
+    if (!(few ? find<true>(g, true, s, f) : find<false>(g, true, s, f)) || f.parts <= 1) return;  // one block did it all
+    if (!few && (group >= groups || row >= rows)) return;
     const uint32_t t = g.by_group.div(row), h = kvh * g.group + row - t * g.group;
     const RowRange of = row_range(g, seq, s, t);
     float *to = g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + 4 * lane;
@@ -1198,18 +1215,13 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_b
         if (!few || group == 0) *reinterpret_cast<f32x4 *>(to) = zero;
         return;
     }
-    uint32_t count, apart;  // partial results, and how many rows they are apart
-    size_t at;
-    if (few) {
-        Found f;
-        if (!find(g, true, s, f) || f.parts <= 1) return;  // one block did it all
-        count = f.parts;
-        at = (size_t)(f.before + (row / 16 * g.kv.kv_heads + kvh) * f.parts) * 16 + row % 16, apart = 16;
-    } else {
-        const uint32_t from = (uint32_t)of.low / share.split_keys;
-        count = (uint32_t)(of.high - 1) / share.split_keys + 1 - from;
-        at = (((size_t)s * g.kv.kv_heads + kvh) * share.rows + row) * share.splits + from, apart = 1;
+    // Partial results, and how many rows they are apart.  A row of few has all; of more, those of the keys that it sees.
+    uint32_t count = f.parts, apart = 16, first = 0, tile = row / 16, inside = row % 16;
+    if (!few) {
+        first = f.part_with(of.low), count = f.part_with(of.high - 1) + 1 - first;
+        apart = TILE_ROWS, tile = row / TILE_ROWS, inside = row % TILE_ROWS;
     }
+    const size_t at = (size_t)(f.before + (tile * g.kv.kv_heads + kvh) * f.parts + first) * apart + inside;
     const float *stats = share.part_stats + 2 * at;
     const f32x4 *parts = reinterpret_cast<const f32x4 *>(share.part_out + at * g.d) + lane;
     const size_t stats_apart = 2 * apart, parts_apart = (size_t)apart * lanes;
@@ -1257,6 +1269,7 @@ constexpr int TILE_CHANNELS = 128;
 
 struct Plan {
     Share few, many;  // their pointers from the start of the workspace, as yet
+    uint32_t few_rows;
     size_t bytes;
 };
 
@@ -1269,50 +1282,30 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const uint32_t rows = (uint32_t)std::min(max_tokens * group, (size_t)1 << 30);
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256, pairs = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads;
     const uint64_t key_bytes = 2 * (uint64_t)cache.head_size * (cache.elem == AHIP_KV_BF16 ? 2 : 4);
-    auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, uint64_t wanted_blocks, uint64_t least) {
-        least = std::max<uint64_t>(least, (max_keys + MOST_SPLITS - 1) / MOST_SPLITS);
+    auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, bool cut, uint64_t at_once, uint64_t least) {
         s.rows = most_rows;
         s.row_tiles = (most_rows + tile - 1) / tile;
-        const uint64_t blocks = std::max<uint64_t>(1, pairs * s.row_tiles), splits = std::max<uint64_t>(1, wanted_blocks / blocks);
-        const uint64_t each = (std::max<uint64_t>(least, (max_keys + splits - 1) / splits) + 63) / 64 * 64;
-        s.split_keys = (uint32_t)std::min<uint64_t>(each, (uint64_t)1 << 31);
-        s.splits = (uint32_t)std::max<uint64_t>(1, (max_keys + s.split_keys - 1) / s.split_keys);
-        s.blocks = (uint32_t)std::min<uint64_t>(blocks * s.splits, UINT32_MAX);
-        if (s.splits > 1) {
-            const size_t parts = pairs * s.rows * s.splits;
-            s.part_stats = reinterpret_cast<float *>(p.bytes);
-            p.bytes += (2 * parts * sizeof(float) + 15) / 16 * 16;
-            s.part_out = reinterpret_cast<float *>(p.bytes);
-            p.bytes += parts * (size_t)cache.head_size * sizeof(float);
-        }
-    };
-    // Few rows: a part for each block that is at work at once, none shorter than 256 KiB of keys and values or 64 keys.
-    p.few.rows = std::min(rows, FEW_ROWS);
-    p.few.row_tiles = (p.few.rows + 15) / 16;
-    p.few.split_keys = (uint32_t)((std::max<uint64_t>(UNIT, 256 * 1024 / key_bytes) + UNIT - 1) / UNIT * UNIT);
-    const uint64_t few_pairs = pairs * p.few.row_tiles, units = few_pairs * ((max_keys + UNIT - 1) / UNIT);
-    p.few.splits = max_keys > p.few.split_keys && units < UINT32_MAX ? 2 : 1;
-    p.few.blocks = (uint32_t)std::min<uint64_t>(few_pairs, UINT32_MAX);
-    if (p.few.splits > 1) {
-        const uint64_t at_once = cus * (cache.head_size <= 64 || (cache.elem == AHIP_KV_BF16 && cache.head_size <= 128) ? 3 : cache.head_size <= 128 ? 2 : 1);
-        p.few.at_once = (uint32_t)std::min<uint64_t>(at_once, MOST_SPLITS);
+        s.split_keys = (uint32_t)((std::max<uint64_t>(UNIT, least) + UNIT - 1) / UNIT * UNIT);
+        const uint64_t tiles = pairs * s.row_tiles, units = tiles * ((max_keys + UNIT - 1) / UNIT);
+        s.splits = cut && max_keys > s.split_keys && units < UINT32_MAX ? 2 : 1;
+        s.blocks = (uint32_t)std::min<uint64_t>(tiles, UINT32_MAX);
+        if (s.splits == 1) return;
+        s.at_once = (uint32_t)std::min<uint64_t>(at_once, MOST_SPLITS);
         // No more parts than both the parts' least size and at_once allow, and one more a pair.
-        p.few.blocks = (uint32_t)(std::min<uint64_t>(p.few.at_once, units * UNIT / p.few.split_keys) + few_pairs);
-        const size_t parts = (size_t)p.few.blocks * 16;
-        p.few.part_stats = reinterpret_cast<float *>(p.bytes);
+        s.blocks = (uint32_t)(std::min<uint64_t>(s.at_once, units * UNIT / s.split_keys) + tiles);
+        const size_t parts = (size_t)s.blocks * tile;
+        s.part_stats = reinterpret_cast<float *>(p.bytes);
         p.bytes += 2 * parts * sizeof(float);
-        p.few.part_out = reinterpret_cast<float *>(p.bytes);
+        s.part_out = reinterpret_cast<float *>(p.bytes);
         p.bytes += parts * (size_t)cache.head_size * sizeof(float);
-    }
-    if (rows > FEW_ROWS) {
-        if (cache.head_size <= TILE_CHANNELS) {
-            // So many blocks are at work at once.  Fewer of them are cut until there are two rounds.
-            const uint64_t at_once = cus * (cache.elem == AHIP_KV_BF16 || cache.head_size <= 64 ? 2 : 1), blocks = std::max<uint64_t>(1, pairs * ((rows + TILE_ROWS - 1) / TILE_ROWS));
-            share(p.many, rows, TILE_ROWS, blocks < at_once / 2 ? 2 * at_once + blocks - 1 : 1, 256);
-        } else {
-            share(p.many, rows, 16, 1, 1);
-        }
-    }
+    };
+    const bool bf16 = cache.elem == AHIP_KV_BF16, tiled = cache.head_size <= TILE_CHANNELS;
+    const uint64_t many_at_once = cus * (bf16 || cache.head_size <= 64 ? 2 : 1);
+    const bool cut = tiled && pairs * ((rows + TILE_ROWS - 1) / TILE_ROWS) < many_at_once / 2;
+    if (rows > FEW_ROWS) share(p.many, rows, tiled ? TILE_ROWS : 16, cut, many_at_once, 256);
+    p.few_rows = p.many.splits > 1 ? FEW_BESIDE_CUT : FEW_ROWS;
+    // A part for each block that is at work at once, none shorter than 256 KiB of keys and values or 64 keys.
+    share(p.few, std::min(rows, p.few_rows), 16, true, cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), 256 * 1024 / key_bytes);
     return p;
 }
 
@@ -1391,14 +1384,14 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
     g.causal = attend.causal, g.window = attend.window, g.slopes = attend.slopes, g.prefix = attend.prefix, g.first_keys = attend.first_keys;
     g.max_tokens = (uint32_t)(attend.max_tokens ? std::min(attend.max_tokens, attend.tokens) : attend.tokens);
     g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
-    g.few = plan.few, g.many = plan.many;
+    g.few = plan.few, g.many = plan.many, g.few_rows = plan.few_rows;
     for (Share *s : {&g.few, &g.many})
         if (s->splits > 1) {
             s->part_stats = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_stats));
             s->part_out = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_out));
         }
     const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, groups = JOIN / (g.d / 4);
-    const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? (pairs * g.many.rows + groups - 1) / groups : 0;
+    const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? pairs * ((g.many.rows + groups - 1) / groups) : 0;
     if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_joins + many_joins >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
     // Pages of whole groups of 16 keys: a group's page is looked up once, not key by key, and its slots lie within 2^31 bytes.
