@@ -31,10 +31,14 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float LOG2E = 1.44269504088896341f;
 // The maximum that weights are relative to stays until one is this much (in powers of two) above it: fp32 holds weights up to 2^8 as
 // exactly as those up to 1, and most of the rescaling of what has been summed falls away.
+// 3 prompts of documents (d = 128, fp32): 88 us, 91 us without the slack; a prompt of 4096 with a window, bf16: 151 and 156 us.
 constexpr float SLACK = 8.0f;
 // Sequences with at most so many rows for a kv head go 16 rows a block (attend_rows16, SPLIT), longer ones 128 (rows128): FEW_ROWS, or
-// FEW_BESIDE_CUT in a batch whose longer ones' keys are cut as well.
-constexpr uint32_t FEW_ROWS = 64, FEW_BESIDE_CUT = 16;
+// FEW_BESIDE_CUT in a batch whose longer ones' keys are cut as well.  4 sequences of 4000 to 8000 keys, 8 kv heads of 128 channels,
+// fp32: 32 rows take 70 us by 16 rows a block and 91 us by 128, 64 rows 104 and 93 us, 128 rows 220 and 105 us; 32 sequences of
+// 2000 to 4000 keys in bf16: 157 and 239, 236 and 242, 384 and 252 us.  Pieces of 57 to 333 rows (5 sequences, 8 heads of 96
+// channels, fp32), the shortest by 16 rows a block, behind the others: 132 us, all by 128: 100 us.
+constexpr uint32_t FEW_ROWS = 32, FEW_BESIDE_CUT = 16;
 constexpr int TILE_ROWS = 128;  // a block's, of the longer ones
 
 // How the blocks share the work on the sequences of one kind.  splits 1: a block per (sequence, kv head, row tile).  Else their keys are
@@ -170,10 +174,15 @@ template <bool BF16> __device__ __forceinline__ float cache_value(const void *ba
 // the k slots of its instructions are declared to be keys in that order.  Keys and values go from memory into registers in the
 // layout of the instructions' first operand, without LDS: a row of keys is read along its channels, 16 bytes a lane, a row of
 // values by 16 lanes side by side, each lane's channels being rows of O^T.
+// Bound by the memory that keys and values come from: no key is read twice for 16 rows.  One row of 65536 keys, 8 kv heads of 128
+// channels, fp32 (537 MB): 107 us with the join of the parts, 5.0 TB/s, where a copy of 1 GiB reads and writes 5.2.  48 sequences of
+// 100 to 8191 bf16 keys (401 MB), 4 kv heads of 128 channels, 8 rows each, scores capped: 99 us, 4.1 TB/s.
 //   fp32 cache: v_mfma_f32_16x16x4_f32.
 //   bf16 cache: v_mfma_f32_16x16x32_bf16 over the channels and _16x16x16_bf16 over the keys; q and the weights as three bf16 numbers
 //   each, whose sum they are exactly, so that each of the three products is exact in the fp32 sum; a lane holds 4 keys x DP / 16
 //   channels of V and turns them with v_perm.
+// Tiles of 16 keys, two on their way (one for DP 256): what registers hold with two or three wavefronts a SIMD.  Tiles of 32
+// keys leave one wavefront fewer.
 constexpr int ROW_WAVES = 4, ROW_KEYS = 16;
 
 template <int DP, bool BF16> struct RowTile {
@@ -193,7 +202,6 @@ template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int 
     return BF16 ? (DP / 16) * (4 * part + r) + i : 64 * (i / 4) + 4 * (4 * part + r) + i % 4;
 }
 
-// UNIFORM: 16 keys that start at a multiple of 16 are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
 template <int DP, bool BF16> struct RowLds {
     static constexpr int PITCH = DP + 4;
     union {
@@ -294,6 +302,7 @@ struct Piece {
     uint32_t slot;
 };
 
+// UNIFORM: 16 keys that start at a multiple of 16 are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
 __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece, RowLds<DP, BF16> &lds) {
     constexpr int KT = ROW_KEYS, NACC = DP / 16, PITCH = RowLds<DP, BF16>::PITCH;
@@ -672,7 +681,7 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds);
 }
 
-// Heads of more than 128 channels have no tiles of their own yet: all their rows go 16 a wavefront.
+// Heads of more than 128 channels have no tiles of 128 rows: all their rows go 16 a wavefront (SPLIT false).
 template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
 __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ? 3 : 2) void attend_rows16(AttendArgs g) {
     __shared__ __align__(16) RowLds<DP, BF16> lds;
@@ -685,7 +694,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ?
 // second product takes its k slots in that order, in which V^T lies in LDS.  Queries and weights are three bf16 numbers each, as
 // above; so are the values of an fp32 cache, split on their way into LDS, and six products of the parts are what fp32 holds of the
 // whole (the three left out are below 2^-24 of it).  A bf16 cache's values are one number: three products.
-//   Two tiles of each operand in LDS, one barrier a tile.
+//   Two tiles of each operand in LDS, one barrier a tile.  Bound by the matrix cores, where all keys are seen: a prompt of 4096 with a
+// window of 1500 (16 heads, 4 of keys, 128 channels, bf16, capped) takes 150 us, 273 TFLOP/s of scores and sums, 820 of the
+// instructions' own, where a large bf16 product reaches 1356; 4 prompts of 1024 (12 heads of 64 channels, fp32) 59 us,
+// 109 and 650.  What is missing: half a causal sequence's tiles lie in blocks that end early, and at 64 channels the exponentials,
+// splits and staging of a tile are as much work for the vector unit as its products for the matrix cores.
 constexpr int TILE_KEYS = 32;
 
 #define ALTIUS_MFMA32_BF16(A, B, C) \
@@ -1125,7 +1138,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         total = lower + upper;
     }
 
-    // As in rows16: what is not finite is computed once more, value by value.
+    // As in piece16: what is not finite is computed once more, value by value.
     float check = total * 0.0f;
 #pragma unroll
     for (int t = 0; t < PARTS; t++)
@@ -1189,7 +1202,8 @@ __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(
 }
 
 // Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
-// channels, four a lane.  few: a block per row, whose groups of lanes deal the splits out among themselves; else a group per row.
+// channels, four a lane.  few: a block per row, whose groups of lanes deal the splits out among themselves; else a group per row.  Bound by
+// latency: the scan for a row's parts, their statistics, their sums.  10 us behind one row's 512 parts, 10 us behind 5 pieces of 57 to 333 rows.
 constexpr int JOIN = 256, MOST_SPLITS = 1024;
 __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_blocks) {
     __shared__ float factors[MOST_SPLITS];
@@ -1287,7 +1301,7 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
         s.row_tiles = (most_rows + tile - 1) / tile;
         s.split_keys = (uint32_t)((std::max<uint64_t>(UNIT, least) + UNIT - 1) / UNIT * UNIT);
         const uint64_t tiles = pairs * s.row_tiles, units = tiles * ((max_keys + UNIT - 1) / UNIT);
-        s.splits = cut && max_keys > s.split_keys && units < UINT32_MAX ? 2 : 1;
+        s.splits = cut && max_keys > 2 * s.split_keys && units < UINT32_MAX ? 2 : 1;
         s.blocks = (uint32_t)std::min<uint64_t>(tiles, UINT32_MAX);
         if (s.splits == 1) return;
         s.at_once = (uint32_t)std::min<uint64_t>(at_once, MOST_SPLITS);
@@ -1302,10 +1316,15 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const bool bf16 = cache.elem == AHIP_KV_BF16, tiled = cache.head_size <= TILE_CHANNELS;
     const uint64_t many_at_once = cus * (bf16 || cache.head_size <= 64 ? 2 : 1);
     const bool cut = tiled && pairs * ((rows + TILE_ROWS - 1) / TILE_ROWS) < many_at_once / 2;
-    if (rows > FEW_ROWS) share(p.many, rows, tiled ? TILE_ROWS : 16, cut, many_at_once, 256);
+    // Prompts whose blocks would leave half the places empty: pieces of 57 to 333 rows, up to 4858 keys, 392 us whole and 100 us cut;
+    // one prompt of 1024, 12 heads of 64 channels, 50 and 37 us.  With three quarters of the places taken (4 such prompts) the cut
+    // costs: 59 us whole, 78 us cut.  Parts of 128 keys at least: a prompt of 400, 16 heads of 128, fp32, 32 us, with 256 36 us.
+    if (rows > FEW_ROWS) share(p.many, rows, tiled ? TILE_ROWS : 16, cut, many_at_once, 128);
     p.few_rows = p.many.splits > 1 ? FEW_BESIDE_CUT : FEW_ROWS;
-    // A part for each block that is at work at once, none shorter than 256 KiB of keys and values or 64 keys.
-    share(p.few, std::min(rows, p.few_rows), 16, true, cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), 256 * 1024 / key_bytes);
+    // A part for each block that is at work at once (as many a CU as registers allow), none shorter than 128 KiB of keys and values or
+    // 64 keys: one token of 1024 keys, 12 heads of 64 channels, fp32, takes 16 us, with parts of 256 KiB 20, of 64 KiB 14 us; of 8192
+    // keys, 8 kv heads of 128: 28, 26 and 28 us.  Nothing is cut into fewer than three: 300 keys take 10 us in one and 15 us in two.
+    share(p.few, std::min(rows, p.few_rows), 16, true, cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), 128 * 1024 / key_bytes);
     return p;
 }
 
@@ -1345,6 +1364,8 @@ template <int DP, bool BF16, bool UNIFORM> int launch_tiled(DeviceCtx &ctx, cons
     return ctx.check(hipGetLastError(), "kv attention launch");
 }
 
+// By the head's channels, rounded up.  Heads of 96 channels have a size of their own: 4 prompts of 512 (16 heads, 4 of keys, fp32)
+// 46 us, at 128 channels 53 us; of 1024, bf16, 8 heads of keys: 63 and 72 us.
 template <bool BF16, bool UNIFORM> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g) {
     if (g.d <= 64) return launch_tiled<64, BF16, UNIFORM>(ctx, g);
     if (g.d <= 96) return launch_tiled<96, BF16, UNIFORM>(ctx, g);
@@ -1394,7 +1415,9 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
     const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? pairs * ((g.many.rows + groups - 1) / groups) : 0;
     if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_joins + many_joins >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
-    // Pages of whole groups of 16 keys: a group's page is looked up once, not key by key, and its slots lie within 2^31 bytes.
+    // Pages of whole groups of 16 keys: a group's page is looked up once, not key by key, and its slots lie within 2^31 bytes.  Pages of
+    // 64, 4 prompts of 1024 (12 heads of 64 channels, fp32): 61.7 us, key by key 67.5; a prompt of 4096 with a window, bf16:
+    // 156 and 166 us; one token of 65536 keys, pages of 16: 111 and 113 us.
     const bool bf16 = cache.elem == AHIP_KV_BF16, uniform = cache.page_size % 16 == 0 && cache.slot_stride < (int64_t)1 << 23;
     int rc = bf16 ? (uniform ? launch_by_size<true, true>(ctx, g) : launch_by_size<true, false>(ctx, g))
                   : (uniform ? launch_by_size<false, true>(ctx, g) : launch_by_size<false, false>(ctx, g));
