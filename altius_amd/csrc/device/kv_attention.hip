@@ -42,7 +42,7 @@ constexpr uint32_t FEW_ROWS = 32, FEW_BESIDE_CUT = 16;
 constexpr int TILE_ROWS = 128;  // a block's, of the longer ones
 
 // How the blocks share the work on the sequences of one kind.  splits 1: a block per (sequence, kv head, row tile).  Else their keys are
-// cut (part_of) so that at_once blocks, which are at work at once, have parts of about the same size, of split_keys keys at least, and
+// cut (find) so that at_once blocks, which are at work at once, have parts of about the same size, of split_keys keys at least, and
 // the partial results of a part's rows wait in the workspace in the place of its number: maximum and sum, and the weighted sum of
 // values.
 struct Share {
@@ -216,7 +216,7 @@ template <int DP, bool BF16> struct RowLds {
 // The keys of the sequences of one kind, cut into parts of about the same size, one a block, whatever the sequences' lengths.  In
 // units of 64 keys: a part is as large as leaves no more parts than blocks that are at work at once, as far as the pairs (row tiles x kv
 // heads of all sequences), which are cut one by one, allow.  Every block finds its part for itself, from the lengths, by a scan over the
-// sequences, 64 at a time.
+// sequences.
 constexpr uint32_t UNIT = 64;
 struct SequenceWork {
     uint32_t units, pairs;  // units of one pair; pairs
@@ -242,23 +242,6 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // over the lanes
     }
     return v;
 }
-// The units of a part: the least of a few that leave no more parts than blocks at work at once, so that few of those go without one.
-template <bool FEW> __device__ __forceinline__ uint32_t part_of(const AttendArgs &g, const SequenceWork &first) {
-    const Share &share = FEW ? g.few : g.many;
-    auto sum = [&](auto of) {
-        uint32_t total = 0;
-        for (uint32_t base = 0; base < g.kv.sequences; base += 64)
-            total += __builtin_amdgcn_readlane(wave_prefix(of(base ? sequence_work<FEW>(g, base + (threadIdx.x & 63u)) : first)), 63);
-        return total;
-    };
-    const uint32_t units = sum([](const SequenceWork &w) { return w.units * w.pairs; });
-    uint32_t part = max((units + share.at_once - 1) / share.at_once, share.split_keys / UNIT);
-    for (int i = 0; i < 4; i++) {
-        if (sum([&](const SequenceWork &w) { return (w.units + part - 1) / part * w.pairs; }) <= share.at_once) break;
-        part += (part + 15) / 16;
-    }
-    return part;
-}
 struct Found {
     uint32_t s, before, parts;  // of a pair; before: the sequence's first block
     SequenceWork work;
@@ -269,26 +252,77 @@ struct Found {
         return (uint32_t)(((uint64_t)((uint32_t)(key - work.begin) / UNIT + 1) * parts - 1) / work.units);
     }
 };
-// The sequence that a block is at work on, or, by_sequence, the one asked for.  False where there is none.
+// The scan over the sequences: a wavefront's own of up to 64, the whole block's of more, 256 at a time.
+constexpr uint32_t SCAN = 256;
+struct ScanLds {
+    uint32_t totals[SCAN / 64];
+    Found found;
+};
+// Sum over the threads up to this one, and over all.
+struct Sums {
+    uint32_t up_to, all;
+};
+__device__ __forceinline__ Sums scan(bool wide, uint32_t v, ScanLds &lds) {
+    Sums r;
+    r.up_to = wave_prefix(v), r.all = __builtin_amdgcn_readlane(r.up_to, 63);
+    if (!wide) return r;
+    const uint32_t wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0) lds.totals[wave] = r.all;
+    __syncthreads();
+    r.all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < SCAN / 64; w++) {
+        const uint32_t total = __builtin_amdgcn_readfirstlane(lds.totals[w]);
+        if (w < wave) r.up_to += total;
+        r.all += total;
+    }
+    return r;
+}
+// The sequence that a block is at work on, or, by_sequence, the one asked for.  False where there is none.  For whole blocks.
 template <bool FEW> __device__ __forceinline__ bool find(const AttendArgs &g, bool by_sequence, uint32_t what, Found &f) {
-    const SequenceWork first = sequence_work<FEW>(g, threadIdx.x & 63u);
-    const uint32_t part = part_of<FEW>(g, first);
+    __shared__ ScanLds lds;
+    const Share &share = FEW ? g.few : g.many;
+    const bool wide = g.kv.sequences > 64;
+    const uint32_t step = wide ? SCAN : 64, index = threadIdx.x & (step - 1);
+    const SequenceWork first = sequence_work<FEW>(g, index);
+    auto sum = [&](auto of) {
+        uint32_t total = 0;
+        for (uint32_t base = 0; base < g.kv.sequences; base += step) total += scan(wide, of(base ? sequence_work<FEW>(g, base + index) : first), lds).all;
+        return total;
+    };
+    // The units of a part: the least of a few that leave no more parts than blocks at work at once, so that few of those go without
+    // one.  (More sequences than lanes leave few anyway.)
+    const uint32_t units = sum([](const SequenceWork &w) { return w.units * w.pairs; });
+    uint32_t part = max((units + share.at_once - 1) / share.at_once, share.split_keys / UNIT);
+    for (int i = 0; i < (wide ? 0 : 4); i++) {
+        if (sum([&](const SequenceWork &w) { return (w.units + part - 1) / part * w.pairs; }) <= share.at_once) break;
+        part += (part + 15) / 16;
+    }
     uint32_t before = 0;
-    for (uint32_t base = 0; base < g.kv.sequences; base += 64) {
-        const uint32_t s = base + (threadIdx.x & 63u);
+    for (uint32_t base = 0; base < g.kv.sequences; base += step) {
+        const uint32_t s = base + index;
         const SequenceWork w = base ? sequence_work<FEW>(g, s) : first;
-        const uint32_t parts = (w.units + part - 1) / part, up_to = wave_prefix(parts * w.pairs);
-        const uint64_t here = __ballot(by_sequence ? s == what : before + up_to > what);
-        if (here) {
-            const int lane = __builtin_ctzll(here);
-            f.s = base + lane;
+        const uint32_t parts = (w.units + part - 1) / part;
+        const Sums sums = scan(wide, parts * w.pairs, lds);
+        const uint32_t mine = before + sums.up_to - parts * w.pairs;
+        if (by_sequence ? what - base < step : before + sums.all > what) {
+            if (wide) {
+                if (by_sequence ? s == what : mine <= what && what < before + sums.up_to) lds.found = {s, mine, parts, w};
+                __syncthreads();
+                f = lds.found;
+                f.s = __builtin_amdgcn_readfirstlane(f.s), f.before = __builtin_amdgcn_readfirstlane(f.before), f.parts = __builtin_amdgcn_readfirstlane(f.parts);
+                f.work.units = __builtin_amdgcn_readfirstlane(f.work.units), f.work.pairs = __builtin_amdgcn_readfirstlane(f.work.pairs);
+                f.work.begin = __builtin_amdgcn_readfirstlane(f.work.begin);
+                return true;
+            }
+            const int lane = __builtin_ctzll(__ballot(by_sequence ? s == what : what < before + sums.up_to));
+            f.s = base + lane, f.before = __builtin_amdgcn_readlane(mine, lane), f.parts = __builtin_amdgcn_readlane(parts, lane);
             f.work.units = __builtin_amdgcn_readlane(w.units, lane), f.work.pairs = __builtin_amdgcn_readlane(w.pairs, lane);
             f.work.begin = __builtin_amdgcn_readlane(w.begin, lane);
-            f.parts = __builtin_amdgcn_readlane(parts, lane);
-            f.before = before + __builtin_amdgcn_readlane(up_to, lane) - f.parts * f.work.pairs;
             return true;
         }
-        before += __builtin_amdgcn_readlane(up_to, 63);
+        before += sums.all;
     }
     return false;
 }
@@ -1278,6 +1312,8 @@ __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_b
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+constexpr uint64_t MOST_ROWS = (uint64_t)1 << 30, MOST_BLOCKS = (uint64_t)1 << 24;  // a grid ends at 2^32 threads
+
 // The largest head that blocks of 128 rows are built for.
 constexpr int TILE_CHANNELS = 128;
 
@@ -1293,7 +1329,7 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const size_t held = std::min((size_t)batch.table_pages * (size_t)cache.page_size, (size_t)INT32_MAX);
     const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
     const size_t max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
-    const uint32_t rows = (uint32_t)std::min(max_tokens * group, (size_t)1 << 30);
+    const uint32_t rows = (uint32_t)(max_tokens * group);
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256, pairs = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads;
     const uint64_t key_bytes = 2 * (uint64_t)cache.head_size * (cache.elem == AHIP_KV_BF16 ? 2 : 4);
     auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, bool cut, uint64_t at_once, uint64_t least) {
@@ -1301,7 +1337,7 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
         s.row_tiles = (most_rows + tile - 1) / tile;
         s.split_keys = (uint32_t)((std::max<uint64_t>(UNIT, least) + UNIT - 1) / UNIT * UNIT);
         const uint64_t tiles = pairs * s.row_tiles, units = tiles * ((max_keys + UNIT - 1) / UNIT);
-        s.splits = cut && max_keys > 2 * s.split_keys && units < UINT32_MAX ? 2 : 1;
+        s.splits = cut && max_keys > 2 * s.split_keys && tiles < MOST_BLOCKS && units < UINT32_MAX ? 2 : 1;
         s.blocks = (uint32_t)std::min<uint64_t>(tiles, UINT32_MAX);
         if (s.splits == 1) return;
         s.at_once = (uint32_t)std::min<uint64_t>(at_once, MOST_SPLITS);
@@ -1324,7 +1360,11 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     // A part for each block that is at work at once (as many a CU as registers allow), none shorter than 128 KiB of keys and values or
     // 64 keys: one token of 1024 keys, 12 heads of 64 channels, fp32, takes 16 us, with parts of 256 KiB 20, of 64 KiB 14 us; of 8192
     // keys, 8 kv heads of 128: 28, 26 and 28 us.  Nothing is cut into fewer than three: 300 keys take 10 us in one and 15 us in two.
-    share(p.few, std::min(rows, p.few_rows), 16, true, cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), 128 * 1024 / key_bytes);
+    // From two blocks a place on nothing is cut: the finding of the parts costs more than a last long sequence would.  bf16, 32 heads,
+    // 8 of keys, 128 channels, sequences of very different lengths: 48 of up to 8191 keys (192 blocks whole) 148 us, cut 98 us; 128 of
+    // up to 4000 (1024) 232 and 233; 512 of up to 2000 (4096) 416 and 464; 1024 of up to 1000 422 and 559 us.
+    const uint64_t few_at_once = cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), few_most = std::min(rows, p.few_rows);
+    share(p.few, (uint32_t)few_most, 16, pairs * ((few_most + 15) / 16) < 2 * few_at_once, few_at_once, 128 * 1024 / key_bytes);
     return p;
 }
 
@@ -1336,6 +1376,10 @@ int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
         return kv_fail(ctx, AHIP_ERR_SHAPE, name + std::to_string(attend->q_heads) + " query heads do not share " + std::to_string(cache->kv_heads) + " heads of keys");
     if (!std::isfinite(attend->scale) || !std::isfinite(attend->softcap) || attend->softcap < 0 || attend->window < 0)
         return kv_fail(ctx, AHIP_ERR_ARG, name + "the scale, the cap or the window is out of range");
+    // Sizes that the plan's products and the kernels' row numbers hold.
+    const uint64_t group = (uint64_t)(attend->q_heads / cache->kv_heads), most_tokens = std::min(attend->max_tokens ? attend->max_tokens : attend->tokens, attend->tokens);
+    if (most_tokens * group > MOST_ROWS) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more than 2^30 rows for a head of keys");
+    if ((uint64_t)batch->sequences * (uint64_t)cache->kv_heads >= MOST_BLOCKS) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     const bool bf16 = cache->elem == AHIP_KV_BF16;
     const int64_t unit = bf16 ? 8 : 4;
     if (cache->head_size > 256 || cache->head_size % unit) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "no kernel for heads of " + std::to_string(cache->head_size));
@@ -1413,7 +1457,7 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
         }
     const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, groups = JOIN / (g.d / 4);
     const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? pairs * ((g.many.rows + groups - 1) / groups) : 0;
-    if ((uint64_t)g.few.blocks + g.many.blocks >= (uint64_t)1 << 24 || few_joins + many_joins >= (uint64_t)1 << 24)  // a grid ends at 2^32 threads
+    if ((uint64_t)g.few.blocks + g.many.blocks >= MOST_BLOCKS || few_joins + many_joins >= MOST_BLOCKS)
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
     // Pages of whole groups of 16 keys: a group's page is looked up once, not key by key, and its slots lie within 2^31 bytes.  Pages of
     // 64, 4 prompts of 1024 (12 heads of 64 channels, fp32): 61.7 us, key by key 67.5; a prompt of 4096 with a window, bf16:

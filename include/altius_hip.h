@@ -346,8 +346,8 @@ int ahip_attention(ahip_ctx *ctx, float *o, const float *q, const float *k, cons
 #define AHIP_ROTARY_HALVES 0
 #define AHIP_ROTARY_INTERLEAVED 1
 /* Pair i of the first `dim` channels of a head, (a, b), becomes magnitude * (a cos t - b sin t, a sin t + b cos t) with
- * t = position * frequencies[i]; the other channels stay.  The angle is reduced in 64 bits, so that far positions turn
- * as exactly as near ones. */
+ * t = position * frequencies[i]; the other channels stay.  The angle is reduced in 64 bits, so that positions up to 2^28
+ * turn as exactly as near ones; |t| stays below 10^15. */
 typedef struct ahip_rotary {
     const double *frequencies; /* device, dim / 2 values: radians per position */
     int32_t dim;               /* even */

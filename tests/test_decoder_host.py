@@ -72,6 +72,27 @@ def test_attention_refuses(code, changed):
     assert e.value.code == code and str(e.value)
 
 
+@pytest.mark.parametrize("changed", [dict(tokens=(1 << 23) - 1, max_tokens=0, q_heads=8 * 129), dict(sequences=1 << 21), dict(sequences=(1 << 31) - 1, kv_heads=32767, q_heads=32767)])
+def test_attention_refuses_what_its_row_numbers_do_not_hold(changed):
+    with pytest.raises(AltiusHipError) as e:
+        workspace(**changed)
+    assert e.value.code == ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("elem", [D.KV_F32, D.KV_BF16])
+@pytest.mark.parametrize("head_size", [64, 96, 128, 256])
+def test_the_workspace_has_an_end(elem, head_size):
+    """However long the sequences and however many, no more parts are kept than blocks at work at once and one a row tile."""
+    cache = dict(elem=elem, head_size=head_size, page_stride=8 * 16 * head_size, head_stride=16 * head_size, slot_stride=head_size)
+    for sequences in (1, 3, 64, 500):
+        for max_tokens in (1, 4, 33, 400):
+            for table_pages in (1, 30, 5000, 1 << 26):
+                bytes_ = workspace(sequences=sequences, tokens=sequences * max_tokens, max_tokens=max_tokens, table_pages=table_pages, table_stride=table_pages, **cache)
+                rows = max_tokens * 4
+                few, many = 8 * sequences * -(-min(rows, 32) // 16), 8 * sequences * -(-rows // 128)
+                assert bytes_ <= ((1024 + few) * 16 + (1024 + many) * 128) * (head_size + 2) * 4
+
+
 def test_null_arguments_are_refused():
     L = _lib.lib()
     n = ctypes.c_size_t()

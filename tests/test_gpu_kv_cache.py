@@ -294,6 +294,30 @@ def test_each_mask_and_bias(here, case, elem, options, n):
     held_to_definition(got, paged, q, **options)
 
 
+MIXED = [  # n, lengths: few and many rows in one batch, whose keys are cut into parts
+    ([57, 20, 16, 33, 200, 0, 1, 9], [600, 900, 700, 64, 1500, 10, 333, 9]),
+    ([1, 40, 1, 300], [2100, 1000, 1, 300]),
+    ([300] + [1] * 60 + [17] * 9 + [34] * 2, [900] + [7 * i + 1 for i in range(60)] + [40 * i + 17 for i in range(9)] + [800, 34]),
+]
+
+
+@pytest.mark.parametrize("n,lengths", MIXED)
+@pytest.mark.parametrize("heads,kv,d,page,elem", [(2, 1, 128, 24, "f32"), (1, 1, 64, 16, "f32"), (2, 2, 96, 16, "f32"), (1, 1, 96, 40, "bf16"), (3, 1, 128, 32, "bf16"), (1, 1, 256, 16, "f32")])
+@pytest.mark.parametrize("options", [dict(), dict(window=130, cap=9.0), dict(causal=False, prefix=True), dict(first=True, slopes=True, prefix=True)])
+def test_batches_of_all_lengths(here, case, n, lengths, heads, kv, d, page, elem, options):
+    case(f"attend mixed {len(n)} heads {heads}/{kv} d {d} page {page} {elem} {sorted(options)}")
+    rng = np.random.default_rng(len(n) + d)
+    paged = Paged(rng, n, lengths, kv, d, page, elem)
+    q = rng.standard_normal((sum(n) + 3, heads, d)).astype(np.float32)
+    options = dict(options)
+    if "prefix" in options: options["prefix"] = rng.integers(-2, 500, len(n)).astype(np.int32)
+    if "first" in options: options["first"] = rng.integers(-3, 700, len(q)).astype(np.int32)
+    if "slopes" in options: options["slopes"] = np.full(heads, 0.03, np.float32)
+    got = attend(here, paged, gpu(q), max_tokens=max(n), max_keys=max(lengths), **options).cpu().numpy()
+    here.sync()
+    held_to_definition(got, paged, q, **options)
+
+
 @pytest.mark.parametrize("elem", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [[1, 1, 2], [80, 5, 30]])
 def test_rows_that_see_nothing_are_zero(here, case, elem, n):
@@ -569,6 +593,36 @@ def test_a_prompt_in_pieces_then_token_by_token(here, case, elem, norm):
         assert (np.abs(keys - want) <= bound + (2.0 ** -8 if elem == "bf16" else 0) * (np.abs(want) + bound)).all()
         raw = x[s][:done[s], heads + kv:]
         np.testing.assert_array_equal(values, bf16(raw) if elem == "bf16" else raw)
+
+
+def test_replayed_with_other_rows(here, case):
+    """One recorded attention whose sequences change from prompts to single tokens and back on the device."""
+    case("attend replayed with other rows")
+    rng = np.random.default_rng(31)
+    stream = torch.cuda.Stream()
+    for d, elem in ((128, "f32"), (64, "bf16")):
+        paged = Paged(rng, [200, 30, 1], [900, 500, 700], 1, d, 16, elem)
+        q, out = gpu(rng.standard_normal((240, 2, d)).astype(np.float32)), torch.full((240, 2, d), 5.0, device="cuda")
+        with D.Context(0, stream=stream.cuda_stream) as c:
+            call = D.KvAttend(tokens=240, q_heads=2, q=q.data_ptr(), out=out.data_ptr(), q_strides=(2 * d, d), out_strides=(2 * d, d), scale=0.125, causal=1, max_tokens=200)
+            room = D.kv_attention_workspace(c, paged.cache(), paged.batch(), call)
+            assert room > 0
+            space = torch.full((room // 4,), math.nan, device="cuda")
+            call.workspace, call.workspace_bytes = space.data_ptr(), room
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                c.kv_attention_raw(paged.cache(), paged.batch(), call)
+            for n, lengths in (([200, 30, 1], [900, 500, 700]), ([1, 1, 1], [900, 1, 12]), ([0, 200, 8], [5, 200, 880]), ([16, 17, 33], [16, 400, 33]), ([200, 0, 40], [201, 0, 40])):
+                paged.n, paged.lengths = n, lengths
+                paged.starts_on.copy_(torch.tensor(np.concatenate([[0], np.cumsum(n)]), dtype=torch.int32))
+                paged.lengths_on.copy_(torch.tensor(lengths, dtype=torch.int32))
+                out.fill_(5.0), space.fill_(math.nan)
+                torch.cuda.synchronize()
+                graph.replay()
+                torch.cuda.synchronize()
+                c.sync()
+                held_to_definition(out.cpu().numpy(), paged, q.cpu().numpy(), scale=0.125)
 
 
 def test_two_contexts_at_once(here, case):
