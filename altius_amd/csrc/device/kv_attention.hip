@@ -1360,9 +1360,9 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     // A part for each block that is at work at once (as many a CU as registers allow), none shorter than 128 KiB of keys and values or
     // 64 keys: one token of 1024 keys, 12 heads of 64 channels, fp32, takes 16 us, with parts of 256 KiB 20, of 64 KiB 14 us; of 8192
     // keys, 8 kv heads of 128: 28, 26 and 28 us.  Nothing is cut into fewer than three: 300 keys take 10 us in one and 15 us in two.
-    // From two blocks a place on nothing is cut: the finding of the parts costs more than a last long sequence would.  bf16, 32 heads,
-    // 8 of keys, 128 channels, sequences of very different lengths: 48 of up to 8191 keys (192 blocks whole) 148 us, cut 98 us; 128 of
-    // up to 4000 (1024) 232 and 233; 512 of up to 2000 (4096) 416 and 464; 1024 of up to 1000 422 and 559 us.
+    // From two blocks a place on nothing is cut: finding the parts costs more than a last long sequence does.  bf16, 128 channels, sequences
+    // of very different lengths: 48 of up to 8191 keys, 4 kv heads (192 blocks whole) 148 us, cut 98 us; with 8 kv heads 128 of up to
+    // 4000 (1024) 232 and 233; 512 of up to 2000 (4096) 416 and 464; 1024 of up to 1000 422 and 559 us.
     const uint64_t few_at_once = cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), few_most = std::min(rows, p.few_rows);
     share(p.few, (uint32_t)few_most, 16, pairs * ((few_most + 15) / 16) < 2 * few_at_once, few_at_once, 128 * 1024 / key_bytes);
     return p;
