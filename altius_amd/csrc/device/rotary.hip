@@ -425,8 +425,9 @@ int make_kv_view(DeviceCtx *ctx, const char *who, const ahip_kv_cache *cache, co
         return kv_fail(ctx, AHIP_ERR_ARG, name + ": a stride of the cache is out of range");
     if (batch->sequences < 0 || batch->table_pages < 0 || batch->table_stride < 0 || batch->table_stride > most)
         return kv_fail(ctx, AHIP_ERR_ARG, name + ": a size of the batch is out of range");
-    if ((int64_t)batch->table_pages * cache->page_size > INT32_MAX)
-        return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + ": sequences of 2^31 tokens and more are not supported");
+    // Kernels look some tiles ahead of a sequence's end.
+    if ((int64_t)batch->table_pages * cache->page_size > INT32_MAX - (1 << 16))
+        return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + ": sequences of 2^31 - 2^16 tokens and more are not supported");
     if (tokens >= ((size_t)1 << 23)) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + ": 2^23 tokens and more in a call are not supported");
     view->keys = cache->keys, view->values = cache->values;
     view->page_stride = cache->page_stride, view->head_stride = cache->head_stride, view->slot_stride = cache->slot_stride;

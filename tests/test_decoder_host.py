@@ -72,7 +72,7 @@ def test_attention_refuses(code, changed):
     assert e.value.code == code and str(e.value)
 
 
-@pytest.mark.parametrize("changed", [dict(tokens=(1 << 23) - 1, max_tokens=0, q_heads=8 * 129), dict(sequences=1 << 21), dict(sequences=(1 << 31) - 1, kv_heads=32767, q_heads=32767)])
+@pytest.mark.parametrize("changed", [dict(tokens=(1 << 23) - 1, max_tokens=0, q_heads=8 * 129), dict(sequences=1 << 21), dict(table_pages=(1 << 27) - 1, table_stride=1 << 27), dict(sequences=(1 << 31) - 1, kv_heads=32767, q_heads=32767)])
 def test_attention_refuses_what_its_row_numbers_do_not_hold(changed):
     with pytest.raises(AltiusHipError) as e:
         workspace(**changed)

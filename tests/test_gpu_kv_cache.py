@@ -384,6 +384,23 @@ def test_infinite_values_and_keys_that_are_seen(here, case, elem, n):
     assert (got[..., 5] == np.inf).all() and (got[..., 6] == -np.inf).all() and np.isfinite(got[..., :5]).all()
 
 
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("d,page", [(64, 16), (96, 24), (128, 32), (256, 16)])
+@pytest.mark.parametrize("n,lengths", [([3, 2], [40, 700]), ([70, 30], [70, 900])])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_queries_that_are_not_finite(here, case, elem, d, page, n, lengths, cap):
+    """Infinity and NaN among the queries reach their own rows and no other."""
+    case(f"attend queries not finite {elem} d {d} page {page} n {n} cap {cap}")
+    rng = np.random.default_rng(21)
+    paged = Paged(rng, n, lengths, 1, d, page, elem)
+    q = rng.standard_normal((sum(n), 2, d)).astype(np.float32)
+    for at, (channel, value) in enumerate([(0, math.inf), (d - 1, -math.inf), (3, math.nan), (d - 4, math.inf)]):
+        q[at % n[0], at % 2, channel] = value
+        q[n[0] + at % n[1], at % 2, channel] = value
+    got = attend(here, paged, gpu(q), cap=cap, max_tokens=max(n)).cpu().numpy()
+    held_to_definition(got, paged, q, cap=cap)
+
+
 def test_a_large_range_of_scores(here, case):
     case("attend peaked scores")
     rng = np.random.default_rng(21)
