@@ -41,13 +41,14 @@ constexpr float SLACK = 8.0f;
 constexpr uint32_t FEW_ROWS = 32, FEW_BESIDE_CUT = 16;
 constexpr int TILE_ROWS = 128;  // a block's, of the longer ones
 
-// How the blocks share the work on the sequences of one kind.  splits 1: a block per (sequence, kv head, row tile).  Else their keys are
-// cut (find) so that at_once blocks, which are at work at once, have parts of about the same size, of split_keys keys at least, and
-// the partial results of a part's rows wait in the workspace in the place of its number: maximum and sum, and the weighted sum of
-// values.
+// How the blocks share the work on the sequences of one kind.  Not listed: a block per (sequence, kv head, row tile of the longest
+// sequence).  Listed: the blocks go through the row tiles that there are (find).  Cut: so they do, and the keys of a row tile are
+// cut so that at_once blocks, which are at work at once, have parts of about the same size, of split_keys keys at least; the partial results
+// of a part's rows wait in the workspace in the place of its number: maximum and sum, and the weighted sum of values.
 struct Share {
-    uint32_t row_tiles, splits, split_keys, rows;
+    uint32_t row_tiles, split_keys, rows;
     uint32_t blocks, at_once;
+    bool listed, cut;
     float *part_stats, *part_out;
 };
 
@@ -299,6 +300,9 @@ template <bool FEW> __device__ __forceinline__ bool find(const AttendArgs &g, bo
         if (sum([&](const SequenceWork &w) { return (w.units + part - 1) / part * w.pairs; }) <= share.at_once) break;
         part += (part + 15) / 16;
     }
+    // Starts out of order can make more rows than the call has, and more blocks than were counted with: what is behind the last stays undone.
+    // (The flag is raised.)
+    auto fits = [&] { return f.before + (uint64_t)f.parts * f.work.pairs <= share.blocks; };
     uint32_t before = 0;
     for (uint32_t base = 0; base < g.kv.sequences; base += step) {
         const uint32_t s = base + index;
@@ -314,13 +318,13 @@ template <bool FEW> __device__ __forceinline__ bool find(const AttendArgs &g, bo
                 f.s = __builtin_amdgcn_readfirstlane(f.s), f.before = __builtin_amdgcn_readfirstlane(f.before), f.parts = __builtin_amdgcn_readfirstlane(f.parts);
                 f.work.units = __builtin_amdgcn_readfirstlane(f.work.units), f.work.pairs = __builtin_amdgcn_readfirstlane(f.work.pairs);
                 f.work.begin = __builtin_amdgcn_readfirstlane(f.work.begin);
-                return true;
+                return fits();
             }
             const int lane = __builtin_ctzll(__ballot(by_sequence ? s == what : what < before + sums.up_to));
             f.s = base + lane, f.before = __builtin_amdgcn_readlane(mine, lane), f.parts = __builtin_amdgcn_readlane(parts, lane);
             f.work.units = __builtin_amdgcn_readlane(w.units, lane), f.work.pairs = __builtin_amdgcn_readlane(w.pairs, lane);
             f.work.begin = __builtin_amdgcn_readlane(w.begin, lane);
-            return true;
+            return fits();
         }
         before += sums.all;
     }
@@ -698,7 +702,7 @@ template <int DP, bool BF16, bool UNIFORM, bool SPLIT>
 __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP, BF16> &lds) {
     const Share &share = SPLIT ? g.few : g.many;
     Piece piece = {0, 0, 0, 0, INT32_MAX, true, 0};
-    if (!SPLIT || share.splits == 1) {
+    if (!SPLIT || !share.listed) {
         const uint32_t outer = id / g.kv.kv_heads;
         piece.kvh = id - outer * g.kv.kv_heads;
         piece.tile = outer % share.row_tiles, piece.s = outer / share.row_tiles;
@@ -761,13 +765,14 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     uint32_t kvh, s, tile;
     int32_t from = 0, to = INT32_MAX;
     bool whole = true;
-    if (share.splits == 1) {
+    const bool first_rows_first = g.first_keys && (g.prefix || !g.causal);
+    if (!share.listed) {
         // The last rows of a causal sequence see most keys: they start first.  Of documents whose first keys are open to all rows (or
         // later ones to earlier rows) the first rows see most.  Blocks that follow each other work on different heads.
         kvh = id % g.kv.kv_heads;
         const uint32_t outer = id / g.kv.kv_heads, order = outer / g.kv.sequences;
         s = outer % g.kv.sequences;
-        tile = g.first_keys && (g.prefix || !g.causal) ? order : share.row_tiles - 1 - order;
+        tile = first_rows_first ? order : share.row_tiles - 1 - order;
     } else {
         Found f;
         if (!find<false>(g, false, id, f)) return;
@@ -775,6 +780,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         s = f.s, tile = pair / g.kv.kv_heads, kvh = pair - tile * g.kv.kv_heads;
         from = f.first_key(part), to = part + 1 == f.parts ? INT32_MAX : f.first_key(part + 1);
         whole = f.parts == 1;
+        if (whole && !first_rows_first) tile = f.work.pairs / g.kv.kv_heads - 1 - tile;
     }
 
     const dev::KvSequence seq = sequence_of(g, s);
@@ -1332,15 +1338,22 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const uint32_t rows = (uint32_t)(max_tokens * group);
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256, pairs = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads;
     const uint64_t key_bytes = 2 * (uint64_t)cache.head_size * (cache.elem == AHIP_KV_BF16 ? 2 : 4);
-    auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, bool cut, uint64_t at_once, uint64_t least) {
+    // tiles: no batch has more row tiles of this kind, times kv heads.
+    auto share = [&](Share &s, uint32_t most_rows, uint32_t tile, uint64_t tiles, bool cut, uint64_t at_once, uint64_t least) {
         s.rows = most_rows;
         s.row_tiles = (most_rows + tile - 1) / tile;
         s.split_keys = (uint32_t)((std::max<uint64_t>(UNIT, least) + UNIT - 1) / UNIT * UNIT);
-        const uint64_t tiles = pairs * s.row_tiles, units = tiles * ((max_keys + UNIT - 1) / UNIT);
-        s.splits = cut && max_keys > 2 * s.split_keys && tiles < MOST_BLOCKS && units < UINT32_MAX ? 2 : 1;
-        s.blocks = (uint32_t)std::min<uint64_t>(tiles, UINT32_MAX);
-        if (s.splits == 1) return;
         s.at_once = (uint32_t)std::min<uint64_t>(at_once, MOST_SPLITS);
+        const uint64_t all = pairs * s.row_tiles, units = tiles * ((max_keys + UNIT - 1) / UNIT);
+        const bool counted = tiles < MOST_BLOCKS && units < UINT32_MAX;
+        s.cut = cut && max_keys > 2 * s.split_keys && counted;
+        // A block without rows costs its place 1 us, the list 3 us a block: 200 single tokens of 1000 keys and a piece of 512 behind
+        // 1488, bf16, 32 heads, 8 of keys, 128 channels (25728 blocks, or 1512): 280 us by all blocks, 249 us by the list; 32
+        // tokens of 4000 keys and the piece (4224, or 400): 166 and 173 us.
+        s.listed = s.cut || (counted && tile == TILE_ROWS && all > tiles + 16 * at_once);
+        if (s.listed && !s.cut) s.split_keys = (uint32_t)1 << 31;
+        s.blocks = (uint32_t)std::min<uint64_t>(s.listed ? tiles : all, UINT32_MAX);
+        if (!s.cut) return;
         // No more parts than both the parts' least size and at_once allow, and one more a pair.
         s.blocks = (uint32_t)(std::min<uint64_t>(s.at_once, units * UNIT / s.split_keys) + tiles);
         const size_t parts = (size_t)s.blocks * tile;
@@ -1351,12 +1364,18 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     };
     const bool bf16 = cache.elem == AHIP_KV_BF16, tiled = cache.head_size <= TILE_CHANNELS;
     const uint64_t many_at_once = cus * (bf16 || cache.head_size <= 64 ? 2 : 1);
-    const bool cut = tiled && pairs * ((rows + TILE_ROWS - 1) / TILE_ROWS) < many_at_once / 2;
+    // A sequence of many rows has more than FEW_BESIDE_CUT, and all have no more than the call: so many tiles are full, and one a
+    // sequence is not.
+    const uint64_t all_rows = attend.tokens * (uint64_t)group, row_tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
+    const uint64_t many_tiles = (uint64_t)cache.kv_heads * std::min(batch.sequences * row_tiles, all_rows / TILE_ROWS + std::min<uint64_t>(batch.sequences, all_rows / (FEW_BESIDE_CUT + 1)));
     // Prompts whose blocks would leave half the places empty: pieces of 57 to 333 rows, up to 4858 keys, 392 us whole and 100 us cut;
     // one prompt of 1024, 12 heads of 64 channels, 50 and 37 us.  With three quarters of the places taken (4 such prompts) the cut
     // costs: 59 us whole, 78 us cut.  Parts of 128 keys at least: a prompt of 400, 16 heads of 128, fp32, 32 us, with 256 36 us.
-    if (rows > FEW_ROWS) share(p.many, rows, tiled ? TILE_ROWS : 16, cut, many_at_once, 128);
-    p.few_rows = p.many.splits > 1 ? FEW_BESIDE_CUT : FEW_ROWS;
+    if (rows > FEW_ROWS) {
+        if (tiled) share(p.many, rows, TILE_ROWS, many_tiles, many_tiles < many_at_once / 2, many_at_once, 128);
+        else share(p.many, rows, 16, pairs * ((rows + 15) / 16), false, 0, 0);
+    }
+    p.few_rows = p.many.cut ? FEW_BESIDE_CUT : FEW_ROWS;
     // A part for each block that is at work at once (as many a CU as registers allow), none shorter than 128 KiB of keys and values or
     // 64 keys: one token of 1024 keys, 12 heads of 64 channels, fp32, takes 16 us, with parts of 256 KiB 20, of 64 KiB 14 us; of 8192
     // keys, 8 kv heads of 128: 28, 26 and 28 us.  Nothing is cut into fewer than three: 300 keys take 10 us in one and 15 us in two.
@@ -1364,7 +1383,8 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     // of very different lengths: 48 of up to 8191 keys, 4 kv heads (192 blocks whole) 148 us, cut 98 us; with 8 kv heads 128 of up to
     // 4000 (1024) 232 and 233; 512 of up to 2000 (4096) 416 and 464; 1024 of up to 1000 422 and 559 us.
     const uint64_t few_at_once = cus * (cache.head_size <= 64 || (bf16 && tiled) ? 3 : tiled ? 2 : 1), few_most = std::min(rows, p.few_rows);
-    share(p.few, (uint32_t)few_most, 16, pairs * ((few_most + 15) / 16) < 2 * few_at_once, few_at_once, 128 * 1024 / key_bytes);
+    const uint64_t few_tiles = pairs * ((few_most + 15) / 16);
+    share(p.few, (uint32_t)few_most, 16, few_tiles, few_tiles < 2 * few_at_once, few_at_once, 128 * 1024 / key_bytes);
     return p;
 }
 
@@ -1451,12 +1471,12 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
     g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
     g.few = plan.few, g.many = plan.many, g.few_rows = plan.few_rows;
     for (Share *s : {&g.few, &g.many})
-        if (s->splits > 1) {
+        if (s->cut) {
             s->part_stats = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_stats));
             s->part_out = reinterpret_cast<float *>(static_cast<char *>(attend.workspace) + reinterpret_cast<uintptr_t>(s->part_out));
         }
     const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, groups = JOIN / (g.d / 4);
-    const uint64_t few_joins = g.few.splits > 1 ? pairs * g.few.rows : 0, many_joins = g.many.splits > 1 ? pairs * ((g.many.rows + groups - 1) / groups) : 0;
+    const uint64_t few_joins = g.few.cut ? pairs * g.few.rows : 0, many_joins = g.many.cut ? pairs * ((g.many.rows + groups - 1) / groups) : 0;
     if ((uint64_t)g.few.blocks + g.many.blocks >= MOST_BLOCKS || few_joins + many_joins >= MOST_BLOCKS)
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
     // Pages of whole groups of 16 keys: a group's page is looked up once, not key by key, and its slots lie within 2^31 bytes.  Pages of

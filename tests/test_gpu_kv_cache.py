@@ -58,7 +58,8 @@ class Paged:
         """Keys and values of sequence s, [length, heads, d] as fp32."""
         at = np.arange(self.lengths[s])
         page, slot = self.table[s][at // self.page], at % self.page
-        return [v.float().cpu().numpy()[page, :, slot] for v in self.views()]
+        page, slot = torch.from_numpy(page.astype(np.int64)).cuda(), torch.from_numpy(slot).cuda()
+        return [v[page, :, slot].float().cpu().numpy() for v in self.views()]
 
 
 # ---- appending -------------------------------------------------------------------------------------------------------
@@ -610,6 +611,40 @@ def test_a_prompt_in_pieces_then_token_by_token(here, case, elem, norm):
         assert (np.abs(keys - want) <= bound + (2.0 ** -8 if elem == "bf16" else 0) * (np.abs(want) + bound)).all()
         raw = x[s][:done[s], heads + kv:]
         np.testing.assert_array_equal(values, bf16(raw) if elem == "bf16" else raw)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("sequences,n,lengths,kv", [(40, 300, 500, 2), (40, 70, 4000, 8), (300, 40, 100, 1)])
+def test_starts_that_jump_back_are_told(here, case, elem, sequences, n, lengths, kv):
+    """Every other sequence takes the first rows once more: more rows in all than the call has."""
+    case(f"attend starts that jump back {elem} {sequences} of {n}")
+    rng = np.random.default_rng(32)
+    paged = Paged(rng, [0] * sequences, [lengths] * sequences, kv, 64, 64, elem)
+    paged.starts_on.copy_(torch.tensor([n if s % 2 else 0 for s in range(sequences + 1)], dtype=torch.int32))
+    q = gpu(rng.standard_normal((n + 2, kv, 64)).astype(np.float32))
+    got = attend(here, paged, q, max_tokens=n, max_keys=lengths)
+    assert (got[n:] == 5.0).all()
+    raises_at_sync(here)
+    paged.n, paged.lengths = [n] + [0] * (sequences - 1), [lengths] * sequences  # the context goes on
+    paged.starts_on.copy_(torch.tensor([0] + [n] * sequences, dtype=torch.int32))
+    got = attend(here, paged, q, max_tokens=n, max_keys=lengths).cpu().numpy()
+    here.sync()
+    held_to_definition(got, paged, q.cpu().numpy())
+
+
+def test_a_piece_beside_many_tokens(here, case):
+    """Blocks for the row tiles that there are, not for as many as the longest sequence has in each."""
+    case("attend a piece beside tokens")
+    rng = np.random.default_rng(33)
+    for elem, d, kv, options in (("f32", 64, 8, {}), ("bf16", 128, 8, dict(window=100)), ("f32", 96, 4, dict(first=True, prefix=True))):
+        n, lengths = [1] * 380 + [150] + [3, 0] * 10 + [90, 1], [60 + s % 50 for s in range(380)] + [350] + [40, 7] * 10 + [90, 1]
+        paged = Paged(rng, n, lengths, kv, d, 16, elem)
+        q = rng.standard_normal((sum(n) + 1, 4 * kv, d)).astype(np.float32)
+        options = dict(options)
+        if "first" in options: options.update(first=rng.integers(0, 60, len(q)).astype(np.int32), prefix=rng.integers(0, 200, len(n)).astype(np.int32))
+        got = attend(here, paged, gpu(q), max_tokens=150, max_keys=350, **options).cpu().numpy()
+        here.sync()
+        held_to_definition(got, paged, q, **options)
 
 
 def test_replayed_with_other_rows(here, case):
