@@ -382,12 +382,20 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     uint32_t q_at = BF16 ? col * (DP + 8) + 8 * part : col * PITCH + 4 * part;
     constexpr int Q_PART = 16 * (DP + 8);
     const float *q_row = g.q + (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
+    // All loads in front of the first use, none behind a condition: a row that is not there is read as row 0, and left out below.  One
+    // token behind 76, 12 heads of 64 channels: 6.6 us, 7.3 with a condition around each load.
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 read[DP / 16];
     if constexpr (BF16) {
 #pragma unroll
         for (int i = 0; i < DP / 32; i++) {
-            const uint32_t c = 32 * i + 8 * part;
-            f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
-            if (valid && c < g.d) lo = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale, hi = *reinterpret_cast<const f32x4 *>(q_row + c + 4) * g.scale;
+            const uint32_t c = 32 * i + 8 * part, at = c < g.d ? c : 0;
+            read[2 * i] = *reinterpret_cast<const f32x4 *>(q_row + at), read[2 * i + 1] = *reinterpret_cast<const f32x4 *>(q_row + at + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+            const bool here = valid && 32 * i + 8 * part < g.d;
+            const f32x4 lo = here ? read[2 * i] * g.scale : zero, hi = here ? read[2 * i + 1] * g.scale : zero;
             u32x4 parts[3];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -402,10 +410,10 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
         }
     } else {
 #pragma unroll
+        for (int i = 0; i < DP / 16; i++) read[i] = *reinterpret_cast<const f32x4 *>(q_row + (16 * i + 4 * part < g.d ? 16 * i + 4 * part : 0));
+#pragma unroll
         for (int i = 0; i < DP / 16; i++) {
-            const uint32_t c = 16 * i + 4 * part;
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (valid && c < g.d) x = *reinterpret_cast<const f32x4 *>(q_row + c) * g.scale;
+            const f32x4 x = valid && 16 * i + 4 * part < g.d ? read[i] * g.scale : zero;
             if constexpr (Q_HERE) *reinterpret_cast<f32x4 *>(&lds.whole_q[q_at + 16 * i]) = x;
             else q[i] = __builtin_bit_cast(u32x4, x);
         }
@@ -733,9 +741,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ?
 // above; so are the values of an fp32 cache, split on their way into LDS, and six products of the parts are what fp32 holds of the
 // whole (the three left out are below 2^-24 of it).  A bf16 cache's values are one number: three products.
 //   Two tiles of each operand in LDS, one barrier a tile.  Bound by the matrix cores, where all keys are seen: a prompt of 4096 with a
-// window of 1500 (16 heads, 4 of keys, 128 channels, bf16, capped) takes 150 us, 273 TFLOP/s of scores and sums, 820 of the
-// instructions' own, where a large bf16 product reaches 1356; 4 prompts of 1024 (12 heads of 64 channels, fp32) 59 us,
-// 109 and 650.  What is missing: half a causal sequence's tiles lie in blocks that end early, and at 64 channels the exponentials,
+// window of 1500 (16 heads, 4 of keys, 128 channels, bf16, capped) takes 148 us, 279 TFLOP/s of scores and sums, 840 of the
+// instructions' own, where a large bf16 product reaches 1356; 4 prompts of 1024 (12 heads of 64 channels, fp32) 58 us,
+// 111 and 670.  What is missing: half a causal sequence's tiles lie in blocks that end early, and at 64 channels the exponentials,
 // splits and staging of a tile are as much work for the vector unit as its products for the matrix cores.
 constexpr int TILE_KEYS = 32;
 
