@@ -436,10 +436,10 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
         const uint32_t key = (uint32_t)tile_key(i < mine ? i : mine - 1), index = g.kv.by_page_size.div(key);
         starts = ((int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
     };
-    // Where they do not: lane l has the row of key l % 16 of a tile, looked up a tile ahead of its use.  Keys behind the last that is
-    // seen have no page: the last one stands in for them.
+    // Where they do not: lane l has the row of key l % 16 of a tile, looked up a tile ahead of its use.  Keys in front of the first that
+    // is seen and behind the last may have no page: those two stand in for them.
     int32_t page_ahead = 0;
-    auto key_ahead = [&](int32_t i) { return (uint32_t)min(tile_key(i) + (int32_t)col, end - 1); };
+    auto key_ahead = [&](int32_t i) { return (uint32_t)max(begin, min(tile_key(i) + (int32_t)col, end - 1)); };
     auto look_up = [&](int32_t i) { page_ahead = g.kv.table[(int64_t)s * g.kv.table_stride + g.kv.by_page_size.div(key_ahead(i))]; };
     auto row_ahead = [&](int32_t i) {  // of tile i, whose pages are known
         const uint32_t key = key_ahead(i);
@@ -847,9 +847,10 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     auto fetch_starts = [&](int32_t from) {
         const int32_t key = (first + from) * TILE_KEYS + 16 * (int32_t)lane;
         if (!UNIFORM) return;
-        const uint32_t index = g.kv.by_page_size.div((uint32_t)min(key, end - 1));
+        // A half that nobody sees any of may have no page: it is read from the start of the cache, and left out.
+        const uint32_t index = g.kv.by_page_size.div((uint32_t)max(begin, min(key, end - 1)));
         starts = ((int64_t)g.kv.page_of(s, index, 0) * g.kv.page_stride + (int64_t)((uint32_t)key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
-        if (key >= end) starts = 0;
+        if (key >= end || key + 16 <= begin) starts = 0;
     };
     auto row_at = [&](uint32_t key) {  // elements from the start of the cache
         const uint32_t index = g.kv.by_page_size.div(key);
@@ -873,11 +874,11 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         }
         return t;
     };
-    // Where they do not: lane l has the row of key l % 32 of a tile, looked up a tile ahead of its first use.  Keys behind the last that
-    // is seen have no page: the last one stands in for them.
+    // Where they do not: lane l has the row of key l % 32 of a tile, looked up a tile ahead of its first use.  Keys in front of the first
+    // that is seen and behind the last may have no page: those two stand in for them.
     int32_t page_ahead = 0;
     int64_t rows_next = 0, rows_ahead = 0;  // bytes from the start of the cache, of tiles i + 1 and i + 2 while tile i is computed
-    auto key_ahead = [&](int32_t i) { return (uint32_t)min((first + i) * TILE_KEYS + (int32_t)col, end - 1); };
+    auto key_ahead = [&](int32_t i) { return (uint32_t)max(begin, min((first + i) * TILE_KEYS + (int32_t)col, end - 1)); };
     auto look_up = [&](int32_t i) { page_ahead = g.kv.table[(int64_t)s * g.kv.table_stride + g.kv.by_page_size.div(key_ahead(i))]; };
     auto advance = [&](int32_t i) {  // to tile i, whose pages are known
         const uint32_t key = key_ahead(i);

@@ -395,7 +395,9 @@ typedef struct ahip_kv_cache {
 /* The sequences of a call.  Rows query_starts[s] .. query_starts[s + 1] - 1 of its tensors are the newest tokens of
  * sequence s, which holds lengths[s] tokens with them; none is a sequence that sits the call out.  Rows behind the last
  * sequence's are padding: not read, and left as they are where written.  The token at place j of sequence s is in slot
- * j % page_size of page page_table[s * table_stride + j / page_size].  All three arrays are device memory. */
+ * j % page_size of page page_table[s * table_stride + j / page_size].  Entries of pages that hold no key between the first and the
+ * last one that a sequence's rows see are not used: pages that a window has left may be given to others.  All three arrays are
+ * device memory. */
 typedef struct ahip_kv_batch {
     int32_t sequences, table_pages; /* table_pages: entries of one sequence's row of the table */
     int64_t table_stride;

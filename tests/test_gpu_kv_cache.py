@@ -713,3 +713,24 @@ def test_the_same_call_gives_the_same_bits(here, case):
         first = attend(here, paged, q).cpu().numpy()
         for _ in range(3):
             np.testing.assert_array_equal(attend(here, paged, q).cpu().numpy().view(np.uint32), first.view(np.uint32))
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("d,page", [(64, 8), (64, 16), (64, 24), (64, 64), (128, 16), (96, 8), (256, 8), (256, 24)])
+@pytest.mark.parametrize("n,lengths", [([1, 3], [1000, 500]), ([100, 70], [1000, 700])])
+@pytest.mark.parametrize("mask", ["window", "first"])
+def test_pages_in_front_of_the_first_key_seen_may_be_gone(here, case, elem, d, page, n, lengths, mask):
+    """A window has left them, or no document reaches back to them: their entries, and those behind the end, hold nothing that is a page."""
+    case(f"attend released pages {elem} d {d} page {page} n {n} {mask}")
+    rng = np.random.default_rng(34)
+    paged = Paged(rng, n, lengths, 1, d, page, elem, table_pages=1008 // page + 3)
+    options = dict(window=300) if mask == "window" else dict(first=np.concatenate([np.full(m, max(0, l - m - 250), np.int32) for m, l in zip(n, lengths)]))
+    for s, (m, l) in enumerate(zip(n, lengths)):
+        low = ranges(m, l, True, options.get("window", 0), None, options["first"][sum(n[:s]):][:m] if mask == "first" else None)[0].min()
+        assert low > 100
+        paged.table_on[s, :low // page] = -1 if s else paged.pages + 7
+        paged.table_on[s, -(-l // page):] = -1
+    q = rng.standard_normal((sum(n), 2, d)).astype(np.float32)
+    got = attend(here, paged, gpu(q), **options).cpu().numpy()
+    here.sync()  # nothing to tell
+    held_to_definition(got, paged, q, **options)
