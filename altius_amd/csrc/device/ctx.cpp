@@ -110,16 +110,24 @@ int check_device_flags(DeviceCtx &ctx) {
     if (!raised[0] && !raised[1] && !raised[2]) return AHIP_OK;
     rc = ctx.check(hipMemset(ctx.flags, 0, sizeof(raised)), "hipMemset(flags)");
     if (rc) return rc;
+    // All that is raised is told at once, by the code of the first: it is cleared, and no later call would tell it.
+    int code = AHIP_OK;
+    std::string said;
+    auto tell = [&](int its_code, const char *what) {
+        if (!code) code = its_code;
+        else said += "; ";
+        said += what;
+    };
     if (raised[1]) {
         // The placement the probe measured did not hold for a launch: the product just computed is not to be
         // trusted, and the cut stays off for the rest of this context's life.
         ctx.xcd_round_robin = false;
-        return ctx.fail(AHIP_ERR_HIP, "MatMul: the slices of a tile cut along k ran on different XCDs, so their partial sums could not be "
-                                      "combined; the in-kernel cut is now switched off for this context, run the product again");
+        tell(AHIP_ERR_HIP, "MatMul: the slices of a tile cut along k ran on different XCDs, so their partial sums could not be "
+                           "combined; the in-kernel cut is now switched off for this context, run the product again");
     }
-    if (raised[2])
-        return ctx.fail(AHIP_ERR_ARG, "paged cache: a sequence's rows, length or pages do not fit the call's tensors, page table or cache");
-    return ctx.fail(AHIP_ERR_ARG, "Gather: an index is outside the gathered axis");
+    if (raised[2]) tell(AHIP_ERR_ARG, "paged cache: a sequence's rows, length or pages do not fit the call's tensors, page table or cache");
+    if (raised[0]) tell(AHIP_ERR_ARG, "Gather: an index is outside the gathered axis");
+    return ctx.fail(code, said);
 }
 
 bool stream_is_recording(const DeviceCtx &ctx) {

@@ -734,3 +734,20 @@ def test_pages_in_front_of_the_first_key_seen_may_be_gone(here, case, elem, d, p
     got = attend(here, paged, gpu(q), **options).cpu().numpy()
     here.sync()  # nothing to tell
     held_to_definition(got, paged, q, **options)
+
+
+def test_a_bad_page_and_a_bad_index_are_both_told(here, case):
+    """Two kernels raise their flags in front of one synchronisation."""
+    case("bad page beside a bad index")
+    rng = np.random.default_rng(35)
+    paged = Paged(rng, [1], [20], 1, 64, 16)
+    x = gpu(rng.standard_normal((1, 1, 64)).astype(np.float32))
+    table, index, out = torch.zeros(6, device="cuda"), torch.tensor([6], device="cuda"), torch.zeros(1, device="cuda")
+    torch.cuda.synchronize()
+    assert here.L.ahip_gather(here.handle, out.data_ptr(), table.data_ptr(), index.data_ptr(), 8, 4, 1, 6, 1, 1) == 0
+    paged.table_on[0, 1] = -1
+    append(here, paged, None, x, x)
+    with pytest.raises(AltiusHipError) as e:
+        here.sync()
+    assert e.value.code == ERR_ARG and "paged cache" in str(e.value) and "Gather" in str(e.value)
+    here.sync()  # told once
