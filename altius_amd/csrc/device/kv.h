@@ -51,9 +51,9 @@ __device__ __forceinline__ KvSequence kv_checked(const KvView &kv, int32_t start
 }
 __device__ __forceinline__ KvSequence kv_sequence(const KvView &kv, uint32_t s) { return kv_checked(kv, kv.starts[s], kv.starts[s + 1], kv.lengths[s]); }
 
-// The sequence that row `token` belongs to, kv.sequences if it is behind the last one's, and what there is to know of it.  For whole
-// wavefronts: up to 64 sequences are read at once, a lane each.  More are searched, one row per sequence first, then by cutting the range
-// in eight with loads that do not wait for each other.
+// The sequence that row `token` belongs to, kv.sequences if it is behind the last one's, 0 if it is in front of the first one's, and what
+// there is to know of it.  For whole wavefronts: up to 64 sequences are read at once, a lane each.  More are searched, one row per sequence
+// first, then by cutting the range in eight with loads that do not wait for each other.
 __device__ __forceinline__ uint32_t kv_sequence_of(const KvView &kv, uint32_t token, KvSequence &q) {
     const int32_t t = (int32_t)token;
     if (kv.sequences <= 64) {

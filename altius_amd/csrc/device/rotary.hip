@@ -101,7 +101,7 @@ __device__ __forceinline__ Slot slot_of(const dev::KvView &kv, uint32_t token, i
     place = 0;
     dev::KvSequence q = {};
     const uint32_t s = dev::kv_sequence_of(kv, token, q);
-    if (s >= kv.sequences) return slot;  // padding behind the last sequence
+    if (s >= kv.sequences || (s == 0 && (int64_t)token < q.start)) return slot;  // padding behind the last sequence or in front of the first
     const int64_t p = (int64_t)q.length - q.n + ((int64_t)token - q.start);
     if (q.n == 0 || (int64_t)token < q.start || (int64_t)token >= (int64_t)q.start + q.n || p < 0) {  // starts out of order, or shorter than its rows
         *kv.flag = 1;

@@ -393,8 +393,9 @@ typedef struct ahip_kv_cache {
 } ahip_kv_cache;
 
 /* The sequences of a call.  Rows query_starts[s] .. query_starts[s + 1] - 1 of its tensors are the newest tokens of
- * sequence s, which holds lengths[s] tokens with them; none is a sequence that sits the call out.  Rows behind the last
- * sequence's are padding: not read, and left as they are where written.  The token at place j of sequence s is in slot
+ * sequence s, which holds lengths[s] tokens with them; none is a sequence that sits the call out.  Rows in front of the first
+ * sequence's and behind the last one's are padding: not read, and left as they are where written, so that a call can take some of a
+ * larger batch's sequences.  The token at place j of sequence s is in slot
  * j % page_size of page page_table[s * table_stride + j / page_size].  Entries of pages that hold no key between the first and the
  * last one that a sequence's rows see are not used: pages that a window has left may be given to others.  All three arrays are
  * device memory. */

@@ -751,3 +751,34 @@ def test_a_bad_page_and_a_bad_index_are_both_told(here, case):
         here.sync()
     assert e.value.code == ERR_ARG and "paged cache" in str(e.value) and "Gather" in str(e.value)
     here.sync()  # told once
+
+
+@pytest.mark.parametrize("n,lengths,left", [([4, 2, 70], [20, 9, 100], 1), ([3, 0, 2], [5, 7, 40], 2), ([2] * 80, list(range(10, 90)), 7), ([5, 1], [9, 3], 2)])
+def test_some_of_a_batchs_sequences(here, case, n, lengths, left):
+    """A call whose first sequence's rows do not start at row 0: the rows in front are padding, for either operator."""
+    case(f"sequences {left} on of {len(n)}")
+    rng = np.random.default_rng(36)
+    paged = Paged(rng, n, lengths, 1, 64, 16, fill=7.0)
+    packed = rng.standard_normal((sum(n) + 2, 4, 64)).astype(np.float32)
+    on, q = gpu(packed), torch.full((sum(n) + 2, 2, 64), 5.0, device="cuda")
+    some = paged.batch()
+    some.sequences = len(n) - left
+    some.query_starts, some.lengths, some.page_table = paged.starts_on[left:].data_ptr(), paged.lengths_on[left:].data_ptr(), paged.table_on[left:].data_ptr()
+    paged.batch = lambda: some
+    append(here, paged, on[:, :2], on[:, 2:3], on[:, 3:], None, q)
+    here.sync()
+    at, end = sum(n[:left]), sum(n)
+    got = q.cpu().numpy()
+    assert (got[:at] == 5.0).all() and (got[end:] == 5.0).all()
+    np.testing.assert_array_equal(got[at:end], packed[at:end, :2])
+    for s, (m, l) in enumerate(zip(n, lengths)):
+        values = paged.dense(s)[1]
+        assert (values[:l - m] == 7.0).all()
+        np.testing.assert_array_equal(values[l - m:, 0], packed[sum(n[:s]):sum(n[:s + 1]), 3] if s >= left else np.full((m, 64), 7.0))
+    for x in paged.views():
+        x.copy_(gpu(rng.standard_normal(tuple(x.shape)).astype(np.float32)))
+    got = attend(here, paged, q).cpu().numpy()
+    here.sync()
+    assert (got[:at] == 5.0).all()
+    paged.n, paged.lengths, paged.table = n[left:], lengths[left:], paged.table[left:]
+    held_to_definition(got[at:], paged, packed[at:, :2])
