@@ -1464,6 +1464,7 @@ int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_k
     if (attend.tokens == 0 || batch.sequences == 0) return AHIP_OK;
     if (int rc = require_kv_arrays(ctx, "kv attention", cache, batch)) return rc;
     if (!attend.q || !attend.out) return ctx.fail(AHIP_ERR_ARG, "kv attention: null pointer");
+    if (attend.out == attend.q) return ctx.fail(AHIP_ERR_ARG, "kv attention: out is q");
     const Plan plan = plan_of(&ctx, cache, batch, attend);
     if (plan.bytes && (!attend.workspace || attend.workspace_bytes < plan.bytes))
         return ctx.fail(AHIP_ERR_ARG, "kv attention: the workspace holds " + std::to_string(attend.workspace ? attend.workspace_bytes : 0) + " bytes of " +

@@ -454,7 +454,7 @@ int ahip_kv_attention_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const
                                 const ahip_kv_attend *attend, size_t *bytes);
 /* head_size up to 256 and a multiple of 4 (of 8 with a bf16 cache); q, out and the cache, with their strides, on 16-byte
  * boundaries (AHIP_ERR_UNSUPPORTED otherwise, nothing launched).  The workspace holds partial results during the call:
- * calls that run at the same time need one each.  out must not overlap q. */
+ * calls that run at the same time need one each.  out must not overlap q (the same pointer is refused). */
 int ahip_kv_attention(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend);
 
 /* Which kernel ahip_gemm (and the MatMul / Gemm / Conv2d operators of a session on this context) uses

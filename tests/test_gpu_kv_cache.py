@@ -782,3 +782,16 @@ def test_some_of_a_batchs_sequences(here, case, n, lengths, left):
     assert (got[:at] == 5.0).all()
     paged.n, paged.lengths, paged.table = n[left:], lengths[left:], paged.table[left:]
     held_to_definition(got[at:], paged, packed[at:, :2])
+
+
+def test_results_in_the_place_of_queries_are_refused(here, case):
+    case("attend out is q")
+    rng = np.random.default_rng(37)
+    paged = Paged(rng, [1], [40], 1, 64, 16)
+    q = rng.standard_normal((1, 2, 64)).astype(np.float32)
+    on = gpu(q)
+    with pytest.raises(AltiusHipError) as e:
+        attend(here, paged, on, out=on)
+    assert e.value.code == ERR_ARG
+    here.sync()
+    np.testing.assert_array_equal(on.cpu().numpy(), q)
