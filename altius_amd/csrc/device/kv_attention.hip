@@ -1403,8 +1403,13 @@ int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
     if (int rc = make_kv_view(ctx, "kv attention", cache, batch, attend->tokens, view)) return rc;
     if (attend->q_heads <= 0 || attend->q_heads > 65535 || attend->q_heads % cache->kv_heads)
         return kv_fail(ctx, AHIP_ERR_SHAPE, name + std::to_string(attend->q_heads) + " query heads do not share " + std::to_string(cache->kv_heads) + " heads of keys");
-    if (!std::isfinite(attend->scale) || !std::isfinite(attend->softcap) || attend->softcap < 0 || attend->window < 0)
+    if (!std::isfinite(attend->scale * LOG2E) || !std::isfinite(attend->softcap) || attend->softcap < 0 || attend->window < 0)
         return kv_fail(ctx, AHIP_ERR_ARG, name + "the scale, the cap or the window is out of range");
+    // Queries are scaled by scale / cap in fp32, whose parts in bf16 reach 2^-24 below them, and scores multiplied by the cap: with a
+    // quotient outside 2^-64 .. 2^64 the parts would be flushed to zero, or the quotient or the product infinite.
+    const double beside_cap = attend->softcap != 0.0f ? std::fabs((double)attend->scale) / attend->softcap : 0.0;
+    if (beside_cap != 0.0 && !(beside_cap >= 0x1p-64 && beside_cap <= 0x1p64)) return kv_fail(ctx, AHIP_ERR_ARG, name + "the cap is out of range beside the scale");
+    if (!std::isfinite(attend->softcap * LOG2E)) return kv_fail(ctx, AHIP_ERR_ARG, name + "the cap is out of range");
     // Sizes that the plan's products and the kernels' row numbers hold.
     const uint64_t group = (uint64_t)(attend->q_heads / cache->kv_heads), most_tokens = std::min(attend->max_tokens ? attend->max_tokens : attend->tokens, attend->tokens);
     if (most_tokens * group > MOST_ROWS) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more than 2^30 rows for a head of keys");

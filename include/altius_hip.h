@@ -439,7 +439,7 @@ typedef struct ahip_kv_attend {
     const float *q;
     float *out;
     size_t q_strides[2], out_strides[2]; /* token, head */
-    float scale, softcap;                /* softcap 0: none */
+    float scale, softcap;                /* softcap 0: none; |scale| / softcap from 2^-64 to 2^64, or 0 */
     int32_t causal, window;              /* window 0: none */
     const float *slopes;                 /* device, q_heads; NULL: none */
     const int32_t *prefix;               /* device, sequences; NULL: none */

@@ -101,3 +101,13 @@ def test_null_arguments_are_refused():
     assert L.ahip_rotary_heads(None, None, None) == ERR_ARG and L.ahip_kv_append(None, None, None, None, None) == ERR_ARG
     assert L.ahip_kv_attention(None, None, None, None) == ERR_ARG
     assert L.ahip_rotary_frequencies(None, 8, 10000.0, 0, 1.0, 0.0, 0.0, 0.0) == ERR_ARG
+
+
+@pytest.mark.parametrize("changed", [dict(softcap=1e-40), dict(softcap=1e-30), dict(softcap=1e30), dict(softcap=2e38), dict(softcap=3e38, scale=0.0), dict(softcap=3e38, scale=1e20),
+                                     dict(softcap=1.0, scale=1e-20), dict(softcap=1.0, scale=-1e20), dict(scale=3e38)])
+def test_caps_that_fp32_does_not_hold_beside_the_scale_are_refused(changed):
+    with pytest.raises(AltiusHipError) as e:
+        workspace(**changed)
+    assert e.value.code == ERR_ARG
+    for fine in (dict(softcap=1e-18), dict(softcap=1e18), dict(softcap=50.0, scale=-0.1), dict(softcap=1e-30, scale=0.0), dict(softcap=2e38, scale=1e20)):
+        workspace(**fine)

@@ -795,3 +795,20 @@ def test_results_in_the_place_of_queries_are_refused(here, case):
     assert e.value.code == ERR_ARG
     here.sync()
     np.testing.assert_array_equal(on.cpu().numpy(), q)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [[2], [70]])
+@pytest.mark.parametrize("cap", [1e-18, 1e-3, 1e6, 1e18])
+def test_caps_far_from_the_scores(here, case, elem, n, cap):
+    """The smallest make all weights alike, the largest do nothing."""
+    case(f"attend cap {cap} {elem} n {n}")
+    rng = np.random.default_rng(38)
+    paged = Paged(rng, n, [90], 1, 64, 16, elem)
+    q = rng.standard_normal((n[0], 2, 64)).astype(np.float32)
+    got = attend(here, paged, gpu(q), cap=float(np.float32(cap))).cpu().numpy()
+    k, v = paged.dense(0)
+    low, high, place = ranges(n[0], 90, True, 0, None, None)
+    # A cap of 1000 times the scores and more changes them by less than 2^-21 of themselves; 8 steps of a large cap are not 8 of the score.
+    want, bound = attended(q, k, v, low, high, place, 0.125, 0.0 if cap > 1e3 else cap, None)
+    assert (np.abs(got - want) <= bound).all()
