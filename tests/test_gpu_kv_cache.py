@@ -9,6 +9,7 @@ import torch
 from altius_amd import device as D
 from altius_amd._lib import ERR_ARG, ERR_UNSUPPORTED, AltiusHipError
 from decoder_oracle import attended, bf16, normed, ranges, turned, turned_bound
+from decoder_precision import WINDOWS, expected, keys, queries, values
 
 pytestmark = pytest.mark.gpu
 
@@ -812,3 +813,30 @@ def test_caps_far_from_the_scores(here, case, elem, n, cap):
     # A cap of 1000 times the scores and more changes them by less than 2^-21 of themselves; 8 steps of a large cap are not 8 of the score.
     want, bound = attended(q, k, v, low, high, place, 0.125, 0.0 if cap > 1e3 else cap, None)
     assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("what", sorted(WINDOWS))
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 80, 96, 128, 256])
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("n,lengths,heads,kv", [([2] * 12, [30 + 9 * i for i in range(12)], 16, 4), ([70, 40, 1], [200, 40, 300], 4, 2), ([2, 1], [1500, 700], 16, 1)])
+def test_no_part_of_a_number_is_lost(here, case, what, elem, d, page, n, lengths, heads, kv):
+    """Held to bounds that a dropped third part or product of parts exceeds (decoder_precision.py)."""
+    case(f"attend precision {what} {elem} d {d} page {page} n {n[:3]}")
+    rng = np.random.default_rng(d + page)
+    paged = Paged(rng, n, lengths, kv, d, page, elem)
+    for x, make in zip(paged.on, (keys, values)):
+        x.copy_(gpu(make(rng, what, tuple(x.shape), elem)))
+    q = queries(rng, what, sum(n) * heads, d).reshape(sum(n), heads, d)
+    got = attend(here, paged, gpu(q), window=WINDOWS[what], scale=1.0).cpu().numpy()
+    here.sync()
+    at = 0
+    for s, (m, l) in enumerate(zip(n, lengths)):
+        k, v = paged.dense(s)
+        low, high, _ = ranges(m, l, True, WINDOWS[what], None, None)
+        seen = (np.arange(l) >= low[:, None]) & (np.arange(l) < high[:, None])
+        for h in range(heads):
+            want, bound = expected(what, q[at:at + m, h], k[:, h // (heads // kv)], v[:, h // (heads // kv)], seen)
+            off = np.abs(got[at:at + m, h] - want)
+            assert (off <= bound).all(), f"sequence {s} head {h}: off by {off.max():.3g}, {(off / np.maximum(bound, 1e-30)).max():.3g} times the bound"
+        at += m
