@@ -840,3 +840,70 @@ def test_no_part_of_a_number_is_lost(here, case, what, elem, d, page, n, lengths
             off = np.abs(got[at:at + m, h] - want)
             assert (off <= bound).all(), f"sequence {s} head {h}: off by {off.max():.3g}, {(off / np.maximum(bound, 1e-30)).max():.3g} times the bound"
         at += m
+
+
+def sharing_pages(rng, n, lengths, kv_heads, d, page, elem):
+    """Long sequences out of few pages, which several of them read."""
+    paged = Paged(rng, [0], [1], kv_heads, d, page, elem, table_pages=60)
+    paged.n, paged.lengths, paged.per = n, lengths, -(-max(lengths) // page)
+    paged.table = rng.integers(0, paged.pages, (len(n), paged.per)).astype(np.int32)
+    paged.starts_on, paged.lengths_on, paged.table_on = gpu(np.concatenate([[0], np.cumsum(n)]).astype(np.int32)), gpu(np.array(lengths, np.int32)), gpu(paged.table)
+    return paged
+
+
+@pytest.mark.parametrize("d,page,elem,sequences,kv", [(64, 16, "f32", 200, 8), (64, 32, "bf16", 200, 8), (64, 24, "f32", 200, 8), (128, 16, "f32", 130, 8), (128, 64, "bf16", 200, 8),
+                                                      (256, 16, "f32", 66, 8), (256, 20, "f32", 66, 8), (256, 16, "bf16", 66, 8), (200, 48, "f32", 66, 8)])
+def test_long_sequences_among_many(here, case, d, page, elem, sequences, kv):
+    """So many sequences that no keys are cut: a wavefront goes through up to 140 tiles of 16 keys, and the starts of its pages, 64 tiles at a
+    time, are looked up anew."""
+    case(f"attend long among many d {d} page {page} {elem}")
+    rng = np.random.default_rng(39)
+    lengths = [1 + 37 * s % 90 for s in range(sequences)]
+    lengths[3], lengths[40], lengths[-1] = 8999, 4097, 5000
+    paged = sharing_pages(rng, [1] * sequences, lengths, kv, d, page, elem)
+    q = rng.standard_normal((sequences, kv, d)).astype(np.float32)
+    got = attend(here, paged, gpu(q), max_tokens=1, max_keys=9000).cpu().numpy()
+    here.sync()
+    held_to_definition(got, paged, q)
+
+
+@pytest.mark.parametrize("page,elem", [(16, "f32"), (48, "f32"), (24, "f32"), (16, "bf16"), (20, "bf16")])
+@pytest.mark.parametrize("sequences,lengths", [(16, 1000), (16, 4000), (3, 20000)])
+@pytest.mark.parametrize("d", [132, 256])
+def test_many_tiles_of_wide_heads(here, case, page, elem, sequences, lengths, d):
+    """Heads of more than 128 channels whose keys are cut into parts of 4 and more tiles a wavefront."""
+    case(f"attend wide heads d {d} page {page} {elem} {sequences} of {lengths}")
+    if elem == "bf16" and d == 132:
+        d = 136  # a multiple of 8
+    rng = np.random.default_rng(40)
+    paged = sharing_pages(rng, [1] * sequences, [lengths - 31 * s for s in range(sequences)], 4, d, page, elem)
+    q = rng.standard_normal((sequences, 8, d)).astype(np.float32)
+    got = attend(here, paged, gpu(q), max_tokens=1, max_keys=lengths).cpu().numpy()
+    here.sync()
+    held_to_definition(got, paged, q)
+
+
+@pytest.mark.parametrize("d,page,elem,kv", [(64, 16, "f32", 8), (64, 24, "f32", 8), (64, 64, "bf16", 8), (96, 16, "f32", 8), (128, 32, "f32", 8), (128, 16, "bf16", 8), (256, 16, "f32", 2),
+                                            (256, 24, "bf16", 2)])
+def test_pieces_behind_long_sequences_among_many(here, case, d, page, elem, kv):
+    """Pieces whose blocks are enough uncut: a block of 128 rows goes through up to 125 tiles of 32 keys, and the starts of its pages, 32 tiles
+    at a time, are looked up anew; so does one of 16 rows of wide heads."""
+    case(f"attend pieces behind long sequences d {d} page {page} {elem}")
+    rng = np.random.default_rng(41)
+    n, lengths = [40] * 32, [45 + s for s in range(32)]
+    lengths[5], lengths[20], lengths[-1] = 1100, 4000, 2500
+    paged = sharing_pages(rng, n, lengths, kv, d, page, elem)
+    q = rng.standard_normal((sum(n), kv, d)).astype(np.float32)
+    got = attend(here, paged, gpu(q), max_tokens=40, max_keys=4000).cpu().numpy()
+    here.sync()
+    held_to_definition(got, paged, q)
+
+
+@pytest.mark.parametrize("sequences,most", [(65, 3), (66, 1), (100, 9), (513, 4), (1000, 2)])
+@pytest.mark.parametrize("d,elem", [(64, "f32"), (20, "bf16"), (7, "f32")])
+def test_tokens_of_many_sequences_land_in_their_slots(here, case, sequences, most, d, elem):
+    """More than 64 sequences with none to several rows each: a row's sequence is searched for."""
+    rng = np.random.default_rng(sequences + most)
+    n = [int(m) for m in rng.integers(0, most + 1, sequences)]
+    lengths = [m + int(x) if m else int(x) for m, x in zip(n, rng.integers(0, 30, sequences))]
+    test_tokens_land_in_their_slots(here, case, n, lengths, 3, 1, d, 6, 8, elem, "head", False, d == 64)
