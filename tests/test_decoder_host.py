@@ -111,3 +111,25 @@ def test_caps_that_fp32_does_not_hold_beside_the_scale_are_refused(changed):
     assert e.value.code == ERR_ARG
     for fine in (dict(softcap=1e-18), dict(softcap=1e18), dict(softcap=50.0, scale=-0.1), dict(softcap=1e-30, scale=0.0), dict(softcap=2e38, scale=1e20)):
         workspace(**fine)
+
+
+def parts_bytes(units, tile, at_once, least, tiles, head_size=128):
+    """Parts of at least `least` units of 64 keys, as many as blocks at work at once and one more a row tile and kv head; rows of a maximum, a
+    sum and head_size channels."""
+    return (min(at_once, units * tiles // least) + tiles) * tile * (2 + head_size) * 4
+
+
+def test_the_workspace_is_what_the_parts_hold():
+    """256 CUs: 512 blocks of 16 rows at work at once (fp32, 128 channels), 256 of 128 rows; parts of 128 keys at least."""
+    # 4 tokens of up to 800 keys: 13 units of 64 keys for each of 32 (sequence, kv head).
+    assert workspace() == parts_bytes(13, 16, 512, 2, 32)
+    # One token of up to 65536 keys: more units than blocks at work at once.
+    one = dict(sequences=1, tokens=1, table_pages=4096, table_stride=4096)
+    assert workspace(**one) == parts_bytes(1024, 16, 512, 2, 8)
+    # 200 tokens: two blocks a place and more, nothing is cut.
+    assert workspace(sequences=200, tokens=200) == 0
+    # A piece of 300 tokens (10 row tiles of 128 rows) behind 65536 keys at most, whose keys are cut, and 16 rows of it if it is shorter.
+    assert workspace(sequences=1, tokens=300, max_tokens=300, table_pages=4096, table_stride=4096) == parts_bytes(1024, 128, 256, 2, 80) + parts_bytes(1024, 16, 512, 2, 8)
+    # Prompts of so many row tiles that none is cut: what remains is for 32 rows of a shorter piece, and does not grow with the prompt.
+    long = [workspace(sequences=1, tokens=t, max_tokens=t, table_pages=8000, table_stride=8000) for t in (1000, 10000, 100000)]
+    assert long == [parts_bytes(2000, 16, 512, 2, 16)] * 3
