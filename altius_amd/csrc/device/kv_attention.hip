@@ -96,20 +96,11 @@ __device__ __forceinline__ float weight_of(float m, float top) { return m == -IN
 
 // tanh, as dev::rational_tanh has it, but for the division: a reciprocal and one step of Newton's, off by an fp32 step more at most.
 __device__ __forceinline__ float fast_tanh(float v) {
-    v = dev::rclamp(v, -9.0f, 9.0f);
-    const float v2 = v * v;
-    float p = __builtin_fmaf(v2, -2.76076847742355e-16f, 2.00018790482477e-13f);
-    p = __builtin_fmaf(p, v2, -8.60467152213735e-11f);
-    p = __builtin_fmaf(p, v2, 5.12229709037114e-08f);
-    p = __builtin_fmaf(p, v2, 1.48572235717979e-05f);
-    p = __builtin_fmaf(p, v2, 6.37261928875436e-04f);
-    p = __builtin_fmaf(p, v2, 4.89352455891786e-03f);
-    float q = __builtin_fmaf(v2, 1.19825839466702e-06f, 1.18534705686654e-04f);
-    q = __builtin_fmaf(q, v2, 2.26843463243900e-03f);
-    q = __builtin_fmaf(q, v2, 4.89352518554385e-03f);
+    float p, q;
+    dev::rational_tanh_parts(dev::rclamp(v, -9.0f, 9.0f), p, q);
     float r = __builtin_amdgcn_rcpf(q);
     r = __builtin_fmaf(__builtin_fmaf(-q, r, 1.0f), r, r);
-    return p * v * r;
+    return p * r;
 }
 
 // Products of a (scaled) query and keys become scores in units of log2(e): capped, biased.  Key place(r) of the tile, which starts

@@ -78,8 +78,8 @@ __device__ __forceinline__ float sigmoid_elem(float x) {
 }
 
 // The 13/6-degree rational tanh shared by Op::Tanh (session.rs:860-877) and
-// Op::Gelu (fast_math.rs:306-322), applied to an already clamped argument.
-__device__ __forceinline__ float rational_tanh(float v) {
+// Op::Gelu (fast_math.rs:306-322), of an already clamped argument, as numerator and denominator.
+__device__ __forceinline__ void rational_tanh_parts(float v, float &p, float &q) {
     constexpr float ALPHA_13 = -2.76076847742355e-16f;
     constexpr float ALPHA_11 = 2.00018790482477e-13f;
     constexpr float ALPHA_9 = -8.60467152213735e-11f;
@@ -92,16 +92,20 @@ __device__ __forceinline__ float rational_tanh(float v) {
     constexpr float BETA_2 = 2.26843463243900e-03f;
     constexpr float BETA_0 = 4.89352518554385e-03f;
     float v2 = v * v;
-    float p = __builtin_fmaf(v2, ALPHA_13, ALPHA_11);
+    p = __builtin_fmaf(v2, ALPHA_13, ALPHA_11);
     p = __builtin_fmaf(p, v2, ALPHA_9);
     p = __builtin_fmaf(p, v2, ALPHA_7);
     p = __builtin_fmaf(p, v2, ALPHA_5);
     p = __builtin_fmaf(p, v2, ALPHA_3);
     p = __builtin_fmaf(p, v2, ALPHA_1);
     p = p * v;
-    float q = __builtin_fmaf(v2, BETA_6, BETA_4);
+    q = __builtin_fmaf(v2, BETA_6, BETA_4);
     q = __builtin_fmaf(q, v2, BETA_2);
     q = __builtin_fmaf(q, v2, BETA_0);
+}
+__device__ __forceinline__ float rational_tanh(float v) {
+    float p, q;
+    rational_tanh_parts(v, p, q);
     return p / q;
 }
 
