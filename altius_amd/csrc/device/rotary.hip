@@ -459,6 +459,7 @@ int rotary_frequencies(double *frequencies, int dim, double base, int scaling, d
     if (scaling == AHIP_ROTARY_TURNS && (!(length > 0) || !std::isfinite(length) || !(slow_turns < fast_turns) || !std::isfinite(slow_turns) || !std::isfinite(fast_turns)))
         return kv_fail(nullptr, AHIP_ERR_ARG, std::string(who) + "turns need a length, and fewer slow turns than fast ones");
     if (scaling == AHIP_ROTARY_BASE) base *= std::pow(factor, (double)dim / (dim - 2));
+    if (!(base > 0) || !std::isfinite(base)) return kv_fail(nullptr, AHIP_ERR_ARG, std::string(who) + "the stretched base is out of range");
     for (int i = 0; i < dim / 2; i++) {
         double f = std::pow(base, -2.0 * i / dim);
         if (scaling == AHIP_ROTARY_LINEAR) f /= factor;

@@ -133,3 +133,10 @@ def test_the_workspace_is_what_the_parts_hold():
     # Prompts of so many row tiles that none is cut: what remains is for 32 rows of a shorter piece, and does not grow with the prompt.
     long = [workspace(sequences=1, tokens=t, max_tokens=t, table_pages=8000, table_stride=8000) for t in (1000, 10000, 100000)]
     assert long == [parts_bytes(2000, 16, 512, 2, 16)] * 3
+
+
+@pytest.mark.parametrize("arguments", [dict(dim=4, factor=1e200), dict(dim=4, factor=1e-200), dict(dim=8, base=1e300, factor=1e10)])
+def test_a_stretched_base_that_64_bits_do_not_hold_is_refused(arguments):
+    with pytest.raises(AltiusHipError) as e:
+        D.rotary_frequencies(scaling=D.ROTARY_BASE, **arguments)
+    assert e.value.code == ERR_ARG
