@@ -731,11 +731,11 @@ __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ?
 // second product takes its k slots in that order, in which V^T lies in LDS.  Queries and weights are three bf16 numbers each, as
 // above; so are the values of an fp32 cache, split on their way into LDS, and six products of the parts are what fp32 holds of the
 // whole (the three left out are below 2^-24 of it).  A bf16 cache's values are one number: three products.
-//   Two tiles of each operand in LDS, one barrier a tile.  Bound by the matrix cores, where all keys are seen: a prompt of 4096 with a
-// window of 1500 (16 heads, 4 of keys, 128 channels, bf16, capped) takes 148 us, 279 TFLOP/s of scores and sums, 840 of the
-// instructions' own, where a large bf16 product reaches 1356; 4 prompts of 1024 (12 heads of 64 channels, fp32) 58 us,
-// 111 and 670.  What is missing: half a causal sequence's tiles lie in blocks that end early, and at 64 channels the exponentials,
-// splits and staging of a tile are as much work for the vector unit as its products for the matrix cores.
+//   Two tiles of each operand in LDS, one barrier a tile.  A prompt of 4096 with a window of 1500 (16 heads, 4 of keys, 128
+// channels, bf16, capped) takes 150 us, 275 TFLOP/s of scores and sums, 825 of the instructions' own, where a large bf16 product
+// reaches 1356; 4 prompts of 1024 (12 heads of 64 channels, fp32) 58 us, 111 and 670.  The matrix cores are busy 29 and 26 % of the time, the
+// vector unit 35 and 28 %: bound by waits with one or two wavefronts a SIMD and by places left empty, since blocks see different numbers of keys
+// (1.25 times the mean the longest with the window, 4 to 32 tiles in the prompts).
 constexpr int TILE_KEYS = 32;
 
 #define ALTIUS_MFMA32_BF16(A, B, C) \
@@ -1243,7 +1243,8 @@ __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(
 
 // Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
 // channels, four a lane.  few: a block per row, whose groups of lanes deal the splits out among themselves; else a group per row.  Bound by
-// latency: the scan for a row's parts, their statistics, their sums.  10 us behind one row's 512 parts, 10 us behind 5 pieces of 57 to 333 rows.
+// latency: the scan for a row's parts, their statistics, their sums.  10 us behind one row's 512 parts, 10 us behind 5 pieces of 57 to 333 rows,
+// 4 to 5 us where the sizes allow parts and there are none.
 constexpr int JOIN = 256, MOST_SPLITS = 1024;
 __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_blocks) {
     __shared__ float factors[MOST_SPLITS];
@@ -1369,8 +1370,8 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     const uint64_t all_rows = attend.tokens * (uint64_t)group, row_tiles = (rows + TILE_ROWS - 1) / TILE_ROWS;
     const uint64_t many_tiles = (uint64_t)cache.kv_heads * std::min(batch.sequences * row_tiles, all_rows / TILE_ROWS + std::min<uint64_t>(batch.sequences, all_rows / (FEW_BESIDE_CUT + 1)));
     // Prompts whose blocks would leave half the places empty: pieces of 57 to 333 rows, up to 4858 keys, 392 us whole and 100 us cut;
-    // one prompt of 1024, 12 heads of 64 channels, 50 and 37 us.  With three quarters of the places taken (4 such prompts) the cut
-    // costs: 59 us whole, 78 us cut.  Parts of 128 keys at least: a prompt of 400, 16 heads of 128, fp32, 32 us, with 256 36 us.
+    // one prompt of 1024, 12 heads of 64 channels, 50 and 37 us.  With three quarters of the places taken (4 such prompts) this cut
+    // costs (59 us whole, 78 us cut): it gives every row tile parts of the whole sequence, half of which a causal prompt does not see.  Parts of 128 keys at least: a prompt of 400, 16 heads of 128, fp32, 32 us, with 256 36 us.
     if (rows > FEW_ROWS) {
         if (tiled) share(p.many, rows, TILE_ROWS, many_tiles, many_tiles < many_at_once / 2, many_at_once, 128);
         else share(p.many, rows, 16, pairs * ((rows + 15) / 16), false, 0, 0);

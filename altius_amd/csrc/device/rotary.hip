@@ -124,7 +124,8 @@ __device__ __forceinline__ Slot slot_of(const dev::KvView &kv, uint32_t token, i
 // Rows that are normed have a power of two of lanes, which add up their squares; others exactly as many as they need.
 //   Bound by memory: 4096 tokens x 16 heads of 128 channels, normed, 67 MB in 14.0 us, 4.8 TB/s, where a copy of 1 GiB moves 5.2;
 // 9 prompts into a bf16 cache, 117 MB in 30 us, 3.9 TB/s, whose rows of 256 bytes are written out of order; interleaved pairs of half
-// of 80 channels, 31 MB in 9.0 us, 3.4 TB/s, by the angles.  One token of 12 heads: 3.2 us, a launch.
+// of 80 channels, 31 MB in 9.0 us, 3.4 TB/s, by waits: each frequency is loaded behind a condition and waited for by itself, behind the
+// position's wait, five trips to memory in a row.  One token of 12 heads: 3.2 us, a launch.
 template <int N, bool CACHE, bool BF16>
 __global__ __launch_bounds__(BLOCK) void rotate_rows_vec4(RotateArgs g) {
     const uint32_t mine = blockIdx.x * BLOCK + threadIdx.x, thread = min(mine, g.threads - 1);

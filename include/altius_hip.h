@@ -359,7 +359,8 @@ typedef struct ahip_rotary {
  * needed).  PLAIN: as they are.  LINEAR: all divided by factor (positions interpolated).  BASE: base multiplied by
  * factor^(dim / (dim - 2)), which leaves the fastest pair and divides the slowest by factor.  TURNS: a pair that makes at
  * most slow_turns turns over `length` positions is divided by factor, one that makes at least fast_turns is left, between
- * the two the frequency is the mean of both weighted by where its turns lie. */
+ * the two the frequency is the mean of both weighted by where its turns lie (not its number among the pairs: a scheme that goes by that
+ * has other frequencies, which the caller computes). */
 enum ahip_rotary_scaling { AHIP_ROTARY_PLAIN = 0, AHIP_ROTARY_LINEAR = 1, AHIP_ROTARY_BASE = 2, AHIP_ROTARY_TURNS = 3 };
 int ahip_rotary_frequencies(double *frequencies, int dim, double base, int scaling, double factor, double length,
                             double slow_turns, double fast_turns);
@@ -421,7 +422,8 @@ typedef struct ahip_kv_tokens {
     int32_t position_size; /* 4 or 8 */
 } ahip_kv_tokens;
 /* Writes each token's keys, normed and turned as ahip_rotary_heads does it, and its values into its slot, and turns the
- * queries on the way: one launch.  rotary may be NULL.  Two tokens of a call must not have the same slot. */
+ * queries on the way: one launch.  rotary may be NULL.  Two tokens of a call must not have the same slot.  Rows of a sequence that is shorter
+ * than they are have no slot in front of place 0: they are left out, and the next ahip_sync fails. */
 int ahip_kv_append(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_tokens *tokens,
                    const ahip_rotary *rotary);
 
@@ -432,7 +434,10 @@ int ahip_kv_append(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batc
  * with the score  x = q k * scale,  softcap ? softcap * tanh(x / softcap) : x,  less slopes[h] * |p - j|.
  * out = sum softmax(score) v; a row that sees no key is 0.  Documents packed into one sequence have their first keys as
  * first_keys.  What lies in slots that a row does not see never reaches it, not even as infinity or NaN; sums and the
- * softmax are held in 32 bits, and a bf16 cache's products with q and with the weights are exact to fp32. */
+ * softmax are held in 32 bits, and a bf16 cache's products with q and with the weights are exact to fp32.  Where fp32 ends: a sum of weights
+ * times values beyond it, before it is divided by the sum of weights, is infinite; of magnitudes below 2^-100 some bits are lost.
+ * Rows of a sequence that is shorter than they are (n > lengths[s]) have places below 0 and see what the formulas say, which is nothing where
+ * causal without a prefix. */
 typedef struct ahip_kv_attend {
     size_t tokens; /* rows of q and out, padding included */
     int32_t q_heads;
