@@ -398,7 +398,7 @@ typedef struct ahip_kv_cache {
  * sequence's and behind the last one's are padding: not read, and left as they are where written, so that a call can take some of a
  * larger batch's sequences.  The token at place j of sequence s is in slot
  * j % page_size of page page_table[s * table_stride + j / page_size].  Entries of pages that hold no key between the first and the
- * last one that a sequence's rows see are not used: pages that a window has left may be given to others.  All three arrays are
+ * last one that a sequence's rows see are not used by attention: pages that a window has left may be given to others.  All three arrays are
  * device memory. */
 typedef struct ahip_kv_batch {
     int32_t sequences, table_pages; /* table_pages: entries of one sequence's row of the table */

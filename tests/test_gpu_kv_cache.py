@@ -907,3 +907,20 @@ def test_tokens_of_many_sequences_land_in_their_slots(here, case, sequences, mos
     n = [int(m) for m in rng.integers(0, most + 1, sequences)]
     lengths = [m + int(x) if m else int(x) for m, x in zip(n, rng.integers(0, 30, sequences))]
     test_tokens_land_in_their_slots(here, case, n, lengths, 3, 1, d, 6, 8, elem, "head", False, d == 64)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [[3], [70]])
+@pytest.mark.parametrize("size", [1.5e38, 2.0 ** -90])
+def test_values_near_the_ends_of_fp32(here, case, elem, d, n, size):
+    """Two keys a row: their weights relative to the larger one add up to 2 at most, and 2 x 1.5e38 is finite."""
+    case(f"attend values of {size:.3g} {elem} d {d} n {n}")
+    rng = np.random.default_rng(42)
+    paged = Paged(rng, n, [120], 1, d, 16, elem)
+    paged.on[1].copy_(size * (2 * torch.rand(paged.on[1].shape, device="cuda", generator=torch.Generator("cuda").manual_seed(42)) - 1))
+    q = rng.standard_normal((n[0], 4, d)).astype(np.float32)
+    got = attend(here, paged, gpu(q), window=2, scale=3.0 / d).cpu().numpy()
+    here.sync()
+    assert np.isfinite(got).all()
+    held_to_definition(got, paged, q, window=2, scale=3.0 / d)
