@@ -101,6 +101,30 @@ class KvAttend(_Described):
     _defaults = {"scale": 1.0, "causal": 1}
 
 
+class KvHistory(_Described):
+    """ahip_kv_history"""
+    _fields_ = [("mass", c_void_p), ("positions", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64)]
+
+
+class KvEviction(_Described):
+    """ahip_kv_eviction"""
+    _fields_ = [("budget", ctypes.c_int32), ("recent", ctypes.c_int32), ("first", ctypes.c_int32), ("most", ctypes.c_int32), ("max_keys", c_size_t),
+                ("sources", c_void_p), ("targets", c_void_p), ("counts", c_void_p), ("lengths", c_void_p)]
+
+
+class KvMoves(_Described):
+    """ahip_kv_moves; strides as tuples (sequence, head)."""
+    _fields_ = [("sources", c_void_p), ("targets", c_void_p), ("counts", c_void_p), ("strides", c_int64 * 2), ("count_strides", c_int64 * 2),
+                ("most", ctypes.c_int32), ("apart", ctypes.c_int32)]
+
+
+class KvSparse(_Described):
+    """ahip_kv_sparse"""
+    _fields_ = [("means", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64), ("chosen", c_void_p), ("most", ctypes.c_int32),
+                ("first", ctypes.c_int32), ("last", ctypes.c_int32)]
+    _defaults = {"last": 1}
+
+
 FUSED_ACC = -1
 FUSED_MAX_INPUTS = 6
 FUSED_MAX_STEPS = 16
@@ -155,6 +179,14 @@ def _declare(L):
     f("ahip_kv_append", [c_void_p, P(KvCache), P(KvBatch), P(KvTokens), P(Rotary)])
     f("ahip_kv_attention_workspace", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), P(c_size_t)])
     f("ahip_kv_attention", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend)])
+    f("ahip_kv_attention_tree", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), c_void_p])
+    f("ahip_kv_attention_mass_workspace", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), P(c_size_t)])
+    f("ahip_kv_attention_mass", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), P(KvHistory), c_float, c_void_p])
+    f("ahip_kv_evict", [c_void_p, P(KvCache), P(KvBatch), P(KvHistory), P(KvEviction)])
+    f("ahip_kv_move", [c_void_p, P(KvCache), P(KvBatch), P(KvMoves), P(KvHistory)])
+    f("ahip_kv_attention_sparse_workspace", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), P(KvSparse), P(c_size_t)])
+    f("ahip_kv_attention_sparse", [c_void_p, P(KvCache), P(KvBatch), P(KvAttend), P(KvSparse)])
+    f("ahip_kv_page_means", [c_void_p, P(KvCache), P(KvBatch), P(KvSparse), c_size_t, c_size_t])
     f("ahip_gemm_set_algorithm", [c_void_p, c_int])
     f("ahip_set_streaming_threshold", [c_void_p, c_size_t])
     f("ahip_set_load_streaming_threshold", [c_void_p, c_size_t])

@@ -623,6 +623,72 @@ int ahip_kv_attention(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_b
     return altius::caught_at_boundary("ahip_kv_attention");
 }
 
+int ahip_kv_attention_tree(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const int32_t *parents) try {
+    REQUIRE_CTX(ctx, "ahip_kv_attention_tree");
+    if (!cache || !batch || !attend) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_attention_tree: null argument");
+    arm_flags(ctx->d);
+    return altius::launch_kv_attention_tree(ctx->d, *cache, *batch, *attend, parents);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention_tree");
+}
+
+int ahip_kv_attention_mass_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, size_t *bytes) try {
+    return altius::kv_attention_mass_workspace(ctx ? &ctx->d : nullptr, cache, batch, attend, bytes);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention_mass_workspace");
+}
+
+int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const ahip_kv_history *history, float decay, const int32_t *row_positions) try {
+    REQUIRE_CTX(ctx, "ahip_kv_attention_mass");
+    if (!cache || !batch || !attend || !history) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_attention_mass: null argument");
+    arm_flags(ctx->d);
+    return altius::launch_kv_attention_mass(ctx->d, *cache, *batch, *attend, *history, decay, row_positions);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention_mass");
+}
+
+int ahip_kv_evict(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_history *history, const ahip_kv_eviction *eviction) try {
+    REQUIRE_CTX(ctx, "ahip_kv_evict");
+    if (!cache || !batch || !history || !eviction) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_evict: null argument");
+    arm_flags(ctx->d);
+    return altius::launch_kv_evict(ctx->d, *cache, *batch, *history, *eviction);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_evict");
+}
+
+int ahip_kv_move(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_moves *moves, const ahip_kv_history *history) try {
+    REQUIRE_CTX(ctx, "ahip_kv_move");
+    if (!cache || !batch || !moves) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_move: null argument");
+    arm_flags(ctx->d);
+    return altius::launch_kv_move(ctx->d, *cache, *batch, *moves, history);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_move");
+}
+
+int ahip_kv_attention_sparse_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const ahip_kv_sparse *sparse, size_t *bytes) try {
+    return altius::kv_attention_sparse_workspace(ctx ? &ctx->d : nullptr, cache, batch, attend, sparse, bytes);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention_sparse_workspace");
+}
+
+int ahip_kv_attention_sparse(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const ahip_kv_sparse *sparse) try {
+    REQUIRE_CTX(ctx, "ahip_kv_attention_sparse");
+    if (!cache || !batch || !attend || !sparse) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_attention_sparse: null argument");
+    arm_flags(ctx->d);
+    return altius::launch_kv_attention_sparse(ctx->d, *cache, *batch, *attend, *sparse);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_attention_sparse");
+}
+
+int ahip_kv_page_means(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_sparse *sparse, size_t tokens, size_t max_tokens) try {
+    REQUIRE_CTX(ctx, "ahip_kv_page_means");
+    if (!cache || !batch || !sparse) return ctx->d.fail(AHIP_ERR_ARG, "ahip_kv_page_means: null argument");
+    arm_flags(ctx->d);
+    return altius::launch_kv_page_means(ctx->d, *cache, *batch, *sparse, tokens, max_tokens);
+} catch (...) {
+    return altius::caught_at_boundary("ahip_kv_page_means");
+}
+
 int ahip_gemm_set_algorithm(ahip_ctx *ctx, int algorithm) try {
     REQUIRE_CTX(ctx, "ahip_gemm_set_algorithm");
     if (algorithm != AHIP_GEMM_AUTO && algorithm != AHIP_GEMM_FP32 && algorithm != AHIP_GEMM_BF16X3)

@@ -125,7 +125,7 @@ int check_device_flags(DeviceCtx &ctx) {
         tell(AHIP_ERR_HIP, "MatMul: the slices of a tile cut along k ran on different XCDs, so their partial sums could not be "
                            "combined; the in-kernel cut is now switched off for this context, run the product again");
     }
-    if (raised[2]) tell(AHIP_ERR_ARG, "paged cache: a sequence's rows, length or pages do not fit the call's tensors, page table or cache");
+    if (raised[2]) tell(AHIP_ERR_ARG, "paged cache: a sequence's rows, length, pages, parents or moves do not fit the call's tensors, page table or cache");
     if (raised[0]) tell(AHIP_ERR_ARG, "Gather: an index is outside the gathered axis");
     return ctx.fail(code, said);
 }

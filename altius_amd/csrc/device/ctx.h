@@ -259,6 +259,17 @@ int launch_kv_append(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_b
 int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend);
 // Host only; ctx may be null.
 int kv_attention_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, size_t *bytes);
+// Trees of drafted tokens (kv_tree.hip), masses (kv_mass.hip), eviction and moves (kv_evict.hip), chosen pages (kv_sparse.hip).
+int launch_kv_attention_tree(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const int32_t *parents);
+int kv_attention_mass_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, size_t *bytes);
+int launch_kv_attention_mass(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const ahip_kv_history &history,
+                             float decay, const int32_t *row_positions);
+int launch_kv_evict(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_history &history, const ahip_kv_eviction &eviction);
+int launch_kv_move(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_moves &moves, const ahip_kv_history *history);
+int kv_attention_sparse_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const ahip_kv_sparse *sparse,
+                                  size_t *bytes);
+int launch_kv_attention_sparse(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const ahip_kv_sparse &sparse);
+int launch_kv_page_means(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_sparse &sparse, size_t tokens, size_t max_tokens);
 int rotary_frequencies(double *frequencies, int dim, double base, int scaling, double factor, double length, double slow_turns, double fast_turns);
 
 // The same product for one batch through three bf16 planes per operand and six bf16 MFMAs per fp32

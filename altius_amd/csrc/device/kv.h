@@ -20,14 +20,14 @@ struct KvView {
     uint32_t pages, page_size, kv_heads, sequences, tokens;
     FastDiv by_page_size;
     const int32_t *table, *starts, *lengths;
-    int64_t table_stride;
+    int64_t table_stride, table_head;  // entries from one sequence's row to the next's, and from one kv head's (0: all share)
     uint32_t table_pages;
     int *flag;
 
     // The page that place `j` (< table_pages * page_size, which is below 2^31) of sequence s is in.  One outside the cache
     // raises the flag and reads as `instead`.
-    __device__ __forceinline__ int32_t page_of(uint32_t s, uint32_t index, int32_t instead) const {
-        const int32_t page = table[(int64_t)s * table_stride + index];
+    __device__ __forceinline__ int32_t page_of(uint32_t s, uint32_t index, int32_t instead, uint32_t head = 0) const {
+        const int32_t page = table[(int64_t)s * table_stride + (int64_t)head * table_head + index];
         if ((uint32_t)page < pages) return page;
         *flag = 1;
         return instead;

@@ -1,0 +1,470 @@
+// Attention over the pages of a cache that a cheap score selects: means of the pages that fill, a score for each page from its mean, the best pages of each
+// row and head of keys, and attention (kv_attend.h) over those, each row being a sequence of its own with a page table of its own for each head.
+//   Scores are sums of products of fp32 values in 64 bits, where no product is rounded: two pages change places only if their scores agree to about 2^-50,
+// whatever order the sums are made in.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kv_attend.h"
+
+namespace altius {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t BLOCK = 256, WAVES = BLOCK / 64;
+constexpr uint32_t HELD = 16384;     // images of pages in LDS
+constexpr uint32_t SCORED = 64;      // pages of a block that does nothing but score
+constexpr uint32_t MOST_CHANNELS = 256;
+
+struct SparseArgs {
+    dev::KvView kv;
+    float *means;
+    int64_t means_page, means_head;
+    int32_t *chosen;
+    const float *q;
+    int64_t q_token, q_head;
+    uint32_t d, group, q_heads, most, first, last;
+    uint32_t max_tokens, max_keys, max_pages, held, chunks;
+    bool bf16, fills;   // fills: choose_pages makes the mean of a page that its row fills
+    double *scores;     // [row][kv head][max_pages]; null: choose_pages makes them itself
+    int32_t *table, *starts, *lengths;  // of the sequences that attention sees
+};
+
+// ---------------------------------------------------------------- means
+// The mean of page `page` for one head, by a block: lanes side by side take 4 channels each, groups of lanes the slots in turn; sums in 64 bits, rounded once.
+__device__ __forceinline__ void page_mean(const SparseArgs &g, int32_t page, uint32_t head) {
+    __shared__ double sums[BLOCK][4];
+    const uint32_t lanes = g.d / 4, groups = BLOCK / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    const int64_t at = (int64_t)page * g.kv.page_stride + (int64_t)head * g.kv.head_stride + 4 * lane;
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    if (group < groups) {
+#pragma unroll 4
+        for (uint32_t slot = group; slot < g.kv.page_size; slot += groups) {
+            const int64_t from = at + (int64_t)slot * g.kv.slot_stride;
+            if (g.bf16) {
+                const u16x4 x = *reinterpret_cast<const u16x4 *>(static_cast<const uint16_t *>(g.kv.keys) + from);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[e] += (double)__uint_as_float((uint32_t)x[e] << 16);
+            } else {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(g.kv.keys) + from);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[e] += (double)x[e];
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; e++) sums[threadIdx.x][e] = sum[e];
+    __syncthreads();
+    if (group == 0) {
+        f32x4 mean;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            for (uint32_t i = 1; i < groups; i++) sum[e] += sums[i * lanes + lane][e];
+            mean[e] = (float)(sum[e] / (double)g.kv.page_size);
+        }
+        *reinterpret_cast<f32x4 *>(g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head + 4 * lane) = mean;
+    }
+}
+
+__device__ __forceinline__ dev::KvSequence within(const SparseArgs &g, dev::KvSequence q) {
+    if ((uint32_t)q.n > g.max_tokens || (uint32_t)q.length > g.max_keys) {
+        *g.kv.flag = 1;
+        q.n = 0;
+    }
+    return q;
+}
+
+// A block for each sequence, page that its rows can have filled, and head.
+__global__ __launch_bounds__(BLOCK) void mean_pages(SparseArgs g) {
+    const uint32_t outer = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - outer * g.kv.kv_heads, s = outer / g.chunks, i = outer - s * g.chunks;
+    const dev::KvSequence q = within(g, dev::kv_sequence(g.kv, s));
+    if (q.n == 0) return;
+    const uint32_t base = (uint32_t)max(0, q.length - q.n), index = g.kv.by_page_size.div(base) + i;
+    if ((uint64_t)(index + 1) * g.kv.page_size > (uint32_t)q.length) return;
+    const int32_t page = g.kv.page_of(s, index, -1);
+    if (page >= 0) page_mean(g, page, head);
+}
+
+// ---------------------------------------------------------------- scores
+template <int CONTROL> __device__ __forceinline__ double moved(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CONTROL, 0xF, 0xF, false);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CONTROL, 0xF, 0xF, false);
+    return __longlong_as_double((long long)((uint64_t)high << 32 | low));
+}
+constexpr int ROR8 = dev::DPP_ROW_ROR + 8;
+// v[h] summed over a row of 16 lanes, the largest of the sums in all of them.  Of two lanes that meet each keeps half of the heads, so that 8
+// sums take 8 exchanges and not 32.
+template <int HEADS> __device__ __forceinline__ double largest_sum(double (&v)[HEADS]) {
+    const uint32_t lane = threadIdx.x;
+    int left = HEADS;
+    auto halve = [&](auto move, bool upper) {
+        left /= 2;
+#pragma unroll
+        for (int h = 0; h < HEADS / 2; h++) {
+            if (h >= left) break;
+            const double keep = upper ? v[h + left] : v[h], give = upper ? v[h] : v[h + left];
+            v[h] = keep + move(give);
+        }
+    };
+    halve([](double x) { return moved<ROR8>(x); }, lane & 8u);
+    halve([](double x) { return moved<dev::DPP_ROW_HALF_MIRROR>(x); }, lane & 4u);
+    if (HEADS == 8) halve([](double x) { return moved<dev::DPP_QUAD_XOR2>(x); }, lane & 2u);
+    else v[0] += moved<dev::DPP_QUAD_XOR2>(v[0]);
+    v[0] += moved<dev::DPP_QUAD_XOR1>(v[0]);
+    double best = fmax(v[0], moved<ROR8>(v[0]));
+    best = fmax(best, moved<dev::DPP_ROW_HALF_MIRROR>(best));
+    if (HEADS == 8) best = fmax(best, moved<dev::DPP_QUAD_XOR2>(best));
+    return best;
+}
+
+// Scores of pages from .. to - 1 of a row's sequence, by a block: 16 lanes a page, 4 J channels each, HEADS queries of the group at a time in registers.
+// put(page, score, again): again: the larger of it and what is there.
+template <int J, int HEADS, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t from, uint32_t to, Put put) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, l = lane & 15u;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t h0 = 0; h0 < g.group; h0 += HEADS) {
+        double q[HEADS][J][4];
+#pragma unroll
+        for (int h = 0; h < HEADS; h++) {
+            const uint32_t its = head * g.group + min(h0 + h, g.group - 1);  // the last one again counts once
+            const float *from_q = g.q + (int64_t)row * g.q_token + (int64_t)its * g.q_head;
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const uint32_t c = 64 * j + 4 * l;
+                const f32x4 x = c < g.d ? *reinterpret_cast<const f32x4 *>(from_q + c) : zero;
+#pragma unroll
+                for (int e = 0; e < 4; e++) q[h][j][e] = (double)x[e];
+            }
+        }
+        for (uint32_t base = from + 4 * wave; base < to; base += 4 * WAVES) {
+            const uint32_t index = base + (lane >> 4);
+            const int32_t page = index < to ? g.kv.page_of(s, index, -1) : -1;
+            const float *mean = g.means + (int64_t)max(page, 0) * g.means_page + (int64_t)head * g.means_head;
+            f32x4 x[J];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const uint32_t c = 64 * j + 4 * l;
+                x[j] = *reinterpret_cast<const f32x4 *>(mean + (c < g.d ? c : 0));
+                if (c >= g.d) x[j] = zero;
+            }
+            double v[HEADS];
+#pragma unroll
+            for (int h = 0; h < HEADS; h++) {
+                v[h] = 0.0;
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[h] = __builtin_fma(q[h][j][e], (double)x[j][e], v[h]);
+            }
+            const double best = largest_sum(v);
+            if (l == 0 && index < to) put(index, best, h0 != 0);
+        }
+    }
+}
+
+// The row's place in its sequence, and the pages in front of it with its own: 0 where there is no such row.
+struct Row {
+    uint32_t s, pages, place;
+    bool live;
+};
+__device__ __forceinline__ Row row_of(const SparseArgs &g, uint32_t row) {
+    dev::KvSequence q = {0, 0, 0};
+    Row r = {0, 0, 0, false};
+    r.s = dev::kv_sequence_of(g.kv, row, q);
+    if (r.s >= g.kv.sequences) return r;
+    q = within(g, q);
+    const int32_t t = (int32_t)row - q.start;
+    if (t < 0 || t >= q.n) return r;
+    r.live = true;
+    const int32_t place = q.length - q.n + t;
+    if (place < 0) return r;
+    r.place = (uint32_t)place, r.pages = g.kv.by_page_size.div(r.place) + 1;
+    return r;
+}
+
+template <int J, int HEADS> __global__ __launch_bounds__(BLOCK) void score_pages(SparseArgs g) {
+    const uint32_t outer = blockIdx.x / g.chunks, chunk = blockIdx.x - outer * g.chunks, row = outer / g.kv.kv_heads, head = outer - row * g.kv.kv_heads;
+    const Row r = row_of(g, row);
+    if (r.pages <= g.most) return;  // all are chosen
+    const uint32_t from = max(chunk * SCORED, g.first), to = min((chunk + 1) * SCORED, r.pages - g.last);
+    double *to_scores = g.scores + (size_t)outer * g.max_pages;
+    score_range<J, HEADS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
+}
+
+// ---------------------------------------------------------------- the best
+// Larger for larger scores, 0 for NaN.
+__device__ __forceinline__ uint64_t rank_image(double score) {
+    if (score != score) return 0;
+    const uint64_t u = (uint64_t)__double_as_longlong(score + 0.0);
+    return u >> 63 ? ~u : u | (uint64_t)1 << 63;
+}
+
+// A block for each row and head of keys.  The smallest image that is chosen is found by halving the range between the smallest and the largest, until
+// exactly as many as are wanted are at or above the middle; equal ones go by their number.  Then the pages are listed in order.
+template <int J, int HEADS> __global__ __launch_bounds__(BLOCK) void choose_pages(SparseArgs g) {
+    extern __shared__ uint64_t images[];
+    __shared__ uint64_t ends[WAVES][2];
+    __shared__ uint32_t totals[2][WAVES][2];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t row = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - row * g.kv.kv_heads;
+    const Row r = row_of(g, row);
+    const int32_t first_row = g.kv.starts[0], end_row = g.kv.starts[g.kv.sequences];
+    if (head == 0 && tid < 2 && (tid == 0 || row + 1 == g.kv.tokens)) {
+        const int32_t at = (int32_t)(row + tid);
+        g.starts[at] = max(0, min(min(max(at, first_row), end_row), (int32_t)g.kv.tokens));
+    }
+    if (!r.live) {
+        // In front of the sequences or behind them: a sequence without rows; in one that does not fit: left out.
+        if (head == 0 && tid == 0) g.lengths[row] = (int32_t)row < first_row || (int32_t)row >= end_row ? 0 : -1;
+        return;
+    }
+    const size_t list = ((size_t)row * g.kv.kv_heads + head) * g.most;
+    const uint32_t count = min(r.pages, g.most);
+    if (head == 0 && tid == 0) g.lengths[row] = count ? (int32_t)((count - 1) * g.kv.page_size + (r.place - (r.pages - 1) * g.kv.page_size) + 1) : 0;
+    for (uint32_t i = count + tid; i < g.most; i += BLOCK) g.chosen[list + i] = -1;
+    if (g.fills && count && r.place + 1 == r.pages * g.kv.page_size) {
+        const int32_t page = g.kv.page_of(r.s, r.pages - 1, -1);
+        if (page >= 0) page_mean(g, page, head);
+    }
+    auto put = [&](uint32_t at, uint32_t page) {
+        g.chosen[list + at] = (int32_t)page;
+        g.table[list + at] = g.kv.page_of(r.s, page, -1);
+    };
+    if (r.pages <= g.most) {
+        for (uint32_t i = tid; i < count; i += BLOCK) put(i, i);
+        return;
+    }
+
+    const uint32_t from = g.first, to = r.pages - g.last, want = g.most - g.first - g.last;  // of the pages from .. to - 1, of which there are more
+    const double *scores = J ? nullptr : g.scores + ((size_t)row * g.kv.kv_heads + head) * g.max_pages;
+    if constexpr (J != 0) {
+        score_range<J, HEADS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) {
+            const uint64_t v = rank_image(score);
+            images[page] = again ? max(images[page], v) : v;
+        });
+    } else {
+        for (uint32_t page = from + tid; page < min(to, g.held); page += BLOCK) images[page] = rank_image(scores[page]);
+    }
+    __syncthreads();
+    auto image = [&](uint32_t page) { return J != 0 || page < g.held ? images[page] : rank_image(scores[page]); };
+
+    // low: at least as many as wanted are at or above it; high: fewer are.
+    uint64_t low = ~(uint64_t)0, high = 0;
+    for (uint32_t page = from + tid; page < to; page += BLOCK) {
+        const uint64_t v = image(page);
+        low = min(low, v), high = max(high, v);
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) low = min(low, (uint64_t)__shfl_xor((unsigned long long)low, m)), high = max(high, (uint64_t)__shfl_xor((unsigned long long)high, m));
+    if (lane == 0) ends[wave][0] = low, ends[wave][1] = high;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; w++) low = min(low, ends[w][0]), high = max(high, ends[w][1]);
+    uint32_t above = 0;  // how many are at or above `high`
+    bool exact = want == 0;
+    uint64_t least = high + 1;
+    high++;  // images are below 2^64 - 1: that would be a NaN
+    for (int turn = 0; !exact && high - low > 1; turn ^= 1) {
+        const uint64_t middle = low + (high - low) / 2;
+        uint32_t n = 0;
+        for (uint32_t page = from + tid; page < to; page += BLOCK) n += image(page) >= middle ? 1u : 0u;
+#pragma unroll
+        for (int m = 32; m; m >>= 1) n += __shfl_xor(n, m);
+        if (lane == 0) totals[turn][wave][0] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; w++) n += totals[turn][w][0];
+        if (n == want) exact = true, least = middle;
+        else if (n > want) low = middle;
+        else high = middle, above = n;
+    }
+    // Either all at or above `least`, or all above `low` (as many as at or above `high`) and the first of those at it.
+    const uint32_t ties = exact ? 0 : want - above;
+    if (!exact) least = low;
+    uint32_t listed = 0, tied = 0;
+    for (uint32_t base = 0, turn = 0; base < r.pages; base += BLOCK, turn ^= 1) {
+        const uint32_t page = base + tid;
+        const bool there = page < r.pages, always = there && (page < from || page >= to);
+        const uint64_t v = there && !always ? image(page) : 0;
+        const bool over = there && !always && (exact ? v >= least && want != 0 : v > least), tie = there && !always && !exact && v == least;
+        const uint64_t before = ((uint64_t)1 << lane) - 1, tie_mask = __ballot(tie);
+        // Ties of the wavefronts in front count first.
+        __syncthreads();
+        if (lane == 0) totals[turn][wave][1] = (uint32_t)__popcll(tie_mask);
+        __syncthreads();
+        uint32_t tie_at = tied;
+        for (uint32_t w = 0; w < WAVES; w++) {
+            if (w < wave) tie_at += totals[turn][w][1];
+            tied += totals[turn][w][1];
+        }
+        const bool stays = always || over || (tie && tie_at + (uint32_t)__popcll(tie_mask & before) < ties);
+        const uint64_t stay_mask = __ballot(stays);
+        if (lane == 0) totals[turn][wave][0] = (uint32_t)__popcll(stay_mask);
+        __syncthreads();
+        uint32_t at = listed;
+        for (uint32_t w = 0; w < WAVES; w++) {
+            if (w < wave) at += totals[turn][w][0];
+            listed += totals[turn][w][0];
+        }
+        if (stays) put(at + (uint32_t)__popcll(stay_mask & before), page);
+    }
+}
+
+// ---------------------------------------------------------------- the host's part
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+constexpr int64_t MOST_STRIDE = (int64_t)1 << 48;
+constexpr uint64_t MOST_GRID = (uint64_t)1 << 24;
+
+int check_means(DeviceCtx *ctx, const std::string &name, const ahip_kv_cache &cache, const ahip_kv_sparse &sparse) {
+    if (sparse.page_stride < 0 || sparse.head_stride < 0 || sparse.page_stride > MOST_STRIDE || sparse.head_stride > MOST_STRIDE)
+        return kv_fail(ctx, AHIP_ERR_ARG, name + "a stride of the means is out of range");
+    const int64_t unit = cache.elem == AHIP_KV_BF16 ? 8 : 4;
+    if (cache.head_size > (int32_t)MOST_CHANNELS || cache.head_size % unit) return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "no kernel for heads of " + std::to_string(cache.head_size));
+    if (!aligned16(sparse.means) || sparse.page_stride % 4 || sparse.head_stride % 4 || !aligned16(cache.keys) || cache.page_stride % unit || cache.head_stride % unit ||
+        cache.slot_stride % unit)
+        return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "a tensor or stride is not on 16-byte boundaries");
+    return AHIP_OK;
+}
+
+struct SparsePlan {
+    ahip_kv_batch batch;    // as attention sees it
+    ahip_kv_attend attend;
+    size_t attend_bytes, starts, lengths, table, scores, bytes;
+    uint64_t max_pages, rows;  // rows: times heads of keys
+    bool split;                // scores by a launch of their own
+};
+
+SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const ahip_kv_sparse &sparse) {
+    SparsePlan p = {};
+    p.batch = {(int32_t)attend.tokens, sparse.most, (int64_t)sparse.most * cache.kv_heads, nullptr, nullptr, nullptr};
+    p.attend = attend;
+    p.attend.max_tokens = 1, p.attend.max_keys = 0;
+    const size_t held = (size_t)batch.table_pages * (size_t)cache.page_size, max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
+    p.max_pages = (max_keys + cache.page_size - 1) / cache.page_size;
+    p.rows = attend.tokens * (uint64_t)cache.kv_heads;
+    const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
+    p.split = p.max_pages > HELD || (p.rows < cus && p.max_pages > 4 * SCORED);
+    p.attend_bytes = attend::plan_of(ctx, cache, p.batch, p.attend).bytes;
+    p.starts = up16(p.attend_bytes);
+    p.lengths = up16(p.starts + (attend.tokens + 1) * sizeof(int32_t));
+    p.table = up16(p.lengths + attend.tokens * sizeof(int32_t));
+    p.scores = up16(p.table + p.rows * (size_t)sparse.most * sizeof(int32_t));
+    p.bytes = p.split ? p.scores + p.rows * p.max_pages * sizeof(double) : p.scores;
+    return p;
+}
+
+int check_sparse(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const ahip_kv_sparse *sparse, dev::KvView *view) {
+    const std::string name = "kv attention over chosen pages: ";
+    if (!sparse) return kv_fail(ctx, AHIP_ERR_ARG, name + "null sparse");
+    if (int rc = attend::check_attend(ctx, cache, batch, attend, view)) return rc;
+    if (!attend->causal || attend->window || attend->slopes || attend->prefix || attend->first_keys)
+        return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "causal attention without window, slopes, prefix and first keys only");
+    if (sparse->first < 0 || sparse->last < 1 || (int64_t)sparse->first + sparse->last > sparse->most)
+        return kv_fail(ctx, AHIP_ERR_ARG, name + "the first and the last pages, one of those at least, fit into what is chosen");
+    if ((int64_t)sparse->most * cache->page_size > INT32_MAX - (1 << 16) || attend->tokens * (uint64_t)cache->kv_heads >= MOST_GRID)
+        return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more chosen keys, or rows, than are supported");
+    return check_means(ctx, name, *cache, *sparse);
+}
+
+template <int J, int HEADS> void launch_choice(hipStream_t stream, const SparseArgs &g, const SparsePlan &p) {
+    const dim3 grid((uint32_t)p.rows), block(BLOCK);
+    const uint32_t held = (uint32_t)(g.held * sizeof(uint64_t));
+    if (p.split) {
+        hipLaunchKernelGGL((score_pages<J, HEADS>), dim3((uint32_t)(p.rows * g.chunks)), block, 0, stream, g);
+        hipLaunchKernelGGL((choose_pages<0, 1>), grid, block, held, stream, g);
+    } else {
+        hipLaunchKernelGGL((choose_pages<J, HEADS>), grid, block, held, stream, g);
+    }
+}
+
+SparseArgs args_of(const dev::KvView &view, const ahip_kv_cache &cache, const ahip_kv_sparse &sparse) {
+    SparseArgs g = {};
+    g.kv = view;
+    g.means = sparse.means, g.means_page = sparse.page_stride, g.means_head = sparse.head_stride;
+    g.d = (uint32_t)cache.head_size, g.bf16 = cache.elem == AHIP_KV_BF16;
+    return g;
+}
+
+// Pages that the rows of a call can fill: g.chunks, and a launch over them.
+int launch_means(DeviceCtx &ctx, SparseArgs g, const std::string &name) {
+    g.chunks = g.max_tokens / g.kv.page_size + 1;
+    const uint64_t blocks = (uint64_t)g.kv.sequences * g.kv.kv_heads * g.chunks;
+    if (blocks >= MOST_GRID) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
+    hipLaunchKernelGGL(mean_pages, dim3((uint32_t)blocks), dim3(BLOCK), 0, ctx.stream, g);
+    return ctx.check(hipGetLastError(), "kv page means launch");
+}
+
+}  // namespace
+
+int launch_kv_page_means(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_sparse &sparse, size_t tokens, size_t max_tokens) {
+    const std::string name = "kv page means: ";
+    dev::KvView view = {};
+    if (int rc = make_kv_view(&ctx, "kv page means", &cache, &batch, tokens, &view)) return rc;
+    if (int rc = check_means(&ctx, name, cache, sparse)) return rc;
+    if (tokens == 0 || batch.sequences == 0) return AHIP_OK;
+    if (int rc = require_kv_arrays(ctx, "kv page means", cache, batch)) return rc;
+    if (!sparse.means) return ctx.fail(AHIP_ERR_ARG, name + "null means");
+    SparseArgs g = args_of(view, cache, sparse);
+    g.max_tokens = (uint32_t)std::min(max_tokens ? max_tokens : tokens, tokens), g.max_keys = INT32_MAX;
+    return launch_means(ctx, g, name);
+}
+
+int kv_attention_sparse_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, const ahip_kv_sparse *sparse,
+                                  size_t *bytes) {
+    if (!bytes) return kv_fail(ctx, AHIP_ERR_ARG, "kv attention over chosen pages: null output");
+    *bytes = 0;
+    dev::KvView view = {};
+    if (int rc = check_sparse(ctx, cache, batch, attend, sparse, &view)) return rc;
+    *bytes = sparse_plan(ctx, *cache, *batch, *attend, *sparse).bytes;
+    return AHIP_OK;
+}
+
+int launch_kv_attention_sparse(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const ahip_kv_sparse &sparse) {
+    const std::string name = "kv attention over chosen pages: ";
+    dev::KvView view = {};
+    if (int rc = check_sparse(&ctx, &cache, &batch, &attend, &sparse, &view)) return rc;
+    if (attend.tokens == 0 || batch.sequences == 0) return AHIP_OK;
+    if (int rc = require_kv_arrays(ctx, "kv attention over chosen pages", cache, batch)) return rc;
+    if (!sparse.means || !sparse.chosen || !attend.q) return ctx.fail(AHIP_ERR_ARG, name + "null pointer");
+    SparsePlan p = sparse_plan(&ctx, cache, batch, attend, sparse);
+    if (!attend.workspace || attend.workspace_bytes < p.bytes)
+        return ctx.fail(AHIP_ERR_ARG, name + "the workspace holds " + std::to_string(attend.workspace ? attend.workspace_bytes : 0) + " bytes of " + std::to_string(p.bytes));
+    char *space = static_cast<char *>(attend.workspace);
+    SparseArgs g = args_of(view, cache, sparse);
+    g.chosen = sparse.chosen, g.q = attend.q, g.q_token = (int64_t)attend.q_strides[0], g.q_head = (int64_t)attend.q_strides[1];
+    g.q_heads = (uint32_t)attend.q_heads, g.group = (uint32_t)(attend.q_heads / cache.kv_heads);
+    g.most = (uint32_t)sparse.most, g.first = (uint32_t)sparse.first, g.last = (uint32_t)sparse.last;
+    g.max_tokens = (uint32_t)std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
+    g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
+    g.max_pages = (uint32_t)p.max_pages, g.held = (uint32_t)std::min<uint64_t>(p.max_pages, HELD);
+    g.chunks = (uint32_t)((p.max_pages + SCORED - 1) / SCORED);
+    g.starts = reinterpret_cast<int32_t *>(space + p.starts), g.lengths = reinterpret_cast<int32_t *>(space + p.lengths), g.table = reinterpret_cast<int32_t *>(space + p.table);
+    g.scores = p.split ? reinterpret_cast<double *>(space + p.scores) : nullptr;
+    if (p.split && p.rows * g.chunks >= MOST_GRID) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
+    // What attention will see, before anything is launched.
+    p.batch.query_starts = g.starts, p.batch.lengths = g.lengths, p.batch.page_table = g.table;
+    p.attend.workspace_bytes = p.attend_bytes;
+    attend::AttendArgs a = {};
+    if (int rc = attend::begin_attend(ctx, cache, p.batch, p.attend, &a)) return rc;
+    a.kv.table_head = sparse.most;
+
+    // A single row fills a page for later calls only; several may score a page that one of them has filled.
+    g.fills = g.max_tokens == 1;
+    if (!g.fills)
+        if (int rc = launch_means(ctx, g, name)) return rc;
+    if (g.d <= 64) g.group <= 4 ? launch_choice<1, 4>(ctx.stream, g, p) : launch_choice<1, 8>(ctx.stream, g, p);
+    else if (g.d <= 128) g.group <= 4 ? launch_choice<2, 4>(ctx.stream, g, p) : launch_choice<2, 8>(ctx.stream, g, p);
+    else launch_choice<4, 4>(ctx.stream, g, p);
+    if (int rc = ctx.check(hipGetLastError(), "kv attention over chosen pages launch")) return rc;
+    return attend::launch_attend_rows(ctx, a, g.bf16);
+}
+
+}  // namespace altius

@@ -1,0 +1,26 @@
+// Attention of trees of drafted tokens over a paged cache: the kernels of kv_attend.h, with a mask of a row's own tree beside its range of keys.
+// 16 trees of 16 to 48 tokens behind 300 to 8000 (bf16, 32 heads, 8 of keys, 128 channels) and 2 of 40 to 61 behind 20011 to 30000 (fp32, 16 heads,
+// 4 of keys, 96 channels, biased): the tree costs a load of the parents and the walk up at a block's start, and a look at the mask in the last one or
+// two tiles of a sequence.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kv_attend.h"
+
+namespace altius {
+
+int launch_kv_attention_tree(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const int32_t *parents) {
+    const std::string name = "kv attention of a tree: ";
+    if (!attend.causal || attend.prefix) return ctx.fail(AHIP_ERR_ARG, name + "a tree is causal and has no prefix");
+    if (attend.max_tokens > attend::TREE_ROWS) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more than 256 rows a sequence");
+    attend::AttendArgs g = {};
+    if (int rc = attend::begin_attend(ctx, cache, batch, attend, &g)) return rc;
+    if (!g.q) return AHIP_OK;
+    if (!parents) return ctx.fail(AHIP_ERR_ARG, name + "null parents");
+    g.parents = parents;
+    g.max_tokens = std::min(g.max_tokens, attend::TREE_ROWS);
+    return attend::launch_attend<true>(ctx, g, cache.elem == AHIP_KV_BF16);
+}
+
+}  // namespace altius

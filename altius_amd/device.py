@@ -9,7 +9,8 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from ._lib import HeadRows, KvAttend, KvBatch, KvCache, KvTokens, Rotary, check, i64_array  # noqa: F401 (described here for callers)
+from ._lib import (HeadRows, KvAttend, KvBatch, KvCache, KvEviction, KvHistory, KvMoves, KvSparse, KvTokens, Rotary, check,  # noqa: F401 (described here for callers)
+                   i64_array)
 
 ADD, SUB, MUL, DIV, POW = 0, 1, 2, 3, 4
 SQRT, ERF, GELU, SIGMOID, HARDSIGMOID, RELU, TANH, LEAKYRELU, EXP, ROUND, CLIP = range(11)
@@ -53,6 +54,22 @@ def kv_attention_workspace(ctx, cache, batch, attend):
     n = ctypes.c_size_t()
     handle = ctx.handle if ctx else None
     check(_lib.lib().ahip_kv_attention_workspace(handle, ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(attend), ctypes.byref(n)), handle)
+    return n.value
+
+
+def kv_attention_mass_workspace(ctx, cache, batch, attend):
+    """Bytes of workspace that kv_attention_mass_raw wants for these arguments; ctx may be None (host only)."""
+    n = ctypes.c_size_t()
+    handle = ctx.handle if ctx else None
+    check(_lib.lib().ahip_kv_attention_mass_workspace(handle, ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(attend), ctypes.byref(n)), handle)
+    return n.value
+
+
+def kv_attention_sparse_workspace(ctx, cache, batch, attend, sparse):
+    """Bytes of workspace that kv_attention_sparse_raw wants for these arguments; ctx may be None (host only)."""
+    n = ctypes.c_size_t()
+    handle = ctx.handle if ctx else None
+    check(_lib.lib().ahip_kv_attention_sparse_workspace(handle, ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(attend), ctypes.byref(sparse), ctypes.byref(n)), handle)
     return n.value
 
 
@@ -229,6 +246,42 @@ class Context:
     def kv_attention_raw(self, cache, batch, attend):
         """ahip_kv_attention."""
         rc = self.L.ahip_kv_attention(self.handle, cache, batch, attend)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_attention_tree_raw(self, cache, batch, attend, parents):
+        """ahip_kv_attention_tree: the rows of each sequence are a tree, by the row that each follows (device pointer, i32)."""
+        rc = self.L.ahip_kv_attention_tree(self.handle, cache, batch, attend, parents)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_attention_mass_raw(self, cache, batch, attend, history, decay=1.0, row_positions=None):
+        """ahip_kv_attention_mass: attention, and what it gave each key added to the KvHistory."""
+        rc = self.L.ahip_kv_attention_mass(self.handle, cache, batch, attend, history, decay, row_positions)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_evict_raw(self, cache, batch, history, eviction):
+        """ahip_kv_evict: which slots stay, as the lists of a KvEviction."""
+        rc = self.L.ahip_kv_evict(self.handle, cache, batch, history, eviction)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_move_raw(self, cache, batch, moves, history=None):
+        """ahip_kv_move: the slots of KvMoves to their new places."""
+        rc = self.L.ahip_kv_move(self.handle, cache, batch, moves, history)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_attention_sparse_raw(self, cache, batch, attend, sparse):
+        """ahip_kv_attention_sparse: attention over the pages that their means select."""
+        rc = self.L.ahip_kv_attention_sparse(self.handle, cache, batch, attend, sparse)
+        if rc:
+            check(rc, self.handle)
+
+    def kv_page_means_raw(self, cache, batch, sparse, tokens, max_tokens=0):
+        """ahip_kv_page_means: the means of the pages that the batch's newest rows fill."""
+        rc = self.L.ahip_kv_page_means(self.handle, cache, batch, sparse, tokens, max_tokens)
         if rc:
             check(rc, self.handle)
 

@@ -462,6 +462,85 @@ int ahip_kv_attention_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const
  * calls that run at the same time need one each.  out must not overlap q (the same pointer is refused). */
 int ahip_kv_attention(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend);
 
+/* Attention of drafted tokens: the newest rows of a sequence are a tree.  Row t of the sequence's n follows its row parents[start + t] < t,
+ * or, -1, the last token in front of the rows.  With depth(t) rows above it and base = lengths[s] - n tokens in front, its position is
+ * base + depth(t), and it sees, of the slots in front of the rows, those of ahip_kv_attend at that position (window and first_keys), and of the
+ * rows' own slots its own and those of the rows it follows, less than a window above it; |p - j| of the slopes is the distance of the
+ * positions.  Everything else, the workspace too, is ahip_kv_attention's.  Up to 256 rows a sequence; causal, without a prefix (AHIP_ERR_ARG
+ * otherwise).  A sequence of more rows is left out, a row that follows none in front of it is taken for one that follows no row, and the next
+ * ahip_sync fails. */
+#define AHIP_KV_TREE_ROWS 256
+int ahip_kv_attention_tree(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
+                           const int32_t *parents);
+
+/* What a cache remembers of each slot and head of keys, at page * page_stride + head * head_stride + slot (elements): how much attention it was
+ * given, and the position of its token, which is not its place any more once slots have moved. */
+typedef struct ahip_kv_history {
+    float *mass;
+    int32_t *positions; /* may be NULL for ahip_kv_attention_mass and ahip_kv_move */
+    int64_t page_stride, head_stride;
+} ahip_kv_history;
+/* ahip_kv_attention, and what it gave each key: for every slot of the sequences that have rows in the call and every head of keys,
+ *     mass = decay * mass + the sum of the softmax's weights over the sequence's rows and the head's group of query heads,
+ * where the rows' own slots start from 0, and so do all where decay is 0: what was there is not read then.  positions (if not NULL) of the rows'
+ * own slots become row_positions[row], or their place where that is NULL.  decay from 0 to 1.  The weights are added in the same order in
+ * every call.  A sequence whose rows are more than its tokens is left out. */
+int ahip_kv_attention_mass_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
+                                     size_t *bytes);
+int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
+                           const ahip_kv_history *history, float decay, const int32_t *row_positions);
+
+/* Which slots stay where a sequence is longer than its budget, for each head of keys by itself: those with a position below `first` or of
+ * the `recent` newest (above the largest less `recent`), then those with the largest mass; of equal ones the lowest place.  NaN counts as
+ * less than all else.  The i-th place from `budget` on that stays is sources[i], the i-th place below it that does not is targets[i], for i <
+ * counts; behind that the lists stay as they were.  ahip_kv_move with these lists (apart) leaves what stays in the first `budget` places, in no order
+ * of positions.  lengths[s] becomes min(length, budget).  Lists of sequence s and head h start at (s * kv_heads + h) * most, counts at
+ * s * kv_heads + h.  Of the batch, query_starts is not read (it may be NULL); of the cache, neither keys nor values. */
+typedef struct ahip_kv_eviction {
+    int32_t budget, recent, first; /* recent + first up to the budget */
+    int32_t most;                  /* no list is longer: at least min(budget, max_keys - budget) */
+    size_t max_keys;               /* no sequence is longer; 0: as the table allows */
+    int32_t *sources, *targets, *counts, *lengths; /* device */
+} ahip_kv_eviction;
+int ahip_kv_evict(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_history *history,
+                  const ahip_kv_eviction *eviction);
+
+/* Slots that go to other places of their sequence: keys, values and, where history is not NULL, masses and positions.  Head h of sequence s moves
+ * sources[at + i] to targets[at + i] for i < counts[s * count_strides[0] + h * count_strides[1]], at = s * strides[0] + h * strides[1]: a
+ * head stride of 0 is one list for all heads.  apart: no place of a list is both a source and a target, and all moves are made at once.  Otherwise
+ * they are made in order, and none may read a place that an earlier one wrote (its value is either's then), as in the accepted branch of
+ * a tree that goes to the front.  No two targets of a list may be the same.  Of the batch, only sequences and the page table are read.  A place
+ * outside the table or a page outside the cache is left out, a count outside 0 .. most moves nothing, and the next ahip_sync fails. */
+typedef struct ahip_kv_moves {
+    const int32_t *sources, *targets, *counts; /* device */
+    int64_t strides[2], count_strides[2];
+    int32_t most, apart;
+} ahip_kv_moves;
+int ahip_kv_move(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_moves *moves, const ahip_kv_history *history);
+
+/* Attention over the pages that a cheap score selects.  The row at place p stands in page o = p / page_size.  For each head of keys it sees the keys
+ * up to p of `most` of the pages 0 .. o, of all where there are no more: the first `first`, the `last` newest (o - last + 1 .. o), then those with
+ * the largest score, of equal ones the lowest page.  A page's score is the largest product of a query of the head's group with the mean of the
+ * page's keys, in 64 bits, NaN counting as less than all else; that mean, of head_size values at page * page_stride + head * head_stride, is held
+ * in 32 bits.  The call writes the means of the pages that its rows fill, before they are used; those filled earlier have to be there, from
+ * earlier calls or from ahip_kv_page_means.  chosen becomes, at (row * kv_heads + head) * most, the pages in ascending order with -1 behind them; rows
+ * that see none, and none of the rows that are padding, are written all -1 and left as they were.  attend: causal, no window, slopes, prefix or
+ * first_keys (AHIP_ERR_UNSUPPORTED). */
+typedef struct ahip_kv_sparse {
+    float *means;
+    int64_t page_stride, head_stride;
+    int32_t *chosen;
+    int32_t most, first, last; /* last at least 1, first + last up to most */
+} ahip_kv_sparse;
+int ahip_kv_attention_sparse_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
+                                       const ahip_kv_sparse *sparse, size_t *bytes);
+int ahip_kv_attention_sparse(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
+                             const ahip_kv_sparse *sparse);
+/* The means of the pages that the newest rows of each sequence fill, as ahip_kv_attention_sparse writes them: behind a prompt that went through
+ * ahip_kv_attention.  tokens: rows of the batch's tensors; max_tokens: no sequence has more of them (0: tokens).  Of sparse, only the means. */
+int ahip_kv_page_means(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_sparse *sparse, size_t tokens,
+                       size_t max_tokens);
+
 /* Which kernel ahip_gemm (and the MatMul / Gemm / Conv2d operators of a session on this context) uses
  * for a single-batch product.  AHIP_GEMM_FP32: v_mfma_f32_32x32x2_f32 on the operands as they are.
  * AHIP_GEMM_BF16X3: every operand value is split exactly into three bf16 numbers and six bf16 MFMAs per
