@@ -65,6 +65,10 @@ struct AttendArgs {
     uint32_t max_tokens, max_keys;
     const int32_t *parents;  // of a tree's rows (TREE)
     float *stats;            // of each row and query head: the maximum that its weights are relative to, and 1 / their sum; null: nobody asks
+    // The scores of sequences of few rows, where somebody asks for them: of row r (below score_rows) of a pair (sequence, kv head) and key j that
+    // some row sees at (pair * score_rows + r) * score_keys + j.  score_keys: a multiple of 16, all of a tile's are written.
+    float *scores;
+    uint32_t score_rows, score_keys;
     Share few, many;  // of sequences with up to few_rows rows, and with more
 };
 
@@ -77,6 +81,10 @@ __device__ __forceinline__ dev::KvSequence sequence_of(const AttendArgs &g, uint
     }
     return q;
 }
+
+// What a kernel is built for.  PLAIN: ahip_kv_attention.  TREE: the rows are a tree.  KEPT: page tables may differ by head, and the rows' statistics and scores
+// may be asked for.  (One kernel that asks while it runs takes up to 3 % longer: 4 prompts of 1024, 12 heads of 64 channels, fp32, 58.2 and 60.2 us.)
+constexpr int PLAIN = 0, TREE = 1, KEPT = 2;
 
 struct RowRange {
     int32_t low, high, place;
@@ -101,7 +109,7 @@ __device__ __forceinline__ void put_stats(const AttendArgs &g, int32_t token, ui
 // follows, less than a window above it.  Every block walks up from its own rows, in LDS: one load of the parents, and a step of LDS for each
 // level.  A mask of 256 bits a row says which rows it sees.
 constexpr uint32_t TREE_ROWS = 256;
-template <bool TREE, int ROWS> struct TreeLds {
+template <bool, int ROWS> struct TreeLds {
     int16_t parent[TREE_ROWS], depth[TREE_ROWS];
     uint32_t mask[ROWS][TREE_ROWS / 32];
 };
@@ -402,8 +410,8 @@ struct Piece {
 };
 
 // UNIFORM: 16 keys that start at a multiple of 16 are in one page.  SPLIT: sequences of few rows, whose keys several blocks share.
-template <int DP, bool BF16, bool UNIFORM, bool SPLIT, bool TREE, int TREE_LDS>
-__device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece, RowLds<DP, BF16> &lds, TreeLds<TREE, TREE_LDS> &tree) {
+template <int DP, bool BF16, bool UNIFORM, bool SPLIT, int MODE, int TREE_LDS>
+__device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece, RowLds<DP, BF16> &lds, TreeLds<MODE == TREE, TREE_LDS> &tree) {
     constexpr int KT = ROW_KEYS, NACC = DP / 16, PITCH = RowLds<DP, BF16>::PITCH;
     auto &sums = lds.sums;
     auto &stats = lds.stats;
@@ -419,7 +427,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     const uint32_t token = g.by_group.div(valid ? row : 0), head = kvh * g.group + (valid ? row : 0) - token * g.group;
     RowRange range;
     const int32_t base_key = seq.length - seq.n;  // TREE: the first of the rows' own
-    if constexpr (TREE) {
+    if constexpr (MODE == TREE) {
         read_tree(g, seq, tile * 16, tree);
         range = tree_range(g, seq, token, tree.depth[token]);
     } else {
@@ -430,11 +438,11 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     const float slope = g.slopes ? g.slopes[head] * LOG2E : 0.0f;
     // Whether the row sees key `key` of [low, high), and the scores of keys key0 + place_in(r).
     auto in_tree = [&](int32_t key) {
-        if constexpr (TREE) return (tree_bits(tree, col, key, base_key) & 1u) != 0;
+        if constexpr (MODE == TREE) return (tree_bits(tree, col, key, base_key) & 1u) != 0;
         else return true;
     };
     auto score_keys = [&](auto &x, int32_t key0, auto place_in) {
-        if constexpr (TREE) {
+        if constexpr (MODE == TREE) {
             cap_scores(g, x);
             if (g.slopes) {
 #pragma unroll
@@ -446,7 +454,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     };
 
     // What any row sees, and what all see.
-    int32_t any_low = sees ? low : INT32_MAX, any_high = sees ? high : 0, all_low = valid ? low : 0, all_high = valid ? (TREE ? min(high, base_key) : high) : INT32_MAX;
+    int32_t any_low = sees ? low : INT32_MAX, any_high = sees ? high : 0, all_low = valid ? low : 0, all_high = valid ? (MODE == TREE ? min(high, base_key) : high) : INT32_MAX;
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {
         any_low = min(any_low, __shfl_xor(any_low, m)), any_high = max(any_high, __shfl_xor(any_high, m));
@@ -459,7 +467,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     const char *keys = static_cast<const char *>(g.kv.keys), *values = static_cast<const char *>(g.kv.values);
     constexpr int SIZE = BF16 ? 2 : 4;
     const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
-    const int32_t *const table = g.kv.table + (int64_t)s * g.kv.table_stride + (int64_t)kvh * g.kv.table_head;
+    const int32_t *const table = g.kv.table + (int64_t)s * g.kv.table_stride + (MODE == KEPT ? (int64_t)kvh * g.kv.table_head : 0);
 
     // fp32: channels 16 i + 4 part on; bf16: parts of channels 32 i + 8 part on.
     constexpr bool Q_HERE = DP > 128 && !BF16;
@@ -509,7 +517,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     auto tile_key = [&](int32_t i) { return (first + (int32_t)wave + i * ROW_WAVES) * KT; };
     auto row_at = [&](uint32_t key) {  // elements from the start of the cache
         const uint32_t index = g.kv.by_page_size.div(key);
-        return (int64_t)g.kv.page_of(s, index, 0, kvh) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
+        return (int64_t)g.kv.page_of(s, index, 0, MODE == KEPT ? kvh : 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
     };
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
     // Where pages hold whole tiles: where the wavefront's next 64 tiles start, in bytes from the start of the cache, a tile a lane.  A
@@ -519,7 +527,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     auto fetch_starts = [&](int32_t from) {
         const int32_t i = from + (int32_t)lane;
         const uint32_t key = (uint32_t)tile_key(i < mine ? i : mine - 1), index = g.kv.by_page_size.div(key);
-        starts = ((int64_t)g.kv.page_of(s, index, 0, kvh) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
+        starts = ((int64_t)g.kv.page_of(s, index, 0, MODE == KEPT ? kvh : 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
     };
     // Where they do not: lane l has the row of key l % 16 of a tile, looked up a tile ahead of its use.  Keys in front of the first that
     // is seen and behind the last may have no page: those two stand in for them.
@@ -602,18 +610,20 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
 #pragma unroll
     for (int i = 0; i < NACC; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
+    float *const scores_here = g.scores + ((int64_t)(s * g.kv.kv_heads + kvh) * g.score_rows + row) * g.score_keys;
     // Scores of the tile (NS registers a lane, key0 + value_key(r)), running maximum and sum, weights in their place.
     constexpr int NS = 4;
     auto weigh = [&](int32_t key0, float (&x)[NS]) {
         const bool full = key0 >= all_low && key0 + KT <= all_high && key0 >= begin && key0 + KT <= end;
         score_keys(x, key0, value_key);
+        if (SPLIT && MODE == KEPT && g.scores && valid) __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(scores_here + key0 + 4 * part));
         uint32_t bits = 0xffffffffu;
-        if constexpr (TREE) bits = full ? bits : tree_bits(tree, col, key0, base_key);
+        if constexpr (MODE == TREE) bits = full ? bits : tree_bits(tree, col, key0, base_key);
         float most = -INFINITY;
 #pragma unroll
         for (int r = 0; r < NS; r++) {
             const int32_t key = key0 + value_key(r);
-            if (full || (key >= low && key < high && key >= begin && key < end && (!TREE || (bits >> value_key(r) & 1u)))) most = fmaxf(most, x[r]);
+            if (full || (key >= low && key < high && key >= begin && key < end && (MODE != TREE || (bits >> value_key(r) & 1u)))) most = fmaxf(most, x[r]);
         }
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
@@ -629,7 +639,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
 #pragma unroll
         for (int r = 0; r < NS; r++) {
             const int32_t key = key0 + value_key(r);
-            const bool seen = full || (key >= low && key < high && key >= begin && key < end && (!TREE || (bits >> value_key(r) & 1u)));
+            const bool seen = full || (key >= low && key < high && key >= begin && key < end && (MODE != TREE || (bits >> value_key(r) & 1u)));
             x[r] = seen ? exp2_fast(x[r] - base) : 0.0f;
             total += x[r];
         }
@@ -740,6 +750,7 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
                 if (!sees || key < low || key >= high || !in_tree(key)) continue;
                 float x[1] = {dot};
                 score_keys(x, key, [](int) { return 0; });
+                if (SPLIT && MODE == KEPT && g.scores && part == 0) scores_here[key] = x[0];
                 const float now_top = fmaxf(top, x[0]);
                 const float corr = weight_of(top, now_top), p = exp2_fast(x[0] - (now_top == -INFINITY ? 0.0f : now_top));
                 top = now_top;
@@ -785,24 +796,24 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
             if (c == 0) g.few.part_stats[2 * at] = m, g.few.part_stats[2 * at + 1] = l;
         } else {
             const uint32_t t = g.by_group.div(mine_row), h = kvh * g.group + mine_row - t * g.group;
-            const RowRange of = TREE ? tree_range(g, seq, t, 0) : row_range(g, seq, s, t);
+            const RowRange of = MODE == TREE ? tree_range(g, seq, t, 0) : row_range(g, seq, s, t);
             const float recip = of.low < of.high ? 1.0f / l : 0.0f;
-            if (c == 0 && g.stats) put_stats(g, seq.start + (int32_t)t, h, m, l);
+            if (c == 0 && MODE == KEPT && g.stats) put_stats(g, seq.start + (int32_t)t, h, m, l);
             *reinterpret_cast<f32x4 *>(g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + c) =
                 of.low < of.high ? o * recip : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
 }
 
-template <int DP, bool BF16, bool UNIFORM, bool SPLIT, bool TREE, int TREE_LDS>
-__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP, BF16> &lds, TreeLds<TREE, TREE_LDS> &tree) {
+template <int DP, bool BF16, bool UNIFORM, bool SPLIT, int MODE, int TREE_LDS>
+__device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<DP, BF16> &lds, TreeLds<MODE == TREE, TREE_LDS> &tree) {
     const Share &share = SPLIT ? g.few : g.many;
     Piece piece = {0, 0, 0, 0, INT32_MAX, true, 0};
     if (!SPLIT || !share.listed) {
         const uint32_t outer = id / g.kv.kv_heads;
         piece.kvh = id - outer * g.kv.kv_heads;
         piece.tile = outer % share.row_tiles, piece.s = outer / share.row_tiles;
-        piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds, tree);
+        piece16<DP, BF16, UNIFORM, SPLIT, MODE>(g, piece, lds, tree);
         return;
     }
     Found f;
@@ -812,15 +823,15 @@ __device__ __forceinline__ void rows16(const AttendArgs &g, uint32_t id, RowLds<
     piece.from = f.first_key(part), piece.to = part + 1 == f.parts ? INT32_MAX : f.first_key(part + 1);
     piece.whole = f.parts == 1;
     piece.slot = id;
-    piece16<DP, BF16, UNIFORM, SPLIT>(g, piece, lds, tree);
+    piece16<DP, BF16, UNIFORM, SPLIT, MODE>(g, piece, lds, tree);
 }
 
 // Heads of more than 128 channels have no tiles of 128 rows: all their rows go 16 a wavefront (SPLIT false).
-template <int DP, bool BF16, bool UNIFORM, bool SPLIT, bool TREE>
+template <int DP, bool BF16, bool UNIFORM, bool SPLIT, int MODE>
 __global__ __launch_bounds__(64 * ROW_WAVES, DP == 256 ? 1 : BF16 && DP == 128 ? 3 : 2) void attend_rows16(AttendArgs g) {
     __shared__ __align__(16) RowLds<DP, BF16> lds;
-    __shared__ TreeLds<TREE, 16> tree;
-    rows16<DP, BF16, UNIFORM, SPLIT>(g, blockIdx.x, lds, tree);
+    __shared__ TreeLds<MODE == TREE, 16> tree;
+    rows16<DP, BF16, UNIFORM, SPLIT, MODE>(g, blockIdx.x, lds, tree);
 }
 
 // ---------------------------------------------------------------- 128 rows a block, keys through LDS
@@ -850,8 +861,8 @@ template <int DP, bool BF16> struct TileLds {
     int32_t bounds[4][2];
 };
 
-template <int DP, bool BF16, bool UNIFORM, bool TREE>
-__device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLds<DP, BF16> &lds, TreeLds<TREE, TILE_ROWS> &tree) {
+template <int DP, bool BF16, bool UNIFORM, int MODE>
+__device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLds<DP, BF16> &lds, TreeLds<MODE == TREE, TILE_ROWS> &tree) {
     using Lds = TileLds<DP, BF16>;
     constexpr int PLANES = Lds::PLANES, K_PITCH = Lds::K_PITCH, V_PITCH = Lds::V_PITCH;
     constexpr int STEPS = DP / 16, PARTS = DP / 32;
@@ -888,7 +899,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     const uint32_t token = g.by_group.div(valid ? row : 0), head = kvh * g.group + (valid ? row : 0) - token * g.group;
     RowRange range;
     const int32_t base_key = seq.length - seq.n;  // TREE: the first of the rows' own
-    if constexpr (TREE) {
+    if constexpr (MODE == TREE) {
         read_tree(g, seq, tile * TILE_ROWS, tree);
         range = tree_range(g, seq, token, tree.depth[token]);
     } else {
@@ -899,11 +910,11 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     const float slope = g.slopes ? g.slopes[head] * LOG2E : 0.0f;
     // Whether the row sees key `key` of [low, high), and the scores of keys key0 + place_in(r).
     auto in_tree = [&](int32_t key) {
-        if constexpr (TREE) return (tree_bits(tree, wave * 32 + col, key, base_key) & 1u) != 0;
+        if constexpr (MODE == TREE) return (tree_bits(tree, wave * 32 + col, key, base_key) & 1u) != 0;
         else return true;
     };
     auto score_keys = [&](auto &x, int32_t key0, auto place_in) {
-        if constexpr (TREE) {
+        if constexpr (MODE == TREE) {
             cap_scores(g, x);
             if (g.slopes) {
 #pragma unroll
@@ -914,7 +925,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         }
     };
 
-    int32_t any_low = sees ? low : INT32_MAX, any_high = sees ? high : 0, all_low = valid ? low : 0, all_high = valid ? (TREE ? min(high, base_key) : high) : INT32_MAX;
+    int32_t any_low = sees ? low : INT32_MAX, any_high = sees ? high : 0, all_low = valid ? low : 0, all_high = valid ? (MODE == TREE ? min(high, base_key) : high) : INT32_MAX;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
         any_low = min(any_low, __shfl_xor(any_low, m)), any_high = max(any_high, __shfl_xor(any_high, m));
@@ -936,7 +947,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     const char *keys = static_cast<const char *>(g.kv.keys), *values = static_cast<const char *>(g.kv.values);
     constexpr int SIZE = BF16 ? 2 : 4;
     const int64_t head_at = (int64_t)kvh * g.kv.head_stride;
-    const int32_t *const table = g.kv.table + (int64_t)s * g.kv.table_stride + (int64_t)kvh * g.kv.table_head;
+    const int32_t *const table = g.kv.table + (int64_t)s * g.kv.table_stride + (MODE == KEPT ? (int64_t)kvh * g.kv.table_head : 0);
 
     // Staging.  Keys: 16-byte units, a row after the other.  Values: blocks of 4 keys (which lie side by side in V^T) and VC
     // channels.  All threads do the same, without a branch: where the units or blocks are fewer, some are fetched and written twice.
@@ -962,12 +973,12 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         if (!UNIFORM) return;
         // A half that nobody sees any of may have no page: it is read from the start of the cache, and left out.
         const uint32_t index = g.kv.by_page_size.div((uint32_t)max(begin, min(key, end - 1)));
-        starts = ((int64_t)g.kv.page_of(s, index, 0, kvh) * g.kv.page_stride + (int64_t)((uint32_t)key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
+        starts = ((int64_t)g.kv.page_of(s, index, 0, MODE == KEPT ? kvh : 0) * g.kv.page_stride + (int64_t)((uint32_t)key - index * g.kv.page_size) * g.kv.slot_stride + head_at) * SIZE;
         if (key >= end || key + 16 <= begin) starts = 0;
     };
     auto row_at = [&](uint32_t key) {  // elements from the start of the cache
         const uint32_t index = g.kv.by_page_size.div(key);
-        return (int64_t)g.kv.page_of(s, index, 0, kvh) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
+        return (int64_t)g.kv.page_of(s, index, 0, MODE == KEPT ? kvh : 0) * g.kv.page_stride + (int64_t)(key - index * g.kv.page_size) * g.kv.slot_stride + head_at;
     };
     const uint32_t slot_bytes = (uint32_t)g.kv.slot_stride * SIZE;
     // No load below depends on a condition, which would have the compiler wait for those before it.  Channels that a head does not
@@ -1239,7 +1250,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
                 const int32_t from = max(low, begin) - key0, to = min(high, end) - key0;
 #pragma unroll
                 for (int r = 0; r < 16; r++) x[r] = key_of(r) >= from && key_of(r) < to ? x[r] : -INFINITY;
-                if constexpr (TREE) {
+                if constexpr (MODE == TREE) {
                     const uint32_t bits = tree_bits(tree, wave * 32 + col, key0, base_key);
 #pragma unroll
                     for (int r = 0; r < 16; r++) x[r] = bits >> key_of(r) & 1u ? x[r] : -INFINITY;
@@ -1345,7 +1356,7 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
     float *const row_out = whole ? g.out + (int64_t)(seq.start + (int32_t)token) * g.out_token + (int64_t)head * g.out_head : share.part_out + at * g.d;
     const float factor = !whole ? 1.0f : 1.0f / total;
     if (!whole && h == 0) share.part_stats[2 * at] = top, share.part_stats[2 * at + 1] = total;
-    if (whole && h == 0 && g.stats) put_stats(g, seq.start + (int32_t)token, head, top, total);
+    if (whole && h == 0 && MODE == KEPT && g.stats) put_stats(g, seq.start + (int32_t)token, head, top, total);
 #pragma unroll
     for (int t = 0; t < PARTS; t++)
 #pragma unroll
@@ -1359,15 +1370,15 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
 
 // Prompts, and the sequences of few rows that share a batch with them: the last blocks are the latter's, and end at once where there
 // are none.
-template <int DP, bool BF16, bool UNIFORM, bool TREE>
+template <int DP, bool BF16, bool UNIFORM, int MODE>
 __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(AttendArgs g) {
     __shared__ __align__(16) union {
         RowLds<DP <= 64 ? 64 : 128, BF16> few;
         TileLds<DP, BF16> many;
     } lds;
-    __shared__ TreeLds<TREE, TILE_ROWS> tree;
-    if (blockIdx.x < g.many.blocks) rows128<DP, BF16, UNIFORM>(g, blockIdx.x, lds.many, tree);
-    else rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true>(g, blockIdx.x - g.many.blocks, lds.few, tree);
+    __shared__ TreeLds<MODE == TREE, TILE_ROWS> tree;
+    if (blockIdx.x < g.many.blocks) rows128<DP, BF16, UNIFORM, MODE>(g, blockIdx.x, lds.many, tree);
+    else rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true, MODE>(g, blockIdx.x - g.many.blocks, lds.few, tree);
 }
 
 // Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
@@ -1375,7 +1386,7 @@ __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(
 // latency: the scan for a row's parts, their statistics, their sums.  10 us behind one row's 512 parts, 10 us behind 5 pieces of 57 to 333 rows,
 // 4 to 5 us where the sizes allow parts and there are none.
 constexpr int JOIN = 256, MOST_SPLITS = 1024;
-template <bool TREE> __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_blocks) {
+template <int MODE> __global__ __launch_bounds__(JOIN) void join_splits(AttendArgs g, uint32_t few_blocks) {
     __shared__ float factors[MOST_SPLITS];
     __shared__ __align__(16) f32x4 sums[JOIN];
     __shared__ float totals[JOIN / 64];
@@ -1392,7 +1403,7 @@ template <bool TREE> __global__ __launch_bounds__(JOIN) void join_splits(AttendA
     if (!(few ? find<true>(g, true, s, f) : find<false>(g, true, s, f)) || f.parts <= 1) return;  // one block did it all
     if (!few && (group >= groups || row >= rows)) return;
     const uint32_t t = g.by_group.div(row), h = kvh * g.group + row - t * g.group;
-    const RowRange of = TREE ? tree_range(g, seq, t, 0) : row_range(g, seq, s, t);
+    const RowRange of = MODE == TREE ? tree_range(g, seq, t, 0) : row_range(g, seq, s, t);
     float *to = g.out + (int64_t)(seq.start + (int32_t)t) * g.out_token + (int64_t)h * g.out_head + 4 * lane;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     if (of.low >= of.high) {
@@ -1420,7 +1431,7 @@ template <bool TREE> __global__ __launch_bounds__(JOIN) void join_splits(AttendA
             o += parts[i * parts_apart] * f;
         }
         *reinterpret_cast<f32x4 *>(to) = o * (1.0f / total);
-        if (lane == 0 && g.stats) put_stats(g, seq.start + (int32_t)t, h, top, total);
+        if (lane == 0 && MODE == KEPT && g.stats) put_stats(g, seq.start + (int32_t)t, h, top, total);
         return;
     }
     // Every wavefront finds the maximum by itself; the weights of the splits wait in LDS.
@@ -1445,7 +1456,7 @@ template <bool TREE> __global__ __launch_bounds__(JOIN) void join_splits(AttendA
     for (int w = 0; w < JOIN / 64; w++) total += totals[w];
     for (uint32_t i = 1; i < groups; i++) o += sums[i * lanes + lane];
     *reinterpret_cast<f32x4 *>(to) = o * (1.0f / total);
-    if (lane == 0 && g.stats) put_stats(g, seq.start + (int32_t)t, h, top, total);
+    if (lane == 0 && MODE == KEPT && g.stats) put_stats(g, seq.start + (int32_t)t, h, top, total);
 }
 
 constexpr uint64_t MOST_ROWS = (uint64_t)1 << 30, MOST_BLOCKS = (uint64_t)1 << 24;  // a grid ends at 2^32 threads
@@ -1453,44 +1464,44 @@ constexpr uint64_t MOST_ROWS = (uint64_t)1 << 30, MOST_BLOCKS = (uint64_t)1 << 2
 // The largest head that blocks of 128 rows are built for.
 constexpr int TILE_CHANNELS = 128;
 
-template <int DP, bool BF16, bool UNIFORM, bool TREE> int launch_wide(DeviceCtx &ctx, const AttendArgs &g) {
-    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, true, TREE>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+template <int DP, bool BF16, bool UNIFORM, int MODE> int launch_wide(DeviceCtx &ctx, const AttendArgs &g) {
+    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, true, MODE>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
     if (int rc = ctx.check(hipGetLastError(), "kv attention launch")) return rc;
     if (!g.many.blocks) return AHIP_OK;
-    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, false, TREE>), dim3(g.many.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+    hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, false, MODE>), dim3(g.many.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
     return ctx.check(hipGetLastError(), "kv attention launch");
 }
-template <int DP, bool BF16, bool UNIFORM, bool TREE> int launch_tiled(DeviceCtx &ctx, const AttendArgs &g) {
+template <int DP, bool BF16, bool UNIFORM, int MODE> int launch_tiled(DeviceCtx &ctx, const AttendArgs &g) {
     if (!g.many.blocks)
-        hipLaunchKernelGGL((attend_rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true, TREE>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+        hipLaunchKernelGGL((attend_rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true, MODE>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
     else
-        hipLaunchKernelGGL((attend_rows128<DP, BF16, UNIFORM, TREE>), dim3(g.few.blocks + g.many.blocks), dim3(256), 0, ctx.stream, g);
+        hipLaunchKernelGGL((attend_rows128<DP, BF16, UNIFORM, MODE>), dim3(g.few.blocks + g.many.blocks), dim3(256), 0, ctx.stream, g);
     return ctx.check(hipGetLastError(), "kv attention launch");
 }
 
 // By the head's channels, rounded up.  Heads of 96 channels have a size of their own: 4 prompts of 512 (16 heads, 4 of keys, fp32)
 // 46 us, at 128 channels 53 us; of 1024, bf16, 8 heads of keys: 63 and 72 us.
-template <bool BF16, bool UNIFORM, bool TREE> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g) {
-    if (g.d <= 64) return launch_tiled<64, BF16, UNIFORM, TREE>(ctx, g);
-    if (g.d <= 96) return launch_tiled<96, BF16, UNIFORM, TREE>(ctx, g);
-    if (g.d <= TILE_CHANNELS) return launch_tiled<128, BF16, UNIFORM, TREE>(ctx, g);
-    return launch_wide<256, BF16, UNIFORM, TREE>(ctx, g);
+template <bool BF16, bool UNIFORM, int MODE> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g) {
+    if (g.d <= 64) return launch_tiled<64, BF16, UNIFORM, MODE>(ctx, g);
+    if (g.d <= 96) return launch_tiled<96, BF16, UNIFORM, MODE>(ctx, g);
+    if (g.d <= TILE_CHANNELS) return launch_tiled<128, BF16, UNIFORM, MODE>(ctx, g);
+    return launch_wide<256, BF16, UNIFORM, MODE>(ctx, g);
 }
 
 
 // Both launches of a call whose arguments and cut are known.  Pages of whole groups of 16 keys: a group's page is looked up once, not key by
 // key, and its slots lie within 2^31 bytes.  Pages of 64, 4 prompts of 1024 (12 heads of 64 channels, fp32): 61.7 us, key by key 67.5; a
 // prompt of 4096 with a window, bf16: 156 and 166 us; one token of 65536 keys, pages of 16: 111 and 113 us.
-template <bool TREE> int launch_attend(DeviceCtx &ctx, const AttendArgs &g, bool bf16) {
+template <int MODE> int launch_attend(DeviceCtx &ctx, const AttendArgs &g, bool bf16) {
     const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads, groups = JOIN / (g.d / 4);
     const uint64_t few_joins = g.few.cut ? pairs * g.few.rows : 0, many_joins = g.many.cut ? pairs * ((g.many.rows + groups - 1) / groups) : 0;
     if ((uint64_t)g.few.blocks + g.many.blocks >= MOST_BLOCKS || few_joins + many_joins >= MOST_BLOCKS)
         return ctx.fail(AHIP_ERR_UNSUPPORTED, "kv attention: more blocks than a grid holds");
     const bool uniform = g.kv.page_size % 16 == 0 && g.kv.slot_stride < (int64_t)1 << 23;
-    int rc = bf16 ? (uniform ? launch_by_size<true, true, TREE>(ctx, g) : launch_by_size<true, false, TREE>(ctx, g))
-                  : (uniform ? launch_by_size<false, true, TREE>(ctx, g) : launch_by_size<false, false, TREE>(ctx, g));
+    int rc = bf16 ? (uniform ? launch_by_size<true, true, MODE>(ctx, g) : launch_by_size<true, false, MODE>(ctx, g))
+                  : (uniform ? launch_by_size<false, true, MODE>(ctx, g) : launch_by_size<false, false, MODE>(ctx, g));
     if (rc || few_joins + many_joins == 0) return rc;
-    hipLaunchKernelGGL(join_splits<TREE>, dim3((uint32_t)(few_joins + many_joins)), dim3(JOIN), 0, ctx.stream, g, (uint32_t)few_joins);
+    hipLaunchKernelGGL(join_splits<MODE>, dim3((uint32_t)(few_joins + many_joins)), dim3(JOIN), 0, ctx.stream, g, (uint32_t)few_joins);
     return ctx.check(hipGetLastError(), "kv attention launch");
 }
 
@@ -1504,7 +1515,7 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
 int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, dev::KvView *view);
 // Checks the call and describes it for the kernels; q stays null where there is nothing to do.
 int begin_attend(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, AttendArgs *args);
-int launch_attend_rows(DeviceCtx &ctx, const AttendArgs &g, bool bf16);
+int launch_attend_kept(DeviceCtx &ctx, const AttendArgs &g, bool bf16);  // kv_kept.hip
 
 }  // namespace attend
 }  // namespace altius

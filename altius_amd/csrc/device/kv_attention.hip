@@ -133,8 +133,6 @@ int begin_attend(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch
     return AHIP_OK;
 }
 
-int launch_attend_rows(DeviceCtx &ctx, const AttendArgs &g, bool bf16) { return launch_attend<false>(ctx, g, bf16); }
-
 }  // namespace attend
 
 int kv_attention_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, size_t *bytes) {
@@ -150,7 +148,7 @@ int kv_attention_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahi
 int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
     attend::AttendArgs g = {};
     if (int rc = attend::begin_attend(ctx, cache, batch, attend, &g)) return rc;
-    return g.q ? attend::launch_attend_rows(ctx, g, cache.elem == AHIP_KV_BF16) : AHIP_OK;
+    return g.q ? attend::launch_attend<attend::PLAIN>(ctx, g, cache.elem == AHIP_KV_BF16) : AHIP_OK;
 }
 
 }  // namespace altius

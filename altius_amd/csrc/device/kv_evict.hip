@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "kv.h"
+#include "kv_rank.h"
 
 namespace altius {
 
@@ -19,12 +20,12 @@ struct History {
 };
 
 // ---------------------------------------------------------------- who stays
-// A block for each sequence and head of keys.  The budget's smallest value is found digit by digit of an order-preserving image of the
-// masses (11, 11 and 10 bits): a histogram of the values that share the digits so far, in LDS, and the bin that the rank falls into.  What is kept
-// by its position is counted apart, so that it does not all meet in one bin.  The image waits in LDS as far as that goes (32768 places), what
-// is behind is read anew, out of L2.  Then wavefronts take runs of places in order: one walk counts, one writes the lists.
-// Bound by latency: the walks of one block, one after the other.  48 sequences of 1025 places, 8 heads: 13.4 us; 4 of 20011 to 50000: 131 us.
-constexpr uint32_t EVICT = 1024, WAVES = EVICT / 64, BINS = 2048, HELD = 32768;
+// A block for each sequence and head of keys, a wavefront for each run of places.  Masses become an order-preserving image of 32 bits; the smallest that
+// stays is found among them (kv_rank.h), then the runs are counted and listed in order.  What stays for its position is counted apart.
+//   Up to 2048 places 256 threads hold 8 images each.  48 sequences of 1025 places, 8 heads: 8.2 us.
+//   Up to 57344 places 1024 threads hold 56.  4 sequences of 20011 to 50000 places: 72.7 us, bound by the vector unit of one CU a block and the latency of its
+// walks over the places.  Beyond, images wait in LDS as far as that goes, and what is behind is read anew, out of L2: 103 us with the same lengths.
+constexpr uint32_t HELD = 28672, PAGES = 4096, SMALL = 256, SMALL_EACH = 8, LARGE = 1024, LARGE_EACH = 56;
 constexpr uint32_t KEPT = 0xffffffffu;  // by its position; above every mass
 
 struct EvictArgs {
@@ -41,11 +42,15 @@ __device__ __forceinline__ uint32_t rank_image(float mass) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(EVICT) void choose_evicted(EvictArgs g) {
+// EACH: images that a thread holds; 0: they are in LDS and memory.
+template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS) void choose_evicted(EvictArgs g) {
+    constexpr uint32_t WAVES = THREADS / 64, AHEAD = 8;  // loads of a thread that are on their way at once
+    constexpr bool STARTS = EACH != AHEAD;               // where pages start is looked up once
+    static_assert(EACH % AHEAD == 0, "whole sweeps");
     extern __shared__ uint32_t held[];
-    __shared__ uint32_t bins[BINS];
-    __shared__ uint32_t per_wave[WAVES][4];
-    __shared__ uint32_t found[2];
+    __shared__ int64_t page_starts[STARTS ? PAGES : 1];
+    __shared__ uint32_t per_wave[2][WAVES][4];
+    __shared__ dev::RankLds rank_lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t s = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - s * g.kv.kv_heads;
     const int32_t length = g.kv.lengths[s];
@@ -55,133 +60,184 @@ __global__ __launch_bounds__(EVICT) void choose_evicted(EvictArgs g) {
         if (tid == 0) {
             *count = 0;
             if (!fits) *g.kv.flag = 1;
-            else if (head == 0) g.lengths[s] = length;
+            else if (head == 0 && g.lengths) g.lengths[s] = length;
         }
         return;
     }
     const uint32_t n = (uint32_t)length;
-    if (tid == 0 && head == 0) g.lengths[s] = (int32_t)g.budget;
-    auto slot_of = [&](uint32_t place) {
-        const uint32_t index = g.kv.by_page_size.div(place);
-        return (int64_t)g.kv.page_of(s, index, 0) * g.history.page_stride + (int64_t)head * g.history.head_stride + (place - index * g.kv.page_size);
+    if (tid == 0 && head == 0 && g.lengths) g.lengths[s] = (int32_t)g.budget;
+    // This wavefront's places: at most 64 EACH.
+    const uint32_t run = (n + THREADS - 1) / THREADS * 64, from = min(wave * run, n), to = min(from + run, n);
+
+    const int32_t *const table = g.kv.table + (int64_t)s * g.kv.table_stride;
+    bool outside = false;  // the flag is raised in the end: no branch in front of a load
+    auto start_of = [&](uint32_t index) {
+        const uint32_t page = (uint32_t)table[index];
+        outside = outside || page >= g.kv.pages;
+        return (int64_t)(page < g.kv.pages ? page : 0) * g.history.page_stride + (int64_t)head * g.history.head_stride;
+    };
+    if constexpr (STARTS) {
+        for (uint32_t index = tid; index < PAGES && (uint64_t)index * g.kv.page_size < n; index += THREADS) page_starts[index] = start_of(index);
+        __syncthreads();
+    }
+    // The next AHEAD x 64 places (behind the end the last one again), all loads on their way before the first is used: left to itself the compiler
+    // waits for one at a time.
+    auto ahead = [&](uint32_t base, auto load) {
+        int64_t at[AHEAD];
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; u++) {
+            const uint32_t place = min(base + 64 * u + lane, n - 1), index = g.kv.by_page_size.div(place);
+            at[u] = (!STARTS || index >= PAGES ? start_of(index) : page_starts[index]) + (place - index * g.kv.page_size);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; u++) load(u, at[u]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Over the block: what the wavefronts have, joined; one barrier.
+    int turn = 0;
+    auto all_waves = [&](uint32_t mine, auto join) {
+        turn ^= 1;
+        if (lane == 0) per_wave[turn][wave][0] = mine;
+        __syncthreads();
+        uint32_t v = per_wave[turn][0][0];
+#pragma unroll
+        for (uint32_t w = 1; w < WAVES; w++) v = join(v, per_wave[turn][w][0]);
+        return v;
     };
 
-    // The newest position.
-    int32_t newest = INT32_MIN;
-    for (uint32_t place = tid; place < n; place += EVICT) newest = max(newest, g.history.positions[slot_of(place)]);
+    // The newest position, and what stays for its own.
+    int32_t newest = INT32_MIN, its[AHEAD];
+    float masses[AHEAD];
+    if constexpr (EACH == AHEAD) {
+        ahead(from, [&](uint32_t u, int64_t at) { its[u] = g.history.positions[at], masses[u] = g.history.mass[at]; });
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, its[u]);
+    } else {
+        for (uint32_t base = from; base < to; base += 64 * AHEAD) {
+            ahead(base, [&](uint32_t u, int64_t at) { its[u] = g.history.positions[at]; });
+#pragma unroll
+            for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, its[u]);
+        }
+    }
 #pragma unroll
     for (int m = 32; m; m >>= 1) newest = max(newest, __shfl_xor(newest, m));
-    if (lane == 0) per_wave[wave][0] = (uint32_t)newest;
-    for (uint32_t b = tid; b < BINS; b += EVICT) bins[b] = 0;
-    __syncthreads();
+    newest = (int32_t)all_waves((uint32_t)newest, [](uint32_t a, uint32_t b) { return (uint32_t)max((int32_t)a, (int32_t)b); });
+    const int64_t above_recent = (int64_t)newest - g.recent;
+    // Images of the places from `base` on, 0 behind the end.
+    auto take_images = [&](uint32_t base, uint32_t *v) {
+        if constexpr (EACH != AHEAD) ahead(base, [&](uint32_t u, int64_t at) { its[u] = g.history.positions[at], masses[u] = g.history.mass[at]; });
 #pragma unroll
-    for (uint32_t w = 0; w < WAVES; w++) newest = max(newest, (int32_t)per_wave[w][0]);
-    const int64_t above = (int64_t)newest - g.recent;
-
-    auto image_of = [&](uint32_t place) {
-        const int64_t at = slot_of(place);
-        const int32_t position = g.history.positions[at];
-        return position < g.first || position > above ? KEPT : rank_image(g.history.mass[at]);
+        for (uint32_t u = 0; u < AHEAD; u++)
+            v[u] = base + 64 * u + lane >= to ? 0 : its[u] < g.first || its[u] > above_recent ? KEPT : rank_image(masses[u]);
     };
-    auto image = [&](uint32_t place) { return place < g.held ? held[place] : image_of(place); };
-
-    // The first digit's histogram, the images into LDS, and how many are kept by their position.
-    uint32_t kept = 0;
-    for (uint32_t place = tid; place < n; place += EVICT) {
-        const uint32_t v = image_of(place);
-        if (place < g.held) held[place] = v;
-        if (v == KEPT) kept++;
-        else atomicAdd(&bins[v >> 21], 1u);
+    uint32_t kept = 0;  // how many stay for their position
+    uint32_t images[EACH ? EACH : 1];
+    if constexpr (EACH != 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; i += AHEAD) {
+            if (EACH > AHEAD && from + 64 * i >= to) break;
+            take_images(from + 64 * i, images + i);
+#pragma unroll
+            for (uint32_t u = 0; u < AHEAD; u++) kept += (uint32_t)__popcll(__ballot(images[i + u] == KEPT));
+        }
+    } else {
+        for (uint32_t base = from; base < to; base += 64 * AHEAD) {
+            uint32_t v[AHEAD];
+            take_images(base, v);
+#pragma unroll
+            for (uint32_t u = 0; u < AHEAD; u++) {
+                if (base + 64 * u < to && base + 64 * u < g.held) held[base + 64 * u + lane] = v[u];
+                kept += (uint32_t)__popcll(__ballot(v[u] == KEPT));
+            }
+        }
     }
+    // what(base, v) for every 64 places of the run in order: this lane's image, 0 behind the end.
+    auto each = [&](auto what) {
+        if constexpr (EACH != 0) {
 #pragma unroll
-    for (int m = 32; m; m >>= 1) kept += __shfl_xor(kept, m);
-    __syncthreads();  // behind the readers of per_wave
-    if (lane == 0) per_wave[wave][0] = kept;
-    __syncthreads();
-    kept = 0;
+            for (uint32_t i = 0; i < EACH; i++) {
+                if (from + 64 * i >= to) break;
+                what(from + 64 * i, images[i]);
+            }
+        } else {
+            for (uint32_t base = from; base < to; base += 64 * AHEAD) {
+                uint32_t v[AHEAD];
+                if (base + 64 * AHEAD <= g.held) {
 #pragma unroll
-    for (uint32_t w = 0; w < WAVES; w++) kept += per_wave[w][0];
+                    for (uint32_t u = 0; u < AHEAD; u++) v[u] = held[base + 64 * u + lane];
+                } else {
+                    take_images(base, v);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < AHEAD; u++)
+                    if (base + 64 * u < to) what(base + 64 * u, v[u]);
+            }
+        }
+    };
+    kept = all_waves(kept, [](uint32_t a, uint32_t b) { return a + b; });
 
-    // least: the smallest image that stays; ties: how many of that image do.
+    // least: the smallest image that stays; ties: of how many of that image, all where that is exact.
     uint32_t least = KEPT, ties = g.budget;
     if (kept < g.budget) {
-        uint32_t need = g.budget - kept;  // of those that share the digits so far
-        least = 0;
-        for (int digit = 0; digit < 3; digit++) {
-            const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
-            const uint32_t width = digit == 2 ? 1024 : 2048;
-            if (digit) {
-                __syncthreads();
-                for (uint32_t b = tid; b < BINS; b += EVICT) bins[b] = 0;
-                __syncthreads();
-                const int known = digit == 1 ? 21 : 10;
-                for (uint32_t place = tid; place < n; place += EVICT) {
-                    const uint32_t v = image(place);
-                    if (v != KEPT && v >> known == least >> known) atomicAdd(&bins[v >> shift & (width - 1)], 1u);
-                }
-                __syncthreads();
-            }
-            // Thread t has bins 2 t and 2 t + 1: how many values are above them.
-            const uint32_t low = bins[2 * tid], high = bins[2 * tid + 1];
-            uint32_t up_to = low + high;  // from this lane's bins on, within the wavefront
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const uint32_t t = __shfl_down(up_to, m);
-                if (lane + m < 64) up_to += t;
-            }
-            __syncthreads();
-            if (lane == 0) per_wave[wave][1] = up_to;
-            __syncthreads();
-            uint32_t over = up_to - low - high;
-            for (uint32_t w = wave + 1; w < WAVES; w++) over += per_wave[w][1];
-            if (over < need && need <= over + high) found[0] = 2 * tid + 1, found[1] = over;
-            else if (over + high < need && need <= over + high + low) found[0] = 2 * tid, found[1] = over + high;
-            __syncthreads();
-            least |= found[0] << shift;
-            need -= found[1];
-        }
-        ties = need;
+        const auto ranked = dev::rank_largest<uint32_t>(rank_lds, g.budget - kept, [&](auto count_in) {
+            each([&](uint32_t base, uint32_t v) {
+                if (base + lane < to && v != KEPT) count_in(v);
+            });
+        });
+        least = ranked.least, ties = ranked.exact ? n : ranked.ties;
     }
 
-    // Runs of places, a wavefront each, in order: what each has above `least` and at it, below the budget and from it on.
-    const uint32_t run = (n + EVICT - 1) / EVICT * 64, from = min(wave * run, n), to = min(from + run, n);
+    // What each run has above `least` and at it, below the budget and from it on: masks of 64 places.
+    auto first_of = [](uint32_t base, uint32_t end) { return base >= end ? 0 : end - base >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << (end - base)) - 1; };
     uint32_t counts[4] = {0, 0, 0, 0};
-    for (uint32_t base = from; base < to; base += 64) {
-        const uint32_t place = base + lane, v = place < to ? image(place) : 0;
-        const bool there = place < to, low = place < g.budget;
-        counts[0] += (uint32_t)__popcll(__ballot(there && low && v > least));
-        counts[1] += (uint32_t)__popcll(__ballot(there && low && v == least));
-        counts[2] += (uint32_t)__popcll(__ballot(there && !low && v > least));
-        counts[3] += (uint32_t)__popcll(__ballot(there && !low && v == least));
+    each([&](uint32_t base, uint32_t v) {
+        const uint64_t there = first_of(base, to), low = first_of(base, g.budget), over = __ballot(v > least) & there, at = __ballot(v == least) & there;
+        counts[0] += (uint32_t)__popcll(over & low), counts[1] += (uint32_t)__popcll(at & low);
+        counts[2] += (uint32_t)__popcll(over & ~low), counts[3] += (uint32_t)__popcll(at & ~low);
+    });
+    turn ^= 1;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) per_wave[turn][wave][i] = counts[i];
     }
-    __syncthreads();
-    if (lane < 4) per_wave[wave][lane] = counts[lane];
     __syncthreads();
     // What the runs in front leave: ties already kept, holes and movers already listed.
     uint32_t tied = 0, holes = 0, movers = 0;
     for (uint32_t w = 0; w < wave; w++) {
         const uint32_t start = min(w * run, n), end = min(start + run, n), lows = min(end, g.budget) - min(start, g.budget);
-        const uint32_t left = ties - tied, stay_low = min(per_wave[w][1], left), stay_high = min(per_wave[w][3], left - stay_low);
-        holes += lows - per_wave[w][0] - stay_low;
-        movers += per_wave[w][2] + stay_high;
+        const uint32_t *of = per_wave[turn][w], left = ties - tied, stay_low = min(of[1], left), stay_high = min(of[3], left - stay_low);
+        holes += lows - of[0] - stay_low;
+        movers += of[2] + stay_high;
         tied += stay_low + stay_high;
     }
     const int64_t list = ((int64_t)s * g.kv.kv_heads + head) * g.most;
     const uint64_t before = ((uint64_t)1 << lane) - 1;
-    for (uint32_t base = from; base < to; base += 64) {
-        const uint32_t place = base + lane, v = place < to ? image(place) : 0;
-        const bool there = place < to, low = place < g.budget, tie = there && v == least;
-        const uint64_t tie_mask = __ballot(tie);
-        const bool stays = there && (v > least || (tie && tied + (uint32_t)__popcll(tie_mask & before) < ties));
-        const bool hole = there && low && !stays, mover = stays && !low;
-        const uint64_t hole_mask = __ballot(hole), mover_mask = __ballot(mover);
-        const uint32_t hole_at = holes + (uint32_t)__popcll(hole_mask & before), mover_at = movers + (uint32_t)__popcll(mover_mask & before);
-        if (hole && hole_at < g.most) g.targets[list + hole_at] = (int32_t)place;
-        if (mover && mover_at < g.most) g.sources[list + mover_at] = (int32_t)place;
-        holes += (uint32_t)__popcll(hole_mask), movers += (uint32_t)__popcll(mover_mask);
-        tied += (uint32_t)__popcll(tie_mask);
-    }
-    if (tid == EVICT - 64) *count = (int32_t)min(movers, g.most);  // the last run's: all of them
+    auto put = [&](int32_t *to_list, uint64_t mask, uint32_t listed, uint32_t base) {
+        const uint32_t at = listed + (uint32_t)__popcll(mask & before);
+        if ((mask >> lane & 1) && at < g.most) to_list[list + at] = (int32_t)(base + lane);
+    };
+    each([&](uint32_t base, uint32_t v) {
+        const uint64_t there = first_of(base, to), low = first_of(base, g.budget), at = __ballot(v == least) & there;
+        uint64_t stay = __ballot(v > least) & there;
+        if (at) {
+            stay |= __ballot((at >> lane & 1) && tied + (uint32_t)__popcll(at & before) < ties);
+            tied += (uint32_t)__popcll(at);
+        }
+        const uint64_t hole = there & low & ~stay, mover = stay & ~low;
+        if (hole) put(g.targets, hole, holes, base), holes += (uint32_t)__popcll(hole);
+        if (mover) put(g.sources, mover, movers, base), movers += (uint32_t)__popcll(mover);
+    });
+    if (tid == THREADS - 64) *count = (int32_t)min(movers, g.most);  // the last run's: all of them
+    if (outside) *g.kv.flag = 1;
+}
+
+// Where the new lengths go into the place of the old ones: once all blocks have read those.
+__global__ __launch_bounds__(256) void shorten(EvictArgs g, int32_t *lengths) {
+    const uint32_t s = blockIdx.x * 256 + threadIdx.x;
+    if (s >= g.kv.sequences) return;
+    const int32_t length = lengths[s];
+    if (length >= 0 && (uint64_t)length <= (uint64_t)g.kv.table_pages * g.kv.page_size && (uint32_t)length <= g.max_keys && (uint32_t)length > g.budget) lengths[s] = (int32_t)g.budget;
 }
 
 // ---------------------------------------------------------------- moves
@@ -309,9 +365,21 @@ int launch_kv_evict(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_ba
     if (blocks >= MOST_BLOCKS) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     g.budget = (uint32_t)eviction.budget, g.most = (uint32_t)eviction.most, g.max_keys = (uint32_t)max_keys;
     g.recent = eviction.recent, g.first = eviction.first;
-    g.sources = eviction.sources, g.targets = eviction.targets, g.counts = eviction.counts, g.lengths = eviction.lengths;
-    g.held = (uint32_t)std::min<size_t>(max_keys, HELD);
-    hipLaunchKernelGGL(choose_evicted, dim3((uint32_t)blocks), dim3(EVICT), g.held * sizeof(uint32_t), ctx.stream, g);
+    const bool in_place = eviction.lengths == batch.lengths;
+    const int64_t apart = reinterpret_cast<intptr_t>(eviction.lengths) - reinterpret_cast<intptr_t>(batch.lengths), all = (int64_t)sizeof(int32_t) * batch.sequences;
+    if (!in_place && apart < all && apart > -all) return ctx.fail(AHIP_ERR_ARG, name + "the new lengths overlap the batch's and are not in their place");
+    g.sources = eviction.sources, g.targets = eviction.targets, g.counts = eviction.counts, g.lengths = in_place ? nullptr : eviction.lengths;
+    if (max_keys <= SMALL * SMALL_EACH) {
+        hipLaunchKernelGGL((choose_evicted<SMALL, SMALL_EACH>), dim3((uint32_t)blocks), dim3(SMALL), 0, ctx.stream, g);
+    } else if (max_keys <= LARGE * LARGE_EACH) {
+        hipLaunchKernelGGL((choose_evicted<LARGE, LARGE_EACH>), dim3((uint32_t)blocks), dim3(LARGE), 0, ctx.stream, g);
+    } else {
+        g.held = HELD;
+        hipLaunchKernelGGL((choose_evicted<LARGE, 0>), dim3((uint32_t)blocks), dim3(LARGE), HELD * sizeof(uint32_t), ctx.stream, g);
+    }
+    if (int rc = ctx.check(hipGetLastError(), "kv evict launch")) return rc;
+    if (!in_place) return AHIP_OK;
+    hipLaunchKernelGGL(shorten, dim3(((uint32_t)batch.sequences + 255) / 256), dim3(256), 0, ctx.stream, g, eviction.lengths);
     return ctx.check(hipGetLastError(), "kv evict launch");
 }
 

@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "kv_attend.h"
+#include "kv_rank.h"
 
 namespace altius {
 
@@ -91,79 +92,62 @@ __global__ __launch_bounds__(BLOCK) void mean_pages(SparseArgs g) {
 }
 
 // ---------------------------------------------------------------- scores
-template <int CONTROL> __device__ __forceinline__ double moved(double v) {
+// The larger of a lane's value and that of the lane that CONTROL names.
+template <int CONTROL> __device__ __forceinline__ double larger(double v) {
     const uint64_t u = (uint64_t)__double_as_longlong(v);
     const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CONTROL, 0xF, 0xF, false);
     const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CONTROL, 0xF, 0xF, false);
-    return __longlong_as_double((long long)((uint64_t)high << 32 | low));
-}
-constexpr int ROR8 = dev::DPP_ROW_ROR + 8;
-// v[h] summed over a row of 16 lanes, the largest of the sums in all of them.  Of two lanes that meet each keeps half of the heads, so that 8
-// sums take 8 exchanges and not 32.
-template <int HEADS> __device__ __forceinline__ double largest_sum(double (&v)[HEADS]) {
-    const uint32_t lane = threadIdx.x;
-    int left = HEADS;
-    auto halve = [&](auto move, bool upper) {
-        left /= 2;
-#pragma unroll
-        for (int h = 0; h < HEADS / 2; h++) {
-            if (h >= left) break;
-            const double keep = upper ? v[h + left] : v[h], give = upper ? v[h] : v[h + left];
-            v[h] = keep + move(give);
-        }
-    };
-    halve([](double x) { return moved<ROR8>(x); }, lane & 8u);
-    halve([](double x) { return moved<dev::DPP_ROW_HALF_MIRROR>(x); }, lane & 4u);
-    if (HEADS == 8) halve([](double x) { return moved<dev::DPP_QUAD_XOR2>(x); }, lane & 2u);
-    else v[0] += moved<dev::DPP_QUAD_XOR2>(v[0]);
-    v[0] += moved<dev::DPP_QUAD_XOR1>(v[0]);
-    double best = fmax(v[0], moved<ROR8>(v[0]));
-    best = fmax(best, moved<dev::DPP_ROW_HALF_MIRROR>(best));
-    if (HEADS == 8) best = fmax(best, moved<dev::DPP_QUAD_XOR2>(best));
-    return best;
+    return fmax(v, __longlong_as_double((long long)((uint64_t)high << 32 | low)));
 }
 
-// Scores of pages from .. to - 1 of a row's sequence, by a block: 16 lanes a page, 4 J channels each, HEADS queries of the group at a time in registers.
+// Scores of pages from .. to - 1 of a row's sequence, by a block, 16 a wavefront, with v_mfma_f64_4x4x4_4b_f64: four blocks of 4 pages by 4 heads, 4
+// channels at a time.  Lane 16 k + p has page p, lane 16 k + 4 b + j head j, and either channels 16 u + 4 k .. + 3 for u < UNITS; the result of page 4 b + i and
+// head j is in lane 16 i + 4 b + j.  No sum goes from lane to lane, and 16 pages of 128 channels and 4 heads take 32 instructions; the same with the vector
+// unit, 16 lanes a page, spent more on adding up the lanes than on products (one token, 48 texts, group of 8: 34.5 us, so 26).
 // put(page, score, again): again: the larger of it and what is there.
-template <int J, int HEADS, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t from, uint32_t to, Put put) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, l = lane & 15u;
+template <uint32_t UNITS, int FOURS, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t from, uint32_t to, Put put) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, k = lane >> 4;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t h0 = 0; h0 < g.group; h0 += HEADS) {
-        double q[HEADS][J][4];
+    for (uint32_t h0 = 0; h0 < g.group; h0 += 4 * FOURS) {
+        double q[FOURS][UNITS][4];
 #pragma unroll
-        for (int h = 0; h < HEADS; h++) {
-            const uint32_t its = head * g.group + min(h0 + h, g.group - 1);  // the last one again counts once
+        for (int f = 0; f < FOURS; f++) {
+            const uint32_t its = head * g.group + min(h0 + 4 * f + (lane & 3u), g.group - 1);  // the last one more than once: the largest is the same
             const float *from_q = g.q + (int64_t)row * g.q_token + (int64_t)its * g.q_head;
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                const uint32_t c = 64 * j + 4 * l;
+            for (uint32_t u = 0; u < UNITS; u++) {
+                const uint32_t c = 16 * u + 4 * k;
                 const f32x4 x = c < g.d ? *reinterpret_cast<const f32x4 *>(from_q + c) : zero;
 #pragma unroll
-                for (int e = 0; e < 4; e++) q[h][j][e] = (double)x[e];
+                for (int e = 0; e < 4; e++) q[f][u][e] = (double)x[e];
             }
         }
-        for (uint32_t base = from + 4 * wave; base < to; base += 4 * WAVES) {
-            const uint32_t index = base + (lane >> 4);
-            const int32_t page = index < to ? g.kv.page_of(s, index, -1) : -1;
-            const float *mean = g.means + (int64_t)max(page, 0) * g.means_page + (int64_t)head * g.means_head;
-            f32x4 x[J];
+        for (uint32_t base = from + 16 * wave; base < to; base += 16 * WAVES) {
+            const uint32_t index = base + (lane & 15u);
+            const int32_t page = index < to ? g.kv.page_of(s, index, 0) : 0;
+            const float *mean = g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head;
+            f32x4 x[UNITS];
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                const uint32_t c = 64 * j + 4 * l;
-                x[j] = *reinterpret_cast<const f32x4 *>(mean + (c < g.d ? c : 0));
-                if (c >= g.d) x[j] = zero;
+            for (uint32_t u = 0; u < UNITS; u++) x[u] = *reinterpret_cast<const f32x4 *>(mean + (16 * u + 4 * k < g.d ? 16 * u + 4 * k : 0));
+            double v[FOURS];
+#pragma unroll
+            for (int f = 0; f < FOURS; f++) v[f] = 0.0;
+#pragma unroll
+            for (uint32_t u = 0; u < UNITS; u++) {
+                if (16 * u >= g.d) break;
+                if (16 * u + 4 * k >= g.d) x[u] = zero;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const double mine = (double)x[u][e];
+#pragma unroll
+                    for (int f = 0; f < FOURS; f++) v[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(mine, q[f][u][e], v[f], 0, 0, 0);
+                }
             }
-            double v[HEADS];
 #pragma unroll
-            for (int h = 0; h < HEADS; h++) {
-                v[h] = 0.0;
-#pragma unroll
-                for (int j = 0; j < J; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[h] = __builtin_fma(q[h][j][e], (double)x[j][e], v[h]);
-            }
-            const double best = largest_sum(v);
-            if (l == 0 && index < to) put(index, best, h0 != 0);
+            for (int f = 1; f < FOURS; f++) v[0] = fmax(v[0], v[f]);
+            const double best = larger<dev::DPP_QUAD_XOR2>(larger<dev::DPP_QUAD_XOR1>(v[0]));
+            const uint32_t its = base + (lane & 12u) + (lane >> 4);
+            if ((lane & 3u) == 0 && its < to) put(its, best, h0 != 0);
         }
     }
 }
@@ -188,13 +172,13 @@ __device__ __forceinline__ Row row_of(const SparseArgs &g, uint32_t row) {
     return r;
 }
 
-template <int J, int HEADS> __global__ __launch_bounds__(BLOCK) void score_pages(SparseArgs g) {
+template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void score_pages(SparseArgs g) {
     const uint32_t outer = blockIdx.x / g.chunks, chunk = blockIdx.x - outer * g.chunks, row = outer / g.kv.kv_heads, head = outer - row * g.kv.kv_heads;
     const Row r = row_of(g, row);
     if (r.pages <= g.most) return;  // all are chosen
     const uint32_t from = max(chunk * SCORED, g.first), to = min((chunk + 1) * SCORED, r.pages - g.last);
     double *to_scores = g.scores + (size_t)outer * g.max_pages;
-    score_range<J, HEADS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
+    score_range<UNITS, FOURS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
 }
 
 // ---------------------------------------------------------------- the best
@@ -205,12 +189,11 @@ __device__ __forceinline__ uint64_t rank_image(double score) {
     return u >> 63 ? ~u : u | (uint64_t)1 << 63;
 }
 
-// A block for each row and head of keys.  The smallest image that is chosen is found by halving the range between the smallest and the largest, until
-// exactly as many as are wanted are at or above the middle; equal ones go by their number.  Then the pages are listed in order.
-template <int J, int HEADS> __global__ __launch_bounds__(BLOCK) void choose_pages(SparseArgs g) {
+// A block for each row and head of keys: the smallest image that is chosen (kv_rank.h), equal ones by their number, then the pages in order.
+template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void choose_pages(SparseArgs g) {
     extern __shared__ uint64_t images[];
-    __shared__ uint64_t ends[WAVES][2];
     __shared__ uint32_t totals[2][WAVES][2];
+    __shared__ dev::RankLds rank_lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t row = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - row * g.kv.kv_heads;
     const Row r = row_of(g, row);
@@ -242,70 +225,49 @@ template <int J, int HEADS> __global__ __launch_bounds__(BLOCK) void choose_page
     }
 
     const uint32_t from = g.first, to = r.pages - g.last, want = g.most - g.first - g.last;  // of the pages from .. to - 1, of which there are more
-    const double *scores = J ? nullptr : g.scores + ((size_t)row * g.kv.kv_heads + head) * g.max_pages;
-    if constexpr (J != 0) {
-        score_range<J, HEADS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) {
-            const uint64_t v = rank_image(score);
-            images[page] = again ? max(images[page], v) : v;
-        });
+    const double *scores = UNITS ? nullptr : g.scores + ((size_t)row * g.kv.kv_heads + head) * g.max_pages;
+    if constexpr (UNITS != 0) {
+        if (want)
+            score_range<UNITS, FOURS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) {
+                const uint64_t v = rank_image(score);
+                images[page] = again ? max(images[page], v) : v;
+            });
     } else {
         for (uint32_t page = from + tid; page < min(to, g.held); page += BLOCK) images[page] = rank_image(scores[page]);
     }
     __syncthreads();
-    auto image = [&](uint32_t page) { return J != 0 || page < g.held ? images[page] : rank_image(scores[page]); };
+    auto image = [&](uint32_t page) { return UNITS != 0 || page < g.held ? images[page] : rank_image(scores[page]); };
 
-    // low: at least as many as wanted are at or above it; high: fewer are.
-    uint64_t low = ~(uint64_t)0, high = 0;
-    for (uint32_t page = from + tid; page < to; page += BLOCK) {
-        const uint64_t v = image(page);
-        low = min(low, v), high = max(high, v);
-    }
-#pragma unroll
-    for (int m = 32; m; m >>= 1) low = min(low, (uint64_t)__shfl_xor((unsigned long long)low, m)), high = max(high, (uint64_t)__shfl_xor((unsigned long long)high, m));
-    if (lane == 0) ends[wave][0] = low, ends[wave][1] = high;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < WAVES; w++) low = min(low, ends[w][0]), high = max(high, ends[w][1]);
-    uint32_t above = 0;  // how many are at or above `high`
-    bool exact = want == 0;
-    uint64_t least = high + 1;
-    high++;  // images are below 2^64 - 1: that would be a NaN
-    for (int turn = 0; !exact && high - low > 1; turn ^= 1) {
-        const uint64_t middle = low + (high - low) / 2;
-        uint32_t n = 0;
-        for (uint32_t page = from + tid; page < to; page += BLOCK) n += image(page) >= middle ? 1u : 0u;
-#pragma unroll
-        for (int m = 32; m; m >>= 1) n += __shfl_xor(n, m);
-        if (lane == 0) totals[turn][wave][0] = n;
-        __syncthreads();
-        n = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < WAVES; w++) n += totals[turn][w][0];
-        if (n == want) exact = true, least = middle;
-        else if (n > want) low = middle;
-        else high = middle, above = n;
-    }
-    // Either all at or above `least`, or all above `low` (as many as at or above `high`) and the first of those at it.
-    const uint32_t ties = exact ? 0 : want - above;
-    if (!exact) least = low;
+    dev::Ranked<uint64_t> ranked = {0, 0, true};
+    if (want)
+        ranked = dev::rank_largest<uint64_t>(rank_lds, want, [&](auto count_in) {
+            for (uint32_t page = from + tid; page < to; page += BLOCK) count_in(image(page));
+        });
+    const uint64_t least = ranked.least;
+    const bool exact = ranked.exact;
+    const uint32_t ties = ranked.ties;
     uint32_t listed = 0, tied = 0;
+    const uint64_t before = ((uint64_t)1 << lane) - 1;
     for (uint32_t base = 0, turn = 0; base < r.pages; base += BLOCK, turn ^= 1) {
         const uint32_t page = base + tid;
         const bool there = page < r.pages, always = there && (page < from || page >= to);
-        const uint64_t v = there && !always ? image(page) : 0;
-        const bool over = there && !always && (exact ? v >= least && want != 0 : v > least), tie = there && !always && !exact && v == least;
-        const uint64_t before = ((uint64_t)1 << lane) - 1, tie_mask = __ballot(tie);
-        // Ties of the wavefronts in front count first.
-        __syncthreads();
-        if (lane == 0) totals[turn][wave][1] = (uint32_t)__popcll(tie_mask);
-        __syncthreads();
-        uint32_t tie_at = tied;
-        for (uint32_t w = 0; w < WAVES; w++) {
-            if (w < wave) tie_at += totals[turn][w][1];
-            tied += totals[turn][w][1];
+        const uint64_t v = there && !always && want ? image(page) : 0;
+        bool stays = always || (there && want && (exact ? v >= least : v > least));
+        if (!exact) {  // ties of the wavefronts in front count first
+            const bool tie = there && !always && v == least;
+            const uint64_t tie_mask = __ballot(tie);
+            __syncthreads();
+            if (lane == 0) totals[turn][wave][1] = (uint32_t)__popcll(tie_mask);
+            __syncthreads();
+            uint32_t tie_at = tied;
+            for (uint32_t w = 0; w < WAVES; w++) {
+                if (w < wave) tie_at += totals[turn][w][1];
+                tied += totals[turn][w][1];
+            }
+            stays = stays || (tie && tie_at + (uint32_t)__popcll(tie_mask & before) < ties);
         }
-        const bool stays = always || over || (tie && tie_at + (uint32_t)__popcll(tie_mask & before) < ties);
         const uint64_t stay_mask = __ballot(stays);
+        __syncthreads();
         if (lane == 0) totals[turn][wave][0] = (uint32_t)__popcll(stay_mask);
         __syncthreads();
         uint32_t at = listed;
@@ -374,14 +336,14 @@ int check_sparse(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
     return check_means(ctx, name, *cache, *sparse);
 }
 
-template <int J, int HEADS> void launch_choice(hipStream_t stream, const SparseArgs &g, const SparsePlan &p) {
+template <uint32_t UNITS, int FOURS> void launch_choice(hipStream_t stream, const SparseArgs &g, const SparsePlan &p) {
     const dim3 grid((uint32_t)p.rows), block(BLOCK);
     const uint32_t held = (uint32_t)(g.held * sizeof(uint64_t));
     if (p.split) {
-        hipLaunchKernelGGL((score_pages<J, HEADS>), dim3((uint32_t)(p.rows * g.chunks)), block, 0, stream, g);
+        hipLaunchKernelGGL((score_pages<UNITS, FOURS>), dim3((uint32_t)(p.rows * g.chunks)), block, 0, stream, g);
         hipLaunchKernelGGL((choose_pages<0, 1>), grid, block, held, stream, g);
     } else {
-        hipLaunchKernelGGL((choose_pages<J, HEADS>), grid, block, held, stream, g);
+        hipLaunchKernelGGL((choose_pages<UNITS, FOURS>), grid, block, held, stream, g);
     }
 }
 
@@ -460,11 +422,11 @@ int launch_kv_attention_sparse(DeviceCtx &ctx, const ahip_kv_cache &cache, const
     g.fills = g.max_tokens == 1;
     if (!g.fills)
         if (int rc = launch_means(ctx, g, name)) return rc;
-    if (g.d <= 64) g.group <= 4 ? launch_choice<1, 4>(ctx.stream, g, p) : launch_choice<1, 8>(ctx.stream, g, p);
-    else if (g.d <= 128) g.group <= 4 ? launch_choice<2, 4>(ctx.stream, g, p) : launch_choice<2, 8>(ctx.stream, g, p);
-    else launch_choice<4, 4>(ctx.stream, g, p);
+    if (g.d <= 64) g.group <= 4 ? launch_choice<4, 1>(ctx.stream, g, p) : launch_choice<4, 2>(ctx.stream, g, p);
+    else if (g.d <= 128) g.group <= 4 ? launch_choice<8, 1>(ctx.stream, g, p) : launch_choice<8, 2>(ctx.stream, g, p);
+    else launch_choice<16, 1>(ctx.stream, g, p);
     if (int rc = ctx.check(hipGetLastError(), "kv attention over chosen pages launch")) return rc;
-    return attend::launch_attend_rows(ctx, a, g.bf16);
+    return attend::launch_attend_kept(ctx, a, g.bf16);
 }
 
 }  // namespace altius

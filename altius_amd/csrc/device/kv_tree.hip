@@ -20,7 +20,7 @@ int launch_kv_attention_tree(DeviceCtx &ctx, const ahip_kv_cache &cache, const a
     if (!parents) return ctx.fail(AHIP_ERR_ARG, name + "null parents");
     g.parents = parents;
     g.max_tokens = std::min(g.max_tokens, attend::TREE_ROWS);
-    return attend::launch_attend<true>(ctx, g, cache.elem == AHIP_KV_BF16);
+    return attend::launch_attend<attend::TREE>(ctx, g, cache.elem == AHIP_KV_BF16);
 }
 
 }  // namespace altius

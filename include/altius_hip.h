@@ -484,7 +484,7 @@ typedef struct ahip_kv_history {
  *     mass = decay * mass + the sum of the softmax's weights over the sequence's rows and the head's group of query heads,
  * where the rows' own slots start from 0, and so do all where decay is 0: what was there is not read then.  positions (if not NULL) of the rows'
  * own slots become row_positions[row], or their place where that is NULL.  decay from 0 to 1.  The weights are added in the same order in
- * every call.  A sequence whose rows are more than its tokens is left out. */
+ * every call.  No two sequences of a call may share pages. */
 int ahip_kv_attention_mass_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
                                      size_t *bytes);
 int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
@@ -494,7 +494,7 @@ int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip
  * the `recent` newest (above the largest less `recent`), then those with the largest mass; of equal ones the lowest place.  NaN counts as
  * less than all else.  The i-th place from `budget` on that stays is sources[i], the i-th place below it that does not is targets[i], for i <
  * counts; behind that the lists stay as they were.  ahip_kv_move with these lists (apart) leaves what stays in the first `budget` places, in no order
- * of positions.  lengths[s] becomes min(length, budget).  Lists of sequence s and head h start at (s * kv_heads + h) * most, counts at
+ * of positions.  lengths[s] becomes min(length, budget); it may be the batch's own array (one launch more).  Lists of sequence s and head h start at (s * kv_heads + h) * most, counts at
  * s * kv_heads + h.  Of the batch, query_starts is not read (it may be NULL); of the cache, neither keys nor values. */
 typedef struct ahip_kv_eviction {
     int32_t budget, recent, first; /* recent + first up to the budget */

@@ -256,15 +256,19 @@ class Evict:
         self.most = most if most is not None else max(0, min(budget, (max_keys or per * page) - budget))
         self.max_keys = max_keys
 
-    def run(self, ctx):
+    in_place = False
+
+    def run(self, ctx, overlap=0):
         on = dict(mass=gpu(self.mass), positions=gpu(self.positions), table=gpu(self.table), lengths=gpu(np.array(self.lengths, np.int32)))
         self.lists = [torch.full((len(self.lengths), self.kv, max(1, self.most)), -9, device="cuda", dtype=torch.int32) for _ in range(2)]
         self.counts, self.kept = torch.full((len(self.lengths), self.kv), -9, device="cuda", dtype=torch.int32), torch.full((len(self.lengths),), -9, device="cuda", dtype=torch.int32)
+        if self.in_place:
+            self.kept = on["lengths"]
         cache = D.KvCache(kv_heads=self.kv, head_size=8, page_size=self.page, pages=self.pages)
         batch = D.KvBatch(sequences=len(self.lengths), table_pages=self.table.shape[1], table_stride=self.table.shape[1], lengths=on["lengths"].data_ptr(), page_table=on["table"].data_ptr())
         history = D.KvHistory(mass=on["mass"].data_ptr(), positions=on["positions"].data_ptr(), page_stride=self.kv * self.page, head_stride=self.page)
         eviction = D.KvEviction(budget=self.budget, recent=self.recent, first=self.first, most=self.most, max_keys=self.max_keys, sources=self.lists[0].data_ptr(),
-                                targets=self.lists[1].data_ptr(), counts=self.counts.data_ptr(), lengths=self.kept.data_ptr())
+                                targets=self.lists[1].data_ptr(), counts=self.counts.data_ptr(), lengths=self.kept.data_ptr() + overlap)
         torch.cuda.synchronize()
         ctx.kv_evict_raw(cache, batch, history, eviction)
         torch.cuda.synchronize()
@@ -359,6 +363,23 @@ def test_evictions_that_are_refused(here, case):  # noqa: F811
             e.run(here)
         assert error.value.code == ERR_ARG
     here.sync()
+
+
+@pytest.mark.parametrize("longest", [150, 5000])
+def test_new_lengths_in_the_place_of_the_old_ones(here, case, longest):  # noqa: F811
+    """Every head of a sequence goes by the old length, however late its block starts: many more blocks than run at once."""
+    case(f"evict in place, {longest}")
+    rng = np.random.default_rng(5)
+    lengths = [int(x) for x in rng.integers(90, longest + 1, 150)]
+    e = Evict(rng, lengths, 32, 50, 100, 20, 4, max_keys=longest)
+    e.in_place = True
+    e.run(here)
+    here.sync()
+    e.held()
+    with pytest.raises(AltiusHipError) as error:
+        e.in_place = 1
+        e.run(here, overlap=4)
+    assert error.value.code == ERR_ARG
 
 
 @pytest.mark.parametrize("elem", ["f32", "bf16"])
