@@ -1511,10 +1511,14 @@ struct Plan {
     uint32_t few_rows;
     size_t bytes;
 };
-Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend);
+Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, bool tree = false);
+// Calls that ahip_kv_attention_tree takes and whose sequences may all be trees.
+inline bool may_be_trees(const ahip_kv_attend &a) {
+    return (a.max_tokens && a.max_tokens < a.tokens ? a.max_tokens : a.tokens) <= TREE_ROWS && a.causal && !a.prefix;
+}
 int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend, dev::KvView *view);
 // Checks the call and describes it for the kernels; q stays null where there is nothing to do.
-int begin_attend(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, AttendArgs *args);
+int begin_attend(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, bool tree, AttendArgs *args);
 int launch_attend_kept(DeviceCtx &ctx, const AttendArgs &g, bool bf16);  // kv_kept.hip
 
 }  // namespace attend

@@ -14,7 +14,7 @@ namespace {
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 }  // namespace
 
-Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
+Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, bool tree) {
     Plan p = {};
     const uint32_t group = (uint32_t)(attend.q_heads / cache.kv_heads);
     const size_t held = std::min((size_t)batch.table_pages * (size_t)cache.page_size, (size_t)INT32_MAX);
@@ -57,7 +57,9 @@ Plan plan_of(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_bat
     // one prompt of 1024, 12 heads of 64 channels, 50 and 37 us.  With three quarters of the places taken (4 such prompts) this cut
     // costs (59 us whole, 78 us cut): it gives every row tile parts of the whole sequence, half of which a causal prompt does not see.  Parts of 128 keys at least: a prompt of 400, 16 heads of 128, fp32, 32 us, with 256 36 us.
     if (rows > FEW_ROWS) {
-        if (tiled) share(p.many, rows, TILE_ROWS, many_tiles, many_tiles < many_at_once / 2, many_at_once, 128);
+        // Trees see nearly all of their sequence, whatever its length: 16 of 48 tokens behind 8000 (8 heads of keys of 128 channels, bf16) 482 us whole, 347 cut, of 16 to
+        // 48 behind 300 to 8000 in fp32 617 and 519.
+        if (tiled) share(p.many, rows, TILE_ROWS, many_tiles, many_tiles < (tree ? 4 * many_at_once : many_at_once / 2), many_at_once, 128);
         else share(p.many, rows, 16, pairs * ((rows + 15) / 16), false, 0, 0);
     }
     p.few_rows = p.many.cut ? FEW_BESIDE_CUT : FEW_ROWS;
@@ -103,14 +105,14 @@ int check_attend(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
     return AHIP_OK;
 }
 
-int begin_attend(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, AttendArgs *args) {
+int begin_attend(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, bool tree, AttendArgs *args) {
     AttendArgs &g = *args;
     if (int rc = check_attend(&ctx, &cache, &batch, &attend, &g.kv)) return rc;
     if (attend.tokens == 0 || batch.sequences == 0) return AHIP_OK;
     if (int rc = require_kv_arrays(ctx, "kv attention", cache, batch)) return rc;
     if (!attend.q || !attend.out) return ctx.fail(AHIP_ERR_ARG, "kv attention: null pointer");
     if (attend.out == attend.q) return ctx.fail(AHIP_ERR_ARG, "kv attention: out is q");
-    const Plan plan = plan_of(&ctx, cache, batch, attend);
+    const Plan plan = plan_of(&ctx, cache, batch, attend, tree);
     if (plan.bytes && (!attend.workspace || attend.workspace_bytes < plan.bytes))
         return ctx.fail(AHIP_ERR_ARG, "kv attention: the workspace holds " + std::to_string(attend.workspace ? attend.workspace_bytes : 0) + " bytes of " +
                                           std::to_string(plan.bytes));
@@ -141,13 +143,15 @@ int kv_attention_workspace(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahi
     dev::KvView view = {};
     // The sizes alone: neither the tensors nor the arrays on the device need exist yet.
     if (int rc = attend::check_attend(ctx, cache, batch, attend, &view)) return rc;
-    *bytes = attend::plan_of(ctx, *cache, *batch, *attend).bytes;
+    *bytes = attend::plan_of(ctx, *cache, *batch, *attend, false).bytes;
+    // The rows may be trees, whose keys are cut where a piece's are not.
+    if (attend::may_be_trees(*attend)) *bytes = std::max(*bytes, attend::plan_of(ctx, *cache, *batch, *attend, true).bytes);
     return AHIP_OK;
 }
 
 int launch_kv_attention(DeviceCtx &ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
     attend::AttendArgs g = {};
-    if (int rc = attend::begin_attend(ctx, cache, batch, attend, &g)) return rc;
+    if (int rc = attend::begin_attend(ctx, cache, batch, attend, false, &g)) return rc;
     return g.q ? attend::launch_attend<attend::PLAIN>(ctx, g, cache.elem == AHIP_KV_BF16) : AHIP_OK;
 }
 

@@ -417,7 +417,7 @@ int launch_kv_attention_mass(DeviceCtx &ctx, const ahip_kv_cache &cache, const a
     const uint64_t finish = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads * (((uint64_t)plan.max_keys + 255) / 256);
     if ((plan.many && (plan.blocks >= MOST_BLOCKS || attend.tokens * (uint64_t)attend.q_heads * plan.channels / 1024 >= MOST_BLOCKS)) || finish >= MOST_BLOCKS)
         return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
-    if (int rc = begin_attend(ctx, cache, batch, attend, &m.at)) return rc;
+    if (int rc = begin_attend(ctx, cache, batch, attend, false, &m.at)) return rc;
     char *space = static_cast<char *>(attend.workspace);
     m.at.stats = reinterpret_cast<float *>(space + plan.stats);
     if (plan.score_rows) {

@@ -17,8 +17,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t BLOCK = 256, WAVES = BLOCK / 64;
-constexpr uint32_t HELD = 16384;     // images of pages in LDS
-constexpr uint32_t SCORED = 64;      // pages of a block that does nothing but score
+constexpr uint32_t HELD = 8192;      // images of pages in LDS
+constexpr uint32_t SCORED = 64;      // pages of a block that does nothing but score a row
+constexpr uint32_t SCORED_ROWS = 8, ROW_PAGES = 256;  // rows and pages of one that scores several
 constexpr uint32_t MOST_CHANNELS = 256;
 
 struct SparseArgs {
@@ -30,7 +31,7 @@ struct SparseArgs {
     int64_t q_token, q_head;
     uint32_t d, group, q_heads, most, first, last;
     uint32_t max_tokens, max_keys, max_pages, held, chunks;
-    bool bf16, fills;   // fills: choose_pages makes the mean of a page that its row fills
+    bool bf16, fills;   // fills: as many blocks again make the mean of the page that a row fills
     double *scores;     // [row][kv head][max_pages]; null: choose_pages makes them itself
     int32_t *table, *starts, *lengths;  // of the sequences that attention sees
 };
@@ -122,13 +123,25 @@ template <uint32_t UNITS, int FOURS, class Put> __device__ __forceinline__ void 
                 for (int e = 0; e < 4; e++) q[f][u][e] = (double)x[e];
             }
         }
-        for (uint32_t base = from + 16 * wave; base < to; base += 16 * WAVES) {
-            const uint32_t index = base + (lane & 15u);
-            const int32_t page = index < to ? g.kv.page_of(s, index, 0) : 0;
+        // The means of 16 pages while those in front are multiplied.
+        auto page_at = [&](uint32_t base) { return base + (lane & 15u) < to ? g.kv.page_of(s, base + (lane & 15u), 0) : 0; };
+        f32x4 ahead[UNITS];
+        auto fetch = [&](int32_t page) {
             const float *mean = g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head;
+#pragma unroll
+            for (uint32_t u = 0; u < UNITS; u++) ahead[u] = *reinterpret_cast<const f32x4 *>(mean + (16 * u + 4 * k < g.d ? 16 * u + 4 * k : 0));
+        };
+        const uint32_t start = from + 16 * wave;
+        fetch(page_at(start));
+        int32_t page = page_at(start + 16 * WAVES);
+        for (uint32_t base = start; base < to; base += 16 * WAVES) {
             f32x4 x[UNITS];
 #pragma unroll
-            for (uint32_t u = 0; u < UNITS; u++) x[u] = *reinterpret_cast<const f32x4 *>(mean + (16 * u + 4 * k < g.d ? 16 * u + 4 * k : 0));
+            for (uint32_t u = 0; u < UNITS; u++) x[u] = ahead[u];
+            if (base + 16 * WAVES < to) {
+                fetch(page);
+                page = page_at(base + 32 * WAVES);
+            }
             double v[FOURS];
 #pragma unroll
             for (int f = 0; f < FOURS; f++) v[f] = 0.0;
@@ -155,18 +168,21 @@ template <uint32_t UNITS, int FOURS, class Put> __device__ __forceinline__ void 
 // The row's place in its sequence, and the pages in front of it with its own: 0 where there is no such row.
 struct Row {
     uint32_t s, pages, place;
+    int32_t signed_place;  // below 0 in a sequence that is shorter than its rows
     bool live;
 };
-__device__ __forceinline__ Row row_of(const SparseArgs &g, uint32_t row) {
+// behind: the first row behind the sequence's, where it is live.
+__device__ __forceinline__ Row row_of(const SparseArgs &g, uint32_t row, uint32_t *behind = nullptr) {
     dev::KvSequence q = {0, 0, 0};
-    Row r = {0, 0, 0, false};
+    Row r = {0, 0, 0, 0, false};
     r.s = dev::kv_sequence_of(g.kv, row, q);
     if (r.s >= g.kv.sequences) return r;
     q = within(g, q);
     const int32_t t = (int32_t)row - q.start;
     if (t < 0 || t >= q.n) return r;
     r.live = true;
-    const int32_t place = q.length - q.n + t;
+    if (behind) *behind = (uint32_t)(q.start + q.n);
+    const int32_t place = r.signed_place = q.length - q.n + t;
     if (place < 0) return r;
     r.place = (uint32_t)place, r.pages = g.kv.by_page_size.div(r.place) + 1;
     return r;
@@ -179,6 +195,67 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void sc
     const uint32_t from = max(chunk * SCORED, g.first), to = min((chunk + 1) * SCORED, r.pages - g.last);
     double *to_scores = g.scores + (size_t)outer * g.max_pages;
     score_range<UNITS, FOURS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
+}
+
+// The same for SCORED_ROWS rows next to each other, whose queries wait in LDS: rows of one sequence read its means together.  309 rows behind 6001 to 12000 tokens in
+// pages of 16, 4 heads of keys of 80 channels: 39 us with the choice; each row by itself, in the block that chooses, 52.
+template <uint32_t UNITS> __global__ __launch_bounds__(BLOCK) void score_rows(SparseArgs g) {
+    __shared__ double queries[SCORED_ROWS][UNITS][4][16];  // [row][u][e][4 k + j]: of channel 16 u + 4 k + e and head j
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = lane >> 4;
+    const uint32_t outer = blockIdx.x / g.chunks, chunk = blockIdx.x - outer * g.chunks, group = outer / g.kv.kv_heads, head = outer - group * g.kv.kv_heads;
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t end_row = min((group + 1) * SCORED_ROWS, g.kv.tokens);
+    for (uint32_t row = group * SCORED_ROWS, rows; row < end_row; row += rows) {
+        uint32_t behind;  // the first row that is another sequence's
+        const Row r = row_of(g, row, &behind);
+        rows = r.live ? min(behind, end_row) - row : 1;
+        // The last row has most pages.
+        const uint32_t last_pages = r.live ? (uint32_t)max(0, (int32_t)g.kv.by_page_size.div((uint32_t)max(0, r.signed_place + (int32_t)rows - 1)) + 1) : 0;
+        if (!r.live || r.signed_place + (int32_t)rows <= 0 || last_pages <= g.most) continue;
+        const uint32_t from = max(chunk * ROW_PAGES, g.first), to = min((chunk + 1) * ROW_PAGES, last_pages - g.last);
+        if (from >= to) continue;
+        for (uint32_t h0 = 0; h0 < g.group; h0 += 4) {
+            __syncthreads();
+            for (uint32_t i = tid; i < rows * UNITS * 16; i += BLOCK) {  // 4 channels of a query each
+                const uint32_t j = i & 3u, its_k = i >> 2 & 3u, u = i / 16 % UNITS, its = i / (16 * UNITS), c = 16 * u + 4 * its_k;
+                const uint32_t h = head * g.group + min(h0 + j, g.group - 1);  // the last one more than once
+                const f32x4 x = c < g.d ? *reinterpret_cast<const f32x4 *>(g.q + (int64_t)(row + its) * g.q_token + (int64_t)h * g.q_head + c) : zero;
+#pragma unroll
+                for (int e = 0; e < 4; e++) queries[its][u][e][4 * its_k + j] = (double)x[e];
+            }
+            __syncthreads();
+            for (uint32_t base = from + 16 * wave; base < to; base += 16 * WAVES) {
+                const uint32_t index = base + (lane & 15u);
+                const int32_t page = index < to ? g.kv.page_of(r.s, index, 0) : 0;
+                const float *mean = g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head;
+                double mine[UNITS][4];
+#pragma unroll
+                for (uint32_t u = 0; u < UNITS; u++) {
+                    const uint32_t c = 16 * u + 4 * k;
+                    f32x4 x = *reinterpret_cast<const f32x4 *>(mean + (c < g.d ? c : 0));
+                    if (c >= g.d) x = zero;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mine[u][e] = (double)x[e];
+                }
+                const uint32_t its_page = base + (lane & 12u) + (lane >> 4);
+                for (uint32_t its = 0; its < rows; its++) {
+                    double v = 0.0;
+#pragma unroll
+                    for (uint32_t u = 0; u < UNITS; u++) {
+                        if (16 * u < g.d) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v = __builtin_amdgcn_mfma_f64_4x4x4f64(mine[u][e], queries[its][u][e][4 * k + (lane & 3u)], v, 0, 0, 0);
+                        }
+                    }
+                    const double best = larger<dev::DPP_QUAD_XOR2>(larger<dev::DPP_QUAD_XOR1>(v));
+                    if ((lane & 3u) == 0 && its_page < to) {
+                        double *put = g.scores + ((size_t)(row + its) * g.kv.kv_heads + head) * g.max_pages + its_page;
+                        *put = h0 ? fmax(*put, best) : best;
+                    }
+                }
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------- the best
@@ -195,8 +272,13 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     __shared__ uint32_t totals[2][WAVES][2];
     __shared__ dev::RankLds rank_lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t row = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - row * g.kv.kv_heads;
+    const uint32_t rows = g.kv.tokens * g.kv.kv_heads, id = blockIdx.x < rows ? blockIdx.x : blockIdx.x - rows, row = id / g.kv.kv_heads, head = id - row * g.kv.kv_heads;
     const Row r = row_of(g, row);
+    if (blockIdx.x >= rows) {  // where rows fill pages for later calls: beside the choice (behind it, one token of 1024 pages takes 5 us more)
+        const int32_t page = r.pages && r.place + 1 == r.pages * g.kv.page_size ? g.kv.page_of(r.s, r.pages - 1, -1) : -1;
+        if (page >= 0) page_mean(g, page, head);
+        return;
+    }
     const int32_t first_row = g.kv.starts[0], end_row = g.kv.starts[g.kv.sequences];
     if (head == 0 && tid < 2 && (tid == 0 || row + 1 == g.kv.tokens)) {
         const int32_t at = (int32_t)(row + tid);
@@ -211,10 +293,6 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     const uint32_t count = min(r.pages, g.most);
     if (head == 0 && tid == 0) g.lengths[row] = count ? (int32_t)((count - 1) * g.kv.page_size + (r.place - (r.pages - 1) * g.kv.page_size) + 1) : 0;
     for (uint32_t i = count + tid; i < g.most; i += BLOCK) g.chosen[list + i] = -1;
-    if (g.fills && count && r.place + 1 == r.pages * g.kv.page_size) {
-        const int32_t page = g.kv.page_of(r.s, r.pages - 1, -1);
-        if (page >= 0) page_mean(g, page, head);
-    }
     auto put = [&](uint32_t at, uint32_t page) {
         g.chosen[list + at] = (int32_t)page;
         g.table[list + at] = g.kv.page_of(r.s, page, -1);
@@ -223,6 +301,7 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
         for (uint32_t i = tid; i < count; i += BLOCK) put(i, i);
         return;
     }
+    uint32_t *const in_order = reinterpret_cast<uint32_t *>(images + g.held);  // g.most of them
 
     const uint32_t from = g.first, to = r.pages - g.last, want = g.most - g.first - g.last;  // of the pages from .. to - 1, of which there are more
     const double *scores = UNITS ? nullptr : g.scores + ((size_t)row * g.kv.kv_heads + head) * g.max_pages;
@@ -233,7 +312,15 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
                 images[page] = again ? max(images[page], v) : v;
             });
     } else {
-        for (uint32_t page = from + tid; page < min(to, g.held); page += BLOCK) images[page] = rank_image(scores[page]);
+        const uint32_t end = min(to, g.held);
+        for (uint32_t base = from + tid; base < end; base += 4 * BLOCK) {  // four loads on their way at once
+            double v[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) v[u] = scores[min(base + u * BLOCK, end - 1)];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++)
+                if (base + u * BLOCK < end) images[base + u * BLOCK] = rank_image(v[u]);
+        }
     }
     __syncthreads();
     auto image = [&](uint32_t page) { return UNITS != 0 || page < g.held ? images[page] : rank_image(scores[page]); };
@@ -275,15 +362,18 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
             if (w < wave) at += totals[turn][w][0];
             listed += totals[turn][w][0];
         }
-        if (stays) put(at + (uint32_t)__popcll(stay_mask & before), page);
+        if (stays) in_order[at + (uint32_t)__popcll(stay_mask & before)] = page;
     }
+    // Their places in the cache are looked up together, not as each is found.
+    __syncthreads();
+    for (uint32_t i = tid; i < g.most; i += BLOCK) put(i, in_order[i]);
 }
 
 // ---------------------------------------------------------------- the host's part
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 constexpr int64_t MOST_STRIDE = (int64_t)1 << 48;
-constexpr uint64_t MOST_GRID = (uint64_t)1 << 24;
+constexpr uint64_t MOST_GRID = (uint64_t)1 << 24, SCORES = (uint64_t)1 << 28;
 
 int check_means(DeviceCtx *ctx, const std::string &name, const ahip_kv_cache &cache, const ahip_kv_sparse &sparse) {
     if (sparse.page_stride < 0 || sparse.head_stride < 0 || sparse.page_stride > MOST_STRIDE || sparse.head_stride > MOST_STRIDE)
@@ -300,8 +390,8 @@ struct SparsePlan {
     ahip_kv_batch batch;    // as attention sees it
     ahip_kv_attend attend;
     size_t attend_bytes, starts, lengths, table, scores, bytes;
-    uint64_t max_pages, rows;  // rows: times heads of keys
-    bool split;                // scores by a launch of their own
+    uint64_t max_pages, rows, score_blocks;  // rows: times heads of keys
+    bool split, by_rows;                     // scores by a launch of their own, for rows next to each other at once
 };
 
 SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const ahip_kv_sparse &sparse) {
@@ -313,7 +403,15 @@ SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const a
     p.max_pages = (max_keys + cache.page_size - 1) / cache.page_size;
     p.rows = attend.tokens * (uint64_t)cache.kv_heads;
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
-    p.split = p.max_pages > HELD || (p.rows < cus && p.max_pages > 4 * SCORED);
+    // A block that chooses makes its scores itself where there are blocks for all CUs, or few pages: 48 tokens of up to 500 pages, 4 heads of keys, 66 us
+    // with their attention, 76 by launches of their own; one token of 1024 pages, 8 heads, 50 us and 31.
+    p.split = p.max_pages > HELD || (p.rows < cus && p.max_pages > 8 * SCORED);
+    // Rows of one sequence read its means together, as far as their scores fit into SCORES bytes.
+    const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
+    p.by_rows = max_tokens >= SCORED_ROWS && p.max_pages > SCORED && (p.split || p.rows * p.max_pages * sizeof(double) <= SCORES);
+    p.split = p.split || p.by_rows;
+    p.score_blocks = p.by_rows ? (attend.tokens + SCORED_ROWS - 1) / SCORED_ROWS * cache.kv_heads * ((p.max_pages + ROW_PAGES - 1) / ROW_PAGES)
+                               : p.rows * ((p.max_pages + SCORED - 1) / SCORED);
     p.attend_bytes = attend::plan_of(ctx, cache, p.batch, p.attend).bytes;
     p.starts = up16(p.attend_bytes);
     p.lengths = up16(p.starts + (attend.tokens + 1) * sizeof(int32_t));
@@ -331,16 +429,20 @@ int check_sparse(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
         return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "causal attention without window, slopes, prefix and first keys only");
     if (sparse->first < 0 || sparse->last < 1 || (int64_t)sparse->first + sparse->last > sparse->most)
         return kv_fail(ctx, AHIP_ERR_ARG, name + "the first and the last pages, one of those at least, fit into what is chosen");
-    if ((int64_t)sparse->most * cache->page_size > INT32_MAX - (1 << 16) || attend->tokens * (uint64_t)cache->kv_heads >= MOST_GRID)
+    if ((int64_t)sparse->most * cache->page_size > INT32_MAX - (1 << 16) || attend->tokens * (uint64_t)cache->kv_heads >= MOST_GRID / 2)
         return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more chosen keys, or rows, than are supported");
     return check_means(ctx, name, *cache, *sparse);
 }
 
 template <uint32_t UNITS, int FOURS> void launch_choice(hipStream_t stream, const SparseArgs &g, const SparsePlan &p) {
-    const dim3 grid((uint32_t)p.rows), block(BLOCK);
-    const uint32_t held = (uint32_t)(g.held * sizeof(uint64_t));
-    if (p.split) {
-        hipLaunchKernelGGL((score_pages<UNITS, FOURS>), dim3((uint32_t)(p.rows * g.chunks)), block, 0, stream, g);
+    const dim3 grid((uint32_t)(g.fills ? 2 * p.rows : p.rows)), block(BLOCK);
+    // What a block holds: images, and the list of a row that has more pages than it chooses.
+    const uint32_t held = (uint32_t)(g.held * sizeof(uint64_t) + (g.most < g.max_pages ? g.most * sizeof(uint32_t) : 0));
+    if (p.by_rows) {
+        hipLaunchKernelGGL((score_rows<UNITS>), dim3((uint32_t)p.score_blocks), block, 0, stream, g);
+        hipLaunchKernelGGL((choose_pages<0, 1>), grid, block, held, stream, g);
+    } else if (p.split) {
+        hipLaunchKernelGGL((score_pages<UNITS, FOURS>), dim3((uint32_t)p.score_blocks), block, 0, stream, g);
         hipLaunchKernelGGL((choose_pages<0, 1>), grid, block, held, stream, g);
     } else {
         hipLaunchKernelGGL((choose_pages<UNITS, FOURS>), grid, block, held, stream, g);
@@ -407,15 +509,15 @@ int launch_kv_attention_sparse(DeviceCtx &ctx, const ahip_kv_cache &cache, const
     g.max_tokens = (uint32_t)std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
     g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
     g.max_pages = (uint32_t)p.max_pages, g.held = (uint32_t)std::min<uint64_t>(p.max_pages, HELD);
-    g.chunks = (uint32_t)((p.max_pages + SCORED - 1) / SCORED);
+    g.chunks = (uint32_t)(p.by_rows ? (p.max_pages + ROW_PAGES - 1) / ROW_PAGES : (p.max_pages + SCORED - 1) / SCORED);
     g.starts = reinterpret_cast<int32_t *>(space + p.starts), g.lengths = reinterpret_cast<int32_t *>(space + p.lengths), g.table = reinterpret_cast<int32_t *>(space + p.table);
     g.scores = p.split ? reinterpret_cast<double *>(space + p.scores) : nullptr;
-    if (p.split && p.rows * g.chunks >= MOST_GRID) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
+    if (p.split && p.score_blocks >= MOST_GRID) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     // What attention will see, before anything is launched.
     p.batch.query_starts = g.starts, p.batch.lengths = g.lengths, p.batch.page_table = g.table;
     p.attend.workspace_bytes = p.attend_bytes;
     attend::AttendArgs a = {};
-    if (int rc = attend::begin_attend(ctx, cache, p.batch, p.attend, &a)) return rc;
+    if (int rc = attend::begin_attend(ctx, cache, p.batch, p.attend, false, &a)) return rc;
     a.kv.table_head = sparse.most;
 
     // A single row fills a page for later calls only; several may score a page that one of them has filled.
