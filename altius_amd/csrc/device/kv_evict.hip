@@ -21,9 +21,9 @@ struct History {
 
 // ---------------------------------------------------------------- who stays
 // A block for each sequence and head of keys, a wavefront for each run of places.  Masses become an order-preserving image of 32 bits; the smallest that
-// stays is found among them (kv_rank.h), then the runs are counted and listed in order.  What stays for its position is counted apart.
-//   Up to 2048 places 256 threads hold 8 images each.  48 sequences of 1025 places, 8 heads: 8.2 us.
-//   Up to 57344 places 1024 threads hold 56.  4 sequences of 20011 to 50000 places: 72.7 us, bound by the vector unit of one CU a block and the latency of its
+// stays is found among them (kv_rank.h), then the runs are counted and listed in order.
+//   Up to 2048 places 256 threads hold 8 images each.  48 sequences of 1025 places, 8 heads: 7.9 us.
+//   Up to 57344 places 1024 threads hold 56.  4 sequences of 20011 to 50000 places: 62 us, bound by the vector unit of one CU a block and the latency of its
 // walks over the places.  Beyond, images wait in LDS as far as that goes, and what is behind is read anew, out of L2: 103 us with the same lengths.
 constexpr uint32_t HELD = 28672, PAGES = 4096, SMALL = 256, SMALL_EACH = 8, LARGE = 1024, LARGE_EACH = 56;
 constexpr uint32_t KEPT = 0xffffffffu;  // by its position; above every mass
@@ -49,7 +49,7 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
     static_assert(EACH % AHEAD == 0, "whole sweeps");
     extern __shared__ uint32_t held[];
     __shared__ int64_t page_starts[STARTS ? PAGES : 1];
-    __shared__ uint32_t per_wave[2][WAVES][4];
+    __shared__ uint32_t per_wave[WAVES][4];
     __shared__ dev::RankLds rank_lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t s = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - s * g.kv.kv_heads;
@@ -94,62 +94,51 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
         for (uint32_t u = 0; u < AHEAD; u++) load(u, at[u]);
         __builtin_amdgcn_sched_barrier(0);
     };
-    // Over the block: what the wavefronts have, joined; one barrier.
-    int turn = 0;
-    auto all_waves = [&](uint32_t mine, auto join) {
-        turn ^= 1;
-        if (lane == 0) per_wave[turn][wave][0] = mine;
-        __syncthreads();
-        uint32_t v = per_wave[turn][0][0];
-#pragma unroll
-        for (uint32_t w = 1; w < WAVES; w++) v = join(v, per_wave[turn][w][0]);
-        return v;
-    };
-
-    // The newest position, and what stays for its own.
-    int32_t newest = INT32_MIN, its[AHEAD];
-    float masses[AHEAD];
+    // The newest position, and what stays for its own: above every mass.
+    int32_t newest = INT32_MIN, positions[AHEAD];
+    uint32_t masses[AHEAD];
     if constexpr (EACH == AHEAD) {
-        ahead(from, [&](uint32_t u, int64_t at) { its[u] = g.history.positions[at], masses[u] = g.history.mass[at]; });
+        ahead(from, [&](uint32_t u, int64_t at) { positions[u] = g.history.positions[at], masses[u] = __float_as_uint(g.history.mass[at]); });
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, its[u]);
-    } else {
+        for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, positions[u]);
+    } else {  // (56 positions a thread beside as many images leave no registers: 69 us instead of 62)
         for (uint32_t base = from; base < to; base += 64 * AHEAD) {
-            ahead(base, [&](uint32_t u, int64_t at) { its[u] = g.history.positions[at]; });
+            ahead(base, [&](uint32_t u, int64_t at) { positions[u] = g.history.positions[at]; });
 #pragma unroll
-            for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, its[u]);
+            for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, positions[u]);
         }
     }
 #pragma unroll
     for (int m = 32; m; m >>= 1) newest = max(newest, __shfl_xor(newest, m));
-    newest = (int32_t)all_waves((uint32_t)newest, [](uint32_t a, uint32_t b) { return (uint32_t)max((int32_t)a, (int32_t)b); });
+    if (lane == 0) per_wave[wave][0] = (uint32_t)newest;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; w++) newest = max(newest, (int32_t)per_wave[w][0]);
     const int64_t above_recent = (int64_t)newest - g.recent;
+    const int32_t recent_from = above_recent < INT32_MIN ? INT32_MIN : (int32_t)above_recent + 1;  // recent is at least 0: no overflow
+    const bool no_recent = g.recent == 0;
+    auto image_of = [&](int32_t position, uint32_t mass) { return position < g.first || (position >= recent_from && !no_recent) ? KEPT : rank_image(__uint_as_float(mass)); };
     // Images of the places from `base` on, 0 behind the end.
     auto take_images = [&](uint32_t base, uint32_t *v) {
-        if constexpr (EACH != AHEAD) ahead(base, [&](uint32_t u, int64_t at) { its[u] = g.history.positions[at], masses[u] = g.history.mass[at]; });
+        if constexpr (EACH != AHEAD) ahead(base, [&](uint32_t u, int64_t at) { positions[u] = g.history.positions[at], masses[u] = __float_as_uint(g.history.mass[at]); });
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; u++)
-            v[u] = base + 64 * u + lane >= to ? 0 : its[u] < g.first || its[u] > above_recent ? KEPT : rank_image(masses[u]);
+        for (uint32_t u = 0; u < AHEAD; u++) v[u] = base + 64 * u + lane < to ? image_of(positions[u], masses[u]) : 0;
     };
-    uint32_t kept = 0;  // how many stay for their position
     uint32_t images[EACH ? EACH : 1];
     if constexpr (EACH != 0) {
 #pragma unroll
         for (uint32_t i = 0; i < EACH; i += AHEAD) {
             if (EACH > AHEAD && from + 64 * i >= to) break;
             take_images(from + 64 * i, images + i);
-#pragma unroll
-            for (uint32_t u = 0; u < AHEAD; u++) kept += (uint32_t)__popcll(__ballot(images[i + u] == KEPT));
         }
-    } else {
-        for (uint32_t base = from; base < to; base += 64 * AHEAD) {
+    }
+    if constexpr (EACH == 0) {
+        for (uint32_t base = from; base < min(to, g.held); base += 64 * AHEAD) {
             uint32_t v[AHEAD];
             take_images(base, v);
 #pragma unroll
-            for (uint32_t u = 0; u < AHEAD; u++) {
+            for (uint32_t u = 0; u < AHEAD; u++)
                 if (base + 64 * u < to && base + 64 * u < g.held) held[base + 64 * u + lane] = v[u];
-                kept += (uint32_t)__popcll(__ballot(v[u] == KEPT));
-            }
         }
     }
     // what(base, v) for every 64 places of the run in order: this lane's image, 0 behind the end.
@@ -175,38 +164,35 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
             }
         }
     };
-    kept = all_waves(kept, [](uint32_t a, uint32_t b) { return a + b; });
 
-    // least: the smallest image that stays; ties: of how many of that image, all where that is exact.
-    uint32_t least = KEPT, ties = g.budget;
-    if (kept < g.budget) {
-        const auto ranked = dev::rank_largest<uint32_t>(rank_lds, g.budget - kept, [&](auto count_in) {
-            each([&](uint32_t base, uint32_t v) {
-                if (base + lane < to && v != KEPT) count_in(v);
-            });
-        });
-        least = ranked.least, ties = ranked.exact ? n : ranked.ties;
-    }
+    // The smallest image that stays, and of how many of it.  The zeros behind the end are among the values: none is larger than any, and they have no place.
+    const auto ranked = dev::rank_largest<uint32_t>(rank_lds, g.budget, [&](auto count_in) { each([&](uint32_t, uint32_t v) { count_in(v); }); });
+    const uint32_t least = ranked.least, ties = ranked.exact ? n : ranked.ties;
 
     // What each run has above `least` and at it, below the budget and from it on: masks of 64 places.
-    auto first_of = [](uint32_t base, uint32_t end) { return base >= end ? 0 : end - base >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << (end - base)) - 1; };
+    auto first_of = [](uint32_t base, uint32_t end) { return base + 64 <= end ? ~(uint64_t)0 : base >= end ? 0 : ((uint64_t)1 << (end - base)) - 1; };
     uint32_t counts[4] = {0, 0, 0, 0};
     each([&](uint32_t base, uint32_t v) {
-        const uint64_t there = first_of(base, to), low = first_of(base, g.budget), over = __ballot(v > least) & there, at = __ballot(v == least) & there;
-        counts[0] += (uint32_t)__popcll(over & low), counts[1] += (uint32_t)__popcll(at & low);
-        counts[2] += (uint32_t)__popcll(over & ~low), counts[3] += (uint32_t)__popcll(at & ~low);
+        const uint64_t over = __ballot(v > least), at = __ballot(v == least) & first_of(base, to);
+        if (base >= g.budget) {  // nearly all of a long sequence
+            counts[2] += (uint32_t)__popcll(over), counts[3] += (uint32_t)__popcll(at);
+        } else {
+            const uint64_t low = first_of(base, g.budget);
+            counts[0] += (uint32_t)__popcll(over & low), counts[1] += (uint32_t)__popcll(at & low);
+            counts[2] += (uint32_t)__popcll(over & ~low), counts[3] += (uint32_t)__popcll(at & ~low);
+        }
     });
-    turn ^= 1;
+    __syncthreads();
     if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) per_wave[turn][wave][i] = counts[i];
+        for (int i = 0; i < 4; i++) per_wave[wave][i] = counts[i];
     }
     __syncthreads();
     // What the runs in front leave: ties already kept, holes and movers already listed.
     uint32_t tied = 0, holes = 0, movers = 0;
     for (uint32_t w = 0; w < wave; w++) {
         const uint32_t start = min(w * run, n), end = min(start + run, n), lows = min(end, g.budget) - min(start, g.budget);
-        const uint32_t *of = per_wave[turn][w], left = ties - tied, stay_low = min(of[1], left), stay_high = min(of[3], left - stay_low);
+        const uint32_t *of = per_wave[w], left = ties - tied, stay_low = min(of[1], left), stay_high = min(of[3], left - stay_low);
         holes += lows - of[0] - stay_low;
         movers += of[2] + stay_high;
         tied += stay_low + stay_high;
@@ -218,14 +204,18 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
         if ((mask >> lane & 1) && at < g.most) to_list[list + at] = (int32_t)(base + lane);
     };
     each([&](uint32_t base, uint32_t v) {
-        const uint64_t there = first_of(base, to), low = first_of(base, g.budget), at = __ballot(v == least) & there;
-        uint64_t stay = __ballot(v > least) & there;
+        uint64_t stay = __ballot(v > least);
+        const uint64_t at = __ballot(v == least) & first_of(base, to);
         if (at) {
             stay |= __ballot((at >> lane & 1) && tied + (uint32_t)__popcll(at & before) < ties);
             tied += (uint32_t)__popcll(at);
         }
-        const uint64_t hole = there & low & ~stay, mover = stay & ~low;
-        if (hole) put(g.targets, hole, holes, base), holes += (uint32_t)__popcll(hole);
+        uint64_t mover = stay;
+        if (base < g.budget) {
+            const uint64_t low = first_of(base, g.budget), hole = low & first_of(base, to) & ~stay;
+            mover &= ~low;
+            if (hole) put(g.targets, hole, holes, base), holes += (uint32_t)__popcll(hole);
+        }
         if (mover) put(g.sources, mover, movers, base), movers += (uint32_t)__popcll(mover);
     });
     if (tid == THREADS - 64) *count = (int32_t)min(movers, g.most);  // the last run's: all of them
