@@ -18,6 +18,7 @@ typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t BLOCK = 256, WAVES = BLOCK / 64;
 constexpr uint32_t HELD = 8192;      // images of pages in LDS
+constexpr uint32_t LISTED = 16384;   // chosen pages in LDS, of a row that has more
 constexpr uint32_t SCORED = 64;      // pages of a block that does nothing but score a row
 constexpr uint32_t SCORED_ROWS = 8, ROW_PAGES = 256;  // rows and pages of one that scores several
 constexpr uint32_t MOST_CHANNELS = 256;
@@ -394,13 +395,18 @@ struct SparsePlan {
     bool split, by_rows;                     // scores by a launch of their own, for rows next to each other at once
 };
 
+// No sequence of the call has more.
+uint64_t most_pages(const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
+    const size_t held = (size_t)batch.table_pages * (size_t)cache.page_size, max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
+    return (max_keys + cache.page_size - 1) / cache.page_size;
+}
+
 SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend, const ahip_kv_sparse &sparse) {
     SparsePlan p = {};
     p.batch = {(int32_t)attend.tokens, sparse.most, (int64_t)sparse.most * cache.kv_heads, nullptr, nullptr, nullptr};
     p.attend = attend;
     p.attend.max_tokens = 1, p.attend.max_keys = 0;
-    const size_t held = (size_t)batch.table_pages * (size_t)cache.page_size, max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
-    p.max_pages = (max_keys + cache.page_size - 1) / cache.page_size;
+    p.max_pages = most_pages(cache, batch, attend);
     p.rows = attend.tokens * (uint64_t)cache.kv_heads;
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
     // A block that chooses makes its scores itself where there are blocks for all CUs, or few pages: 48 tokens of up to 500 pages, 4 heads of keys, 66 us
@@ -431,6 +437,8 @@ int check_sparse(DeviceCtx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
         return kv_fail(ctx, AHIP_ERR_ARG, name + "the first and the last pages, one of those at least, fit into what is chosen");
     if ((int64_t)sparse->most * cache->page_size > INT32_MAX - (1 << 16) || attend->tokens * (uint64_t)cache->kv_heads >= MOST_GRID / 2)
         return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more chosen keys, or rows, than are supported");
+    if (sparse->most > (int32_t)LISTED && (uint64_t)sparse->most < most_pages(*cache, *batch, *attend))
+        return kv_fail(ctx, AHIP_ERR_UNSUPPORTED, name + "more than " + std::to_string(LISTED) + " pages chosen of more");
     return check_means(ctx, name, *cache, *sparse);
 }
 

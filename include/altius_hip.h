@@ -484,7 +484,7 @@ typedef struct ahip_kv_history {
  *     mass = decay * mass + the sum of the softmax's weights over the sequence's rows and the head's group of query heads,
  * where the rows' own slots start from 0, and so do all where decay is 0: what was there is not read then.  positions (if not NULL) of the rows'
  * own slots become row_positions[row], or their place where that is NULL.  decay from 0 to 1.  The weights are added in the same order in
- * every call.  No two sequences of a call may share pages. */
+ * every call.  No two sequences of a call may share pages, and calls that run at the same time need a workspace each. */
 int ahip_kv_attention_mass_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
                                      size_t *bytes);
 int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
@@ -494,8 +494,10 @@ int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip
  * the `recent` newest (above the largest less `recent`), then those with the largest mass; of equal ones the lowest place.  NaN counts as
  * less than all else.  The i-th place from `budget` on that stays is sources[i], the i-th place below it that does not is targets[i], for i <
  * counts; behind that the lists stay as they were.  ahip_kv_move with these lists (apart) leaves what stays in the first `budget` places, in no order
- * of positions.  lengths[s] becomes min(length, budget); it may be the batch's own array (one launch more).  Lists of sequence s and head h start at (s * kv_heads + h) * most, counts at
- * s * kv_heads + h.  Of the batch, query_starts is not read (it may be NULL); of the cache, neither keys nor values. */
+ * of positions.  lengths[s] becomes min(length, budget); it may be the batch's own array (one launch more) but not overlap it otherwise.  Lists of sequence s and
+ * head h start at (s * kv_heads + h) * most, counts at s * kv_heads + h.  Of the batch, query_starts is not read (it may be NULL); of the cache, neither keys
+ * nor values.  A sequence that is longer than max_keys or its table has no moves and its new length is not written, the lists of one with a page
+ * outside the cache mean nothing, and the next ahip_sync fails. */
 typedef struct ahip_kv_eviction {
     int32_t budget, recent, first; /* recent + first up to the budget */
     int32_t most;                  /* no list is longer: at least min(budget, max_keys - budget) */
@@ -509,7 +511,8 @@ int ahip_kv_evict(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch
  * sources[at + i] to targets[at + i] for i < counts[s * count_strides[0] + h * count_strides[1]], at = s * strides[0] + h * strides[1]: a
  * head stride of 0 is one list for all heads.  apart: no place of a list is both a source and a target, and all moves are made at once.  Otherwise
  * they are made in order, and none may read a place that an earlier one wrote (its value is either's then), as in the accepted branch of
- * a tree that goes to the front.  No two targets of a list may be the same.  Of the batch, only sequences and the page table are read.  A place
+ * a tree that goes to the front.  No two targets of a call may be the same slot, and no source
+ * of one list the target of another: sequences that share a page move nothing in it.  Of the batch, only sequences and the page table are read.  A place
  * outside the table or a page outside the cache is left out, a count outside 0 .. most moves nothing, and the next ahip_sync fails. */
 typedef struct ahip_kv_moves {
     const int32_t *sources, *targets, *counts; /* device */
@@ -523,9 +526,10 @@ int ahip_kv_move(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch 
  * the largest score, of equal ones the lowest page.  A page's score is the largest product of a query of the head's group with the mean of the
  * page's keys, in 64 bits, NaN counting as less than all else; that mean, of head_size values at page * page_stride + head * head_stride, is held
  * in 32 bits.  The call writes the means of the pages that its rows fill, before they are used; those filled earlier have to be there, from
- * earlier calls or from ahip_kv_page_means.  chosen becomes, at (row * kv_heads + head) * most, the pages in ascending order with -1 behind them; rows
- * that see none, and none of the rows that are padding, are written all -1 and left as they were.  attend: causal, no window, slopes, prefix or
- * first_keys (AHIP_ERR_UNSUPPORTED). */
+ * earlier calls or from ahip_kv_page_means.  chosen becomes, at (row * kv_heads + head) * most, the pages in ascending order with -1 behind them; a row
+ * that stands in front of its sequence's first place has -1 only, and padding is left as it was.  attend: causal, no window, slopes, prefix or
+ * first_keys, and up to 16384 pages are chosen where sequences may have more (AHIP_ERR_UNSUPPORTED).  Calls that run at the same time need a workspace
+ * each; the memory of the pages that a call's rows fill, and their means, belong to one sequence. */
 typedef struct ahip_kv_sparse {
     float *means;
     int64_t page_stride, head_stride;

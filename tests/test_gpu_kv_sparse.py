@@ -102,6 +102,8 @@ SHAPES = [  # n, lengths, heads, kv heads, d, page, type, order, most, first, la
     ([1, 1], [640, 640], 4, 1, 64, 64, "f32", "head", 4, 0, 4),
     ([1], [700], 7, 1, 64, 250, "f32", "slot", 2, 1, 1),
     ([1], [20000], 4, 1, 64, 1, "f32", "head", 64, 4, 8),
+    ([1], [9000], 2, 1, 64, 1, "f32", "head", 8700, 4, 8),
+    ([1, 2], [17000, 20], 1, 1, 8, 1, "bf16", "slot", 16384, 0, 3),
 ]
 
 
