@@ -269,7 +269,9 @@ template <int DP, bool BF16> struct RowTile {
 
 // Row of O^T (channel) of accumulator i, register r, in lane group `part` = lane / 16.
 template <int DP, bool BF16> __device__ __forceinline__ uint32_t channel_of(int i, int r, uint32_t part) {
-    return BF16 ? (DP / 16) * (4 * part + r) + i : 64 * (i / 4) + 4 * (4 * part + r) + i % 4;
+    if constexpr (BF16) return (DP / 16) * (4 * part + r) + i;
+    const int words = DP / 16 - i / 4 * 4 < 4 ? DP / 16 % 4 : 4;  // of a lane, of these 64 channels
+    return 64 * (i / 4) + words * (4 * part + r) + i % 4;
 }
 
 template <int DP, bool BF16> struct RowLds {
@@ -542,11 +544,15 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     };
 
     // A lane's parts of a tile: of row `col` of the keys 16 bytes at 64 c + 16 part; of row 4 part + r of the values, fp32: 16 bytes at
-    // 256 j + 16 col, bf16: DP / 8 bytes.  No load depends on a condition, which would have the compiler wait for those before it:
+    // 256 j + 16 col and behind the last whole 64 channels as many words as there are left for 16 lanes, bf16: DP / 8 bytes.  No load depends on a condition, which would have the compiler wait for those before it:
     // channels that a head does not have are read as others (their queries are 0, their sums go nowhere).
     typedef RowTile<DP, BF16> Tile;
     const uint32_t row_bytes = g.d * SIZE;
     constexpr uint32_t V_STEP = BF16 ? DP / 8 : 16;
+    // Lanes without channels of their own read the first ones.
+    const uint32_t k_byte = 16 * part < row_bytes ? 16 * part : 0, v_byte = V_STEP * col < row_bytes ? V_STEP * col : 0;
+    constexpr int LEFT = BF16 ? 0 : DP / 16 % 4;
+    static_assert(LEFT == 0 || LEFT == 1 || LEFT == 2, "aligned words");
     auto load_parts = [&](Tile &t, auto whole, const char *k_row, auto v_row) {
         constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
@@ -569,11 +575,20 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
 #pragma unroll
                     for (int e = 0; e < 4; e++) t.v[r][4 * w + e] = x[e];
                 }
+                if constexpr (LEFT != 0) {
+                    typedef uint32_t Left __attribute__((ext_vector_type(LEFT == 1 ? 2 : LEFT)));
+                    constexpr uint32_t AT = 64 * (DP / 64);
+                    const char *at = p - v_byte + (WHOLE || AT + LEFT * col < g.d ? 4 * (AT + LEFT * col) : 0);
+                    if constexpr (LEFT == 1) t.v[r][AT / 16] = *reinterpret_cast<const uint32_t *>(at);
+                    else {
+                        const Left x = *reinterpret_cast<const Left *>(at);
+#pragma unroll
+                        for (int e = 0; e < LEFT; e++) t.v[r][AT / 16 + e] = x[e];
+                    }
+                }
             }
         }
     };
-    // Lanes without channels of their own read the first ones.
-    const uint32_t k_byte = 16 * part < row_bytes ? 16 * part : 0, v_byte = V_STEP * col < row_bytes ? V_STEP * col : 0;
     const uint32_t k_off = col * slot_bytes + k_byte, v_off = 4 * part * slot_bytes + v_byte;
     auto load = [&](int32_t i, Tile &t) {
         if constexpr (UNIFORM) {
@@ -770,10 +785,14 @@ __device__ __forceinline__ void piece16(const AttendArgs &g, const Piece &piece,
     if (BF16 || Q_HERE) __syncthreads();
     if (part == 0) stats[wave][0][col] = top, stats[wave][1][col] = total;
 #pragma unroll
-    for (int i = 0; i < NACC; i += 4)
+    for (int i = 0; i + 4 <= NACC; i += 4)
 #pragma unroll
         for (int r = 0; r < 4; r++)
             *reinterpret_cast<f32x4 *>(&sums[wave][col * PITCH + channel_of<DP, BF16>(i, r, part)]) = f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+#pragma unroll
+    for (int i = NACC - LEFT; i < NACC; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sums[wave][col * PITCH + channel_of<DP, BF16>(i, r, part)] = acc[i][r];
     __syncthreads();
 
     for (uint32_t unit = threadIdx.x; unit < 16 * (DP / 4); unit += 64 * ROW_WAVES) {
@@ -1368,17 +1387,21 @@ __device__ __forceinline__ void rows128(const AttendArgs &g, uint32_t id, TileLd
         }
 }
 
+// What few rows are computed with: the fp32 matrix instructions of channels that are not there cost as much as the others.  309 rows of 976 chosen keys, 16 heads
+// of 80 channels, 4 of keys: 95 us, with 128 channels 132.
+template <int DP, bool BF16> constexpr int few_channels() { return DP <= 64 ? 64 : DP <= 96 && !BF16 ? 96 : 128; }
+
 // Prompts, and the sequences of few rows that share a batch with them: the last blocks are the latter's, and end at once where there
 // are none.
 template <int DP, bool BF16, bool UNIFORM, int MODE>
 __global__ __launch_bounds__(256, BF16 || DP == 64 ? 2 : 1) void attend_rows128(AttendArgs g) {
     __shared__ __align__(16) union {
-        RowLds<DP <= 64 ? 64 : 128, BF16> few;
+        RowLds<few_channels<DP, BF16>(), BF16> few;
         TileLds<DP, BF16> many;
     } lds;
     __shared__ TreeLds<MODE == TREE, TILE_ROWS> tree;
     if (blockIdx.x < g.many.blocks) rows128<DP, BF16, UNIFORM, MODE>(g, blockIdx.x, lds.many, tree);
-    else rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true, MODE>(g, blockIdx.x - g.many.blocks, lds.few, tree);
+    else rows16<few_channels<DP, BF16>(), BF16, UNIFORM, true, MODE>(g, blockIdx.x - g.many.blocks, lds.few, tree);
 }
 
 // Joins the splits of a row, of which only those that hold keys that it sees were computed for it.  A group of lanes holds the row's
@@ -1483,9 +1506,9 @@ template <int DP, bool BF16, bool UNIFORM, int MODE> int launch_wide(DeviceCtx &
     hipLaunchKernelGGL((attend_rows16<DP, BF16, UNIFORM, false, MODE>), dim3(g.many.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
     return ctx.check(hipGetLastError(), "kv attention launch");
 }
-template <int DP, bool BF16, bool UNIFORM, int MODE> int launch_tiled(DeviceCtx &ctx, const AttendArgs &g) {
+template <int DP, bool BF16, bool UNIFORM, int MODE, int ROWS_DP = few_channels<DP, BF16>()> int launch_tiled(DeviceCtx &ctx, const AttendArgs &g) {
     if (!g.many.blocks)
-        hipLaunchKernelGGL((attend_rows16<DP <= 64 ? 64 : 128, BF16, UNIFORM, true, MODE>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
+        hipLaunchKernelGGL((attend_rows16<ROWS_DP, BF16, UNIFORM, true, MODE>), dim3(g.few.blocks), dim3(64 * ROW_WAVES), 0, ctx.stream, g);
     else
         hipLaunchKernelGGL((attend_rows128<DP, BF16, UNIFORM, MODE>), dim3(g.few.blocks + g.many.blocks), dim3(256), 0, ctx.stream, g);
     return ctx.check(hipGetLastError(), "kv attention launch");
@@ -1495,6 +1518,9 @@ template <int DP, bool BF16, bool UNIFORM, int MODE> int launch_tiled(DeviceCtx 
 // 46 us, at 128 channels 53 us; of 1024, bf16, 8 heads of keys: 63 and 72 us.
 template <bool BF16, bool UNIFORM, int MODE> int launch_by_size(DeviceCtx &ctx, const AttendArgs &g) {
     if (g.d <= 64) return launch_tiled<64, BF16, UNIFORM, MODE>(ctx, g);
+    if constexpr (!BF16) {
+        if (g.d <= 80) return launch_tiled<96, BF16, UNIFORM, MODE, 80>(ctx, g);
+    }
     if (g.d <= 96) return launch_tiled<96, BF16, UNIFORM, MODE>(ctx, g);
     if (g.d <= TILE_CHANNELS) return launch_tiled<128, BF16, UNIFORM, MODE>(ctx, g);
     return launch_wide<256, BF16, UNIFORM, MODE>(ctx, g);
