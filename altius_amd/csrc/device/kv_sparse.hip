@@ -16,7 +16,8 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t BLOCK = 256, WAVES = BLOCK / 64;
+// LARGE: of a block that makes its scores itself (48 tokens of up to 500 pages, 4 heads of keys: 20.3 us, with 256 threads 23.8; 1024 leave no registers, 63).
+constexpr uint32_t BLOCK = 256, LARGE = 512;
 constexpr uint32_t HELD = 8192;      // images of pages in LDS
 constexpr uint32_t LISTED = 16384;   // chosen pages in LDS, of a row that has more
 constexpr uint32_t SCORED = 64;      // pages of a block that does nothing but score a row
@@ -39,9 +40,9 @@ struct SparseArgs {
 
 // ---------------------------------------------------------------- means
 // The mean of page `page` for one head, by a block: lanes side by side take 4 channels each, groups of lanes the slots in turn; sums in 64 bits, rounded once.
-__device__ __forceinline__ void page_mean(const SparseArgs &g, int32_t page, uint32_t head) {
-    __shared__ double sums[BLOCK][4];
-    const uint32_t lanes = g.d / 4, groups = BLOCK / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+template <uint32_t THREADS> __device__ __forceinline__ void page_mean(const SparseArgs &g, int32_t page, uint32_t head) {
+    __shared__ double sums[THREADS][4];
+    const uint32_t lanes = g.d / 4, groups = THREADS / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
     const int64_t at = (int64_t)page * g.kv.page_stride + (int64_t)head * g.kv.head_stride + 4 * lane;
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
     if (group < groups) {
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(BLOCK) void mean_pages(SparseArgs g) {
     const uint32_t base = (uint32_t)max(0, q.length - q.n), index = g.kv.by_page_size.div(base) + i;
     if ((uint64_t)(index + 1) * g.kv.page_size > (uint32_t)q.length) return;
     const int32_t page = g.kv.page_of(s, index, -1);
-    if (page >= 0) page_mean(g, page, head);
+    if (page >= 0) page_mean<BLOCK>(g, page, head);
 }
 
 // ---------------------------------------------------------------- scores
@@ -107,7 +108,7 @@ template <int CONTROL> __device__ __forceinline__ double larger(double v) {
 // head j is in lane 16 i + 4 b + j.  No sum goes from lane to lane, and 16 pages of 128 channels and 4 heads take 32 instructions; the same with the vector
 // unit, 16 lanes a page, spent more on adding up the lanes than on products (one token, 48 texts, group of 8: 34.5 us, so 26).
 // put(page, score, again): again: the larger of it and what is there.
-template <uint32_t UNITS, int FOURS, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t from, uint32_t to, Put put) {
+template <uint32_t UNITS, int FOURS, uint32_t WAVES, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t from, uint32_t to, Put put) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, k = lane >> 4;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t h0 = 0; h0 < g.group; h0 += 4 * FOURS) {
@@ -195,7 +196,7 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void sc
     if (r.pages <= g.most) return;  // all are chosen
     const uint32_t from = max(chunk * SCORED, g.first), to = min((chunk + 1) * SCORED, r.pages - g.last);
     double *to_scores = g.scores + (size_t)outer * g.max_pages;
-    score_range<UNITS, FOURS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
+    score_range<UNITS, FOURS, BLOCK / 64>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
 }
 
 // The same for SCORED_ROWS rows next to each other, whose queries wait in LDS: rows of one sequence read its means together.  309 rows behind 6001 to 12000 tokens in
@@ -225,7 +226,7 @@ template <uint32_t UNITS> __global__ __launch_bounds__(BLOCK) void score_rows(Sp
                 for (int e = 0; e < 4; e++) queries[its][u][e][4 * its_k + j] = (double)x[e];
             }
             __syncthreads();
-            for (uint32_t base = from + 16 * wave; base < to; base += 16 * WAVES) {
+            for (uint32_t base = from + 16 * wave; base < to; base += BLOCK / 4) {
                 const uint32_t index = base + (lane & 15u);
                 const int32_t page = index < to ? g.kv.page_of(r.s, index, 0) : 0;
                 const float *mean = g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head;
@@ -268,7 +269,8 @@ __device__ __forceinline__ uint64_t rank_image(double score) {
 }
 
 // A block for each row and head of keys: the smallest image that is chosen (kv_rank.h), equal ones by their number, then the pages in order.
-template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void choose_pages(SparseArgs g) {
+template <uint32_t UNITS, int FOURS, uint32_t THREADS> __global__ __launch_bounds__(THREADS) void choose_pages(SparseArgs g) {
+    constexpr uint32_t WAVES = THREADS / 64;
     extern __shared__ uint64_t images[];
     __shared__ uint32_t totals[2][WAVES][2];
     __shared__ dev::RankLds rank_lds;
@@ -277,7 +279,7 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     const Row r = row_of(g, row);
     if (blockIdx.x >= rows) {  // where rows fill pages for later calls: beside the choice (behind it, one token of 1024 pages takes 5 us more)
         const int32_t page = r.pages && r.place + 1 == r.pages * g.kv.page_size ? g.kv.page_of(r.s, r.pages - 1, -1) : -1;
-        if (page >= 0) page_mean(g, page, head);
+        if (page >= 0) page_mean<THREADS>(g, page, head);
         return;
     }
     const int32_t first_row = g.kv.starts[0], end_row = g.kv.starts[g.kv.sequences];
@@ -293,13 +295,13 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     const size_t list = ((size_t)row * g.kv.kv_heads + head) * g.most;
     const uint32_t count = min(r.pages, g.most);
     if (head == 0 && tid == 0) g.lengths[row] = count ? (int32_t)((count - 1) * g.kv.page_size + (r.place - (r.pages - 1) * g.kv.page_size) + 1) : 0;
-    for (uint32_t i = count + tid; i < g.most; i += BLOCK) g.chosen[list + i] = -1;
+    for (uint32_t i = count + tid; i < g.most; i += THREADS) g.chosen[list + i] = -1;
     auto put = [&](uint32_t at, uint32_t page) {
         g.chosen[list + at] = (int32_t)page;
         g.table[list + at] = g.kv.page_of(r.s, page, -1);
     };
     if (r.pages <= g.most) {
-        for (uint32_t i = tid; i < count; i += BLOCK) put(i, i);
+        for (uint32_t i = tid; i < count; i += THREADS) put(i, i);
         return;
     }
     uint32_t *const in_order = reinterpret_cast<uint32_t *>(images + g.held);  // g.most of them
@@ -308,19 +310,19 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     const double *scores = UNITS ? nullptr : g.scores + ((size_t)row * g.kv.kv_heads + head) * g.max_pages;
     if constexpr (UNITS != 0) {
         if (want)
-            score_range<UNITS, FOURS>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) {
+            score_range<UNITS, FOURS, WAVES>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) {
                 const uint64_t v = rank_image(score);
                 images[page] = again ? max(images[page], v) : v;
             });
     } else {
         const uint32_t end = min(to, g.held);
-        for (uint32_t base = from + tid; base < end; base += 4 * BLOCK) {  // four loads on their way at once
+        for (uint32_t base = from + tid; base < end; base += 4 * THREADS) {  // four loads on their way at once
             double v[4];
 #pragma unroll
-            for (uint32_t u = 0; u < 4; u++) v[u] = scores[min(base + u * BLOCK, end - 1)];
+            for (uint32_t u = 0; u < 4; u++) v[u] = scores[min(base + u * THREADS, end - 1)];
 #pragma unroll
             for (uint32_t u = 0; u < 4; u++)
-                if (base + u * BLOCK < end) images[base + u * BLOCK] = rank_image(v[u]);
+                if (base + u * THREADS < end) images[base + u * THREADS] = rank_image(v[u]);
         }
     }
     __syncthreads();
@@ -329,14 +331,14 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     dev::Ranked<uint64_t> ranked = {0, 0, true};
     if (want)
         ranked = dev::rank_largest<uint64_t>(rank_lds, want, [&](auto count_in) {
-            for (uint32_t page = from + tid; page < to; page += BLOCK) count_in(image(page));
+            for (uint32_t page = from + tid; page < to; page += THREADS) count_in(image(page));
         });
     const uint64_t least = ranked.least;
     const bool exact = ranked.exact;
     const uint32_t ties = ranked.ties;
     uint32_t listed = 0, tied = 0;
     const uint64_t before = ((uint64_t)1 << lane) - 1;
-    for (uint32_t base = 0, turn = 0; base < r.pages; base += BLOCK, turn ^= 1) {
+    for (uint32_t base = 0, turn = 0; base < r.pages; base += THREADS, turn ^= 1) {
         const uint32_t page = base + tid;
         const bool there = page < r.pages, always = there && (page < from || page >= to);
         const uint64_t v = there && !always && want ? image(page) : 0;
@@ -367,7 +369,7 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void ch
     }
     // Their places in the cache are looked up together, not as each is found.
     __syncthreads();
-    for (uint32_t i = tid; i < g.most; i += BLOCK) put(i, in_order[i]);
+    for (uint32_t i = tid; i < g.most; i += THREADS) put(i, in_order[i]);
 }
 
 // ---------------------------------------------------------------- the host's part
@@ -409,7 +411,7 @@ SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const a
     p.max_pages = most_pages(cache, batch, attend);
     p.rows = attend.tokens * (uint64_t)cache.kv_heads;
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
-    // A block that chooses makes its scores itself where there are blocks for all CUs, or few pages: 48 tokens of up to 500 pages, 4 heads of keys, 66 us
+    // A block that chooses makes its scores itself where there are blocks for all CUs, or few pages: 48 tokens of up to 500 pages, 4 heads of keys, 61 us
     // with their attention, 76 by launches of their own; one token of 1024 pages, 8 heads, 50 us and 31.
     p.split = p.max_pages > HELD || (p.rows < cus && p.max_pages > 8 * SCORED);
     // Rows of one sequence read its means together, as far as their scores fit into SCORES bytes.
@@ -448,12 +450,12 @@ template <uint32_t UNITS, int FOURS> void launch_choice(hipStream_t stream, cons
     const uint32_t held = (uint32_t)(g.held * sizeof(uint64_t) + (g.most < g.max_pages ? g.most * sizeof(uint32_t) : 0));
     if (p.by_rows) {
         hipLaunchKernelGGL((score_rows<UNITS>), dim3((uint32_t)p.score_blocks), block, 0, stream, g);
-        hipLaunchKernelGGL((choose_pages<0, 1>), grid, block, held, stream, g);
+        hipLaunchKernelGGL((choose_pages<0, 1, BLOCK>), grid, block, held, stream, g);
     } else if (p.split) {
         hipLaunchKernelGGL((score_pages<UNITS, FOURS>), dim3((uint32_t)p.score_blocks), block, 0, stream, g);
-        hipLaunchKernelGGL((choose_pages<0, 1>), grid, block, held, stream, g);
+        hipLaunchKernelGGL((choose_pages<0, 1, BLOCK>), grid, block, held, stream, g);
     } else {
-        hipLaunchKernelGGL((choose_pages<UNITS, FOURS>), grid, block, held, stream, g);
+        hipLaunchKernelGGL((choose_pages<UNITS, FOURS, LARGE>), grid, dim3(LARGE), held, stream, g);
     }
 }
 
