@@ -21,7 +21,7 @@ constexpr uint32_t BLOCK = 256, LARGE = 512;
 constexpr uint32_t HELD = 8192;      // images of pages in LDS
 constexpr uint32_t LISTED = 16384;   // chosen pages in LDS, of a row that has more
 constexpr uint32_t SCORED = 64;      // pages of a block that does nothing but score a row
-constexpr uint32_t SCORED_ROWS = 8, ROW_PAGES = 256;  // rows and pages of one that scores several
+constexpr uint32_t SCORED_ROWS = 8, ROW_PAGES = 128;  // rows and pages of one that scores several
 constexpr uint32_t MOST_CHANNELS = 256;
 
 struct SparseArgs {
@@ -200,7 +200,7 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void sc
 }
 
 // The same for SCORED_ROWS rows next to each other, whose queries wait in LDS: rows of one sequence read its means together.  309 rows behind 6001 to 12000 tokens in
-// pages of 16, 4 heads of keys of 80 channels: 39 us with the choice; each row by itself, in the block that chooses, 52.
+// pages of 16, 4 heads of keys of 80 channels: 34 us with the choice (128 pages a block; 256 leave CUs idle, 39); each row by itself, in the block that chooses, 52.
 template <uint32_t UNITS> __global__ __launch_bounds__(BLOCK) void score_rows(SparseArgs g) {
     __shared__ double queries[SCORED_ROWS][UNITS][4][16];  // [row][u][e][4 k + j]: of channel 16 u + 4 k + e and head j
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = lane >> 4;
