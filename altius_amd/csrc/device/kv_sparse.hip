@@ -2,6 +2,9 @@
 // row and head of keys, and attention (kv_attend.h) over those, each row being a sequence of its own with a page table of its own for each head.
 //   Scores are sums of products of fp32 values in 64 bits, where no product is rounded: two pages change places only if their scores agree to about 2^-50,
 // whatever order the sums are made in.
+//   One token behind 65535 (32 of 1024 pages of 64, 32 heads, 8 of keys, 128 channels, fp32) 31 us, bound by the chains of four launches; 48 behind 100 to 16000 (40
+// pages of 32, 4 heads of keys, bf16) 61 us, 35 of them attention at 3.6 TB/s; 309 rows behind 6001 to 12000 (61 pages of 16, 16 heads, 4 of keys of 80 channels,
+// fp32) 127 us, 95 of them attention, each row's pages for itself, 8 TB/s out of the caches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -1,7 +1,7 @@
 // Attention of trees of drafted tokens over a paged cache: the kernels of kv_attend.h, with a mask of a row's own tree beside its range of keys.
 // The tree costs a load of the parents and the walk up at a block's start, and a look at the mask in the last one or two tiles of a sequence: 8 tokens behind 500 (12
-// heads of 64 channels, fp32) 14.0 us, as a piece 12.6.  16 trees of 16 to 48 tokens behind 300 to 8000 (bf16, 32 heads, 8 of keys, 128 channels) 173 us, 188
-// TFLOP/s; 2 of 40 to 61 behind 20011 to 30000 (fp32, 16 heads, 4 of keys, 96 channels, biased) 190 us, 78.  Bound by rows of the blocks of 128 that are not there (a
+// heads of 64 channels, fp32) 14.0 us, as a piece 12.6.  16 trees of 16 to 48 tokens behind 300 to 8000 (bf16, 32 heads, 8 of keys, 128 channels) 172 us, 189
+// TFLOP/s; 2 of 40 to 61 behind 20011 to 30000 (fp32, 16 heads, 4 of keys, 96 channels, biased) 183 us, 81.  Bound by rows of the blocks of 128 that are not there (a
 // third) and by what bounds rows128.
 #include <hip/hip_runtime.h>
 
