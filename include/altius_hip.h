@@ -484,7 +484,8 @@ typedef struct ahip_kv_history {
  *     mass = decay * mass + the sum of the softmax's weights over the sequence's rows and the head's group of query heads,
  * where the rows' own slots start from 0, and so do all where decay is 0: what was there is not read then.  positions (if not NULL) of the rows'
  * own slots become row_positions[row], or their place where that is NULL.  decay from 0 to 1.  The weights are added in the same order in
- * every call.  No two sequences of a call may share pages, and calls that run at the same time need a workspace each. */
+ * every call.  No two sequences of a call may share pages, the pages of all slots have to be there, also of those that no row sees, and calls that
+ * run at the same time need a workspace each. */
 int ahip_kv_attention_mass_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
                                      size_t *bytes);
 int ahip_kv_attention_mass(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,
@@ -526,7 +527,7 @@ int ahip_kv_move(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch 
  * the largest score, of equal ones the lowest page.  A page's score is the largest product of a query of the head's group with the mean of the
  * page's keys, in 64 bits, NaN counting as less than all else; that mean, of head_size values at page * page_stride + head * head_stride, is held
  * in 32 bits.  The call writes the means of the pages that its rows fill, before they are used; those filled earlier have to be there, from
- * earlier calls or from ahip_kv_page_means.  chosen becomes, at (row * kv_heads + head) * most, the pages in ascending order with -1 behind them; a row
+ * earlier calls or from ahip_kv_page_means; a slot that moves does not change them.  chosen becomes, at (row * kv_heads + head) * most, the pages in ascending order with -1 behind them; a row
  * that stands in front of its sequence's first place has -1 only, and padding is left as it was.  attend: causal, no window, slopes, prefix or
  * first_keys, and up to 16384 pages are chosen where sequences may have more (AHIP_ERR_UNSUPPORTED).  Calls that run at the same time need a workspace
  * each; the memory of the pages that a call's rows fill, and their means, belong to one sequence. */

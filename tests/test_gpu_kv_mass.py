@@ -18,7 +18,7 @@ class Mass:
     """The history of a cache (masses spread over ten powers of two, positions -3 where nothing was written) and one call."""
 
     def __init__(self, ctx, paged, q, rng, decay=1.0, own_positions=True, max_tokens=0, max_keys=0, causal=True, window=0, cap=0.0, slopes=None, prefix=None, first=None, scale=None):
-        self.paged, self.decay = paged, decay
+        self.paged, self.q, self.decay = paged, q, decay
         shape = (paged.pages, paged.kv_heads, paged.page)
         self.before = np.exp2(10 * rng.random(shape) - 5).astype(np.float32)
         self.mass, self.positions = gpu(self.before), torch.full(shape, -3, device="cuda", dtype=torch.int32)
@@ -96,6 +96,8 @@ SHAPES = [  # n, lengths, heads, kv heads, d, page, type, order
     ([257], [400], 8, 1, 128, 250, "f32", "slot"),
     ([600], [600], 4, 1, 64, 16, "bf16", "head"),
     ([70], [90], 2, 2, 200, 32, "f32", "head"),
+    ([5, 40, 1], [3, 25, 0], 4, 2, 64, 16, "f32", "slot"),
+    ([300, 2], [280, 1], 8, 2, 128, 16, "bf16", "head"),
 ]
 
 

@@ -153,3 +153,29 @@ def test_two_calls_at_once(here, case):  # noqa: F811
         mass.decay = 0.0
         held_to_masses(mass, q)
         held_to_choice(sparse, q)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+def test_means_of_pages_that_moved_slots_fill(here, case, elem):  # noqa: F811
+    """Accepted tokens of a tree go to the front and fill a page: its mean is made with them as the newest rows, and the next token chooses by it."""
+    case(f"means behind moves {elem}")
+    rng = np.random.default_rng(92)
+    paged = Paged(rng, [12], [62], 2, 64, 8, elem)
+    sources, targets, count = (gpu(np.array(x, np.int32)) for x in ([50, 52, 55, 56, 58, 61], range(50, 56), [6]))
+    torch.cuda.synchronize()
+    here.kv_move_raw(paged.cache(), paged.batch(), D.KvMoves(sources=sources.data_ptr(), targets=targets.data_ptr(), counts=count.data_ptr(), strides=(6, 0), count_strides=(1, 0), most=6))
+    here.sync()
+    q = rng.standard_normal((1, 8, 64)).astype(np.float32)
+    paged.n, paged.lengths = [1], [57]
+    got = Sparse(here, paged, gpu(q), 4, 1, 1)
+    got.means[int(paged.table[0, 6])] = math.nan
+    for n, length in ((6, 56), (1, 57)):
+        paged.starts_on, paged.lengths_on = gpu(np.array([0, n], np.int32)), gpu(np.array([length], np.int32))
+        torch.cuda.synchronize()
+        if n == 6:
+            here.kv_page_means_raw(paged.cache(), paged.batch(), got.sparse, 6)
+            here.sync()
+        else:
+            got.run(here)
+    here.sync()
+    held_to_choice(got, q)

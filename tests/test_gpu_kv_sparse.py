@@ -24,7 +24,7 @@ class Sparse:
     """The means (NaN where a page is not full yet), the list of chosen pages and the call."""
 
     def __init__(self, ctx, paged, q, most, first=0, last=1, cap=0.0, max_tokens=0, max_keys=0, scale=None):
-        self.paged, self.most, self.first, self.last = paged, most, first, last
+        self.paged, self.q, self.most, self.first, self.last = paged, q, most, first, last
         self.scale, self.cap = scale if scale is not None else 1 / math.sqrt(paged.d), cap
         self.means = torch.full((paged.pages, paged.kv_heads, paged.d), math.nan, device="cuda")
         full = page_means(paged)
