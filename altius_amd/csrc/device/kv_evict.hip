@@ -23,8 +23,9 @@ struct History {
 // A block for each sequence and head of keys, a wavefront for each run of places.  Masses become an order-preserving image of 32 bits; the smallest that
 // stays is found among them (kv_rank.h), then the runs are counted and listed in order.
 //   Up to 2048 places 256 threads hold 8 images each.  48 sequences of 1025 places, 8 heads: 7.9 us.
-//   Up to 57344 places 1024 threads hold 56.  4 sequences of 20011 to 50000 places: 62 us, bound by the vector unit of one CU a block and the latency of its
-// walks over the places.  Beyond, images wait in LDS as far as that goes, and what is behind is read anew, out of L2: 103 us with the same lengths.
+//   Up to 57344 places 1024 threads hold 56.  4 sequences of 20011 to 50000 places: 55 us, bound by the latency of one block's walks over the places, a CU
+// each.  Beyond, images wait in LDS as far as that goes, and what is behind is read anew, out of L2: 103 us with the same lengths and
+// one row of bins.
 constexpr uint32_t HELD = 28672, PAGES = 4096, SMALL = 256, SMALL_EACH = 8, LARGE = 1024, LARGE_EACH = 56;
 constexpr uint32_t KEPT = 0xffffffffu;  // by its position; above every mass
 
@@ -50,7 +51,7 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
     extern __shared__ uint32_t held[];
     __shared__ int64_t page_starts[STARTS ? PAGES : 1];
     __shared__ uint32_t per_wave[WAVES][4];
-    __shared__ dev::RankLds rank_lds;
+    __shared__ dev::RankLds<EACH == SMALL_EACH ? 1 : 8> rank_lds;  // 50000 masses in one row of bins: 62 us; in 8: 55; 1025 have none to wait for
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t s = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - s * g.kv.kv_heads;
     const int32_t length = g.kv.lengths[s];
@@ -101,7 +102,7 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
         ahead(from, [&](uint32_t u, int64_t at) { positions[u] = g.history.positions[at], masses[u] = __float_as_uint(g.history.mass[at]); });
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; u++) newest = max(newest, positions[u]);
-    } else {  // (56 positions a thread beside as many images leave no registers: 69 us instead of 62)
+    } else {  // (56 positions a thread beside as many images leave no registers: 69 us instead of 62, with one row of bins)
         for (uint32_t base = from; base < to; base += 64 * AHEAD) {
             ahead(base, [&](uint32_t u, int64_t at) { positions[u] = g.history.positions[at]; });
 #pragma unroll

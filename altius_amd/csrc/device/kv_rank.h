@@ -19,8 +19,9 @@ __device__ __forceinline__ uint32_t lanes_up_to(uint32_t v) {
     return plus_moved<0x143, 0xC>(v);  // row_bcast 31: lane 31 to the upper half
 }
 
-struct RankLds {
-    uint32_t bins[256], totals[4], found[3];
+// COPIES: bins of some lanes' own, in other banks.  Values share few first bytes, and lanes that count the same one wait for each other.
+template <uint32_t COPIES> struct RankLds {
+    uint32_t bins[COPIES][256 + 32 / COPIES], totals[4], found[3];
 };
 template <class Image> struct Ranked {
     Image least;    // all above it are among the largest
@@ -30,21 +31,23 @@ template <class Image> struct Ranked {
 // each(f) calls f with every value of the calling thread; of all threads' there are more than `want`, which is at least 1.  A byte at a time, from the top: a
 // histogram in LDS of the values that share the bytes so far, and the bin that the rank falls into, until all of a bin are wanted.  For whole blocks of 256
 // threads or more; lds must not be in use.
-template <class Image, class Each> __device__ __forceinline__ Ranked<Image> rank_largest(RankLds &lds, uint32_t want, Each each) {
+template <class Image, uint32_t COPIES, class Each> __device__ __forceinline__ Ranked<Image> rank_largest(RankLds<COPIES> &lds, uint32_t want, Each each) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (tid < 256) lds.bins[tid] = 0;
+    if (tid < 256)
+#pragma unroll
+        for (uint32_t i = 0; i < COPIES; i++) lds.bins[i][tid] = 0;
     __syncthreads();
     Ranked<Image> r = {0, want, false};
     for (int shift = 8 * (int)sizeof(Image) - 8; shift >= 0; shift -= 8) {
         const Image known = shift == 8 * (int)sizeof(Image) - 8 ? 0 : ~(Image)0 << (shift + 8);
         each([&](Image v) {
-            if ((v & known) == r.least) atomicAdd(&lds.bins[(uint32_t)(v >> shift) & 255u], 1u);
+            if ((v & known) == r.least) atomicAdd(&lds.bins[lane % COPIES][(uint32_t)(v >> shift) & 255u], 1u);
         });
         __syncthreads();
         uint32_t count = 0, up_to = 0;
         if (tid < 256) {  // the largest first
-            count = lds.bins[255 - tid];
-            lds.bins[255 - tid] = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < COPIES; i++) count += lds.bins[i][255 - tid], lds.bins[i][255 - tid] = 0;
             up_to = lanes_up_to(count);
             if (lane == 63) lds.totals[wave] = up_to;
         }

@@ -276,7 +276,7 @@ template <uint32_t UNITS, int FOURS, uint32_t THREADS> __global__ __launch_bound
     constexpr uint32_t WAVES = THREADS / 64;
     extern __shared__ uint64_t images[];
     __shared__ uint32_t totals[2][WAVES][2];
-    __shared__ dev::RankLds rank_lds;
+    __shared__ dev::RankLds<1> rank_lds;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t rows = g.kv.tokens * g.kv.kv_heads, id = blockIdx.x < rows ? blockIdx.x : blockIdx.x - rows, row = id / g.kv.kv_heads, head = id - row * g.kv.kv_heads;
     const Row r = row_of(g, row);
