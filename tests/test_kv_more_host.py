@@ -1,6 +1,9 @@
-"""The host side of the operators around a paged cache, no GPU needed: the workspaces that they want, what they refuse, and the sizes of their structures."""
+"""The host side of the operators around a paged cache, no GPU needed: the workspaces that they want, what they refuse, and their structures as the header has them."""
 import ctypes
 import math
+import os
+import shutil
+import subprocess
 
 import pytest
 
@@ -109,3 +112,15 @@ def test_the_workspace_of_attention_is_enough_for_trees():
     """Whose keys are cut where a piece's are not: 16 of up to 48 tokens behind up to 7952."""
     trees = {"cache.elem": D.KV_BF16, "batch.sequences": 16, "batch.table_pages": 500, "batch.table_stride": 500, "attend.tokens": 16 * 48, "attend.max_tokens": 48}
     assert plain_workspace(**trees) > plain_workspace(**{**trees, "attend.causal": 0})
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="no C compiler")
+def test_structures_are_the_headers(tmp_path):
+    kinds = {"ahip_kv_history": D.KvHistory, "ahip_kv_eviction": D.KvEviction, "ahip_kv_moves": D.KvMoves, "ahip_kv_sparse": D.KvSparse}
+    lines = [f'printf("%zu\\n", sizeof({c}));' + "".join(f' printf("%zu\\n", offsetof({c}, {f[0]}));' for f in kind._fields_) for c, kind in kinds.items()]
+    source = tmp_path / "sizes.c"
+    source.write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"altius_hip.h\"\nint main(void) {\n" + "\n".join(lines) + "\nreturn 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-std=c11", "-I", include, str(source), "-o", str(tmp_path / "sizes")], check=True)
+    told = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split()]
+    assert told == [x for kind in kinds.values() for x in [ctypes.sizeof(kind)] + [getattr(kind, f[0]).offset for f in kind._fields_]]
