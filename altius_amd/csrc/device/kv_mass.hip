@@ -7,8 +7,9 @@
 //   Sequences of few rows (16 a block in attention) are bound by the memory that keys come from: attention leaves their scores in the workspace, 4 bytes a row
 // where a key has hundreds, and a launch over the keys adds them up.  24 tokens behind 1000 to 4095 keys, 32 heads, 8 of keys, 128 channels, fp32: 130 us
 // with the attention, computed again 192.
-//   Of many rows: 2 prompts of 1500 to 2048 (16 heads, 4 of keys, 128 channels, bf16) take 140 us of attention, 13 us to split their queries (5.6 TB/s), 65 us
-// here, 32 % of the matrix cores' time, and 5 us to join: bound by waits with two wavefronts a SIMD.
+//   Of many rows: 2 prompts of 1500 to 2048 (16 heads, 4 of keys, 128 channels, bf16) take 140 us of attention and 72 us
+// here, bound by waits with two wavefronts a SIMD (matrix cores 28 % of the time busy); 193 us in all.  Each block splits the queries that it stages:
+// split once, by a launch of its own, they take 217 in all.
 //   No sum is made in an order that changes: where there are few keys the rows are cut into parts, whose sums wait in the workspace and are added in
 // order by a second launch.
 #include <hip/hip_runtime.h>
@@ -37,8 +38,6 @@ struct MassArgs {
     float decay;
     uint32_t parts, max_keys;  // parts of a sequence's rows; keys of the longest sequence
     float *sums;               // [parts][sequence][kv head][max_keys]; null: one part
-    uint16_t *planes;          // split_queries
-    size_t plane;              // values of one
 };
 
 __device__ __forceinline__ void put_mass(const MassArgs &m, const dev::KvSequence &seq, uint32_t s, uint32_t kvh, int32_t key, float sum) {
@@ -49,21 +48,6 @@ __device__ __forceinline__ void put_mass(const MassArgs &m, const dev::KvSequenc
     const int32_t row = key - (seq.length - seq.n);  // its own, where it is the call's
     m.mass[to] = (row >= 0 || m.decay == 0.0f ? 0.0f : m.decay * m.mass[to]) + sum;
     if (row >= 0 && m.positions) m.positions[to] = m.row_positions ? m.row_positions[seq.start + row] : key;
-}
-
-// The scaled queries as three bf16 numbers each, [plane][token][query head][DP]: made once, read by every block of keys.  A thread 4 channels.
-template <int DP> __global__ __launch_bounds__(256) void split_queries(MassArgs m) {
-    const AttendArgs &g = m.at;
-    const uint32_t at = blockIdx.x * 256 + threadIdx.x, row = at / (DP / 4), c = 4 * (at % (DP / 4)), token = row / g.q_heads, head = row - token * g.q_heads;
-    // Rows in front of the sequences and behind them are not read.
-    if (token >= g.kv.tokens || (int32_t)token < g.kv.starts[0] || (int32_t)token >= g.kv.starts[g.kv.sequences]) return;
-    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < g.d) x = *reinterpret_cast<const f32x4 *>(g.q + (int64_t)token * g.q_token + (int64_t)head * g.q_head + c) * g.scale;
-    uint32_t w[3][2];
-    split_pair(x[0], x[1], w[0][0], w[1][0], w[2][0]);
-    split_pair(x[2], x[3], w[0][1], w[1][1], w[2][1]);
-#pragma unroll
-    for (int p = 0; p < 3; p++) *reinterpret_cast<u32x2 *>(m.planes + p * m.plane + (size_t)row * DP + c) = u32x2{w[p][0], w[p][1]};
 }
 
 template <int DP> struct MassLds {
@@ -134,6 +118,7 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
     struct Its {
         RowRange range;
         uint32_t at;  // token times heads, and head
+        int64_t query;
         bool valid;
     };
     auto row_of_tile = [&](uint32_t tile) {
@@ -141,7 +126,9 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
         const uint32_t row = tile * MASS_ROWS + col;
         r.valid = row < rows;
         const uint32_t token = g.by_group.div(r.valid ? row : 0);
-        r.at = (uint32_t)(seq.start + (int32_t)token) * g.q_heads + kvh * g.group + (r.valid ? row : 0) - token * g.group;
+        const uint32_t head = kvh * g.group + (r.valid ? row : 0) - token * g.group;
+        r.at = (uint32_t)(seq.start + (int32_t)token) * g.q_heads + head;
+        r.query = (int64_t)(seq.start + (int32_t)token) * g.q_token + (int64_t)head * g.q_head;
         r.range = row_range(g, seq, s, token);
         if (!r.valid) r.range.low = r.range.high = 0;
         return r;
@@ -154,18 +141,19 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
         }
         return tile;
     };
-    // A tile on its way: its queries' parts, 16 bytes at a time, and what is known of its rows.
-    constexpr int PIECES = MASS_ROWS * DP / 8, EACH = PIECES / 256 ? PIECES / 256 : 1;  // of a plane; of a thread
-    u32x4 stage[3][EACH];
+    // A tile on its way: its queries, 8 channels at a time, and what is known of its rows.
+    constexpr int PIECES = MASS_ROWS * DP / 8, EACH = PIECES / 256 ? PIECES / 256 : 1;  // of a thread
+    f32x4 stage[EACH][2];
     f32x2 stats;
     float its_slope;
+    auto channel_of_piece = [&](int e, int half) { return (uint32_t)(8 * ((tid + 256 * e) % PIECES % (DP / 8)) + 4 * half); };
     auto fetch = [&](const Its &r) {
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const uint32_t piece = (tid + 256 * e) % PIECES, row = piece / (DP / 8);
-            const uint32_t at = __shfl(r.at, row);
+            const uint32_t row = (tid + 256 * e) % PIECES / (DP / 8), low_word = __shfl((int32_t)r.query, row), high_word = __shfl((int32_t)(r.query >> 32), row);
+            const float *from = g.q + (int64_t)((uint64_t)high_word << 32 | low_word);
 #pragma unroll
-            for (int p = 0; p < 3; p++) stage[p][e] = *reinterpret_cast<const u32x4 *>(m.planes + p * m.plane + (size_t)at * DP + 8 * (piece % (DP / 8)));
+            for (int half = 0; half < 2; half++) stage[e][half] = *reinterpret_cast<const f32x4 *>(from + (channel_of_piece(e, half) < g.d ? channel_of_piece(e, half) : 0));
         }
         stats = *reinterpret_cast<const f32x2 *>(g.stats + 2 * (size_t)r.at);
         its_slope = g.slopes ? g.slopes[r.at % g.q_heads] * LOG2E : 0.0f;
@@ -173,9 +161,16 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
     auto park = [&](int buffer, const Its &r) {
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const uint32_t piece = (tid + 256 * e) % PIECES;
+            uint32_t w[3][4];
 #pragma unroll
-            for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4 *>(&lds.q[buffer][p][piece / (DP / 8) * PITCH + 8 * (piece % (DP / 8))]) = stage[p][e];
+            for (int half = 0; half < 2; half++) {
+                const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f}, x = channel_of_piece(e, half) < g.d ? stage[e][half] * g.scale : zero;
+                split_pair(x[0], x[1], w[0][2 * half], w[1][2 * half], w[2][2 * half]);
+                split_pair(x[2], x[3], w[0][2 * half + 1], w[1][2 * half + 1], w[2][2 * half + 1]);
+            }
+            const uint32_t row = (tid + 256 * e) % PIECES / (DP / 8);
+#pragma unroll
+            for (int p = 0; p < 3; p++) *reinterpret_cast<u32x4 *>(&lds.q[buffer][p][row * PITCH + channel_of_piece(e, 0)]) = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
         }
         if (tid < MASS_ROWS) {
             lds.top[buffer][col] = stats.x, lds.recip[buffer][col] = stats.y, lds.slope[buffer][col] = its_slope;
@@ -341,8 +336,7 @@ __global__ __launch_bounds__(256) void finish_masses(MassArgs m) {
 
 struct MassPlan {
     uint64_t parts, blocks;
-    size_t attend, stats, sums, scores, planes;  // where each begins in the workspace
-    uint32_t channels;                           // of a split query
+    size_t attend, stats, sums, scores;  // where each begins in the workspace
     uint32_t max_keys, score_rows, score_keys;  // score_rows 0: no scores are kept
     bool many;                           // sequences may have more than few rows
     size_t bytes;
@@ -357,8 +351,7 @@ MassPlan mass_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_
     const size_t max_keys = std::min(attend.max_keys ? attend.max_keys : held, held);
     const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
     const uint64_t pairs = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads, tiles = (max_tokens * (uint64_t)(attend.q_heads / cache.kv_heads) + MASS_ROWS - 1) / MASS_ROWS;
-    p.channels = cache.head_size <= 64 ? 64 : cache.head_size <= 128 ? 128 : 256;
-    const uint64_t block_keys = cache.elem == AHIP_KV_BF16 ? (p.channels <= 128 ? 256 : 128) : p.channels <= 64 ? 256 : 128, chunks = (max_keys + block_keys - 1) / block_keys;
+    const uint64_t block_keys = cache.head_size <= (cache.elem == AHIP_KV_BF16 ? 128 : 64) ? 256 : 128, chunks = (max_keys + block_keys - 1) / block_keys;
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
     // Rows are cut until there are three blocks a CU, each of at least eight tiles of rows.
     p.parts = 1;
@@ -375,13 +368,11 @@ MassPlan mass_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_
     p.stats = up16(attention.bytes);
     p.sums = up16(p.stats + 2 * attend.tokens * (size_t)attend.q_heads * sizeof(float));
     p.scores = up16(p.sums + (p.many && p.parts > 1 ? p.parts * pairs * max_keys * sizeof(float) : 0));
-    p.planes = up16(p.scores + pairs * p.score_keys * p.score_rows * sizeof(float));
-    p.bytes = p.planes + (p.many ? 3 * attend.tokens * (size_t)attend.q_heads * p.channels * sizeof(uint16_t) : 0);
+    p.bytes = p.scores + pairs * p.score_keys * p.score_rows * sizeof(float);
     return p;
 }
 
 template <int DP, bool BF16> void launch_weigh(hipStream_t stream, uint32_t blocks, const MassArgs &m) {
-    hipLaunchKernelGGL(split_queries<DP>, dim3((uint32_t)((m.plane / 4 + 255) / 256)), dim3(256), 0, stream, m);
     hipLaunchKernelGGL((weigh_keys<DP, BF16>), dim3(blocks), dim3(256), 0, stream, m);
 }
 template <bool BF16> void launch_weigh(hipStream_t stream, uint32_t blocks, const MassArgs &m) {
@@ -417,7 +408,7 @@ int launch_kv_attention_mass(DeviceCtx &ctx, const ahip_kv_cache &cache, const a
     if (!attend.workspace || attend.workspace_bytes < plan.bytes)
         return ctx.fail(AHIP_ERR_ARG, name + "the workspace holds " + std::to_string(attend.workspace ? attend.workspace_bytes : 0) + " bytes of " + std::to_string(plan.bytes));
     const uint64_t finish = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads * (((uint64_t)plan.max_keys + 255) / 256);
-    if ((plan.many && (plan.blocks >= MOST_BLOCKS || attend.tokens * (uint64_t)attend.q_heads * plan.channels / 1024 >= MOST_BLOCKS)) || finish >= MOST_BLOCKS)
+    if ((plan.many && (plan.blocks >= MOST_BLOCKS || attend.tokens * (uint64_t)attend.q_heads > UINT32_MAX)) || finish >= MOST_BLOCKS)
         return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     if (int rc = begin_attend(ctx, cache, batch, attend, false, &m.at)) return rc;
     char *space = static_cast<char *>(attend.workspace);
@@ -434,7 +425,6 @@ int launch_kv_attention_mass(DeviceCtx &ctx, const ahip_kv_cache &cache, const a
     m.parts = (uint32_t)plan.parts, m.max_keys = plan.max_keys;
     m.sums = plan.many && plan.parts > 1 ? reinterpret_cast<float *>(space + plan.sums) : nullptr;
     if (plan.many) {
-        m.planes = reinterpret_cast<uint16_t *>(space + plan.planes), m.plane = attend.tokens * (size_t)attend.q_heads * plan.channels;
         if (bf16) launch_weigh<true>(ctx.stream, (uint32_t)plan.blocks, m);
         else launch_weigh<false>(ctx.stream, (uint32_t)plan.blocks, m);
         if (int rc = ctx.check(hipGetLastError(), "kv attention mass launch")) return rc;

@@ -38,13 +38,15 @@ def plain_workspace(**changed):
 def test_masses_want_statistics_and_scores_beside_attention():
     # 4 tokens of up to 800 keys, 4 query heads for each of 8: attention's own, two numbers a row and head, 4 rows of 800 scores for each of 32 pairs.
     assert mass_workspace() == plain_workspace() + 4 * 32 * 2 * 4 + 32 * 4 * 800 * 4
-    # A prompt's queries are split into three planes of 16 bits, and scores kept for as many rows as a short sequence beside it can have.
+    # A prompt of 1000 tokens: scores are kept for as many rows as a short sequence beside it can have,
+    # 32, and sums of up to 16 parts of its rows.
     prompt = {"batch.sequences": 1, "attend.tokens": 1000, "attend.max_tokens": 1000}
-    assert mass_workspace(**prompt) >= plain_workspace(**prompt) + 1000 * 32 * 2 * 4 + 3 * 1000 * 32 * 128 * 2
+    most = plain_workspace(**prompt) + 1000 * 32 * 2 * 4 + 8 * 32 * 800 * 4 + 16 * 8 * 800 * 4
+    assert most - 16 * 8 * 800 * 4 < mass_workspace(**prompt) <= most + 64
 
 
 def test_the_workspace_of_masses_has_an_end():
-    """Scores are kept up to 2^30 bytes; with more the weights are computed again, from split queries."""
+    """Scores are kept up to 2^30 bytes; with more the weights are computed again."""
     long = {"batch.sequences": 64, "batch.table_pages": 1 << 16, "batch.table_stride": 1 << 16, "attend.tokens": 64}
     assert mass_workspace(**long) < plain_workspace(**long) + (1 << 30)
     assert mass_workspace(**{**long, "attend.max_keys": 4096}) <= plain_workspace(**{**long, "attend.max_keys": 4096}) + 64 * 32 * 2 * 4 + 64 * 8 * 4 * 4096 * 4
