@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from altius_amd import device as D
-from test_gpu_kv_cache import Paged, gpu, here  # noqa: F401 (a fixture)
+from test_gpu_kv_cache import Paged, attend, gpu, held_to_definition, here  # noqa: F401 (a fixture)
 from test_gpu_kv_mass import Mass, held_to_masses
 from test_gpu_kv_sparse import Sparse, held_to_choice, page_means
 from test_gpu_kv_tree import attend_tree, held_to_tree, random_tree
@@ -179,3 +179,19 @@ def test_means_of_pages_that_moved_slots_fill(here, case, elem):  # noqa: F811
             got.run(here)
     here.sync()
     held_to_choice(got, q)
+
+
+@pytest.mark.parametrize("d", [68, 72, 76, 80, 84, 88, 92, 96])
+@pytest.mark.parametrize("page", [5, 16])
+@pytest.mark.parametrize("n,lengths", [([1, 1], [300, 33]), ([3, 50], [90, 120])])
+def test_few_rows_of_heads_of_65_to_96_channels(here, case, d, page, n, lengths):  # noqa: F811
+    """Channels behind the 64th go to the lanes one or two a lane."""
+    case(f"few rows, {d} channels, pages of {page}, {n}")
+    rng = np.random.default_rng(d + page)
+    paged = Paged(rng, n, lengths, 2, d, page)
+    q = rng.standard_normal((sum(n), 6, d)).astype(np.float32)
+    on = gpu(q)
+    held_to_definition(attend(here, paged, on).cpu().numpy(), paged, q)
+    held_to_masses(Mass(here, paged, on, rng).run(here), q)
+    held_to_choice(Sparse(here, paged, on, 3, 1, 1).run(here), q)
+    here.sync()
