@@ -50,6 +50,16 @@ __device__ __forceinline__ void put_mass(const MassArgs &m, const dev::KvSequenc
     if (row >= 0 && m.positions) m.positions[to] = m.row_positions ? m.row_positions[seq.start + row] : key;
 }
 
+// A sum that carries along what its last addition rounded off (Kahan's): off by two steps of itself at most, however many terms there are.  The weight that a key is
+// given by many rows adds up to thousands, beside which a single one is less than a step.
+struct LongSum {
+    float sum = 0.0f, over = 0.0f;  // over: how much too large
+    __device__ __forceinline__ void add(float x) {
+        const float y = x - over, next = sum + y;
+        over = (next - sum) - y, sum = next;
+    }
+};
+
 template <int DP> struct MassLds {
     static constexpr int PITCH = DP + 8;  // 16-bit words; 16 rows of 16-byte reads cover all banks
     uint16_t q[2][3][MASS_ROWS * PITCH];
@@ -177,7 +187,7 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
             lds.low[buffer][col] = r.range.low, lds.high[buffer][col] = r.range.high, lds.place[buffer][col] = r.range.place;
         }
     };
-    float sum[TILES] = {};
+    LongSum sum[TILES];
     // Weights of 16 scores of the lane's key `its` are added to `total`; whole: all rows see all of the wavefront's keys.
     auto add = [&](int buffer, float (&x)[16], int32_t its, bool whole, float &total) {
         cap_scores(g, x);
@@ -250,7 +260,9 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
             float x[16];
 #pragma unroll
             for (int r = 0; r < 16; r++) x[r] = st[t][r];
-            add(buffer, x, key + 32 * t, whole, sum[t]);
+            float of_tile = 0.0f;
+            add(buffer, x, key + 32 * t, whole, of_tile);
+            sum[t].add(of_tile);
         }
         if (behind < to) park(buffer ^ 1, next);
         now = next, tile = behind;
@@ -260,13 +272,13 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
     // more then, value by value.
     float check = 0.0f;
 #pragma unroll
-    for (int t = 0; t < TILES; t++) check = key + 32 * t < seq.length ? __builtin_fmaf(sum[t], 0.0f, check) : check;
+    for (int t = 0; t < TILES; t++) check = key + 32 * t < seq.length ? __builtin_fmaf(sum[t].sum, 0.0f, check) : check;
     if (__any(check != 0.0f)) {
 #pragma unroll 1
         for (int t = 0; t < TILES; t++) {
             const int32_t its = key + 32 * t;
             const int64_t at = t == 0 ? k_at[0] : k_at[TILES - 1];
-            float total = 0.0f;
+            LongSum total;
             for (uint32_t row = from * MASS_ROWS + h; row < min(to * MASS_ROWS, rows); row += 2) {
                 const uint32_t token = g.by_group.div(row), head = kvh * g.group + row - token * g.group;
                 const RowRange range = row_range(g, seq, s, token);
@@ -276,15 +288,15 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
                 for (uint32_t c = 0; c < g.d; c++) x[0] = __builtin_fmaf(q_row[c] * g.scale, cache_value<BF16>(g.kv.keys, at + c), x[0]);
                 scores(g, x, g.slopes ? g.slopes[head] * LOG2E : 0.0f, range.place - its, [](int) { return 0; });
                 const f32x2 its_stats = *reinterpret_cast<const f32x2 *>(g.stats + 2 * ((size_t)(seq.start + (int32_t)token) * g.q_heads + head));
-                total += exp2_fast(x[0] - its_stats.x) * its_stats.y;
+                total.add(exp2_fast(x[0] - its_stats.x) * its_stats.y);
             }
 #pragma unroll
-            for (int e = 0; e < TILES; e++) sum[e] = e == t ? total : sum[e];
+            for (int e = 0; e < TILES; e++) sum[e].sum = e == t ? total.sum : sum[e].sum;
         }
     }
 #pragma unroll
     for (int t = 0; t < TILES; t++) {
-        const float total = sum[t] + __shfl_xor(sum[t], 32);
+        const float total = sum[t].sum + __shfl_xor(sum[t].sum, 32);
         const int32_t its = key + 32 * t;
         if (h != 0 || its >= seq.length) continue;
         if (m.sums) m.sums[((size_t)part * pairs + pair) * m.max_keys + (size_t)its] = total;
