@@ -533,8 +533,9 @@ int launch_kv_attention_sparse(DeviceCtx &ctx, const ahip_kv_cache &cache, const
     if (int rc = attend::begin_attend(ctx, cache, p.batch, p.attend, false, &a)) return rc;
     a.kv.table_head = sparse.most;
 
-    // A single row fills a page for later calls only; several may score a page that one of them has filled.
-    g.fills = g.max_tokens == 1;
+    // A single row fills a page for later calls only; several may score a page that one of them has filled.  Blocks beside the choice are as many again, as far as a
+    // grid of 2^32 threads holds both.
+    g.fills = g.max_tokens == 1 && 2 * p.rows * (p.split ? BLOCK : LARGE) < MOST_GRID * BLOCK;
     if (!g.fills)
         if (int rc = launch_means(ctx, g, name)) return rc;
     if (g.d <= 64) g.group <= 4 ? launch_choice<4, 1>(ctx.stream, g, p) : launch_choice<4, 2>(ctx.stream, g, p);

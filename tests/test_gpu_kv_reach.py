@@ -1,8 +1,12 @@
-"""The operators around a paged cache at sizes that choose among their kernels or that a sum feels: sums of many weights."""
+"""The operators around a paged cache at sizes that choose among their kernels or that a sum feels: sums of many weights, more rows than a grid of
+large blocks has twice."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
+from altius_amd import device as D
 from decoder_oracle import STEP
 from test_gpu_kv_cache import Paged, here  # noqa: F401 (a fixture)
 from test_gpu_kv_mass import Mass
@@ -32,3 +36,43 @@ def test_masses_of_many_rows_are_summed_to_fp32(here, case):  # noqa: F811
     # 2 steps a weight; 16 for a partial sum of as many weights, 2 for a sum that carries its rounding along, 1 for the two halves of a row tile and up to 15 for parts
     # of the rows.
     assert (np.abs(mass - want[:, None]) <= (2 + 16 + 2 + 1 + 15) * STEP * want[:, None] + 1e-9).all(), (np.abs(mass - want[:, None]) / want[:, None]).max() / STEP
+
+
+def test_more_rows_than_twice_a_grid_of_large_blocks(here, case):  # noqa: F811
+    """129 single tokens of 32767 heads, each the sixth of its text, in pages of two: the page that it fills, and the better one of the two in front."""
+    case("chosen pages of 129 x 32767 rows")
+    tokens, heads, d, page, pages = 129, 32767, 4, 2, 3
+    gen = torch.Generator(device="cuda").manual_seed(44)
+    k, v = (torch.randn((tokens * pages, heads, page, d), device="cuda", generator=gen) for _ in range(2))
+    q, out = torch.randn((tokens, heads, d), device="cuda", generator=gen), torch.empty((tokens, heads, d), device="cuda")
+    table = torch.randperm(tokens * pages, device="cuda", generator=gen).int().reshape(tokens, pages)
+    at = table.long()
+    means = torch.full((tokens * pages, heads, d), math.nan, device="cuda")
+    full = k.double().sum(2).div(page).float()
+    means[at[:, :2].flatten()] = full[at[:, :2].flatten()]
+    chosen = torch.full((tokens, heads, 2), -5, device="cuda", dtype=torch.int32)
+    starts, lengths = torch.arange(tokens + 1, device="cuda", dtype=torch.int32), torch.full((tokens,), 6, device="cuda", dtype=torch.int32)
+    cache = D.KvCache(keys=k.data_ptr(), values=v.data_ptr(), elem=D.KV_F32, kv_heads=heads, head_size=d, page_size=page, pages=tokens * pages, page_stride=heads * page * d,
+                      head_stride=page * d, slot_stride=d)
+    batch = D.KvBatch(sequences=tokens, table_pages=pages, table_stride=pages, query_starts=starts.data_ptr(), lengths=lengths.data_ptr(), page_table=table.data_ptr())
+    call = D.KvAttend(tokens=tokens, q_heads=heads, q=q.data_ptr(), out=out.data_ptr(), q_strides=(heads * d, d), out_strides=(heads * d, d), scale=0.5, max_tokens=1)
+    sparse = D.KvSparse(means=means.data_ptr(), page_stride=heads * d, head_stride=d, chosen=chosen.data_ptr(), most=2, first=0, last=1)
+    room = D.kv_attention_sparse_workspace(here, cache, batch, call, sparse)
+    space = torch.empty(room, device="cuda", dtype=torch.uint8)
+    call.workspace, call.workspace_bytes = space.data_ptr(), room
+    torch.cuda.synchronize()
+    here.kv_attention_sparse_raw(cache, batch, call, sparse)
+    here.sync()
+    assert torch.equal(means, full)
+    score = (full[at[:, :2]].double() * q[:, None].double()).sum(-1)  # [tokens, page, heads]
+    best = (score[:, 1] > score[:, 0]).int()
+    assert torch.equal(chosen[..., 0], best) and (chosen[..., 1] == 2).all()
+    take = torch.stack([torch.gather(at[:, None, :].expand(-1, heads, -1), 2, best[..., None].long())[..., 0], at[:, 2:3].expand(-1, heads)], 2)
+    number = torch.arange(heads, device="cuda")[None, :, None]
+    keys, values = (x[take, number].reshape(tokens, heads, 2 * page, d).double() for x in (k, v))
+    x = (keys * q[:, :, None].double()).sum(-1) * 0.5
+    p = torch.softmax(x, -1)
+    want = (p[..., None] * values).sum(2)
+    # A score is off by (d + 4) steps of its terms; a weight by what the worst score and its own are, the sum of 4 and 8 more: twice that with the values' sum.
+    worst = (2 * (d + 4) * ((keys.abs() * q[:, :, None].double().abs()).sum(-1) * 0.5).amax(-1) + 2 * 4 + 8) * STEP
+    assert ((out - want).abs() <= worst[..., None] * (p[..., None] * values.abs()).sum(2) + 1e-37).all()
