@@ -115,10 +115,10 @@ template <uint32_t THREADS, uint32_t EACH> __global__ __launch_bounds__(THREADS)
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < WAVES; w++) newest = max(newest, (int32_t)per_wave[w][0]);
-    const int64_t above_recent = (int64_t)newest - g.recent;
-    const int32_t recent_from = above_recent < INT32_MIN ? INT32_MIN : (int32_t)above_recent + 1;  // recent is at least 0: no overflow
-    const bool no_recent = g.recent == 0;
-    auto image_of = [&](int32_t position, uint32_t mass) { return position < g.first || (position >= recent_from && !no_recent) ? KEPT : rank_image(__uint_as_float(mass)); };
+    // How far a position is behind the newest fits 32 bits without a sign, whatever both are.
+    auto image_of = [&](int32_t position, uint32_t mass) {
+        return position < g.first || (uint32_t)newest - (uint32_t)position < (uint32_t)g.recent ? KEPT : rank_image(__uint_as_float(mass));
+    };
     // Images of the places from `base` on, 0 behind the end.
     auto take_images = [&](uint32_t base, uint32_t *v) {
         if constexpr (EACH != AHEAD) ahead(base, [&](uint32_t u, int64_t at) { positions[u] = g.history.positions[at], masses[u] = __float_as_uint(g.history.mass[at]); });

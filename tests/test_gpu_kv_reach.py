@@ -1,5 +1,5 @@
 """The operators around a paged cache at sizes that choose among their kernels or that a sum feels: sums of many weights, more rows than a grid of
-large blocks has twice."""
+large blocks has twice, positions at the ends of 32 bits."""
 import math
 
 import numpy as np
@@ -9,7 +9,7 @@ import torch
 from altius_amd import device as D
 from decoder_oracle import STEP
 from test_gpu_kv_cache import Paged, here  # noqa: F401 (a fixture)
-from test_gpu_kv_mass import Mass
+from test_gpu_kv_mass import Evict, Mass
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,17 @@ def test_more_rows_than_twice_a_grid_of_large_blocks(here, case):  # noqa: F811
     # A score is off by (d + 4) steps of its terms; a weight by what the worst score and its own are, the sum of 4 and 8 more: twice that with the values' sum.
     worst = (2 * (d + 4) * ((keys.abs() * q[:, :, None].double().abs()).sum(-1) * 0.5).amax(-1) + 2 * 4 + 8) * STEP
     assert ((out - want).abs() <= worst[..., None] * (p[..., None] * values.abs()).sum(2) + 1e-37).all()
+
+
+@pytest.mark.parametrize("longest", [300, 3000, 60000])
+def test_evictions_that_keep_no_recent_position(here, case, longest):  # noqa: F811
+    """Positions at both ends of 32 bits, and none of them kept for being new."""
+    case(f"evict, recent 0, {longest}")
+    rng = np.random.default_rng(43)
+    for values in ([-(1 << 31), (1 << 31) - 1, 0, 5], [(1 << 31) - 1], [-(1 << 31)]):
+        for recent, first in ((0, 40), (0, 0), (1, 0)):
+            e = Evict(rng, [longest, longest - 9], 2, 16, longest // 3, recent, first, max_keys=longest)
+            e.positions = np.array(values, np.int64)[rng.integers(0, len(values), e.positions.shape)].astype(np.int32)
+            e.run(here)
+            here.sync()
+            e.held()
