@@ -1,5 +1,6 @@
 """The operators around a paged cache at sizes that choose among their kernels or that a sum feels: sums of many weights, more rows than a grid of
-large blocks has twice, positions at the ends of 32 bits."""
+large blocks has twice, positions at the ends of 32 bits; weights of few rows that are computed again because their scores would not fit the workspace, scores of many
+pages for wide heads."""
 import math
 
 import numpy as np
@@ -8,8 +9,9 @@ import torch
 
 from altius_amd import device as D
 from decoder_oracle import STEP
-from test_gpu_kv_cache import Paged, here  # noqa: F401 (a fixture)
-from test_gpu_kv_mass import Evict, Mass
+from test_gpu_kv_cache import Paged, gpu, here  # noqa: F401 (a fixture)
+from test_gpu_kv_mass import Evict, Mass, held_to_masses
+from test_gpu_kv_sparse import Sparse, held_to_choice
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +92,39 @@ def test_evictions_that_keep_no_recent_position(here, case, longest):  # noqa: F
             e.run(here)
             here.sync()
             e.held()
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("n,lengths,heads,kv,d", [([1, 1, 1], [1, 300, 77], 8, 2, 64), ([1, 2, 40], [700, 33, 90], 8, 2, 128), ([3, 1, 1], [2, 50, 400], 12, 3, 80),
+                                                  ([1, 1, 9], [600, 5, 130], 8, 2, 256)])
+@pytest.mark.parametrize("plain", [True, False])
+def test_masses_whose_scores_are_not_kept(here, case, elem, n, lengths, heads, kv, d, plain):  # noqa: F811
+    """Short sequences whose page table has room for 2^24 tokens, and no bound on their keys: their scores would take more than the workspace has for them."""
+    case(f"mass, scores not kept {elem} n {n} lengths {lengths} heads {heads}/{kv} d {d} plain {plain}")
+    rng = np.random.default_rng(41 + d)
+    paged = Paged(rng, n, lengths, kv, d, 16, elem)
+    table = np.full((len(n), 1 << 20), -1, np.int32)
+    table[:, :paged.per] = paged.table
+    paged.per, paged.table_on = table.shape[1], gpu(table)
+    q = rng.standard_normal((sum(n) + 2, heads, d)).astype(np.float32)
+    options = dict(decay=0.0) if plain else dict(decay=0.75, own_positions=False, window=100, cap=20.0, slopes=(2.0 ** -np.arange(1, heads + 1)).astype(np.float32),
+                                                 first=rng.integers(-3, 60, sum(n) + 2).astype(np.int32))
+    got = Mass(here, paged, gpu(q), rng, **options)
+    assert got.room < 1 << 29
+    got.run(here)
+    here.sync()
+    held_to_masses(got, q)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("n,lengths,heads,kv,d,page", [([20, 3], [1500, 900], 4, 2, 256, 8), ([9, 1, 30], [700, 800, 1300], 7, 1, 136, 12), ([11], [600], 3, 3, 200, 8),
+                                                       ([1], [9000], 4, 2, 256, 16), ([1, 2], [5000, 8000], 6, 1, 200, 9), ([2], [5300], 2, 2, 136, 8)])
+def test_many_pages_of_wide_heads(here, case, elem, n, lengths, heads, kv, d, page):  # noqa: F811
+    """Scores by launches of their own: of rows next to each other, and of few rows of more than 512 pages."""
+    case(f"sparse, wide heads {elem} n {n} lengths {lengths} heads {heads}/{kv} d {d} page {page}")
+    rng = np.random.default_rng(42 + d)
+    paged = Paged(rng, n, lengths, kv, d, page, elem)
+    q = (1.5 * rng.standard_normal((sum(n) + 2, heads, d))).astype(np.float32)
+    got = Sparse(here, paged, gpu(q), 12, 1, 2).run(here)
+    here.sync()
+    held_to_choice(got, q)
