@@ -37,6 +37,7 @@ struct MassArgs {
     const int32_t *row_positions;
     float decay;
     uint32_t parts, max_keys;  // parts of a sequence's rows; keys of the longest sequence
+    uint32_t chunks, finish_chunks;  // runs of keys of a pair (sequence, kv head) that there are blocks for: a block goes on with every chunks-th behind its own
     float *sums;               // [parts][sequence][kv head][max_keys]; null: one part
 };
 
@@ -69,22 +70,14 @@ template <int DP> struct MassLds {
 // 32 keys a wavefront, or 64, where registers hold them: each part of a query that comes from LDS is then used twice.
 template <int DP, bool BF16> constexpr int mass_tiles() { return (BF16 ? DP <= 128 : DP <= 64) ? 2 : 1; }
 
-template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void weigh_keys(MassArgs m) {
+// A block's keys, from `first` on, and part `part` of the sequence's rows.
+template <int DP, bool BF16>
+__device__ __forceinline__ void weigh_run(const MassArgs &m, MassLds<DP> &lds, const dev::KvSequence &seq, uint32_t s, uint32_t kvh, uint32_t part, int32_t first) {
     constexpr int STEPS = DP / 16, PLANES = BF16 ? 1 : 3, SIZE = BF16 ? 2 : 4, TILES = mass_tiles<DP, BF16>(), KEYS = 128 * TILES;
-    using Lds = MassLds<DP>;
-    constexpr int PITCH = Lds::PITCH;
-    __shared__ __align__(16) Lds lds;
+    constexpr int PITCH = MassLds<DP>::PITCH;
     const AttendArgs &g = m.at;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31u, h = lane >> 5;
-    // The first keys of a causal sequence are seen by most rows: they start first.  Blocks i, i + 8, .. share an XCD: the pairs go round, so that no XCD has the
-    // long sequences to itself.
-    const uint32_t pairs = g.kv.sequences * g.kv.kv_heads, outer = blockIdx.x / pairs, pair = (blockIdx.x + outer) % pairs;
-    const uint32_t chunk = outer / m.parts, part = outer - chunk * m.parts, s = pair / g.kv.kv_heads, kvh = pair - s * g.kv.kv_heads;
-    const dev::KvSequence seq = sequence_of(g, s);
-    const int32_t first = (int32_t)(chunk * KEYS);
-    if (seq.n == 0 || first >= seq.length) return;
-    const uint32_t rows = (uint32_t)seq.n * g.group;
-    if (g.scores && rows <= g.few_rows) return;  // finish_masses has them
+    const uint32_t pairs = g.kv.sequences * g.kv.kv_heads, pair = s * g.kv.kv_heads + kvh, rows = (uint32_t)seq.n * g.group;
 
     // This lane's keys.  Behind the last one that one stands in, and is left out.
     const int32_t mine = first + (int32_t)(wave * 32 * TILES), key = mine + (int32_t)col;
@@ -304,29 +297,50 @@ template <int DP, bool BF16> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2
     }
 }
 
+// LONG: blocks go on with further keys.  (The loop costs registers: of 128 channels, bf16, 234 instead of 208, of fp32 some are spilled.)
+template <int DP, bool BF16, bool LONG> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void weigh_keys(MassArgs m) {
+    constexpr uint32_t KEYS = 128 * mass_tiles<DP, BF16>();
+    __shared__ __align__(16) MassLds<DP> lds;
+    const AttendArgs &g = m.at;
+    // The first keys of a causal sequence are seen by most rows: they start first.  Blocks i, i + 8, .. share an XCD: the pairs go round, so that no XCD has the
+    // long sequences to itself.
+    const uint32_t pairs = g.kv.sequences * g.kv.kv_heads, outer = blockIdx.x / pairs, pair = (blockIdx.x + outer) % pairs;
+    const uint32_t chunk = outer / m.parts, part = outer - chunk * m.parts, s = pair / g.kv.kv_heads, kvh = pair - s * g.kv.kv_heads;
+    const dev::KvSequence seq = sequence_of(g, s);
+    if (seq.n == 0) return;
+    if (g.scores && (uint32_t)seq.n * g.group <= g.few_rows) return;  // finish_masses has them
+    for (uint32_t at = chunk; (uint64_t)at * KEYS < (uint32_t)seq.length; at += m.chunks) {
+        if (at != chunk) __syncthreads();  // behind the last reader of what is in LDS
+        weigh_run<DP, BF16>(m, lds, seq, s, kvh, part, (int32_t)(at * KEYS));
+        if constexpr (!LONG) break;
+    }
+}
+
 // What is left to add up, a thread a key: the scores of sequences of few rows, and the parts of the others' sums, in order.
 __global__ __launch_bounds__(256) void finish_masses(MassArgs m) {
     __shared__ float top[FEW_ROWS], recip[FEW_ROWS];
     __shared__ int32_t low[FEW_ROWS], high[FEW_ROWS];
     const AttendArgs &g = m.at;
-    const uint32_t tid = threadIdx.x, per = (m.max_keys + 255) / 256, pairs = g.kv.sequences * g.kv.kv_heads, pair = blockIdx.x / per, s = pair / g.kv.kv_heads, kvh = pair - s * g.kv.kv_heads;
-    const uint32_t first = (blockIdx.x - pair * per) * 256, key = first + tid;
+    const uint32_t tid = threadIdx.x, per = m.finish_chunks, pairs = g.kv.sequences * g.kv.kv_heads, pair = blockIdx.x / per, s = pair / g.kv.kv_heads, kvh = pair - s * g.kv.kv_heads;
+    const uint32_t first = (blockIdx.x - pair * per) * 256, apart_keys = per * 256;
     const dev::KvSequence seq = sequence_of(g, s);
     const uint32_t rows = (uint32_t)seq.n * g.group;
     if (rows == 0 || first >= (uint32_t)seq.length) return;
-    float sum = 0.0f;
     if (!g.scores || rows > g.few_rows) {
-        if (!m.sums || key >= (uint32_t)seq.length) return;
-        const float *sums = m.sums + (size_t)pair * m.max_keys + key;
-        const size_t apart = (size_t)pairs * m.max_keys;
-        for (uint32_t part = 0; part < m.parts; part += 4) {  // a power of two of them; fewer than four read the last again
-            float its[4];
+        if (!m.sums) return;
+        for (uint32_t key = first + tid; key < (uint32_t)seq.length; key += apart_keys) {
+            float sum = 0.0f;
+            const float *sums = m.sums + (size_t)pair * m.max_keys + key;
+            const size_t apart = (size_t)pairs * m.max_keys;
+            for (uint32_t part = 0; part < m.parts; part += 4) {  // a power of two of them; fewer than four read the last again
+                float its[4];
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) its[e] = sums[min(part + e, m.parts - 1) * apart];
+                for (uint32_t e = 0; e < 4; e++) its[e] = sums[min(part + e, m.parts - 1) * apart];
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) sum += part + e < m.parts ? its[e] : 0.0f;
+                for (uint32_t e = 0; e < 4; e++) sum += part + e < m.parts ? its[e] : 0.0f;
+            }
+            put_mass(m, seq, s, kvh, (int32_t)key, sum);
         }
-        put_mass(m, seq, s, kvh, (int32_t)key, sum);
         return;
     }
     if (tid < rows) {
@@ -336,25 +350,31 @@ __global__ __launch_bounds__(256) void finish_masses(MassArgs m) {
         top[tid] = stats.x, recip[tid] = stats.y, low[tid] = range.low, high[tid] = range.high;
     }
     __syncthreads();
-    if (key >= (uint32_t)seq.length) return;
-    const float *scores = g.scores + (size_t)pair * g.score_rows * g.score_keys + key;
+    for (uint32_t key = first + tid; key < (uint32_t)seq.length; key += apart_keys) {
+        float sum = 0.0f;
+        const float *scores = g.scores + (size_t)pair * g.score_rows * g.score_keys + key;
 #pragma unroll 4
-    for (uint32_t r = 0; r < rows; r++) {
-        const float w = exp2_fast(scores[(size_t)r * g.score_keys] - top[r]) * recip[r];
-        sum += (int32_t)key >= low[r] && (int32_t)key < high[r] ? w : 0.0f;
+        for (uint32_t r = 0; r < rows; r++) {
+            const float w = exp2_fast(scores[(size_t)r * g.score_keys] - top[r]) * recip[r];
+            sum += (int32_t)key >= low[r] && (int32_t)key < high[r] ? w : 0.0f;
+        }
+        put_mass(m, seq, s, kvh, (int32_t)key, sum);
     }
-    put_mass(m, seq, s, kvh, (int32_t)key, sum);
 }
 
 struct MassPlan {
-    uint64_t parts, blocks;
+    uint64_t parts, chunks, finish_chunks, blocks, finish_blocks;
     size_t attend, stats, sums, scores;  // where each begins in the workspace
     uint32_t max_keys, score_rows, score_keys;  // score_rows 0: no scores are kept
     bool many;                           // sequences may have more than few rows
+    bool is_long;                        // blocks go through several runs of keys
     size_t bytes;
 };
 // Scores are kept where they take up to this: a batch of 64 texts of 128 Ki keys and 8 kv heads needs as much.
 constexpr uint64_t MOST_SCORES = (uint64_t)1 << 30;
+// Blocks of a launch, where there are not more pairs: one behind its sequence's end costs 1 ns, and a page table may have room for far more keys than any sequence
+// has.  24 single tokens of 1000 to 4095 keys, 8 heads of keys, in a table for 2^22: 6386 us with a block for each 128 keys of it.
+constexpr uint64_t LAUNCHED = 1 << 14;
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 MassPlan mass_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_kv_batch &batch, const ahip_kv_attend &attend) {
@@ -368,7 +388,10 @@ MassPlan mass_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_
     // Rows are cut until there are three blocks a CU, each of at least eight tiles of rows.
     p.parts = 1;
     while (p.parts < 16 && chunks * pairs * p.parts < 3 * cus && tiles / (2 * p.parts) >= 8) p.parts *= 2;
-    p.blocks = chunks * pairs * p.parts;
+    p.chunks = std::min(chunks, std::max<uint64_t>(1, LAUNCHED / std::max<uint64_t>(1, pairs * p.parts)));
+    p.blocks = p.chunks * pairs * p.parts, p.is_long = p.chunks < chunks;
+    p.finish_chunks = std::min<uint64_t>((max_keys + 255) / 256, std::max<uint64_t>(1, LAUNCHED / std::max<uint64_t>(1, pairs)));
+    p.finish_blocks = p.finish_chunks * pairs;
     const Plan attention = plan_of(ctx, cache, batch, attend);
     const uint64_t rows = max_tokens * (uint64_t)(attend.q_heads / cache.kv_heads);
     p.max_keys = (uint32_t)max_keys;
@@ -384,13 +407,15 @@ MassPlan mass_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const ahip_
     return p;
 }
 
-template <int DP, bool BF16> void launch_weigh(hipStream_t stream, uint32_t blocks, const MassArgs &m) {
-    hipLaunchKernelGGL((weigh_keys<DP, BF16>), dim3(blocks), dim3(256), 0, stream, m);
+template <int DP, bool BF16> void launch_weigh(hipStream_t stream, const MassPlan &plan, const MassArgs &m) {
+    const dim3 grid((uint32_t)plan.blocks);
+    if (plan.is_long) hipLaunchKernelGGL((weigh_keys<DP, BF16, true>), grid, dim3(256), 0, stream, m);
+    else hipLaunchKernelGGL((weigh_keys<DP, BF16, false>), grid, dim3(256), 0, stream, m);
 }
-template <bool BF16> void launch_weigh(hipStream_t stream, uint32_t blocks, const MassArgs &m) {
-    if (m.at.d <= 64) launch_weigh<64, BF16>(stream, blocks, m);
-    else if (m.at.d <= 128) launch_weigh<128, BF16>(stream, blocks, m);
-    else launch_weigh<256, BF16>(stream, blocks, m);
+template <bool BF16> void launch_weigh(hipStream_t stream, const MassPlan &plan, const MassArgs &m) {
+    if (m.at.d <= 64) launch_weigh<64, BF16>(stream, plan, m);
+    else if (m.at.d <= 128) launch_weigh<128, BF16>(stream, plan, m);
+    else launch_weigh<256, BF16>(stream, plan, m);
 }
 
 constexpr int64_t MOST_STRIDE = (int64_t)1 << 48;
@@ -419,8 +444,7 @@ int launch_kv_attention_mass(DeviceCtx &ctx, const ahip_kv_cache &cache, const a
     const MassPlan plan = mass_plan(&ctx, cache, batch, attend);
     if (!attend.workspace || attend.workspace_bytes < plan.bytes)
         return ctx.fail(AHIP_ERR_ARG, name + "the workspace holds " + std::to_string(attend.workspace ? attend.workspace_bytes : 0) + " bytes of " + std::to_string(plan.bytes));
-    const uint64_t finish = (uint64_t)batch.sequences * (uint64_t)cache.kv_heads * (((uint64_t)plan.max_keys + 255) / 256);
-    if ((plan.many && (plan.blocks >= MOST_BLOCKS || attend.tokens * (uint64_t)attend.q_heads > UINT32_MAX)) || finish >= MOST_BLOCKS)
+    if ((plan.many && (plan.blocks >= MOST_BLOCKS || attend.tokens * (uint64_t)attend.q_heads > UINT32_MAX)) || plan.finish_blocks >= MOST_BLOCKS)
         return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     if (int rc = begin_attend(ctx, cache, batch, attend, false, &m.at)) return rc;
     char *space = static_cast<char *>(attend.workspace);
@@ -434,15 +458,15 @@ int launch_kv_attention_mass(DeviceCtx &ctx, const ahip_kv_cache &cache, const a
     if (plan.max_keys == 0) return AHIP_OK;  // no page, no slot
     m.mass = history.mass, m.positions = history.positions, m.page_stride = history.page_stride, m.head_stride = history.head_stride;
     m.row_positions = row_positions, m.decay = decay;
-    m.parts = (uint32_t)plan.parts, m.max_keys = plan.max_keys;
+    m.parts = (uint32_t)plan.parts, m.max_keys = plan.max_keys, m.chunks = (uint32_t)plan.chunks, m.finish_chunks = (uint32_t)plan.finish_chunks;
     m.sums = plan.many && plan.parts > 1 ? reinterpret_cast<float *>(space + plan.sums) : nullptr;
     if (plan.many) {
-        if (bf16) launch_weigh<true>(ctx.stream, (uint32_t)plan.blocks, m);
-        else launch_weigh<false>(ctx.stream, (uint32_t)plan.blocks, m);
+        if (bf16) launch_weigh<true>(ctx.stream, plan, m);
+        else launch_weigh<false>(ctx.stream, plan, m);
         if (int rc = ctx.check(hipGetLastError(), "kv attention mass launch")) return rc;
     }
     if (!plan.score_rows && !m.sums) return AHIP_OK;
-    hipLaunchKernelGGL(finish_masses, dim3((uint32_t)finish), dim3(256), 0, ctx.stream, m);
+    hipLaunchKernelGGL(finish_masses, dim3((uint32_t)plan.finish_blocks), dim3(256), 0, ctx.stream, m);
     return ctx.check(hipGetLastError(), "kv attention mass launch");
 }
 

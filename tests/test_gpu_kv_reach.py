@@ -128,3 +128,42 @@ def test_many_pages_of_wide_heads(here, case, elem, n, lengths, heads, kv, d, pa
     got = Sparse(here, paged, gpu(q), 12, 1, 2).run(here)
     here.sync()
     held_to_choice(got, q)
+
+
+def widened(paged, sequences, table_pages):
+    """The same sequences with others behind them that hold nothing, and a page table with room for more."""
+    table = np.full((sequences, table_pages), -1, np.int32)
+    table[:len(paged.n), :paged.per] = paged.table
+    more = sequences - len(paged.n)
+    paged.n, paged.lengths = paged.n + [0] * more, paged.lengths + [0] * more
+    paged.per, paged.table, paged.table_on = table_pages, table, gpu(table)
+    paged.starts_on, paged.lengths_on = gpu(np.concatenate([[0], np.cumsum(paged.n)]).astype(np.int32)), gpu(np.array(paged.lengths, np.int32))
+    return paged
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("n", [[1], [40, 2]])
+@pytest.mark.parametrize("room", [2512, 1 << 20])
+def test_masses_of_more_keys_than_blocks_are_launched_for(here, case, elem, d, n, room):  # noqa: F811
+    """1024 sequences, of which few hold anything, 2 heads of keys: 8 blocks a head, which go on with the keys behind their own."""
+    case(f"mass, long {elem} d {d} n {n} room {room}")
+    rng = np.random.default_rng(45)
+    lengths = [2500, 1100][:len(n)]
+    paged = widened(Paged(rng, n, lengths, 2, d, 16, elem), 1024, room // 16)
+    q = rng.standard_normal((sum(n) + 2, 4, d)).astype(np.float32)
+    got = Mass(here, paged, gpu(q), rng, decay=0.5).run(here)
+    here.sync()
+    held_to_masses(got, q)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+def test_masses_are_taken_whatever_the_page_table_has_room_for(here, case, elem):  # noqa: F811
+    """32 sequences of 8 heads, whose table has room for 2^24 tokens each: a block for each 256 of those would be more than a grid holds."""
+    case(f"mass, long table {elem}")
+    rng = np.random.default_rng(46)
+    paged = widened(Paged(rng, [1, 3, 1], [500, 70, 1], 8, 64, 16, elem), 32, 1 << 20)
+    q = rng.standard_normal((5, 16, 64)).astype(np.float32)
+    got = Mass(here, paged, gpu(q), rng).run(here)
+    here.sync()
+    held_to_masses(got, q)
