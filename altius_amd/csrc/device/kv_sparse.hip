@@ -106,13 +106,13 @@ template <int CONTROL> __device__ __forceinline__ double larger(double v) {
     return fmax(v, __longlong_as_double((long long)((uint64_t)high << 32 | low)));
 }
 
-// Scores of pages from .. to - 1 of a row's sequence, by a block, 16 a wavefront, with v_mfma_f64_4x4x4_4b_f64: four blocks of 4 pages by 4 heads, 4
+// Scores of pages of a row's sequence, by a block, 16 a wavefront: this wavefront's from `start` on and every `step` behind, below `to`, with v_mfma_f64_4x4x4_4b_f64: four blocks of 4 pages by 4 heads, 4
 // channels at a time.  Lane 16 k + p has page p, lane 16 k + 4 b + j head j, and either channels 16 u + 4 k .. + 3 for u < UNITS; the result of page 4 b + i and
 // head j is in lane 16 i + 4 b + j.  No sum goes from lane to lane, and 16 pages of 128 channels and 4 heads take 32 instructions; the same with the vector
 // unit, 16 lanes a page, spent more on adding up the lanes than on products (one token, 48 texts, group of 8: 34.5 us, so 26).
 // put(page, score, again): again: the larger of it and what is there.
-template <uint32_t UNITS, int FOURS, uint32_t WAVES, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t from, uint32_t to, Put put) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, k = lane >> 4;
+template <uint32_t UNITS, int FOURS, class Put> __device__ __forceinline__ void score_range(const SparseArgs &g, uint32_t s, uint32_t row, uint32_t head, uint32_t start, uint32_t step, uint32_t to, Put put) {
+    const uint32_t lane = threadIdx.x & 63u, k = lane >> 4;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t h0 = 0; h0 < g.group; h0 += 4 * FOURS) {
         double q[FOURS][UNITS][4];
@@ -136,16 +136,15 @@ template <uint32_t UNITS, int FOURS, uint32_t WAVES, class Put> __device__ __for
 #pragma unroll
             for (uint32_t u = 0; u < UNITS; u++) ahead[u] = *reinterpret_cast<const f32x4 *>(mean + (16 * u + 4 * k < g.d ? 16 * u + 4 * k : 0));
         };
-        const uint32_t start = from + 16 * wave;
         fetch(page_at(start));
-        int32_t page = page_at(start + 16 * WAVES);
-        for (uint32_t base = start; base < to; base += 16 * WAVES) {
+        int32_t page = page_at(start + step);
+        for (uint32_t base = start; base < to; base += step) {
             f32x4 x[UNITS];
 #pragma unroll
             for (uint32_t u = 0; u < UNITS; u++) x[u] = ahead[u];
-            if (base + 16 * WAVES < to) {
+            if (base + step < to) {
                 fetch(page);
-                page = page_at(base + 32 * WAVES);
+                page = page_at(base + 2 * step);
             }
             double v[FOURS];
 #pragma unroll
@@ -197,10 +196,12 @@ template <uint32_t UNITS, int FOURS> __global__ __launch_bounds__(BLOCK) void sc
     const uint32_t outer = blockIdx.x / g.chunks, chunk = blockIdx.x - outer * g.chunks, row = outer / g.kv.kv_heads, head = outer - row * g.kv.kv_heads;
     const Row r = row_of(g, row);
     if (r.pages <= g.most) return;  // all are chosen
-    const uint32_t from = max(chunk * SCORED, g.first), to = min((chunk + 1) * SCORED, r.pages - g.last);
     double *to_scores = g.scores + (size_t)outer * g.max_pages;
-    score_range<UNITS, FOURS, BLOCK / 64>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
+    // A run of SCORED pages, and those behind it where there are not blocks for all.  (The first pages, which are chosen anyway, among them.)
+    score_range<UNITS, FOURS>(g, r.s, row, head, chunk * SCORED + 16 * (threadIdx.x >> 6), g.chunks * SCORED, r.pages - g.last,
+                              [&](uint32_t page, double score, bool again) { to_scores[page] = again ? fmax(to_scores[page], score) : score; });
 }
+static_assert(SCORED == BLOCK / 64 * 16, "16 pages a wavefront");
 
 // The same for SCORED_ROWS rows next to each other, whose queries wait in LDS: rows of one sequence read its means together.  309 rows behind 6001 to 12000 tokens in
 // pages of 16, 4 heads of keys of 80 channels: 34 us with the choice (128 pages a block; 256 leave CUs idle, 39); each row by itself, in the block that chooses, 52.
@@ -217,8 +218,8 @@ template <uint32_t UNITS> __global__ __launch_bounds__(BLOCK) void score_rows(Sp
         // The last row has most pages.
         const uint32_t last_pages = r.live ? (uint32_t)max(0, (int32_t)g.kv.by_page_size.div((uint32_t)max(0, r.signed_place + (int32_t)rows - 1)) + 1) : 0;
         if (!r.live || r.signed_place + (int32_t)rows <= 0 || last_pages <= g.most) continue;
-        const uint32_t from = max(chunk * ROW_PAGES, g.first), to = min((chunk + 1) * ROW_PAGES, last_pages - g.last);
-        if (from >= to) continue;
+        const uint32_t most_to = last_pages - g.last;
+        if (chunk * ROW_PAGES >= most_to) continue;
         for (uint32_t h0 = 0; h0 < g.group; h0 += 4) {
             __syncthreads();
             for (uint32_t i = tid; i < rows * UNITS * 16; i += BLOCK) {  // 4 channels of a query each
@@ -229,33 +230,37 @@ template <uint32_t UNITS> __global__ __launch_bounds__(BLOCK) void score_rows(Sp
                 for (int e = 0; e < 4; e++) queries[its][u][e][4 * its_k + j] = (double)x[e];
             }
             __syncthreads();
-            for (uint32_t base = from + 16 * wave; base < to; base += BLOCK / 4) {
-                const uint32_t index = base + (lane & 15u);
-                const int32_t page = index < to ? g.kv.page_of(r.s, index, 0) : 0;
-                const float *mean = g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head;
-                double mine[UNITS][4];
-#pragma unroll
-                for (uint32_t u = 0; u < UNITS; u++) {
-                    const uint32_t c = 16 * u + 4 * k;
-                    f32x4 x = *reinterpret_cast<const f32x4 *>(mean + (c < g.d ? c : 0));
-                    if (c >= g.d) x = zero;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mine[u][e] = (double)x[e];
-                }
-                const uint32_t its_page = base + (lane & 12u) + (lane >> 4);
-                for (uint32_t its = 0; its < rows; its++) {
-                    double v = 0.0;
+            // 16 pages of a wavefront at a time: of this block's run of ROW_PAGES, and of those behind it where there are not blocks for all.
+            for (uint32_t at = chunk; at * ROW_PAGES < most_to; at += g.chunks) {
+                const uint32_t from = max(at * ROW_PAGES, g.first), to = min((at + 1) * ROW_PAGES, most_to);
+                for (uint32_t base = from + 16 * wave; base < to; base += BLOCK / 4) {
+                    const uint32_t index = base + (lane & 15u);
+                    const int32_t page = index < to ? g.kv.page_of(r.s, index, 0) : 0;
+                    const float *mean = g.means + (int64_t)page * g.means_page + (int64_t)head * g.means_head;
+                    double mine[UNITS][4];
 #pragma unroll
                     for (uint32_t u = 0; u < UNITS; u++) {
-                        if (16 * u < g.d) {
+                        const uint32_t c = 16 * u + 4 * k;
+                        f32x4 x = *reinterpret_cast<const f32x4 *>(mean + (c < g.d ? c : 0));
+                        if (c >= g.d) x = zero;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) v = __builtin_amdgcn_mfma_f64_4x4x4f64(mine[u][e], queries[its][u][e][4 * k + (lane & 3u)], v, 0, 0, 0);
-                        }
+                        for (int e = 0; e < 4; e++) mine[u][e] = (double)x[e];
                     }
-                    const double best = larger<dev::DPP_QUAD_XOR2>(larger<dev::DPP_QUAD_XOR1>(v));
-                    if ((lane & 3u) == 0 && its_page < to) {
-                        double *put = g.scores + ((size_t)(row + its) * g.kv.kv_heads + head) * g.max_pages + its_page;
-                        *put = h0 ? fmax(*put, best) : best;
+                    const uint32_t its_page = base + (lane & 12u) + (lane >> 4);
+                    for (uint32_t its = 0; its < rows; its++) {
+                        double v = 0.0;
+#pragma unroll
+                        for (uint32_t u = 0; u < UNITS; u++) {
+                            if (16 * u < g.d) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) v = __builtin_amdgcn_mfma_f64_4x4x4f64(mine[u][e], queries[its][u][e][4 * k + (lane & 3u)], v, 0, 0, 0);
+                            }
+                        }
+                        const double best = larger<dev::DPP_QUAD_XOR2>(larger<dev::DPP_QUAD_XOR1>(v));
+                        if ((lane & 3u) == 0 && its_page < to) {
+                            double *put = g.scores + ((size_t)(row + its) * g.kv.kv_heads + head) * g.max_pages + its_page;
+                            *put = h0 ? fmax(*put, best) : best;
+                        }
                     }
                 }
             }
@@ -313,7 +318,7 @@ template <uint32_t UNITS, int FOURS, uint32_t THREADS> __global__ __launch_bound
     const double *scores = UNITS ? nullptr : g.scores + ((size_t)row * g.kv.kv_heads + head) * g.max_pages;
     if constexpr (UNITS != 0) {
         if (want)
-            score_range<UNITS, FOURS, WAVES>(g, r.s, row, head, from, to, [&](uint32_t page, double score, bool again) {
+            score_range<UNITS, FOURS>(g, r.s, row, head, from + 16 * (tid >> 6), 16 * WAVES, to, [&](uint32_t page, double score, bool again) {
                 const uint64_t v = rank_image(score);
                 images[page] = again ? max(images[page], v) : v;
             });
@@ -380,6 +385,8 @@ bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 constexpr int64_t MOST_STRIDE = (int64_t)1 << 48;
 constexpr uint64_t MOST_GRID = (uint64_t)1 << 24, SCORES = (uint64_t)1 << 28;
+// Blocks that score, where there are not more rows: one without pages costs 1 ns, and a page table may have room for far more than any sequence has.
+constexpr uint64_t LAUNCHED = 1 << 14;
 
 int check_means(DeviceCtx *ctx, const std::string &name, const ahip_kv_cache &cache, const ahip_kv_sparse &sparse) {
     if (sparse.page_stride < 0 || sparse.head_stride < 0 || sparse.page_stride > MOST_STRIDE || sparse.head_stride > MOST_STRIDE)
@@ -396,7 +403,7 @@ struct SparsePlan {
     ahip_kv_batch batch;    // as attention sees it
     ahip_kv_attend attend;
     size_t attend_bytes, starts, lengths, table, scores, bytes;
-    uint64_t max_pages, rows, score_blocks;  // rows: times heads of keys
+    uint64_t max_pages, rows, chunks, score_blocks;  // rows: times heads of keys; chunks: of a row's pages that there are blocks for
     bool split, by_rows;                     // scores by a launch of their own, for rows next to each other at once
 };
 
@@ -421,8 +428,9 @@ SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const a
     const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
     p.by_rows = max_tokens >= SCORED_ROWS && p.max_pages > SCORED && (p.split || p.rows * p.max_pages * sizeof(double) <= SCORES);
     p.split = p.split || p.by_rows;
-    p.score_blocks = p.by_rows ? (attend.tokens + SCORED_ROWS - 1) / SCORED_ROWS * cache.kv_heads * ((p.max_pages + ROW_PAGES - 1) / ROW_PAGES)
-                               : p.rows * ((p.max_pages + SCORED - 1) / SCORED);
+    const uint64_t scored = p.by_rows ? (attend.tokens + SCORED_ROWS - 1) / SCORED_ROWS * cache.kv_heads : p.rows, run = p.by_rows ? ROW_PAGES : SCORED;
+    p.chunks = std::min((p.max_pages + run - 1) / run, std::max<uint64_t>(1, LAUNCHED / std::max<uint64_t>(1, scored)));
+    p.score_blocks = scored * p.chunks;
     p.attend_bytes = attend::plan_of(ctx, cache, p.batch, p.attend).bytes;
     p.starts = up16(p.attend_bytes);
     p.lengths = up16(p.starts + (attend.tokens + 1) * sizeof(int32_t));
@@ -522,10 +530,9 @@ int launch_kv_attention_sparse(DeviceCtx &ctx, const ahip_kv_cache &cache, const
     g.max_tokens = (uint32_t)std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
     g.max_keys = (uint32_t)std::min(attend.max_keys ? attend.max_keys : (size_t)INT32_MAX, (size_t)INT32_MAX);
     g.max_pages = (uint32_t)p.max_pages, g.held = (uint32_t)std::min<uint64_t>(p.max_pages, HELD);
-    g.chunks = (uint32_t)(p.by_rows ? (p.max_pages + ROW_PAGES - 1) / ROW_PAGES : (p.max_pages + SCORED - 1) / SCORED);
+    g.chunks = (uint32_t)p.chunks;
     g.starts = reinterpret_cast<int32_t *>(space + p.starts), g.lengths = reinterpret_cast<int32_t *>(space + p.lengths), g.table = reinterpret_cast<int32_t *>(space + p.table);
     g.scores = p.split ? reinterpret_cast<double *>(space + p.scores) : nullptr;
-    if (p.split && p.score_blocks >= MOST_GRID) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     // What attention will see, before anything is launched.
     p.batch.query_starts = g.starts, p.batch.lengths = g.lengths, p.batch.page_table = g.table;
     p.attend.workspace_bytes = p.attend_bytes;

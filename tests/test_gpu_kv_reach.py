@@ -136,7 +136,7 @@ def widened(paged, sequences, table_pages):
     table[:len(paged.n), :paged.per] = paged.table
     more = sequences - len(paged.n)
     paged.n, paged.lengths = paged.n + [0] * more, paged.lengths + [0] * more
-    paged.per, paged.table, paged.table_on = table_pages, table, gpu(table)
+    paged.table, paged.per, paged.table_on = table[:, :paged.per], table_pages, gpu(table)
     paged.starts_on, paged.lengths_on = gpu(np.concatenate([[0], np.cumsum(paged.n)]).astype(np.int32)), gpu(np.array(paged.lengths, np.int32))
     return paged
 
@@ -167,3 +167,29 @@ def test_masses_are_taken_whatever_the_page_table_has_room_for(here, case, elem)
     got = Mass(here, paged, gpu(q), rng).run(here)
     here.sync()
     held_to_masses(got, q)
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,tokens", [([1, 2, 1], 128), ([9, 3, 20], 2048)])
+@pytest.mark.parametrize("room", [1280, 1 << 14])
+def test_more_pages_than_blocks_are_launched_for(here, case, elem, d, n, tokens, room):  # noqa: F811
+    """Three sequences among rows of padding, 8 heads of keys: blocks for 1024 pages of a row, which go on with the pages behind their own."""
+    case(f"sparse, long {elem} d {d} n {n} tokens {tokens} room {room}")
+    rng = np.random.default_rng(47)
+    paged = widened(Paged(rng, n, [5000, 4300, 30], 8, d, 4, elem), 3, room)
+    q = rng.standard_normal((tokens, 16, d)).astype(np.float32)
+    got = Sparse(here, paged, gpu(q), 20, 3, 2, max_tokens=max(n)).run(here)
+    here.sync()
+    held_to_choice(got, q)
+
+
+def test_chosen_pages_are_taken_whatever_the_page_table_has_room_for(here, case):  # noqa: F811
+    """1024 rows times heads, and a table of 2^20 pages: a block for each 64 of those would be more than a grid holds."""
+    case("sparse, long table")
+    rng = np.random.default_rng(48)
+    paged = widened(Paged(rng, [1, 2, 1], [900, 77, 9], 8, 64, 4), 3, 1 << 20)
+    q = rng.standard_normal((128, 16, 64)).astype(np.float32)
+    got = Sparse(here, paged, gpu(q), 20, 3, 2, max_tokens=2).run(here)
+    here.sync()
+    held_to_choice(got, q)
