@@ -86,15 +86,16 @@ __device__ __forceinline__ dev::KvSequence within(const SparseArgs &g, dev::KvSe
     return q;
 }
 
-// A block for each sequence, page that its rows can have filled, and head.
+// A block for each sequence, page that its rows can have filled, and head; where there are not blocks for all it goes on with every chunks-th page behind its own.
 __global__ __launch_bounds__(BLOCK) void mean_pages(SparseArgs g) {
     const uint32_t outer = blockIdx.x / g.kv.kv_heads, head = blockIdx.x - outer * g.kv.kv_heads, s = outer / g.chunks, i = outer - s * g.chunks;
     const dev::KvSequence q = within(g, dev::kv_sequence(g.kv, s));
     if (q.n == 0) return;
-    const uint32_t base = (uint32_t)max(0, q.length - q.n), index = g.kv.by_page_size.div(base) + i;
-    if ((uint64_t)(index + 1) * g.kv.page_size > (uint32_t)q.length) return;
-    const int32_t page = g.kv.page_of(s, index, -1);
-    if (page >= 0) page_mean<BLOCK>(g, page, head);
+    const uint32_t base = (uint32_t)max(0, q.length - q.n);
+    for (uint32_t index = g.kv.by_page_size.div(base) + i; (uint64_t)(index + 1) * g.kv.page_size <= (uint32_t)q.length; index += g.chunks) {
+        const int32_t page = g.kv.page_of(s, index, -1);
+        if (page >= 0) page_mean<BLOCK>(g, page, head);
+    }
 }
 
 // ---------------------------------------------------------------- scores
@@ -385,7 +386,7 @@ bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 constexpr int64_t MOST_STRIDE = (int64_t)1 << 48;
 constexpr uint64_t MOST_GRID = (uint64_t)1 << 24, SCORES = (uint64_t)1 << 28;
-// Blocks that score, where there are not more rows: one without pages costs 1 ns, and a page table may have room for far more than any sequence has.
+// Blocks that score or make means, where there are not more rows or sequences: one without pages costs 1 ns, and a page table may have room for far more than any sequence has.
 constexpr uint64_t LAUNCHED = 1 << 14;
 
 int check_means(DeviceCtx *ctx, const std::string &name, const ahip_kv_cache &cache, const ahip_kv_sparse &sparse) {
@@ -480,8 +481,9 @@ SparseArgs args_of(const dev::KvView &view, const ahip_kv_cache &cache, const ah
 
 // Pages that the rows of a call can fill: g.chunks, and a launch over them.
 int launch_means(DeviceCtx &ctx, SparseArgs g, const std::string &name) {
-    g.chunks = g.max_tokens / g.kv.page_size + 1;
-    const uint64_t blocks = (uint64_t)g.kv.sequences * g.kv.kv_heads * g.chunks;
+    const uint64_t pairs = (uint64_t)g.kv.sequences * g.kv.kv_heads;
+    g.chunks = (uint32_t)std::min<uint64_t>(g.max_tokens / g.kv.page_size + 1, std::max<uint64_t>(1, LAUNCHED / pairs));
+    const uint64_t blocks = pairs * g.chunks;
     if (blocks >= MOST_GRID) return ctx.fail(AHIP_ERR_UNSUPPORTED, name + "more blocks than a grid holds");
     hipLaunchKernelGGL(mean_pages, dim3((uint32_t)blocks), dim3(BLOCK), 0, ctx.stream, g);
     return ctx.check(hipGetLastError(), "kv page means launch");

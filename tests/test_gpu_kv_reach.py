@@ -11,7 +11,7 @@ from altius_amd import device as D
 from decoder_oracle import STEP
 from test_gpu_kv_cache import Paged, gpu, here  # noqa: F401 (a fixture)
 from test_gpu_kv_mass import Evict, Mass, held_to_masses
-from test_gpu_kv_sparse import Sparse, held_to_choice
+from test_gpu_kv_sparse import Sparse, held_to_choice, page_means
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +193,21 @@ def test_chosen_pages_are_taken_whatever_the_page_table_has_room_for(here, case)
     got = Sparse(here, paged, gpu(q), 20, 3, 2, max_tokens=2).run(here)
     here.sync()
     held_to_choice(got, q)
+
+
+@pytest.mark.parametrize("page", [1, 4, 16])
+def test_means_of_more_pages_than_blocks_are_launched_for(here, case, page):  # noqa: F811
+    """1024 sequences, of which three hold anything, 8 heads of keys: two blocks a head."""
+    case(f"page means, long, pages of {page}")
+    rng = np.random.default_rng(49)
+    n, lengths = [100, 3, 70], [130, 48, 70]
+    paged = widened(Paged(rng, n, lengths, 8, 64, page), 1024, 200)
+    means = torch.full((paged.pages, 8, 64), math.nan, device="cuda")
+    torch.cuda.synchronize()
+    here.kv_page_means_raw(paged.cache(), paged.batch(), D.KvSparse(means=means.data_ptr(), page_stride=8 * 64, head_stride=64), sum(n))
+    here.sync()
+    got, full, written = means.cpu().numpy(), page_means(paged).cpu().numpy(), np.zeros(paged.pages, bool)
+    for s, (m, l) in enumerate(zip(n, lengths)):
+        written[paged.table[s, (l - m) // page:l // page]] = True
+    np.testing.assert_array_equal(got[written], full[written])
+    assert np.isnan(got[~written]).all()
