@@ -453,8 +453,9 @@ typedef struct ahip_kv_attend {
     void *workspace;
     size_t workspace_bytes;
 } ahip_kv_attend;
-/* Bytes of device memory that a call of ahip_kv_attention with these arguments wants as its workspace (often 0), from the
- * sizes alone: the lengths on the device do not matter.  ctx may be NULL (no GPU needed). */
+/* Bytes of device memory that a call of ahip_kv_attention or of ahip_kv_attention_tree with these arguments wants as its workspace (often
+ * 0), from the sizes alone: the lengths on the device do not matter.  ctx may be NULL (no GPU needed).  What ahip_kv_attention wants is the
+ * same with any masks; asked with causal 0, which no tree is, this tells that alone, where trees may want several times as much. */
 int ahip_kv_attention_workspace(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch,
                                 const ahip_kv_attend *attend, size_t *bytes);
 /* head_size up to 256 and a multiple of 4 (of 8 with a bf16 cache); q, out and the cache, with their strides, on 16-byte
@@ -466,8 +467,8 @@ int ahip_kv_attention(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_b
  * or, -1, the last token in front of the rows.  With depth(t) rows above it and base = lengths[s] - n tokens in front, its position is
  * base + depth(t), and it sees, of the slots in front of the rows, those of ahip_kv_attend at that position (window and first_keys), and of the
  * rows' own slots its own and those of the rows it follows, less than a window above it; |p - j| of the slopes is the distance of the
- * positions.  Everything else, the workspace too, is ahip_kv_attention's.  Up to 256 rows a sequence; causal, without a prefix (AHIP_ERR_ARG
- * otherwise).  A sequence of more rows is left out, a row that follows none in front of it is taken for one that follows no row, and the next
+ * positions.  Everything else, the workspace too, is ahip_kv_attention's.  Causal, without a prefix (AHIP_ERR_ARG otherwise), with max_tokens up to
+ * 256, whatever tokens is (AHIP_ERR_UNSUPPORTED otherwise).  A sequence of more than 256 rows is left out, a row that follows none in front of it is taken for one that follows no row, and the next
  * ahip_sync fails. */
 #define AHIP_KV_TREE_ROWS 256
 int ahip_kv_attention_tree(ahip_ctx *ctx, const ahip_kv_cache *cache, const ahip_kv_batch *batch, const ahip_kv_attend *attend,

@@ -8,8 +8,9 @@ import pytest
 import torch
 
 from altius_amd import device as D
+from altius_amd._lib import ERR_ARG, AltiusHipError
 from decoder_oracle import STEP
-from test_gpu_kv_cache import Paged, gpu, here  # noqa: F401 (a fixture)
+from test_gpu_kv_cache import Paged, gpu, held_to_definition, here  # noqa: F401 (a fixture)
 from test_gpu_kv_mass import Evict, Mass, held_to_masses
 from test_gpu_kv_sparse import Sparse, held_to_choice, page_means
 
@@ -211,3 +212,33 @@ def test_means_of_more_pages_than_blocks_are_launched_for(here, case, page):  # 
         written[paged.table[s, (l - m) // page:l // page]] = True
     np.testing.assert_array_equal(got[written], full[written])
     assert np.isnan(got[~written]).all()
+
+
+@pytest.mark.parametrize("elem", ["f32", "bf16"])
+def test_the_workspace_that_plain_attention_wants_is_told(here, case, elem):  # noqa: F811
+    """Where trees want more, the query without `causal` answers for ahip_kv_attention alone, whatever its masks."""
+    case(f"workspace of plain attention {elem}")
+    rng = np.random.default_rng(50)
+    n, lengths = [40] * 16, [int(x) for x in rng.integers(40, 700, 16)]
+    paged = Paged(rng, n, lengths, 8, 64, 16, elem)
+    q = rng.standard_normal((sum(n), 32, 64)).astype(np.float32)
+    on, out, prefix = gpu(q), torch.empty((sum(n), 32, 64), device="cuda"), rng.integers(0, 300, 16).astype(np.int32)
+    call = D.KvAttend(tokens=sum(n), q_heads=32, q=on.data_ptr(), out=out.data_ptr(), q_strides=on.stride()[:2], out_strides=out.stride()[:2], scale=1 / 8, max_tokens=40)
+    asked = D.kv_attention_workspace(here, paged.cache(), paged.batch(), call)
+    call.causal = 0
+    room = D.kv_attention_workspace(here, paged.cache(), paged.batch(), call)
+    assert room < asked
+    space = torch.full((room // 4 + 4,), math.nan, device="cuda")
+    call.workspace, call.workspace_bytes, on_prefix = space.data_ptr(), room, gpu(prefix)
+    for masks in (dict(), dict(causal=False), dict(window=90), dict(prefix=prefix)):
+        call.causal, call.window, call.prefix = int(masks.get("causal", True)), masks.get("window", 0), on_prefix.data_ptr() if "prefix" in masks else None
+        torch.cuda.synchronize()
+        here.kv_attention_raw(paged.cache(), paged.batch(), call)
+        here.sync()
+        held_to_definition(out.cpu().numpy(), paged, q, **masks)
+    assert torch.isnan(space[room // 4:]).all()
+    if room:
+        call.workspace_bytes = room - 4
+        with pytest.raises(AltiusHipError) as e:
+            here.kv_attention_raw(paged.cache(), paged.batch(), call)
+        assert e.value.code == ERR_ARG
