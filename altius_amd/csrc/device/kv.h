@@ -1,4 +1,5 @@
-// A paged cache of keys and values and the sequences of a call as the kernels see them (rotary.hip, kv_attention.hip).
+// A paged cache of keys and values and the sequences of a call as the kernels see them (rotary.hip, kv_attend.h and the other
+// kv_ files).
 // Everything a caller's device memory says -- where a sequence's rows start, how long it is, which page a place is in --
 // is checked here before it becomes an address.
 #pragma once

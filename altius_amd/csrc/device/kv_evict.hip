@@ -24,8 +24,8 @@ struct History {
 // stays is found among them (kv_rank.h), then the runs are counted and listed in order.
 //   Up to 2048 places 256 threads hold 8 images each.  48 sequences of 1025 places, 8 heads: 7.9 us.
 //   Up to 57344 places 1024 threads hold 56.  4 sequences of 20011 to 50000 places: 55 us, bound by the latency of one block's walks over the places, a CU
-// each.  Beyond, images wait in LDS as far as that goes, and what is behind is read anew, out of L2: 103 us with the same lengths and
-// one row of bins.
+// each; 4 of 57344: 63 us.  Beyond, images wait in LDS as far as that goes, and what is behind is read anew, out of L2: 4 of 57345 113 us, of 65536 119, of 131072
+// 246, in pages of 16 435.
 constexpr uint32_t HELD = 28672, PAGES = 4096, SMALL = 256, SMALL_EACH = 8, LARGE = 1024, LARGE_EACH = 56;
 constexpr uint32_t KEPT = 0xffffffffu;  // by its position; above every mass
 

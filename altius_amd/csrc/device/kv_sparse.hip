@@ -1,10 +1,10 @@
 // Attention over the pages of a cache that a cheap score selects: means of the pages that fill, a score for each page from its mean, the best pages of each
 // row and head of keys, and attention (kv_attend.h) over those, each row being a sequence of its own with a page table of its own for each head.
-//   Scores are sums of products of fp32 values in 64 bits, where no product is rounded: two pages change places only if their scores agree to about 2^-50,
-// whatever order the sums are made in.
+//   Scores are sums of products of fp32 values in 64 bits, where no product is rounded: of d channels they are off by d 2^-53 of the sum of |q mean| at most, and only
+// pages whose scores are that near to each other may change places with another order of sums.  All kernels here add in the same order: equal means have equal scores.
 //   One token behind 65535 (32 of 1024 pages of 64, 32 heads, 8 of keys, 128 channels, fp32) 31 us, bound by the chains of four launches; 48 behind 100 to 16000 (40
 // pages of 32, 4 heads of keys, bf16) 61 us, 35 of them attention at 3.6 TB/s; 309 rows behind 6001 to 12000 (61 pages of 16, 16 heads, 4 of keys of 80 channels,
-// fp32) 127 us, 95 of them attention, each row's pages for itself, 8 TB/s out of the caches.
+// fp32) 127 us, 95 of them attention, each row's pages for itself, 820 MB asked of L2.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -423,7 +423,8 @@ SparsePlan sparse_plan(const DeviceCtx *ctx, const ahip_kv_cache &cache, const a
     p.rows = attend.tokens * (uint64_t)cache.kv_heads;
     const uint64_t cus = ctx && ctx->cus_per_xcd ? 8 * ctx->cus_per_xcd : 256;
     // A block that chooses makes its scores itself where there are blocks for all CUs, or few pages: 48 tokens of up to 500 pages, 4 heads of keys, 61 us
-    // with their attention, 76 by launches of their own; one token of 1024 pages, 8 heads, 50 us and 31.
+    // with their attention, 76 by launches of their own; one token of 1024 pages, 8 heads, 50 us and 31.  Of pages of 64, 8 heads of keys: one token of 256 pages 29 us either
+    // way, of 512 33 and 30; 8 tokens of 512 47 and 46; 24 of 512 91 and 97; 48 of 1024 178 and 188.
     p.split = p.max_pages > HELD || (p.rows < cus && p.max_pages > 8 * SCORED);
     // Rows of one sequence read its means together, as far as their scores fit into SCORES bytes.
     const size_t max_tokens = std::min(attend.max_tokens ? attend.max_tokens : attend.tokens, attend.tokens);
